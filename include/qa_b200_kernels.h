@@ -111,6 +111,82 @@ int qa_k_window_attention(const void* qkv, long long T, int dm, int nh, const in
                           int n_windows, int max_window, void* out, int bf16, unsigned* status,
                           void* stream);
 
+/*
+ * The three entry points below serve sessions that grow: a few new tokens for
+ * each of many sequences, against what their caches already hold.  They have no
+ * counterpart in the reference, which prefills a whole clip at once.
+ *
+ * New tokens are packed: sequence s owns rows [q_start[s], q_start[s + 1]) of
+ * every [T]-row buffer, at most max_q of them (0 is allowed), and its cache
+ * holds kv_len[s] tokens, the new ones among them.  q_start [n_seqs + 1],
+ * kv_len [n_seqs] and block_tab [n_seqs][max_pages] are device data; they are
+ * checked on the device, and what contradicts the sizes given here (a sequence
+ * outside [0, T) or longer than max_q or than its table, a page id outside
+ * [0, kv_pages)) sets bit 2 of *status (may be NULL) and is neither read nor
+ * written.  Row strides (ld*) are in elements; head h of a row starts at h * hd,
+ * hd is 64 or 128, nq a multiple of nkv.  Sizes of zero are allowed and do
+ * nothing.
+ */
+
+/*
+ * Rotates q [T][nq * hd] into q_out (which may be q) and appends k (rotated)
+ * and v [T][nkv * hd] to the paged cache at cache indices kv_len[s] - n_s + i.
+ * Pools are [kv_pages][nkv][64][hd].
+ *
+ * Cache format: with kscale / vscale [kv_pages][nkv] (both or neither) the
+ * pools hold e4m3 codes of value code * scale, and a page's scale is the least
+ * power of two (>= 2^-64) that brings its largest finite value to at most 448;
+ * appending to a page that has tokens keeps the larger scale and rescales the
+ * older codes when it grows.  Values that are not finite become NaN codes.
+ * Without scales the pools hold the 16-bit type (what qa_k_causal_attention
+ * reads).  Sequences may share pages that are full, not the page they append to.
+ *
+ * Rotation: cos_t / sin_t [table_rows][hd / 2] f32 (NULL: none), the halves of a
+ * head paired (j, j + hd / 2).  Positions: pos [n_axes][pos_stride], NULL for the
+ * cache index; with n_axes > 1 (at most 4), axis_of [hd / 2] names each
+ * frequency's axis.  A position outside the tables sets bit 2 of *status and
+ * counts as 0.  qn / kn [hd] (both or neither): RMSNorm of each head before the
+ * rotation, with eps.  Arithmetic in f32, rounded once.  kpool, vpool, cos_t and
+ * sin_t are 16-byte aligned.
+ */
+int qa_k_kv_append(const void* q, long long ldq, const void* k, long long ldk, const void* v,
+                   long long ldv, void* q_out, long long ldqo, long long T, int nq, int nkv, int hd,
+                   const int* q_start, const int* kv_len, int n_seqs, int max_q,
+                   const int* block_tab, int max_pages, void* kpool, void* vpool, int kv_pages,
+                   float* kscale, float* vscale, const float* cos_t, const float* sin_t,
+                   int table_rows, const int* pos, long long pos_stride, int n_axes,
+                   const int* axis_of, const float* qn, const float* kn, float eps, int bf16,
+                   unsigned* status, void* stream);
+
+/*
+ * Attention of q [T][nq * hd] over the e4m3 cache: query head h reads K/V head
+ * h / (nq / nkv).  Query i of a sequence sees cache indices below
+ * kv_len - n_s + i + 1 (causal) or kv_len; scores are scale * (q . k).  A row
+ * that sees nothing gets zeros and lse -inf; what lies past a sequence's length
+ * in its last page is never used, whatever it holds.  A page id outside the pool
+ * sets bit 2 of *status and its tokens are left out.  lse [T][nq] f32 (natural
+ * logarithm of the sum of exponentials) may be NULL.  max_kv (the longest
+ * kv_len, as far as the caller knows) only sizes the launch.
+ */
+int qa_k_cache_attention(const void* q, long long ldq, long long T, int nq, int nkv, int hd,
+                         const int* q_start, const int* kv_len, int n_seqs, int max_q, int max_kv,
+                         const int* block_tab, int max_pages, const void* kpool, const void* vpool,
+                         int kv_pages, const float* kscale, const float* vscale, float scale,
+                         int causal, void* out, long long ldo, float* lse, int bf16,
+                         unsigned* status, void* stream);
+
+/*
+ * out [M][N] = x [M][K] . W^T (+ bias [N] f32), the weights in 4 bits:
+ * W[n][k] = scales[n][k / group] * (code[n][k] - zeros[n][k / group]), zeros 8
+ * when NULL.  wq [N] rows of K / 2 bytes, ldw bytes apart, the even k of a pair
+ * in the low nibble; scales [N][K / group] in x's type; group 32, 64 or 128, K a
+ * multiple of it.  f32 sums, one rounding.  Built for few rows, where the
+ * weights are what has to be read; any M is taken.
+ */
+int qa_k_w4_linear(const void* x, long long ldx, int M, int K, const uint8_t* wq, long long ldw,
+                   int N, int group, const void* scales, const uint8_t* zeros, const float* bias,
+                   void* out, long long ldo, int bf16, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

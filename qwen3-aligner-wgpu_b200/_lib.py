@@ -61,7 +61,8 @@ EXPORTED = [
     "qa_head_noalloc", "qa_probe_timeout", "qa_local_head_load", "qa_set_local_head_enabled",
     "qa_local_head_enabled", "qa_local_head_refine",
     "qa_k_gemm", "qa_k_conv3x3s2", "qa_k_causal_attention", "qa_k_window_attention",
-    "qa_k_conv1", "qa_k_gemm_qkv_rope",
+    "qa_k_conv1", "qa_k_gemm_qkv_rope", "qa_k_kv_append", "qa_k_cache_attention",
+    "qa_k_w4_linear",
 ]
 
 c_void_p = ctypes.c_void_p
@@ -190,6 +191,17 @@ def _declare(L: ctypes.CDLL) -> None:
                                         c_int, c_void_p, c_void_p]
     L.qa_k_window_attention.argtypes = [c_void_p, c_ll, c_int, c_int, c_void_p, c_int, c_int,
                                         c_void_p, c_int, c_void_p, c_void_p]
+    L.qa_k_kv_append.argtypes = [c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll,
+                                 c_ll, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int,
+                                 c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                 c_void_p, c_void_p, c_int, c_void_p, c_ll, c_int, c_void_p,
+                                 c_void_p, c_void_p, ctypes.c_float, c_int, c_void_p, c_void_p]
+    L.qa_k_cache_attention.argtypes = [c_void_p, c_ll, c_ll, c_int, c_int, c_int, c_void_p,
+                                       c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p,
+                                       c_void_p, c_int, c_void_p, c_void_p, ctypes.c_float, c_int,
+                                       c_void_p, c_ll, c_void_p, c_int, c_void_p, c_void_p]
+    L.qa_k_w4_linear.argtypes = [c_void_p, c_ll, c_int, c_int, c_void_p, c_ll, c_int, c_int,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_int, c_void_p]
     if hasattr(L, "qa_open"):
         L.qa_open.argtypes = [c_int, c_int, ctypes.POINTER(c_void_p)]
         L.qa_load.argtypes = [c_void_p, c_void_p, c_int, c_void_p]
@@ -371,3 +383,206 @@ def gemm_qkv_rope(A, B, q_out, pos_of, clip_of, block_tab, kc, vc, cos_t, sin_t,
                                    ptr(block_tab), block_tab.shape[1], ptr(kc), ptr(vc),
                                    ptr(cos_t), ptr(sin_t), ptr(qn), ptr(kn), eps, nq, nkv,
                                    ptr(status), force_bn, s))
+
+
+# ---------------------------------------------------------------- growing sessions
+
+def _need(ok, what) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _rows16(t, width, T, dtype, name) -> int:
+    """Row stride of t, which is [T, width] of 16-bit `dtype` with adjacent columns."""
+    ld = t.stride(0) if T > 1 else width
+    _need(t.dim() == 2 and t.shape[0] == T and t.shape[1] == width and t.dtype == dtype
+          and (t.stride(1) == 1 or width == 1) and ld >= width,
+          f"{name}: [{T}, {width}] of {dtype} with adjacent columns")
+    return ld
+
+
+def _on_device(*tensors) -> None:
+    dev = tensors[0].device
+    _need(all(t is None or (t.is_cuda and t.device == dev) for t in tensors),
+          "all tensors on one CUDA device")
+
+
+def _seq_args(T, q_start, kv_len, block_tab, kpool, vpool, max_q) -> tuple:
+    """Shapes of the sequence maps and pools; (n_seqs, max_pages, pages, nkv, hd)."""
+    import torch
+    i32 = torch.int32
+    _need(q_start.dtype == i32 and kv_len.dtype == i32 and block_tab.dtype == i32
+          and q_start.is_contiguous() and kv_len.is_contiguous() and block_tab.is_contiguous()
+          and q_start.dim() == 1 and kv_len.dim() == 1 and block_tab.dim() == 2
+          and q_start.shape[0] == kv_len.shape[0] + 1 == block_tab.shape[0] + 1
+          and block_tab.shape[1] > 0,
+          "q_start int32 [n + 1], kv_len int32 [n], block_tab int32 [n, max_pages], contiguous")
+    ps = kpool.shape
+    _need(len(ps) == 4 and ps == vpool.shape and ps[2] == 64 and ps[3] in (64, 128)
+          and ps[0] > 0 and ps[1] > 0 and kpool.dtype == vpool.dtype
+          and kpool.is_contiguous() and vpool.is_contiguous(),
+          "kpool / vpool [pages, heads, 64, 64 or 128], contiguous, of one type")
+    _need(max_q >= 0, "max_q >= 0")
+    return kv_len.shape[0], block_tab.shape[1], ps[0], ps[1], ps[3]
+
+
+def check_sequences(T, q_start, kv_len, block_tab, pages, max_q, appending) -> None:
+    """Host-side range checks of the sequence maps (copies them to the host;
+    ValueError on failure): what the kernels would otherwise report in *status."""
+    import torch
+    qs, kl, bt = q_start.cpu().long(), kv_len.cpu().long(), block_tab.cpu().long()
+    n = qs.diff()
+    if n.numel() == 0:
+        return
+    _need(int(qs[0]) >= 0 and int(n.min()) >= 0 and int(qs[-1]) <= T, "q_start out of range")
+    _need(int(n.max()) <= max_q, "a sequence has more than max_q new tokens")
+    _need(int(kl.min()) >= 0 and int(kl.max()) <= 64 * bt.shape[1], "kv_len out of range")
+    _need(not appending or bool((kl >= n).all()), "kv_len counts the new tokens")
+    used = torch.arange(bt.shape[1])[None] < ((kl + 63) // 64)[:, None]
+    ids = bt[used]
+    _need(ids.numel() == 0 or (int(ids.min()) >= 0 and int(ids.max()) < pages),
+          "block_tab names a page outside the pools")
+    if appending:
+        first = ((kl - n) // 64)[:, None]
+        written = bt[used & (torch.arange(bt.shape[1])[None] >= first) & (n > 0)[:, None]]
+        _need(written.unique().numel() == written.numel(), "two sequences append to one page")
+
+
+def kv_append(q, k, v, q_out, q_start, kv_len, block_tab, kpool, vpool, *, max_q, kscale=None,
+              vscale=None, cos=None, sin=None, pos=None, axis_of=None, qn=None, kn=None, eps=1e-6,
+              status=None, stream=None, validate=True):
+    """Rotate queries and append keys and values to a paged cache (qa_k_kv_append).
+
+    q [T, nq * hd], k and v [T, nkv * hd] 16-bit (rows may be slices of one
+    packed projection), q_out like q (or q itself); q_start int32 [n + 1],
+    kv_len int32 [n] (the new tokens counted), block_tab int32 [n, max_pages].
+    Pools [pages, nkv, 64, hd]: float8_e4m3fn with kscale / vscale f32 [pages,
+    nkv], or q's type without.  cos / sin f32 [rows, hd / 2]; pos int32 [T] or
+    [axes, T] (None: the cache index) with axis_of int32 [hd / 2] when there are
+    several axes; qn / kn f32 [hd].  `validate` copies the maps and the positions
+    to the host to check them; without it, what is malformed sets bit 2 of
+    `status` (int32 [1]) and is skipped.
+    """
+    import torch
+    T, dt = q.shape[0], q.dtype
+    n, max_pages, pages, nkv, hd = _seq_args(T, q_start, kv_len, block_tab, kpool, vpool, max_q)
+    _need(dt in (torch.float16, torch.bfloat16), "q, k and v are float16 or bfloat16")
+    width = q.shape[1] if q.dim() == 2 else 0
+    nq = width // hd
+    _need(nq > 0 and nq % nkv == 0, "q has a multiple of the cache's heads")
+    ldq, ldqo = _rows16(q, nq * hd, T, dt, "q"), _rows16(q_out, nq * hd, T, dt, "q_out")
+    ldk, ldv = _rows16(k, nkv * hd, T, dt, "k"), _rows16(v, nkv * hd, T, dt, "v")
+    f32 = torch.float32
+    if kscale is None:
+        _need(vscale is None and kpool.dtype == dt, "pools of q's type, or e4m3 with both scales")
+    else:
+        _need(vscale is not None and kpool.dtype == torch.float8_e4m3fn
+              and all(x.dtype == f32 and x.is_contiguous() and tuple(x.shape) == (pages, nkv)
+                      for x in (kscale, vscale)),
+              "e4m3 pools with kscale and vscale f32 [pages, heads]")
+    rows, axes, stride = 0, 1, 0
+    if cos is not None:
+        rows = cos.shape[0]
+        _need(sin is not None and rows > 0
+              and all(x.dtype == f32 and x.is_contiguous() and tuple(x.shape) == (rows, hd // 2)
+                      for x in (cos, sin)), "cos and sin f32 [rows, hd / 2]")
+        if pos is not None:
+            _need(pos.dtype == torch.int32 and pos.dim() in (1, 2) and pos.shape[-1] == T
+                  and (T < 2 or pos.stride(-1) == 1), "pos int32 [T] or [axes, T]")
+            if pos.dim() == 2:
+                axes, stride = pos.shape[0], pos.stride(0)
+            _need(1 <= axes <= 4, "one to four axes")
+            _need(axes == 1 or (axis_of is not None and axis_of.dtype == torch.int32
+                                and axis_of.is_contiguous() and tuple(axis_of.shape) == (hd // 2,)),
+                  "axis_of int32 [hd / 2] for several axes")
+    else:
+        _need(sin is None and pos is None, "sin and pos go with cos")
+    if qn is not None or kn is not None:
+        _need(qn is not None and kn is not None
+              and all(x.dtype == f32 and x.is_contiguous() and tuple(x.shape) == (hd,)
+                      for x in (qn, kn)), "qn and kn f32 [hd]")
+    if validate:
+        check_sequences(T, q_start, kv_len, block_tab, pages, max_q, True)
+        if axes > 1:
+            a = axis_of.cpu()
+            _need(int(a.min()) >= 0 and int(a.max()) < axes, "axis_of out of range")
+        if pos is not None and T:
+            _need(int(pos.min()) >= 0 and int(pos.max()) < rows, "pos outside the tables")
+        elif cos is not None and n:
+            _need(int(kv_len.max()) <= rows, "kv_len outside the tables")
+    _on_device(q, k, v, q_out, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale, cos, sin,
+               pos, axis_of, qn, kn, status)
+    s = stream if stream is not None else torch.cuda.current_stream(q.device).cuda_stream
+    check(lib().qa_k_kv_append(
+        q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
+        q_out.data_ptr(), ldqo, T, nq, nkv, hd, q_start.data_ptr(), kv_len.data_ptr(),
+        n, max_q, block_tab.data_ptr(), max_pages, kpool.data_ptr(), vpool.data_ptr(), pages,
+        ptr(kscale), ptr(vscale), ptr(cos), ptr(sin), rows, ptr(pos), stride, axes, ptr(axis_of),
+        ptr(qn), ptr(kn), eps, 1 if dt == torch.bfloat16 else 0, ptr(status), s))
+
+
+def cache_attention(q, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale, out, *, max_q,
+                    max_kv, causal=True, scale=None, lse=None, status=None, stream=None,
+                    validate=True):
+    """Attention over the e4m3 paged cache (qa_k_cache_attention).
+
+    q and out [T, nq * hd] 16-bit; the maps, pools and scales as for kv_append;
+    lse f32 [T, nq] optional; scale defaults to 1 / sqrt(hd).  max_q and max_kv
+    bound the sequences' new and cached tokens.  `validate` copies the maps to
+    the host to check them.
+    """
+    import torch
+    T, dt = q.shape[0], q.dtype
+    n, max_pages, pages, nkv, hd = _seq_args(T, q_start, kv_len, block_tab, kpool, vpool, max_q)
+    _need(dt in (torch.float16, torch.bfloat16), "q and out are float16 or bfloat16")
+    f32 = torch.float32
+    _need(kpool.dtype == torch.float8_e4m3fn and kscale.dtype == f32 and vscale.dtype == f32
+          and kscale.shape == vscale.shape == (pages, nkv) and kscale.is_contiguous()
+          and vscale.is_contiguous(), "e4m3 pools with kscale and vscale f32 [pages, heads]")
+    nq = q.shape[1] // hd if q.dim() == 2 else 0
+    _need(nq > 0 and nq % nkv == 0, "q has a multiple of the cache's heads")
+    ldq, ldo = _rows16(q, nq * hd, T, dt, "q"), _rows16(out, nq * hd, T, dt, "out")
+    _need(lse is None or (lse.dtype == f32 and lse.is_contiguous() and lse.shape == (T, nq)),
+          "lse f32 [T, heads]")
+    _need(max_kv >= 0, "max_kv >= 0")
+    if validate:
+        check_sequences(T, q_start, kv_len, block_tab, pages, max_q, False)
+        _need(n == 0 or int(kv_len.max()) <= max_kv, "a cache is longer than max_kv")
+    _on_device(q, out, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale, lse, status)
+    s = stream if stream is not None else torch.cuda.current_stream(q.device).cuda_stream
+    check(lib().qa_k_cache_attention(
+        q.data_ptr(), ldq, T, nq, nkv, hd, q_start.data_ptr(), kv_len.data_ptr(), n, max_q,
+        max_kv, block_tab.data_ptr(), max_pages, kpool.data_ptr(), vpool.data_ptr(), pages,
+        kscale.data_ptr(), vscale.data_ptr(), hd ** -0.5 if scale is None else scale,
+        1 if causal else 0, out.data_ptr(), ldo, ptr(lse),
+        1 if dt == torch.bfloat16 else 0, ptr(status), s))
+
+
+def w4_linear(x, wq, scales, out, *, zeros=None, bias=None, stream=None):
+    """out [M, N] = x [M, K] . W^T + bias, W in 4 bits (qa_k_w4_linear).
+
+    wq uint8 [N, K / 2], low nibble first; scales [N, K / group] of x's type with
+    group 32, 64 or 128 (told by the shapes); zeros uint8 like scales (None: 8);
+    bias f32 [N].
+    """
+    import torch
+    dt = x.dtype
+    _need(dt in (torch.float16, torch.bfloat16) and x.dim() == 2, "x [M, K] float16 or bfloat16")
+    M, K = x.shape
+    _need(wq.dim() == 2 and wq.dtype == torch.uint8 and 2 * wq.shape[1] == K
+          and wq.stride(1) == 1 and wq.stride(0) >= wq.shape[1], "wq uint8 [N, K / 2]")
+    N = wq.shape[0]
+    _need(scales.dim() == 2 and scales.dtype == dt and scales.shape[0] == N
+          and scales.is_contiguous() and scales.shape[1] > 0, "scales [N, K / group] of x's type")
+    group = K // scales.shape[1]
+    _need(group in (32, 64, 128) and group * scales.shape[1] == K, "group 32, 64 or 128")
+    _need(zeros is None or (zeros.dtype == torch.uint8 and zeros.shape == scales.shape
+                            and zeros.is_contiguous()), "zeros uint8 [N, K / group]")
+    _need(bias is None or (bias.dtype == torch.float32 and bias.shape == (N,)
+                           and bias.is_contiguous()), "bias f32 [N]")
+    ldx, ldo = _rows16(x, K, M, dt, "x"), _rows16(out, N, M, dt, "out")
+    _on_device(x, wq, scales, out, zeros, bias)
+    s = stream if stream is not None else torch.cuda.current_stream(x.device).cuda_stream
+    check(lib().qa_k_w4_linear(
+        x.data_ptr(), ldx, M, K, wq.data_ptr(), wq.stride(0), N, group, scales.data_ptr(),
+        ptr(zeros), ptr(bias), out.data_ptr(), ldo, 1 if dt == torch.bfloat16 else 0, s))

@@ -200,6 +200,74 @@ int lh_tail(const float* P, const float* kv, const float* audio, const LhClip* c
 int lh_repair(const long long* fixed, const float* offsets, const LhClip* clips, int n_clips,
               double* intervals, cudaStream_t s);
 
+// ---------------------------------------------------------------- growing sessions
+// New tokens of many sequences, packed: sequence s owns rows [q_start[s],
+// q_start[s + 1]) and has kv_len[s] cached tokens, the new ones among them.
+struct SeqMap {
+  const int* q_start;    // [n_seqs + 1]
+  const int* kv_len;     // [n_seqs]
+  int n_seqs;
+  const int* block_tab;  // [n_seqs][max_pages] page ids
+  int max_pages;
+  int max_q;             // most new tokens of a sequence
+};
+
+// One sequence's rows; ok is false where the map contradicts the sizes that
+// the launch was given, and such a sequence is not touched.
+struct SeqSpan {
+  long long t0;
+  int n, len;
+  bool ok;
+};
+
+#ifdef __CUDACC__
+__device__ __forceinline__ SeqSpan seq_span(const SeqMap& m, int s, long long T) {
+  const int a = m.q_start[s], b = m.q_start[s + 1], len = m.kv_len[s];
+  SeqSpan r;
+  r.t0 = a;
+  r.n = b - a;
+  r.len = len;
+  r.ok = a >= 0 && b >= a && b <= T && r.n <= m.max_q && len >= 0 &&
+         len <= 64ll * m.max_pages;
+  return r;
+}
+#endif
+
+// Rotary positions on 1..4 axes.  cos_t / sin_t [rows][hd / 2] f32, null for no
+// rotation; pos [n_axes][T] (rows pos_stride apart), null for the cache index;
+// axis_of [hd / 2], the axis of each frequency, read when n_axes > 1.
+struct RopeAxes {
+  const float* cos_t;
+  const float* sin_t;
+  int rows;
+  const int* pos;
+  long long pos_stride;
+  int n_axes;
+  const int* axis_of;
+};
+
+// Rotated queries, and keys and values appended to a paged cache (kv_append.cu).
+// kscale / vscale [kv_pages][nkvh] given: e4m3 codes; null: the 16-bit type.
+// Malformed sequences, page ids outside the pools and positions outside the
+// tables set status bit 2 and are not read or written.
+int kv_append(const void* q, long long ldq, const void* k, long long ldk, const void* v,
+              long long ldv, void* q_out, long long ldqo, long long T, int nqh, int nkvh, int hd,
+              const SeqMap& seqs, int max_q, PagedKV kv, int kv_pages, float* kscale, float* vscale,
+              const RopeAxes& rope, const float* qn, const float* kn, float eps, bool bf16,
+              unsigned* status, cudaStream_t s);
+
+// Attention over the e4m3 cache (cache_attn.cu); lse [T][nqh] optional.
+int cache_attention(const void* q, long long ldq, long long T, int nqh, int nkvh, int hd,
+                    const SeqMap& seqs, int max_q, int max_kv, const void* kpool, const void* vpool,
+                    int kv_pages, const float* kscale, const float* vscale, float scale, bool causal,
+                    void* out, long long ldo, float* lse, bool bf16, unsigned* status,
+                    cudaStream_t s);
+
+// y = x W^T (+ bias), W in 4 bits with group scales (w4.cu).
+int w4_linear(const void* x, long long ldx, int M, int K, const uint8_t* wq, long long ldw, int N,
+              int group, const void* scales, const uint8_t* zeros, const float* bias, void* out,
+              long long ldo, bool bf16, cudaStream_t s);
+
 // 16-bit [rows][d] -> f32 widening (text_hidden readback).
 int widen16(const void* x, long long n, float* out, bool bf16, cudaStream_t s);
 

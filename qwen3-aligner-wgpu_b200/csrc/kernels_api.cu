@@ -109,3 +109,85 @@ extern "C" int qa_k_conv1(const float* mel, int n, int h, int w, const float* wt
                               static_cast<cudaStream_t>(stream));
   return rc == 0 ? QA_OK : QA_ERR_CUDA;
 }
+
+namespace {
+
+// What both cache entry points ask of their sequences and pools.
+bool cache_args_ok(int nq, int nkv, const int* q_start, const int* kv_len, int n_seqs, int max_q,
+                   const int* block_tab, int max_pages, const void* kpool, const void* vpool,
+                   int kv_pages) {
+  return q_start && kv_len && block_tab && kpool && vpool && n_seqs >= 0 && max_q >= 0 &&
+         max_pages > 0 && kv_pages > 0 && nq > 0 && nkv > 0 && nq % nkv == 0;
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+}  // namespace
+
+extern "C" int qa_k_kv_append(const void* q, long long ldq, const void* k, long long ldk,
+                              const void* v, long long ldv, void* q_out, long long ldqo,
+                              long long T, int nq, int nkv, int hd, const int* q_start,
+                              const int* kv_len, int n_seqs, int max_q, const int* block_tab,
+                              int max_pages, void* kpool, void* vpool, int kv_pages, float* kscale,
+                              float* vscale, const float* cos_t, const float* sin_t, int table_rows,
+                              const int* pos, long long pos_stride, int n_axes, const int* axis_of,
+                              const float* qn, const float* kn, float eps, int bf16,
+                              unsigned* status, void* stream) {
+  if (T == 0 || n_seqs == 0) return QA_OK;
+  if (!cache_args_ok(nq, nkv, q_start, kv_len, n_seqs, max_q, block_tab, max_pages, kpool, vpool,
+                     kv_pages) ||
+      !q || !k || !v || !q_out || T < 0 || T > 0x7FFFFFFFll || !kscale != !vscale ||
+      !cos_t != !sin_t || (cos_t && table_rows <= 0) || n_axes < 1 || n_axes > 4 ||
+      (n_axes > 1 && cos_t && (!pos || !axis_of)) || !qn != !kn)
+    return QA_ERR_ARG;
+  if ((hd != 64 && hd != 128) || ldq < static_cast<long long>(nq) * hd ||
+      ldqo < static_cast<long long>(nq) * hd || ldk < static_cast<long long>(nkv) * hd ||
+      ldv < static_cast<long long>(nkv) * hd)
+    return QA_ERR_SHAPE;
+  if (!aligned16(kpool) || !aligned16(vpool) || !aligned16(cos_t) || !aligned16(sin_t))
+    return QA_ERR_ARG;
+  const SeqMap seqs{q_start, kv_len, n_seqs, block_tab, max_pages, max_q};
+  const RopeAxes rope{cos_t, sin_t, table_rows, pos, pos_stride, n_axes, axis_of};
+  const int rc = kv_append(q, ldq, k, ldk, v, ldv, q_out, ldqo, T, nq, nkv, hd, seqs, max_q,
+                           PagedKV{kpool, vpool, 64}, kv_pages, kscale, vscale, rope, qn, kn, eps,
+                           bf16 != 0, status, static_cast<cudaStream_t>(stream));
+  return rc == 0 ? QA_OK : QA_ERR_CUDA;
+}
+
+extern "C" int qa_k_cache_attention(const void* q, long long ldq, long long T, int nq, int nkv,
+                                    int hd, const int* q_start, const int* kv_len, int n_seqs,
+                                    int max_q, int max_kv, const int* block_tab, int max_pages,
+                                    const void* kpool, const void* vpool, int kv_pages,
+                                    const float* kscale, const float* vscale, float scale,
+                                    int causal, void* out, long long ldo, float* lse, int bf16,
+                                    unsigned* status, void* stream) {
+  if (T == 0 || n_seqs == 0) return QA_OK;
+  if (!cache_args_ok(nq, nkv, q_start, kv_len, n_seqs, max_q, block_tab, max_pages, kpool, vpool,
+                     kv_pages) ||
+      !q || !kscale || !vscale || !out || T < 0 || T > 0x7FFFFFFFll || max_kv < 0 ||
+      !(scale - scale == 0.0f))
+    return QA_ERR_ARG;
+  if ((hd != 64 && hd != 128) || ldq < static_cast<long long>(nq) * hd ||
+      ldo < static_cast<long long>(nq) * hd)
+    return QA_ERR_SHAPE;
+  if (!aligned16(kpool) || !aligned16(vpool)) return QA_ERR_ARG;
+  const SeqMap seqs{q_start, kv_len, n_seqs, block_tab, max_pages, max_q};
+  const int rc = cache_attention(q, ldq, T, nq, nkv, hd, seqs, max_q, max_kv, kpool, vpool,
+                                 kv_pages, kscale, vscale, scale, causal != 0, out, ldo, lse,
+                                 bf16 != 0, status, static_cast<cudaStream_t>(stream));
+  return rc == 0 ? QA_OK : QA_ERR_CUDA;
+}
+
+extern "C" int qa_k_w4_linear(const void* x, long long ldx, int M, int K, const uint8_t* wq,
+                              long long ldw, int N, int group, const void* scales,
+                              const uint8_t* zeros, const float* bias, void* out, long long ldo,
+                              int bf16, void* stream) {
+  if (M == 0 || N == 0) return QA_OK;
+  if (!x || !wq || !scales || !out || M < 0 || N < 0) return QA_ERR_ARG;
+  if ((group != 32 && group != 64 && group != 128) || K <= 0 || K % group != 0 || ldx < K ||
+      ldw < K / 2 || ldo < N)
+    return QA_ERR_SHAPE;
+  const int rc = w4_linear(x, ldx, M, K, wq, ldw, N, group, scales, zeros, bias, out, ldo,
+                           bf16 != 0, static_cast<cudaStream_t>(stream));
+  return rc == 0 ? QA_OK : QA_ERR_CUDA;
+}
