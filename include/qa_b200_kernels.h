@@ -165,15 +165,27 @@ int qa_k_kv_append(const void* q, long long ldq, const void* k, long long ldk, c
  * that sees nothing gets zeros and lse -inf; what lies past a sequence's length
  * in its last page is never used, whatever it holds.  A page id outside the pool
  * sets bit 2 of *status and its tokens are left out.  lse [T][nq] f32 (natural
- * logarithm of the sum of exponentials) may be NULL.  max_kv (the longest
- * kv_len, as far as the caller knows) only sizes the launch.
+ * logarithm of the sum of exponentials) may be NULL.
+ *
+ * max_kv (the longest kv_len, as far as the caller knows) sizes the launch; a
+ * smaller or larger value gives the same results up to the order of sums.
+ *
+ * workspace: device memory, 16-byte aligned, of the size that
+ * qa_k_cache_attention_workspace gives for these arguments (0: none is needed),
+ * its first 2^20 bytes filled with zeros once before its first use; each call
+ * leaves it fit for the next one, of whatever sizes, and two calls that may run
+ * at the same time need one each.  With less of it, or NULL, some or all
+ * sequences are not split over CTAs, which is slow for few long caches.  A
+ * sequence's result does not depend on the others of the batch, as long as the
+ * workspace has the size given.
  */
+int64_t qa_k_cache_attention_workspace(int nq, int nkv, int hd, int n_seqs, int max_q, int max_kv);
 int qa_k_cache_attention(const void* q, long long ldq, long long T, int nq, int nkv, int hd,
                          const int* q_start, const int* kv_len, int n_seqs, int max_q, int max_kv,
                          const int* block_tab, int max_pages, const void* kpool, const void* vpool,
                          int kv_pages, const float* kscale, const float* vscale, float scale,
-                         int causal, void* out, long long ldo, float* lse, int bf16,
-                         unsigned* status, void* stream);
+                         int causal, void* out, long long ldo, float* lse, void* workspace,
+                         long long workspace_bytes, int bf16, unsigned* status, void* stream);
 
 /*
  * out [M][N] = x [M][K] . W^T (+ bias [N] f32), the weights in 4 bits:

@@ -62,7 +62,7 @@ EXPORTED = [
     "qa_local_head_enabled", "qa_local_head_refine",
     "qa_k_gemm", "qa_k_conv3x3s2", "qa_k_causal_attention", "qa_k_window_attention",
     "qa_k_conv1", "qa_k_gemm_qkv_rope", "qa_k_kv_append", "qa_k_cache_attention",
-    "qa_k_w4_linear",
+    "qa_k_cache_attention_workspace", "qa_k_w4_linear",
 ]
 
 c_void_p = ctypes.c_void_p
@@ -199,7 +199,10 @@ def _declare(L: ctypes.CDLL) -> None:
     L.qa_k_cache_attention.argtypes = [c_void_p, c_ll, c_ll, c_int, c_int, c_int, c_void_p,
                                        c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p,
                                        c_void_p, c_int, c_void_p, c_void_p, ctypes.c_float, c_int,
-                                       c_void_p, c_ll, c_void_p, c_int, c_void_p, c_void_p]
+                                       c_void_p, c_ll, c_void_p, c_void_p, c_ll, c_int, c_void_p,
+                                       c_void_p]
+    L.qa_k_cache_attention_workspace.argtypes = [c_int] * 6
+    L.qa_k_cache_attention_workspace.restype = ctypes.c_int64
     L.qa_k_w4_linear.argtypes = [c_void_p, c_ll, c_int, c_int, c_void_p, c_ll, c_int, c_int,
                                  c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_int, c_void_p]
     if hasattr(L, "qa_open"):
@@ -521,6 +524,9 @@ def kv_append(q, k, v, q_out, q_start, kv_len, block_tab, kpool, vpool, *, max_q
         ptr(qn), ptr(kn), eps, 1 if dt == torch.bfloat16 else 0, ptr(status), s))
 
 
+_workspaces: dict = {}  # (device, stream) -> the attention's workspace
+
+
 def cache_attention(q, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale, out, *, max_q,
                     max_kv, causal=True, scale=None, lse=None, status=None, stream=None,
                     validate=True):
@@ -529,7 +535,8 @@ def cache_attention(q, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale,
     q and out [T, nq * hd] 16-bit; the maps, pools and scales as for kv_append;
     lse f32 [T, nq] optional; scale defaults to 1 / sqrt(hd).  max_q and max_kv
     bound the sequences' new and cached tokens.  `validate` copies the maps to
-    the host to check them.
+    the host to check them.  A workspace is kept for each stream and
+    grows with the sizes seen (outside of graph capture).
     """
     import torch
     T, dt = q.shape[0], q.dtype
@@ -550,11 +557,17 @@ def cache_attention(q, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale,
         _need(n == 0 or int(kv_len.max()) <= max_kv, "a cache is longer than max_kv")
     _on_device(q, out, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale, lse, status)
     s = stream if stream is not None else torch.cuda.current_stream(q.device).cuda_stream
+    need = lib().qa_k_cache_attention_workspace(nq, nkv, hd, n, max_q, max_kv)
+    ws = _workspaces.get((q.device, s)) if need else None
+    if need and (ws is None or ws.numel() < need):
+        torch.cuda.synchronize(q.device)  # nobody uses the old one, and the new one is zeroed
+        ws = _workspaces[(q.device, s)] = torch.zeros(need, dtype=torch.uint8, device=q.device)
+        torch.cuda.synchronize(q.device)
     check(lib().qa_k_cache_attention(
         q.data_ptr(), ldq, T, nq, nkv, hd, q_start.data_ptr(), kv_len.data_ptr(), n, max_q,
         max_kv, block_tab.data_ptr(), max_pages, kpool.data_ptr(), vpool.data_ptr(), pages,
         kscale.data_ptr(), vscale.data_ptr(), hd ** -0.5 if scale is None else scale,
-        1 if causal else 0, out.data_ptr(), ldo, ptr(lse),
+        1 if causal else 0, out.data_ptr(), ldo, ptr(lse), ptr(ws), need,
         1 if dt == torch.bfloat16 else 0, ptr(status), s))
 
 

@@ -5,17 +5,22 @@
 // them) sees cache indices c < len - n + i + 1 when causal, c < len otherwise:
 //   s_c = scale kscale[page(c)] (q . kcode_c),  out = sum_c softmax(s)_c vscale[page(c)] vcode_c,
 // lse = log sum_c exp(s_c); a row that sees nothing gets 0 and -inf.
-#include <cuda_fp8.h>
+#include <algorithm>
 
 #include "gemm_tc.cuh"
 #include "kernels.cuh"
 #include "sm100.cuh"
+#include "tma_host.h"
 
 namespace qa {
 
 namespace {
 
 constexpr int kPage = 64;
+constexpr int kMaxCtasPerSm = 3;
+constexpr int kJoin = 16;                        // parts joined at a time
+constexpr int kMaxParts = kJoin * kJoin;         // parts of a unit
+constexpr long long kCounterBytes = 1ll << 20;   // the workspace's counters
 
 struct CacheAttnParams {
   const void* q;
@@ -31,20 +36,35 @@ struct CacheAttnParams {
   long long ldo;
   float* lse;
   int vec;      // q and out rows can be read and written 16 bytes at a time
-  int cluster;  // CTAs that share a sequence's tokens
+  int tiles_max;       // tiles of a sequence of max_q tokens
+  int* arrived;        // workspace: parts that are there, a counter a group and one a unit
+  float* parts;        // workspace: a unit's parts and groups, part_stride floats each
+  long long cap_units; // units that have a place in the workspace
+  int cap_parts;       // parts a unit has place for
+  int part_rows, part_stride;
   unsigned* status;
 };
 
 // ------------------------------------------------------------ few query rows
 // A query row is one (new token, head of the K/V head's group); row r of a
-// sequence is token r / group, head r % group.  A CTA takes up to 8 * NT rows of
-// one sequence and K/V head; a cluster of CTAs splits the cached tokens.
+// sequence is token r / group, head r % group.  A CTA takes up to 8 * NT rows of one
+// sequence and K/V head (a unit) at a time.
 //
 // Bound: the cache's bytes, read once (2 hd a token and head), so what matters
-// is bytes in flight and instructions a byte.  Each of the CTA's warps streams
-// its own slabs of 16 tokens through a private ring of kStages slabs
-// (cp.async), without any CTA-wide barrier in the loop: 12 warps and three slabs
-// of 4 KB each keep 144 KB in flight on an SM.
+// is that every SM reads all the time, bytes in flight and instructions a byte.
+//  - A unit's cached tokens are cut into chunks by the unit's own length alone
+//    (so a sequence's result does not depend on the batch it is in).  The slabs
+//    of 16 tokens of all units, laid end to end, are shared out evenly over the
+//    CTAs that the GPU holds; a CTA takes the chunks that begin in its share,
+//    which it finds from kv_len and q_start itself.
+//  - A unit of one chunk is finished where it is computed.  Otherwise each chunk
+//    leaves its part (m, l, O) in the workspace, and the CTA that completes a
+//    group of 16 parts joins them in order; with more than one group, the CTA
+//    that completes the last group joins the groups.  No second launch, no
+//    atomics on values, the same bits each time.
+//  - Each warp streams its own slabs through a private ring of kStages slabs
+//    (TMA, 128-byte swizzle; hd 64: 64-byte), without any CTA-wide barrier in
+//    the loop.
 //
 // Tokens are the M = 16 side of both products, so 8 rows cost one mma.sync
 // m16n8k16 a 16x16 block and nothing is padded to 16 rows:
@@ -72,7 +92,6 @@ constexpr int kStages = 4;
 constexpr int kSlab = 16;  // tokens
 constexpr float kLift = 8.0f, kSlack = 6.0f;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxCluster = 16;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
@@ -90,36 +109,22 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   return d;
 }
 
-// Two e4m3 codes (low byte first) as f16x2.
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w16) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w16), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+// Four e4m3 codes (low byte first) as two f16x2; NaN codes stay NaN.
+__device__ __forceinline__ void e4m3x4_f16x2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
-}
-__device__ __forceinline__ float ld_cluster_f32(uint32_t a) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t a) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
-  return v;
-}
-// 4 bytes global -> shared.
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(src)) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // Base-2 logarithm and reciprocal of a page's V scale; a scale of 0 (a page of
@@ -140,466 +145,698 @@ __device__ __forceinline__ void store4(T* p, float4 v, bool vec) {
   }
 }
 
+// Slabs of a chunk of a unit of `slabs` slabs: 256 tokens keep a short unit's
+// latency down (16 chunks up to 4096 tokens, joined in one step), 512 the joins
+// of a long one (256 chunks up to 131072 tokens, two steps).
+__host__ __device__ __forceinline__ int chunk_slabs(int slabs) {
+  return slabs <= kJoin * 16 ? 16 : slabs <= kMaxParts * 32 ? 32 : (slabs + kMaxParts - 1) / kMaxParts;
+}
+
+// Shared memory of the few-row kernel besides the ring.
+template <int R>
+struct RowsShared {
+  uint64_t full[kWarps][kStages];
+  float m[kWarps][R], l[kWarps][R];  // the warps' references and sums
+  float cm[R], cl[R];                // the CTA's
+  float w[kJoin][R];                 // weights of joined parts
+  float inv[R];                      // 1 / sum
+  long long scan[kWarps];
+  long long lo, hi;                  // this CTA's share of the slabs
+  long long start;                   // first slab of the first sequence of the share
+  int seq;                           // that sequence
+  int last;
+};
+
+// What a sequence asks of the few-row kernel: tiles x K/V heads units of
+// `slabs` slabs, each in `chunks` chunks of `step` slabs.
+struct SeqPlan {
+  int tiles, slabs, step, chunks;
+  long long cost;  // slabs of all units
+};
+__device__ __forceinline__ SeqPlan seq_plan(const CacheAttnParams& ap, const SeqSpan& sp, int s,
+                                            int group, int R) {
+  SeqPlan c;
+  c.tiles = sp.ok ? (sp.n * group + R - 1) / R : 0;
+  c.slabs = max(1, (sp.len + kSlab - 1) / kSlab);  // an empty cache still owes its rows zeros
+  c.step = chunk_slabs(c.slabs);
+  c.chunks = (c.slabs + c.step - 1) / c.step;
+  if (c.chunks > ap.cap_parts || static_cast<long long>(s + 1) * ap.tiles_max * ap.nkv > ap.cap_units) {
+    c.step = c.slabs;  // no place for the parts
+    c.chunks = 1;
+  }
+  c.cost = static_cast<long long>(c.tiles) * c.slabs * ap.nkv;
+  return c;
+}
+
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(kWarps * 32) cache_attn_rows(CacheAttnParams ap) {
+__global__ void __launch_bounds__(kWarps * 32)
+    cache_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    CacheAttnParams ap) {
   constexpr int R = 8 * NT;          // rows of a tile
-  constexpr int kCpr = HD / 16;      // 16-byte units of a token
-  constexpr int kKc = HD / 64;       // units of K a thread reads a token
+  constexpr int kKc = HD / 64;       // 16-byte units of K a thread reads a token
   constexpr int kMt = HD / 16;       // 16-dim blocks of O^T
   constexpr int kPart = kSlab * HD;  // bytes of a slab's K (or V)
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float s_head[kWarps][kStages][4];  // K scale, V scale, tokens that may be seen
-  __shared__ float s_m[kWarps][R], s_l[kWarps][R];
-  __shared__ float s_cm[R], s_cl[R];            // the CTA's
-  __shared__ float s_w[kMaxCluster][R], s_inv[R];
-
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ RowsShared<R> sh;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int group = ap.nq / ap.nkv, n_seqs = ap.seqs.n_seqs;
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    for (int i = 0; i < kWarps * kStages; ++i) mbar_init(&sh.full[0][0] + i, 1);
+    fence_barrier_init();
+  }
   pdl_wait();
   pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int rank = blockIdx.x % ap.cluster, item = blockIdx.x / ap.cluster;
-  const int s = item % ap.seqs.n_seqs, tile = item / ap.seqs.n_seqs;
-  const int h = blockIdx.y;
-  const SeqSpan sp = seq_span(ap.seqs, s, ap.T);
-  if (!sp.ok) {
-    if (tile == 0 && h == 0 && rank == 0 && threadIdx.x == 0 && ap.status) atomicOr(ap.status, kStatusBadShape);
-    return;
-  }
-  const int group = ap.nq / ap.nkv;
-  const int rows = min(R, sp.n * group - tile * R);
-  if (rows <= 0) return;
-  // tokens that the tile's last row sees, and the CTAs that share them
-  const int past = sp.len - sp.n;  // + i + 1: seen by new token i
-  const int seen = ap.causal ? min(sp.len, max(0, past + (tile * R + rows - 1) / group + 1)) : sp.len;
-  const int slabs = (seen + kSlab - 1) / kSlab;
-  const int cta = min(ap.cluster, max(1, (slabs + 2 * kWarps - 1) / (2 * kWarps)));
-  if (rank >= cta) {
-    if (cta > 1) {  // the cluster's barriers count this CTA too
-      cluster_sync();
-      cluster_sync();
-    }
-    return;
-  }
 
-  // ---- queries: B operands, f16
-  uint32_t qf[NT][HD / 16][2];
-  float fac[NT][2];  // scale log2(e), undoing the row's own scaling, of columns 2t, 2t + 1
-  int lim[NT][2];    // tokens that they see
+  // ---- this CTA's share: thread i adds up sequences [i c, (i + 1) c)
+  {
+    const int c = (n_seqs + kWarps * 32 - 1) / (kWarps * 32);
+    const int s0 = min(n_seqs, static_cast<int>(threadIdx.x) * c), s1 = min(n_seqs, s0 + c);
+    long long mine = 0;
+    for (int i = s0; i < s1; ++i) {
+      const SeqSpan sp = seq_span(ap.seqs, i, ap.T);
+      if (!sp.ok && blockIdx.x == 0 && ap.status) atomicOr(ap.status, kStatusBadShape);
+      mine += seq_plan(ap, sp, i, group, R).cost;
+    }
+    long long before = mine;  // inclusive scan
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = nt * 8 + g, row = tile * R + r;
-    float shift = 1.0f, undo = 1.0f;
-    if (r < rows) {
-      const T* qr = static_cast<const T*>(ap.q) + (sp.t0 + row / group) * ap.ldq +
-                    static_cast<long long>(h * group + row % group) * HD;
-      uint4 raw[kKc][2];
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xFFFFFFFFu, before, o);
+      if (lane >= o) before += y;
+    }
+    if (lane == 31) sh.scan[warp] = before;
+    __syncthreads();
+    long long total = 0;
 #pragma unroll
-      for (int i = 0; i < kKc; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const T* src = qr + 16 * (kKc * t + i) + 8 * j;
-          if (ap.vec) {
-            raw[i][j] = *reinterpret_cast<const uint4*>(src);
-          } else {
-            T* e = reinterpret_cast<T*>(&raw[i][j]);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) e[k] = src[k];
-          }
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += sh.scan[w];
+      total += sh.scan[w];
+    }
+    before -= mine;
+    const long long quot = total / gridDim.x, rem = total % gridDim.x, b = blockIdx.x;
+    const long long lo = quot * b + min(b, rem), hi = lo + quot + (b < rem ? 1 : 0);
+    if (lo >= hi) return;
+    if (lo >= before && lo < before + mine) {  // the share begins in one of mine
+      sh.lo = lo;
+      sh.hi = hi;
+      for (int i = s0; i < s1; ++i) {
+        const long long cost = seq_plan(ap, seq_span(ap.seqs, i, ap.T), i, group, R).cost;
+        if (lo < before + cost) {
+          sh.seq = i;
+          sh.start = before;
+          break;
         }
-      if constexpr (H16Traits<T>::kBf16) {
-        float big = 0.0f;
+        before += cost;
+      }
+    }
+    __syncthreads();
+  }
+  const long long share_hi = sh.hi;
+  uint32_t it = 0;  // slabs this warp has taken through its ring
+  bool ok = true;   // no wait has run out
+  long long x = sh.lo;  // first slab still to be looked at
+  int s = sh.seq, unit, chunk;
+  SeqSpan sp = seq_span(ap.seqs, s, ap.T);
+  SeqPlan plan = seq_plan(ap, sp, s, group, R);
+  {
+    const long long rel = x - sh.start;
+    unit = static_cast<int>(rel / plan.slabs);
+    const int in = static_cast<int>(rel % plan.slabs);
+    chunk = (in + plan.step - 1) / plan.step;  // the first that begins here
+    x += min(plan.slabs, chunk * plan.step) - in;
+  }
+  while (x < share_hi) {
+    if (chunk == plan.chunks) {
+      chunk = 0;
+      ++unit;
+    }
+    if (unit >= plan.tiles * ap.nkv) {
+      ++s;  // x < share_hi <= total: there is another unit
+      unit = chunk = 0;
+      sp = seq_span(ap.seqs, s, ap.T);
+      plan = seq_plan(ap, sp, s, group, R);
+      continue;
+    }
+    const int tile = unit / ap.nkv, h = unit % ap.nkv;
+    const int lo = chunk * plan.step, hi = min(plan.slabs, lo + plan.step);
+    x += hi - lo;
+    const int rows = min(R, sp.n * group - tile * R);
+    const int past = sp.len - sp.n;  // + i + 1: tokens seen by new token i
+    const int seen = ap.causal ? min(sp.len, max(0, past + (tile * R + rows - 1) / group + 1)) : sp.len;
+    const int end = min(hi, (seen + kSlab - 1) / kSlab);
+
+    // ---- the ring's first slabs
+    uint8_t* ring = smem + warp * (kStages * 2 * kPart);
+    const int* bt = ap.seqs.block_tab + static_cast<long long>(s) * ap.seqs.max_pages;
+    const int first = lo + warp;
+    auto page_of = [&](int slab) { return slab < end ? bt[slab / (kPage / kSlab)] : 0; };
+    auto good = [&](int page) { return page >= 0 && page < ap.kv_pages; };
+    auto fetch = [&](int slab, int page, uint32_t n) {
+      if (slab < end && lane == 0) {
+        uint64_t* bar = &sh.full[warp][n % kStages];
+        if (good(page)) {
+          const int row = (page * ap.nkv + h) * kPage + slab % (kPage / kSlab) * kSlab;
+          uint8_t* dst = ring + n % kStages * (2 * kPart);
+          mbar_arrive_expect_tx(bar, 2 * kPart);
+          tma_load_2d(&tmK, bar, dst, 0, row);
+          tma_load_2d(&tmV, bar, dst + kPart, 0, row);
+        } else {
+          if (ap.status) atomicOr(ap.status, kStatusBadShape);
+          mbar_arrive(bar);
+        }
+      }
+    };
+    int pages[kStages];  // of the slabs from the current one on
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) pages[i] = page_of(first + i * kWarps);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) fetch(first + i * kWarps, pages[i], it + i);
+    auto scale_at = [&](const float* p, int page) {
+      return p[static_cast<long long>(good(page) ? page : 0) * ap.nkv + h];
+    };
+    float ks_next = scale_at(ap.kscale, pages[0]), vs_next = scale_at(ap.vscale, pages[0]);
+
+    // ---- queries: B operands, f16
+    uint32_t qf[NT][HD / 16][2];
+    float fac[NT][2];  // scale log2(e), undoing the row's own scaling, of columns 2t, 2t + 1
+    int lim[NT][2];    // tokens that they see
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = nt * 8 + g, row = tile * R + r;
+      float undo = 1.0f;
+      if (r < rows) {
+        const T* qr = static_cast<const T*>(ap.q) + (sp.t0 + row / group) * ap.ldq +
+                      static_cast<long long>(h * group + row % group) * HD;
+        uint4 raw[kKc][2];
 #pragma unroll
         for (int i = 0; i < kKc; ++i)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < 2; ++j) {
+            const T* src = qr + 16 * (kKc * t + i) + 8 * j;
+            if (ap.vec) {
+              raw[i][j] = *reinterpret_cast<const uint4*>(src);
+            } else {
+              T* e = reinterpret_cast<T*>(&raw[i][j]);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              big = fmaxf(big, fabsf(h2f<T>(reinterpret_cast<const T*>(&raw[i][j])[k])));
-        const unsigned quad = 0xFu << (lane & 28);
-        big = fmaxf(big, __shfl_xor_sync(quad, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(quad, big, 2));
-        const int e = (__float_as_int(big) >> 23) - 127;  // 2^e <= big
-        // 2^(14 - e), in reach of a float for every finite row
-        if (big > 0.0f && e < 128) {
-          const int up = min(14 - e, 126);
-          shift = __int_as_float((up + 127) << 23);
-          undo = __int_as_float((127 - up) << 23);
+              for (int k = 0; k < 8; ++k) e[k] = src[k];
+            }
+          }
+        if constexpr (H16Traits<T>::kBf16) {
+          float big = 0.0f, shift = 1.0f;
+#pragma unroll
+          for (int i = 0; i < kKc; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                big = fmaxf(big, fabsf(h2f<T>(reinterpret_cast<const T*>(&raw[i][j])[k])));
+          const unsigned quad = 0xFu << (lane & 28);
+          big = fmaxf(big, __shfl_xor_sync(quad, big, 1));
+          big = fmaxf(big, __shfl_xor_sync(quad, big, 2));
+          const int e = (__float_as_int(big) >> 23) - 127;  // 2^e <= big
+          // 2^(14 - e), in reach of a float for every finite row
+          if (big > 0.0f && e < 128) {
+            const int up = min(14 - e, 126);
+            shift = __int_as_float((up + 127) << 23);
+            undo = __int_as_float((127 - up) << 23);
+          }
+#pragma unroll
+          for (int i = 0; i < kKc; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t* w = reinterpret_cast<uint32_t*>(&raw[i][j]);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const T* e2 = reinterpret_cast<const T*>(&w[k]);
+                w[k] = cvt2_rn<__half>(make_float2(h2f<T>(e2[0]) * shift, h2f<T>(e2[1]) * shift));
+              }
+            }
         }
 #pragma unroll
         for (int i = 0; i < kKc; ++i)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            uint32_t* w = reinterpret_cast<uint32_t*>(&raw[i][j]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const T* e2 = reinterpret_cast<const T*>(&w[k]);
-              w[k] = cvt2_rn<__half>(make_float2(h2f<T>(e2[0]) * shift, h2f<T>(e2[1]) * shift));
-            }
+            qf[nt][4 * i + 2 * j][0] = raw[i][j].x;
+            qf[nt][4 * i + 2 * j][1] = raw[i][j].y;
+            qf[nt][4 * i + 2 * j + 1][0] = raw[i][j].z;
+            qf[nt][4 * i + 2 * j + 1][1] = raw[i][j].w;
           }
+      } else {
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) qf[nt][k][0] = qf[nt][k][1] = 0u;
       }
+      __syncwarp();
 #pragma unroll
-      for (int i = 0; i < kKc; ++i)
+      for (int c = 0; c < 2; ++c) {
+        fac[nt][c] = __shfl_sync(0xFFFFFFFFu, undo, 8 * t + 4 * c) * (ap.scale * kLog2e);
+        const int cr = nt * 8 + 2 * t + c;
+        // columns without a row: zeros that nothing masks and nobody reads
+        lim[nt][c] = cr >= rows ? 0x7FFFFFFF : ap.causal ? max(0, past + (tile * R + cr) / group + 1) : sp.len;
+      }
+    }
+    int all = 0x7FFFFFFF;  // tokens that every row sees
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          qf[nt][4 * i + 2 * j][0] = raw[i][j].x;
-          qf[nt][4 * i + 2 * j][1] = raw[i][j].y;
-          qf[nt][4 * i + 2 * j + 1][0] = raw[i][j].z;
-          qf[nt][4 * i + 2 * j + 1][1] = raw[i][j].w;
+    for (int nt = 0; nt < NT; ++nt) all = min(all, min(lim[nt][0], lim[nt][1]));
+    all = __reduce_min_sync(0xFFFFFFFFu, all);
+
+    float o[kMt][NT][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kMt; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
+    }
+
+    for (int slab = first; slab < end; slab += kWarps, ++it) {
+      fetch(slab + (kStages - 1) * kWarps, pages[kStages - 1], it + kStages - 1);
+      const float ks = ks_next, vs = usable_vscale(vs_next);
+      const int have = good(pages[0]) ? min(kSlab, sp.len - slab * kSlab) : 0;
+#pragma unroll
+      for (int i = 0; i + 1 < kStages; ++i) pages[i] = pages[i + 1];
+      pages[kStages - 1] = page_of(slab + kStages * kWarps);
+      ks_next = scale_at(ap.kscale, pages[0]);
+      vs_next = scale_at(ap.vscale, pages[0]);
+      if (!mbar_wait_warp(&sh.full[warp][it % kStages], (it / kStages) & 1)) {
+        ok = false;
+        for (int i = 1; i < kStages; ++i)  // nothing may still be on its way when the CTA ends
+          if (slab + i * kWarps < end)
+            mbar_wait_warp(&sh.full[warp][(it + i) % kStages], ((it + i) / kStages) & 1);
+        break;
+      }
+      const uint32_t kb = smem_u32(ring) + it % kStages * (2 * kPart), vb = kb + kPart;
+      const float lv = lg2_approx(vs), ivs = rcp_approx(vs);
+
+      float c[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kKc; ++i) {
+        const int u = (kKc * t + i) ^ (HD == 128 ? g & 7 : (g >> 1) & 3);
+        const uint4 ka = lds128(kb + g * HD + 16 * u), kc = lds128(kb + (g + 8) * HD + 16 * u);
+        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wc[4] = {kc.x, kc.y, kc.z, kc.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a[4];
+          e4m3x4_f16x2(wa[j], a[0], a[2]);
+          e4m3x4_f16x2(wc[j], a[1], a[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816(c[nt], a, qf[nt][4 * i + j][0], qf[nt][4 * i + j][1]);
         }
-    } else {
-#pragma unroll
-      for (int k = 0; k < HD / 16; ++k) qf[nt][k][0] = qf[nt][k][1] = 0u;
-    }
-    __syncwarp();
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      fac[nt][c] = __shfl_sync(0xFFFFFFFFu, undo, 8 * t + 4 * c) * (ap.scale * kLog2e);
-      const int cr = nt * 8 + 2 * t + c;
-      // columns without a row: zeros that nothing masks and nobody reads
-      lim[nt][c] = cr >= rows ? 0x7FFFFFFF : ap.causal ? max(0, past + (tile * R + cr) / group + 1) : sp.len;
-    }
-  }
-  int all = 0x7FFFFFFF;  // tokens that every row sees
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) all = min(all, min(lim[nt][0], lim[nt][1]));
-  all = __reduce_min_sync(0xFFFFFFFFu, all);
-
-  // ---- the ring
-  const uint32_t ring = smem_u32(smem) + warp * (kStages * 2 * kPart);
-  const uint32_t head = smem_u32(&s_head[warp][0][0]);
-  const int* bt = ap.seqs.block_tab + static_cast<long long>(s) * ap.seqs.max_pages;
-  const int step = cta * kWarps;
-  const int first = rank * kWarps + warp;
-  auto fetch = [&](int slab, int stage) {
-    if (slab < slabs) {
-      int page = bt[slab / (kPage / kSlab)];
-      int have = min(kSlab, sp.len - slab * kSlab);
-      if (page < 0 || page >= ap.kv_pages) {
-        if (lane == 0 && ap.status) atomicOr(ap.status, kStatusBadShape);
-        page = have = 0;
       }
-      const long long ph = static_cast<long long>(page) * ap.nkv + h;
-      const long long at = ph * (kPage * HD) + (slab % (kPage / kSlab)) * kPart;
-      const uint32_t dst = ring + stage * (2 * kPart);
-#pragma unroll
-      for (int i = 0; i < kSlab * kCpr / 32; ++i) {
-        const int row = i * (32 / kCpr) + lane / kCpr, c = lane % kCpr;
-        const uint32_t to = row * HD + 16 * (c ^ (HD == 128 ? row & 7 : (row >> 1) & 3));
-        const uint32_t n = row < have ? 16 : 0;  // tokens past the end become zeros
-        cp_async16(dst + to, ap.kpool + at + row * HD + 16 * c, n);
-        cp_async16(dst + kPart + to, ap.vpool + at + row * HD + 16 * c, n);
-      }
-      if (lane < 2) cp_async4(head + stage * 16 + 4 * lane, (lane ? ap.vscale : ap.kscale) + ph);
-      if (lane == 2) s_head[warp][stage][2] = __int_as_float(have);
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch(first + i * step, i);
 
-  float o[kMt][NT][4];
-  float m[NT][2], l[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kMt; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
-  }
-
-  int stage = 0;
-  for (int slab = first; slab < slabs; slab += step) {
-    cp_async_wait<kStages - 2>();
-    __syncwarp();  // this slab has landed; the slot refilled below was read by all
-    fetch(slab + (kStages - 1) * step, (stage + kStages - 1) % kStages);
-    const uint32_t kb = ring + stage * (2 * kPart), vb = kb + kPart;
-    const float ks = s_head[warp][stage][0], vs = usable_vscale(s_head[warp][stage][1]);
-    const int have = __float_as_int(s_head[warp][stage][2]);
-    const float lv = log2f(vs), ivs = 1.0f / vs;
-
-    float c[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kKc; ++i) {
-      const int u = (kKc * t + i) ^ (HD == 128 ? g & 7 : (g >> 1) & 3);
-      const uint4 ka = lds128(kb + g * HD + 16 * u), kc = lds128(kb + (g + 8) * HD + 16 * u);
-      const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wc[4] = {kc.x, kc.y, kc.z, kc.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t a[4] = {e4m3x2_f16x2(wa[j] & 0xFFFFu), e4m3x2_f16x2(wc[j] & 0xFFFFu),
-                               e4m3x2_f16x2(wa[j] >> 16), e4m3x2_f16x2(wc[j] >> 16)};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816(c[nt], a, qf[nt][4 * i + j][0], qf[nt][4 * i + j][1]);
-      }
-    }
-
-    // ---- softmax of tokens tok, tok + 8 (c[0..1], c[2..3]) for columns 2t, 2t + 1
-    const int tok = slab * kSlab + g;
-    const bool partial = (slab + 1) * kSlab > all || have < kSlab;
-    bool over = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float x = fmaf(c[nt][e], ks * fac[nt][e & 1], lv);
-        if (partial && (tok + (e >> 1) * 8 >= lim[nt][e & 1] || g + (e >> 1) * 8 >= have)) x = -INFINITY;
-        c[nt][e] = x;
-        over |= x > m[nt][e & 1] + kSlack;
-      }
-    if (__any_sync(0xFFFFFFFFu, over)) {
+      // ---- softmax of tokens tok, tok + 8 (c[0..1], c[2..3]) for columns 2t, 2t + 1
+      const bool partial = (slab + 1) * kSlab > all || have < kSlab;
+      bool over = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float big = fmaxf(c[nt][e], c[nt][e + 2]);
+        for (int e = 0; e < 4; ++e) c[nt][e] = fmaf(c[nt][e], ks * fac[nt][e & 1], lv);
+      if (partial) {
+        const int tok = slab * kSlab + g;
 #pragma unroll
-          for (int w = 4; w < 32; w <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, w));
-          if (big > m[nt][e]) {
-            const float a = ex2_approx(m[nt][e] - big);
-            m[nt][e] = big;
-            l[nt][e] *= a;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < kMt; ++i) {
-              o[i][nt][e] *= a;
-              o[i][nt][e + 2] *= a;
+          for (int e = 0; e < 4; ++e)
+            if (tok + (e >> 1) * 8 >= lim[nt][e & 1] || g + (e >> 1) * 8 >= have) c[nt][e] = -INFINITY;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) over |= fmaxf(c[nt][e], c[nt][e + 2]) > m[nt][e] + kSlack;
+      if (__any_sync(0xFFFFFFFFu, over)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float big = fmaxf(c[nt][e], c[nt][e + 2]);
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, w));
+            if (big > m[nt][e]) {
+              const float a = ex2_approx(m[nt][e] - big);
+              m[nt][e] = big;
+              l[nt][e] *= a;
+#pragma unroll
+              for (int i = 0; i < kMt; ++i) {
+                o[i][nt][e] *= a;
+                o[i][nt][e + 2] *= a;
+              }
             }
           }
+      }
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float ref = m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1];
+          p[e] = ex2_approx(c[nt][e] + (kLift - ref));
+          l[nt][e & 1] = fmaf(p[e], ivs, l[nt][e & 1]);
         }
-    }
-    uint32_t pb[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float p[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float ref = m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1];
-        p[e] = ex2_approx(c[nt][e] + (kLift - ref));
-        l[nt][e & 1] = fmaf(p[e], ivs, l[nt][e & 1]);
+        pb[nt][0] = movmatrix_trans(cvt2_rn<__half>(make_float2(p[0], p[1])));
+        pb[nt][1] = movmatrix_trans(cvt2_rn<__half>(make_float2(p[2], p[3])));
       }
-      pb[nt][0] = movmatrix_trans(cvt2_rn<__half>(make_float2(p[0], p[1])));
-      pb[nt][1] = movmatrix_trans(cvt2_rn<__half>(make_float2(p[2], p[3])));
-    }
 
-    // ---- O^T += V^T P^T: tokens 2t, 2t + 1, 2t + 8, 2t + 9 of dims 2 kMt g ..
-    uint32_t v[4][HD / 32];  // the four tokens' codes
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int row = 2 * t + (k & 1) + (k >> 1) * 8;
-      if constexpr (HD == 128) {
-        const uint4 d = lds128(vb + row * HD + 16 * (g ^ (row & 7)));
-        v[k][0] = d.x;
-        v[k][1] = d.y;
-        v[k][2] = d.z;
-        v[k][3] = d.w;
-      } else {
-        const uint32_t at = vb + row * HD + 16 * ((g >> 1) ^ ((row >> 1) & 3)) + 8 * (g & 1);
-        asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v[k][0]), "=r"(v[k][1]) : "r"(at));
-      }
-    }
-    if (partial) {
-      // 0 . NaN is NaN: a NaN code that some rows do not see is taken out, and
-      // put into the results of the rows that do
-      uint32_t nan[4];  // a bit for each of the thread's dims
-      bool any = false;
+      // ---- O^T += V^T P^T: tokens 2t, 2t + 1, 2t + 8, 2t + 9 of dims 2 kMt g ..
+      uint32_t v[4][HD / 32];  // the four tokens' codes
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        nan[k] = 0;
-#pragma unroll
-        for (int w = 0; w < HD / 32; ++w)
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-            if (((v[k][w] >> (8 * b)) & 0x7Fu) == 0x7Fu) {
-              nan[k] |= 1u << (4 * w + b);
-              v[k][w] &= ~(0xFFu << (8 * b));
-            }
-        any |= nan[k] != 0;
+        const int row = 2 * t + (k & 1) + (k >> 1) * 8;
+        if constexpr (HD == 128) {
+          const uint4 d = lds128(vb + row * HD + 16 * (g ^ (row & 7)));
+          v[k][0] = d.x;
+          v[k][1] = d.y;
+          v[k][2] = d.z;
+          v[k][3] = d.w;
+        } else {
+          const uint32_t at = vb + row * HD + 16 * ((g >> 1) ^ ((row >> 1) & 3)) + 8 * (g & 1);
+          asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v[k][0]), "=r"(v[k][1]) : "r"(at));
+        }
       }
-      if (__any_sync(0xFFFFFFFFu, any)) {
+      if (partial) {
+        // What lies past the sequence's end is not used, whatever it holds.  And
+        // 0 . NaN is NaN: a NaN code that some rows do not see is taken out, and
+        // put into the results of the rows that do.
+        uint32_t nan[4];  // a bit for each of the thread's dims
+        bool any = false;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          for (int from = 0; from < 4; ++from) {
-            const uint32_t bits = __shfl_sync(0xFFFFFFFFu, nan[k], (lane & 28) + from);
-            const int at = 2 * from + (k & 1) + (k >> 1) * 8;
+        for (int k = 0; k < 4; ++k) {
+          nan[k] = 0;
+          const bool in = 2 * t + (k & 1) + (k >> 1) * 8 < have;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+          for (int w = 0; w < HD / 32; ++w) {
+            if (!in) v[k][w] = 0;
 #pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (slab * kSlab + at < lim[nt][e] && at < have)
-#pragma unroll
-                  for (int i = 0; i < kMt; ++i) {
-                    if (bits >> (2 * i) & 1) o[i][nt][e] = NAN;
-                    if (bits >> (2 * i + 1) & 1) o[i][nt][e + 2] = NAN;
-                  }
+            for (int b = 0; b < 4; ++b)
+              if (((v[k][w] >> (8 * b)) & 0x7Fu) == 0x7Fu) {
+                nan[k] |= 1u << (4 * w + b);
+                v[k][w] &= ~(0xFFu << (8 * b));
+              }
           }
+          any |= nan[k] != 0;
+        }
+        if (__any_sync(0xFFFFFFFFu, any)) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            for (int from = 0; from < 4; ++from) {
+              const uint32_t bits = __shfl_sync(0xFFFFFFFFu, nan[k], (lane & 28) + from);
+              const int at = 2 * from + (k & 1) + (k >> 1) * 8;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (slab * kSlab + at < lim[nt][e])
+#pragma unroll
+                    for (int i = 0; i < kMt; ++i) {
+                      if (bits >> (2 * i) & 1) o[i][nt][e] = NAN;
+                      if (bits >> (2 * i + 1) & 1) o[i][nt][e + 2] = NAN;
+                    }
+            }
+        }
       }
+#pragma unroll
+      for (int w = 0; w < HD / 32; ++w)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t b01 = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140);
+          const uint32_t b23 = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
+          uint32_t a[4];
+          e4m3x4_f16x2(b01, a[0], a[1]);
+          e4m3x4_f16x2(b23, a[2], a[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816(o[2 * w + half][nt], a, pb[nt][0], pb[nt][1]);
+        }
+      __syncwarp();  // the slot is refilled next
     }
-#pragma unroll
-    for (int w = 0; w < HD / 32; ++w)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t lo = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140);
-        const uint32_t hi = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
-        const uint32_t a[4] = {e4m3x2_f16x2(lo & 0xFFFFu), e4m3x2_f16x2(lo >> 16),
-                               e4m3x2_f16x2(hi & 0xFFFFu), e4m3x2_f16x2(hi >> 16)};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816(o[2 * w + half][nt], a, pb[nt][0], pb[nt][1]);
-      }
-    stage = (stage + 1) % kStages;
-  }
 
-  // ---- join the warps: O [warp][row][dim] over the ring, scaled to one reference
+    // ---- join the warps: O [warp][row][dim] over the ring, scaled to one reference
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < 2; ++e) {
 #pragma unroll
-      for (int w = 4; w < 32; w <<= 1) l[nt][e] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][e], w);
-      if (g == 0) {
-        s_m[warp][nt * 8 + 2 * t + e] = m[nt][e];
-        s_l[warp][nt * 8 + 2 * t + e] = l[nt][e];
+        for (int w = 4; w < 32; w <<= 1) l[nt][e] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][e], w);
+        if (g == 0) {
+          sh.m[warp][nt * 8 + 2 * t + e] = m[nt][e];
+          sh.l[warp][nt * 8 + 2 * t + e] = l[nt][e];
+        }
       }
-    }
-  cp_async_wait<0>();
-  __syncthreads();
-  float* obuf = reinterpret_cast<float*>(smem);
+    if (__syncthreads_or(!ok)) break;  // every slab has been read
+    float* obuf = reinterpret_cast<float*>(smem);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = nt * 8 + 2 * t + e;
-      float big = s_m[0][r];
+      for (int e = 0; e < 2; ++e) {
+        const int r = nt * 8 + 2 * t + e;
+        float big = sh.m[0][r];
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) big = fmaxf(big, s_m[w][r]);
-      const float ref = big == -INFINITY ? 0.0f : big;
-      const float a = ex2_approx(m[nt][e] - ref);
-      float* dst = obuf + (warp * R + r) * HD + 2 * kMt * g;
+        for (int w = 1; w < kWarps; ++w) big = fmaxf(big, sh.m[w][r]);
+        const float ref = big == -INFINITY ? 0.0f : big;
+        const float a = ex2_approx(m[nt][e] - ref);
+        float* dst = obuf + (warp * R + r) * HD + 2 * kMt * g;
 #pragma unroll
-      for (int i = 0; i < kMt / 2; ++i)
-        *reinterpret_cast<float4*>(dst + 4 * i) = make_float4(
-            o[2 * i][nt][e] * a, o[2 * i][nt][e + 2] * a, o[2 * i + 1][nt][e] * a, o[2 * i + 1][nt][e + 2] * a);
-      if (warp == 0 && g == 0) {
-        float sum = 0.0f;
+        for (int i = 0; i < kMt / 2; ++i)
+          *reinterpret_cast<float4*>(dst + 4 * i) = make_float4(
+              o[2 * i][nt][e] * a, o[2 * i][nt][e + 2] * a, o[2 * i + 1][nt][e] * a, o[2 * i + 1][nt][e + 2] * a);
+        if (warp == 0 && g == 0) {
+          float sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) sum += s_l[w][r] * ex2_approx(s_m[w][r] - ref);
-        s_cm[r] = big;
-        s_cl[r] = sum;
+          for (int w = 0; w < kWarps; ++w) sum += sh.l[w][r] * ex2_approx(sh.m[w][r] - ref);
+          sh.cm[r] = big;
+          sh.cl[r] = sum;
+        }
       }
-    }
-  __syncthreads();
-  if (cta > 1) {
-    for (int i = threadIdx.x; i < R * HD / 4; i += kWarps * 32) {
+    __syncthreads();
+    auto joined = [&](int i) {  // four values of the CTA's O
       float4 v = reinterpret_cast<float4*>(obuf)[i];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) {
-        const float4 x = reinterpret_cast<float4*>(obuf + w * R * HD)[i];
-        v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+        const float4 y = reinterpret_cast<float4*>(obuf + w * R * HD)[i];
+        v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
       }
-      reinterpret_cast<float4*>(obuf)[i] = v;
-    }
-    cluster_sync();  // every part is in its CTA's shared memory
-  }
-  // ---- join the cluster: each CTA finishes a share of the values, parts in rank order
-  if (threadIdx.x < rows) {
-    const int r = threadIdx.x;
-    float big = s_cm[r], sum = s_cl[r];
-    if (cta > 1) {
-      const uint32_t am = smem_u32(&s_cm[r]), al = smem_u32(&s_cl[r]);
-      big = -INFINITY;
-      for (int k = 0; k < cta; ++k) big = fmaxf(big, ld_cluster_f32(mapa_shared(am, k)));
-      const float ref = big == -INFINITY ? 0.0f : big;
-      sum = 0.0f;
-      for (int k = 0; k < cta; ++k) {
-        const float a = ex2_approx(ld_cluster_f32(mapa_shared(am, k)) - ref);
-        s_w[k][r] = a;
-        sum += a * ld_cluster_f32(mapa_shared(al, k));
-      }
-    }
-    s_inv[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (rank == 0 && ap.lse) {
-      const int row = tile * R + r;
-      ap.lse[(sp.t0 + row / group) * ap.nq + h * group + row % group] =
-          sum == 0.0f ? -INFINITY : (big - kLift + log2f(sum)) * 0.69314718055994531f;
-    }
-  }
-  __syncthreads();
-  for (int i = rank * (kWarps * 32) + threadIdx.x; i < rows * (HD / 4); i += cta * (kWarps * 32)) {
-    const int r = i / (HD / 4), row = tile * R + r;
-    float4 v;
-    if (cta > 1) {
-      v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      const uint32_t at = smem_u32(obuf + 4 * i);
-      for (int k = 0; k < cta; ++k) {
-        const float4 x = ld_cluster_f32x4(mapa_shared(at, k));
-        const float a = s_w[k][r];
-        v = make_float4(fmaf(a, x.x, v.x), fmaf(a, x.y, v.y), fmaf(a, x.z, v.z), fmaf(a, x.w, v.w));
-      }
+      return v;
+    };
+
+    // ---- the CTA's O, or the sum of the parts that it completes, and where it goes
+    auto row_of = [&](int r) { return tile * R + r; };
+    auto finish = [&](int i, float4 v) {  // four values of row i / (HD / 4)
+      const int r = i / (HD / 4), row = row_of(r);
+      const float inv = sh.inv[r];
+      store4(static_cast<T*>(ap.out) + (sp.t0 + row / group) * ap.ldo +
+                 static_cast<long long>(h * group + row % group) * HD + 4 * (i % (HD / 4)),
+             make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), ap.vec);
+    };
+    auto close_row = [&](int r, float ref, float sum) {
+      sh.inv[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
+      if (ap.lse)
+        ap.lse[(sp.t0 + row_of(r) / group) * ap.nq + h * group + row_of(r) % group] =
+            sum == 0.0f ? -INFINITY : (ref - kLift + log2f(sum)) * 0.69314718055994531f;
+    };
+    if (plan.chunks == 1) {
+      if (threadIdx.x < rows) close_row(threadIdx.x, sh.cm[threadIdx.x], sh.cl[threadIdx.x]);
+      __syncthreads();
+      for (int i = threadIdx.x; i < rows * (HD / 4); i += kWarps * 32) finish(i, joined(i));
     } else {
-      v = reinterpret_cast<float4*>(obuf)[i];
+      const int groups = (plan.chunks + kJoin - 1) / kJoin;
+      const long long u = (static_cast<long long>(s) * ap.tiles_max + tile) * ap.nkv + h;
+      const int cap_groups = (ap.cap_parts + kJoin - 1) / kJoin;
+      float* parts = ap.parts + u * (ap.cap_parts + cap_groups) * ap.part_stride;
+      int* arrived = ap.arrived + u * (cap_groups + 1);
+      const int l_at = (ap.part_rows + 3) & ~3, o_at = 2 * l_at;
+      // counts an arrival of one of n; true for all threads of the CTA that is the last
+      auto arrive_last = [&](int* counter, int n) {
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          sh.last = atomicAdd(counter, 1) == n - 1;
+          if (sh.last) *counter = 0;  // for the next launch
+          __threadfence();
+        }
+        __syncthreads();
+        return sh.last != 0;
+      };
+      // reference, sum and weights of n parts from `from` on
+      auto weigh = [&](const float* from, int n) {
+        if (threadIdx.x < rows) {
+          const int r = threadIdx.x;
+          float pm[kJoin], pl[kJoin], big = -INFINITY, sum = 0.0f;
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) {
-        const float4 x = reinterpret_cast<float4*>(obuf + w * R * HD)[i];
-        v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+          for (int k = 0; k < kJoin; ++k) {
+            pm[k] = k < n ? __ldcg(from + k * ap.part_stride + r) : -INFINITY;
+            pl[k] = k < n ? __ldcg(from + k * ap.part_stride + l_at + r) : 0.0f;
+            big = fmaxf(big, pm[k]);
+          }
+          const float ref = big == -INFINITY ? 0.0f : big;
+#pragma unroll
+          for (int k = 0; k < kJoin; ++k) {
+            const float w = ex2_approx(pm[k] - ref);
+            sh.w[k][r] = w;
+            sum = fmaf(w, pl[k], sum);
+          }
+          sh.cm[r] = big;
+          sh.cl[r] = sum;
+        }
+        __syncthreads();
+      };
+      auto summed = [&](const float* from, int n, int i) {
+        float4 y[kJoin], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < kJoin; ++k)
+          y[k] = k < n ? __ldcg(reinterpret_cast<const float4*>(from + k * ap.part_stride + o_at) + i) : v;
+#pragma unroll
+        for (int k = 0; k < kJoin; ++k) {
+          const float a = sh.w[k][i / (HD / 4)];
+          if (k < n)
+            v = make_float4(fmaf(a, y[k].x, v.x), fmaf(a, y[k].y, v.y), fmaf(a, y[k].z, v.z),
+                            fmaf(a, y[k].w, v.w));
+        }
+        return v;
+      };
+      float* mine = parts + chunk * ap.part_stride;
+      for (int i = threadIdx.x; i < rows * (HD / 4); i += kWarps * 32)
+        __stcg(reinterpret_cast<float4*>(mine + o_at) + i, joined(i));
+      if (threadIdx.x < rows) {
+        __stcg(mine + threadIdx.x, sh.cm[threadIdx.x]);
+        __stcg(mine + l_at + threadIdx.x, sh.cl[threadIdx.x]);
+      }
+      const int gr = chunk / kJoin, in_group = min(kJoin, plan.chunks - gr * kJoin);
+      if (arrive_last(arrived + gr, in_group)) {
+        const float* from = parts + gr * kJoin * ap.part_stride;
+        int n = in_group;
+        bool all_there = true;
+        weigh(from, n);
+        if (groups > 1) {
+          float* to = parts + (ap.cap_parts + gr) * ap.part_stride;
+          for (int i = threadIdx.x; i < rows * (HD / 4); i += kWarps * 32)
+            __stcg(reinterpret_cast<float4*>(to + o_at) + i, summed(from, n, i));
+          if (threadIdx.x < rows) {
+            __stcg(to + threadIdx.x, sh.cm[threadIdx.x]);
+            __stcg(to + l_at + threadIdx.x, sh.cl[threadIdx.x]);
+          }
+          all_there = arrive_last(arrived + cap_groups, groups);
+          if (all_there) {
+            from = parts + ap.cap_parts * ap.part_stride;
+            n = groups;
+            weigh(from, n);
+          }
+        }
+        if (all_there) {
+          if (threadIdx.x < rows) close_row(threadIdx.x, sh.cm[threadIdx.x], sh.cl[threadIdx.x]);
+          __syncthreads();
+          for (int i = threadIdx.x; i < rows * (HD / 4); i += kWarps * 32) finish(i, summed(from, n, i));
+        }
       }
     }
-    const float inv = s_inv[r];
-    store4(static_cast<T*>(ap.out) + (sp.t0 + row / group) * ap.ldo +
-               static_cast<long long>(h * group + row % group) * HD + 4 * (i % (HD / 4)),
-           make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), ap.vec);
+    ++chunk;
+    fence_proxy_async_smem();  // O is overwritten by the next unit's copies
+    __syncthreads();
   }
-  if (cta > 1) cluster_sync();  // nobody leaves while its part is being read
+  if (!ok && lane == 0 && ap.status) atomicOr(ap.status, kStatusTimeout);
+}
+
+// Rows of a tile of the few-row kernel for sequences of up to `rows` rows.
+int tile_rows(long long rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 24 ? 24 : 32; }
+
+// The workspace of a unit, for caches of up to max_kv tokens.
+struct PartSizes {
+  int tiles, parts, groups, rows, stride;
+  long long unit_bytes;
+};
+PartSizes part_sizes(int nq, int nkv, int hd, int max_q, int max_kv) {
+  PartSizes p;
+  const long long rows = static_cast<long long>(max_q) * (nq / nkv);
+  const int R = tile_rows(rows);
+  p.tiles = static_cast<int>((rows + R - 1) / R);
+  const int slabs = std::max(1, (max_kv + kSlab - 1) / kSlab), step = chunk_slabs(slabs);
+  p.parts = (slabs + step - 1) / step;
+  // just past a change of the step, a shorter cache has more chunks
+  if (slabs >= kJoin * 16) p.parts = std::max(p.parts, kJoin);
+  if (slabs >= kMaxParts * 32) p.parts = kMaxParts;
+  p.groups = (p.parts + kJoin - 1) / kJoin;
+  p.rows = static_cast<int>(std::min<long long>(R, rows));
+  p.stride = 2 * ((p.rows + 3) & ~3) + p.rows * hd;
+  p.unit_bytes = 4ll * (p.parts + p.groups) * p.stride;
+  return p;
+}
+
+// CTAs of a few-row kernel that the GPU holds at once.
+template <typename K>
+int resident_ctas(K kern, size_t smem, cudaError_t* err) {
+  int per = 0;
+  *err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (*err == cudaSuccess) *err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, kWarps * 32, smem);
+  return std::min(per, kMaxCtasPerSm) * device_sm_count();
 }
 
 template <typename T, int HD, int NT>
-cudaError_t launch_rows(CacheAttnParams ap, int max_q, int max_kv, cudaStream_t s) {
+cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int max_kv, cudaStream_t s) {
   constexpr int R = 8 * NT;
-  constexpr int kSmem = kWarps * kStages * 2 * kSlab * HD;  // = the joined O, 4 * kWarps * R * HD at NT = 4
-  static_assert(kSmem >= 4 * kWarps * R * HD, "the warps' O fits the ring");
-  const int group = ap.nq / ap.nkv;
-  const long long tiles = (static_cast<long long>(max_q) * group + R - 1) / R;
-  const long long x = tiles * ap.seqs.n_seqs;
-  // Split until the machine is several times full, while a warp keeps enough slabs.
-  const long long base = x * ap.nkv;
-  const long long want = 12ll * device_sm_count();
-  int c = 1;
-  while (c < kMaxCluster && base * c < want && static_cast<long long>(c) * 2 * kWarps * kSlab * 2 <= max_kv) c *= 2;
-  ap.cluster = c;
-  if (x * c > 0x7FFFFFFFll || ap.nkv > 65535) return cudaErrorInvalidValue;
-  auto k = cache_attn_rows<T, HD, NT>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  if (e == cudaSuccess && c > 8) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(x * c), ap.nkv);
-  cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = c;
-  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, k, ap);
+  // the ring holds the warps' O, 4 kWarps R HD bytes, at NT = 4; and 1 KB to align it
+  constexpr int kSmem = kWarps * kStages * 2 * kSlab * HD + 1024;
+  static_assert(kSmem - 1024 >= 4 * kWarps * R * HD, "the warps' O fits the ring");
+  CUtensorMap tk, tv;
+  const long long rows = static_cast<long long>(ap.kv_pages) * ap.nkv * kPage;
+  if (rows > 0x7FFFFFFFll) return cudaErrorInvalidValue;  // TMA row coordinates
+  // codes in pairs, as 16-bit elements
+  const long long dims[2] = {HD / 2, rows}, stride[1] = {HD};
+  const int box[2] = {HD / 2, kSlab}, step[2] = {1, 1};
+  int rc = make_tmap_nd(&tk, ap.kpool, false, 2, dims, stride, box, step, HD);
+  if (!rc) rc = make_tmap_nd(&tv, ap.vpool, false, 2, dims, stride, box, step, HD);
+  if (rc) return static_cast<cudaError_t>(rc);
+  auto kern = cache_attn_rows<T, HD, NT>;
+  static int resident[64] = {0};  // per instantiation and device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int grid = resident[dev & 63];
+  if (!grid) {
+    cudaError_t e;
+    grid = resident_ctas(kern, kSmem, &e);
+    if (e != cudaSuccess) return e;
+    resident[dev & 63] = grid;
+  }
+  const PartSizes ps = part_sizes(ap.nq, ap.nkv, HD, ap.seqs.max_q, max_kv);
+  ap.tiles_max = ps.tiles;
+  ap.cap_parts = ps.parts;
+  ap.part_rows = ps.rows;
+  ap.part_stride = ps.stride;
+  if (ws && ws_bytes > kCounterBytes) {
+    ap.arrived = static_cast<int*>(ws);
+    ap.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kCounterBytes);
+    ap.cap_units = std::min((ws_bytes - kCounterBytes) / ps.unit_bytes, kCounterBytes / 4 / (ps.groups + 1));
+  }
+  return launch_pdl(kern, dim3(grid), dim3(kWarps * 32), kSmem, s, tk, tv, ap);
 }
 
 template <typename T, int HD>
-cudaError_t launch_any(const CacheAttnParams& ap, int max_q, int max_kv, cudaStream_t s) {
-  const long long rows = static_cast<long long>(max_q) * (ap.nq / ap.nkv);
-  if (rows <= 8) return launch_rows<T, HD, 1>(ap, max_q, max_kv, s);
-  if (rows <= 16) return launch_rows<T, HD, 2>(ap, max_q, max_kv, s);
-  if (rows <= 24) return launch_rows<T, HD, 3>(ap, max_q, max_kv, s);
-  return launch_rows<T, HD, 4>(ap, max_q, max_kv, s);
+cudaError_t launch_any(const CacheAttnParams& ap, void* ws, long long ws_bytes, int max_kv, cudaStream_t s) {
+  switch (tile_rows(static_cast<long long>(ap.seqs.max_q) * (ap.nq / ap.nkv))) {
+    case 8: return launch_rows<T, HD, 1>(ap, ws, ws_bytes, max_kv, s);
+    case 16: return launch_rows<T, HD, 2>(ap, ws, ws_bytes, max_kv, s);
+    case 24: return launch_rows<T, HD, 3>(ap, ws, ws_bytes, max_kv, s);
+    default: return launch_rows<T, HD, 4>(ap, ws, ws_bytes, max_kv, s);
+  }
 }
 
 }  // namespace
 
+long long cache_attention_workspace(int nqh, int nkvh, int hd, int n_seqs, int max_q, int max_kv) {
+  if (nkvh <= 0 || nqh < nkvh || n_seqs <= 0 || max_q <= 0) return 0;
+  const PartSizes p = part_sizes(nqh, nkvh, hd, max_q, max_kv);
+  if (p.parts == 1) return 0;
+  const long long units = static_cast<long long>(n_seqs) * p.tiles * nkvh;
+  return std::min(kCounterBytes + units * p.unit_bytes, 1ll << 28);
+}
+
 int cache_attention(const void* q, long long ldq, long long T, int nqh, int nkvh, int hd,
                     const SeqMap& seqs, int max_q, int max_kv, const void* kpool, const void* vpool,
                     int kv_pages, const float* kscale, const float* vscale, float scale, bool causal,
-                    void* out, long long ldo, float* lse, bool bf16, unsigned* status,
-                    cudaStream_t s) {
+                    void* out, long long ldo, float* lse, void* workspace,
+                    long long workspace_bytes, bool bf16, unsigned* status, cudaStream_t s) {
   if (T <= 0 || seqs.n_seqs <= 0 || max_q <= 0) return 0;
   CacheAttnParams ap{};
   ap.q = q;
@@ -624,11 +861,11 @@ int cache_attention(const void* q, long long ldq, long long T, int nqh, int nkvh
            ((ldq | ldo) % 8 == 0);
   cudaError_t e;
   if (bf16)
-    e = hd == 128 ? launch_any<__nv_bfloat16, 128>(ap, max_q, max_kv, s)
-                  : launch_any<__nv_bfloat16, 64>(ap, max_q, max_kv, s);
+    e = hd == 128 ? launch_any<__nv_bfloat16, 128>(ap, workspace, workspace_bytes, max_kv, s)
+                  : launch_any<__nv_bfloat16, 64>(ap, workspace, workspace_bytes, max_kv, s);
   else
-    e = hd == 128 ? launch_any<__half, 128>(ap, max_q, max_kv, s)
-                  : launch_any<__half, 64>(ap, max_q, max_kv, s);
+    e = hd == 128 ? launch_any<__half, 128>(ap, workspace, workspace_bytes, max_kv, s)
+                  : launch_any<__half, 64>(ap, workspace, workspace_bytes, max_kv, s);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 

@@ -257,11 +257,15 @@ int kv_append(const void* q, long long ldq, const void* k, long long ldk, const 
               unsigned* status, cudaStream_t s);
 
 // Attention over the e4m3 cache (cache_attn.cu); lse [T][nqh] optional.
+// workspace: cache_attention_workspace() bytes (fewer, or null: some or all
+// long caches are not split), its first 2^20 zeroed once before its first use,
+// used by one launch at a time.
 int cache_attention(const void* q, long long ldq, long long T, int nqh, int nkvh, int hd,
                     const SeqMap& seqs, int max_q, int max_kv, const void* kpool, const void* vpool,
                     int kv_pages, const float* kscale, const float* vscale, float scale, bool causal,
-                    void* out, long long ldo, float* lse, bool bf16, unsigned* status,
-                    cudaStream_t s);
+                    void* out, long long ldo, float* lse, void* workspace,
+                    long long workspace_bytes, bool bf16, unsigned* status, cudaStream_t s);
+long long cache_attention_workspace(int nqh, int nkvh, int hd, int n_seqs, int max_q, int max_kv);
 
 // y = x W^T (+ bias), W in 4 bits with group scales (w4.cu).
 int w4_linear(const void* x, long long ldx, int M, int K, const uint8_t* wq, long long ldw, int N,

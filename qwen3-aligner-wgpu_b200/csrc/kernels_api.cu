@@ -159,13 +159,14 @@ extern "C" int qa_k_cache_attention(const void* q, long long ldq, long long T, i
                                     int max_q, int max_kv, const int* block_tab, int max_pages,
                                     const void* kpool, const void* vpool, int kv_pages,
                                     const float* kscale, const float* vscale, float scale,
-                                    int causal, void* out, long long ldo, float* lse, int bf16,
+                                    int causal, void* out, long long ldo, float* lse,
+                                    void* workspace, long long workspace_bytes, int bf16,
                                     unsigned* status, void* stream) {
   if (T == 0 || n_seqs == 0) return QA_OK;
   if (!cache_args_ok(nq, nkv, q_start, kv_len, n_seqs, max_q, block_tab, max_pages, kpool, vpool,
                      kv_pages) ||
       !q || !kscale || !vscale || !out || T < 0 || T > 0x7FFFFFFFll || max_kv < 0 ||
-      !(scale - scale == 0.0f))
+      !(scale - scale == 0.0f) || workspace_bytes < 0 || !aligned16(workspace))
     return QA_ERR_ARG;
   if ((hd != 64 && hd != 128) || ldq < static_cast<long long>(nq) * hd ||
       ldo < static_cast<long long>(nq) * hd)
@@ -174,8 +175,13 @@ extern "C" int qa_k_cache_attention(const void* q, long long ldq, long long T, i
   const SeqMap seqs{q_start, kv_len, n_seqs, block_tab, max_pages, max_q};
   const int rc = cache_attention(q, ldq, T, nq, nkv, hd, seqs, max_q, max_kv, kpool, vpool,
                                  kv_pages, kscale, vscale, scale, causal != 0, out, ldo, lse,
-                                 bf16 != 0, status, static_cast<cudaStream_t>(stream));
+                                 workspace, workspace_bytes, bf16 != 0, status, static_cast<cudaStream_t>(stream));
   return rc == 0 ? QA_OK : QA_ERR_CUDA;
+}
+
+extern "C" int64_t qa_k_cache_attention_workspace(int nq, int nkv, int hd, int n_seqs, int max_q,
+                                                  int max_kv) {
+  return cache_attention_workspace(nq, nkv, hd, n_seqs, max_q, max_kv);
 }
 
 extern "C" int qa_k_w4_linear(const void* x, long long ldx, int M, int K, const uint8_t* wq,

@@ -127,11 +127,11 @@ def test_c_entry_points_answer_bad_arguments():
     assert append(hd=96) == lib.QA_ERR_SHAPE and append(ldq=255) == lib.QA_ERR_SHAPE
     assert append(T=0) == lib.QA_OK and append(n=0) == lib.QA_OK
 
-    def attend(q=p, T=4, nq=4, nkv=2, hd=64, ldo=256, n=1, max_kv=9, ks=p, scale=0.1, out=p, vpool=p):
+    def attend(q=p, T=4, nq=4, nkv=2, hd=64, ldo=256, n=1, ks=p, scale=0.1, out=p, vpool=p, max_kv=9, ws=0, ws_bytes=0):
         return L.qa_k_cache_attention(q, 256, T, nq, nkv, hd, p, p, n, 4, max_kv, p, 2, p, vpool, 3, ks, p, scale, 1, out,
-                                      ldo, 0, 0, 0, 0)
+                                      ldo, 0, ws, ws_bytes, 0, 0, 0)
 
-    for bad in (dict(q=0), dict(out=0), dict(ks=0), dict(vpool=0), dict(vpool=p + 1), dict(max_kv=-1), dict(nq=5),
+    for bad in (dict(q=0), dict(out=0), dict(ks=0), dict(vpool=0), dict(vpool=p + 1), dict(max_kv=-1), dict(ws=p + 8), dict(ws_bytes=-1), dict(nq=5),
                 dict(scale=float("nan")), dict(scale=float("inf")), dict(T=-1)):
         assert attend(**bad) == lib.QA_ERR_ARG, bad
     assert attend(hd=256) == lib.QA_ERR_SHAPE and attend(ldo=100) == lib.QA_ERR_SHAPE
