@@ -55,11 +55,13 @@ struct CacheAttnParams {
 //  - A unit's cached tokens are cut into chunks by the unit's own length alone
 //    (so a sequence's result does not depend on the batch it is in).  The slabs
 //    of 16 tokens of all units, laid end to end, are shared out evenly over the
-//    CTAs that the GPU holds; a CTA takes the chunks that begin in its share,
-//    which it finds from kv_len and q_start itself.
+//    teams that the GPU holds; a team takes the chunks that begin in its share,
+//    which it finds from kv_len and q_start itself.  A team is one warp for up to
+//    8 rows, so that nothing waits for anything else, and a CTA's four warps for
+//    more rows, whose parts are larger and take longer to join.
 //  - A unit of one chunk is finished where it is computed.  Otherwise each chunk
-//    leaves its part (m, l, O) in the workspace, and the CTA that completes a
-//    group of 16 parts joins them in order; with more than one group, the CTA
+//    leaves its part (m, l, O) in the workspace, and the team that completes a
+//    group of 16 parts joins them in order; with more than one group, the team
 //    that completes the last group joins the groups.  No second launch, no
 //    atomics on values, the same bits each time.
 //  - Each warp streams its own slabs through a private ring of kStages slabs
@@ -145,27 +147,41 @@ __device__ __forceinline__ void store4(T* p, float4 v, bool vec) {
   }
 }
 
-// Slabs of a chunk of a unit of `slabs` slabs: 256 tokens keep a short unit's
-// latency down (16 chunks up to 4096 tokens, joined in one step), 512 the joins
-// of a long one (256 chunks up to 131072 tokens, two steps).
-__host__ __device__ __forceinline__ int chunk_slabs(int slabs) {
-  return slabs <= kJoin * 16 ? 16 : slabs <= kMaxParts * 32 ? 32 : (slabs + kMaxParts - 1) / kMaxParts;
+// Slabs of a chunk of a unit of `slabs` slabs.  Short units are cut fine, for
+// their latency: up to 16 chunks, joined in one step; longer ones so that a part
+// (2 (hd + 2) floats a row written and read) stays small next to its chunk's
+// 32 hd bytes a slab, up to 256 chunks, joined in two steps.
+// A team of four warps takes four slabs at a time, so its chunks start at 16.
+__host__ __device__ __forceinline__ int chunk_slabs(int slabs, int team) {
+  if (team == 1 && slabs <= kJoin * 4) return 4;
+  if (team == 1 && slabs <= kJoin * 8) return 8;
+  if (slabs <= (team == 1 ? kMaxParts : kJoin) * 16) return 16;
+  return slabs <= kMaxParts * 32 ? 32 : (slabs + kMaxParts - 1) / kMaxParts;
 }
 
 // Shared memory of the few-row kernel besides the ring.
-template <int R>
+template <int R, int TEAM>
 struct RowsShared {
+  static constexpr int kTeams = kWarps / TEAM;
   uint64_t full[kWarps][kStages];
   float m[kWarps][R], l[kWarps][R];  // the warps' references and sums
-  float cm[R], cl[R];                // the CTA's
-  float w[kJoin][R];                 // weights of joined parts
-  float inv[R];                      // 1 / sum
+  float cm[kTeams][R], cl[kTeams][R];  // the teams'
+  float w[kTeams][kJoin][R];         // weights of joined parts
+  float inv[kTeams][R];              // 1 / sum
   long long scan[kWarps];
-  long long lo, hi;                  // this CTA's share of the slabs
-  long long start;                   // first slab of the first sequence of the share
-  int seq;                           // that sequence
-  int last;
+  long long lo[kTeams], hi[kTeams];  // the teams' shares of the slabs
+  long long start[kTeams];           // first slab of the first sequence of the share
+  int seq[kTeams];                   // that sequence
+  int last[kTeams];
 };
+
+// Counts an arrival; what this thread's warp or CTA wrote before its last
+// barrier is visible to who counts later.
+__device__ __forceinline__ int arrive_count(int* p) {
+  int old;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(p) : "memory");
+  return old;
+}
 
 // What a sequence asks of the few-row kernel: tiles x K/V heads units of
 // `slabs` slabs, each in `chunks` chunks of `step` slabs.
@@ -174,11 +190,11 @@ struct SeqPlan {
   long long cost;  // slabs of all units
 };
 __device__ __forceinline__ SeqPlan seq_plan(const CacheAttnParams& ap, const SeqSpan& sp, int s,
-                                            int group, int R) {
+                                            int group, int R, int team) {
   SeqPlan c;
   c.tiles = sp.ok ? (sp.n * group + R - 1) / R : 0;
   c.slabs = max(1, (sp.len + kSlab - 1) / kSlab);  // an empty cache still owes its rows zeros
-  c.step = chunk_slabs(c.slabs);
+  c.step = chunk_slabs(c.slabs, team);
   c.chunks = (c.slabs + c.step - 1) / c.step;
   if (c.chunks > ap.cap_parts || static_cast<long long>(s + 1) * ap.tiles_max * ap.nkv > ap.cap_units) {
     c.step = c.slabs;  // no place for the parts
@@ -188,7 +204,7 @@ __device__ __forceinline__ SeqPlan seq_plan(const CacheAttnParams& ap, const Seq
   return c;
 }
 
-template <typename T, int HD, int NT>
+template <typename T, int HD, int NT, int TEAM>
 __global__ void __launch_bounds__(kWarps * 32)
     cache_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     CacheAttnParams ap) {
@@ -197,10 +213,16 @@ __global__ void __launch_bounds__(kWarps * 32)
   constexpr int kMt = HD / 16;       // 16-dim blocks of O^T
   constexpr int kPart = kSlab * HD;  // bytes of a slab's K (or V)
   extern __shared__ uint8_t smem_raw[];
-  __shared__ RowsShared<R> sh;
+  constexpr int kTeams = kWarps / TEAM, kTeamThreads = TEAM * 32;
+  __shared__ RowsShared<R, TEAM> sh;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int team = warp / TEAM, tw = warp % TEAM, tid = threadIdx.x % kTeamThreads;
+  auto team_sync = [] {
+    if constexpr (TEAM == 1) __syncwarp();
+    else __syncthreads();
+  };
   const int group = ap.nq / ap.nkv, n_seqs = ap.seqs.n_seqs;
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmK);
@@ -211,7 +233,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   pdl_wait();
   pdl_trigger();
 
-  // ---- this CTA's share: thread i adds up sequences [i c, (i + 1) c)
+  // ---- the teams' shares: thread i adds up sequences [i c, (i + 1) c)
   {
     const int c = (n_seqs + kWarps * 32 - 1) / (kWarps * 32);
     const int s0 = min(n_seqs, static_cast<int>(threadIdx.x) * c), s1 = min(n_seqs, s0 + c);
@@ -219,7 +241,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     for (int i = s0; i < s1; ++i) {
       const SeqSpan sp = seq_span(ap.seqs, i, ap.T);
       if (!sp.ok && blockIdx.x == 0 && ap.status) atomicOr(ap.status, kStatusBadShape);
-      mine += seq_plan(ap, sp, i, group, R).cost;
+      mine += seq_plan(ap, sp, i, group, R, TEAM).cost;
     }
     long long before = mine;  // inclusive scan
 #pragma unroll
@@ -236,33 +258,42 @@ __global__ void __launch_bounds__(kWarps * 32)
       total += sh.scan[w];
     }
     before -= mine;
-    const long long quot = total / gridDim.x, rem = total % gridDim.x, b = blockIdx.x;
-    const long long lo = quot * b + min(b, rem), hi = lo + quot + (b < rem ? 1 : 0);
-    if (lo >= hi) return;
-    if (lo >= before && lo < before + mine) {  // the share begins in one of mine
-      sh.lo = lo;
-      sh.hi = hi;
-      for (int i = s0; i < s1; ++i) {
-        const long long cost = seq_plan(ap, seq_span(ap.seqs, i, ap.T), i, group, R).cost;
-        if (lo < before + cost) {
-          sh.seq = i;
-          sh.start = before;
-          break;
+    const long long n_teams = static_cast<long long>(gridDim.x) * kTeams;
+    const long long quot = total / n_teams, rem = total % n_teams;
+#pragma unroll
+    for (int k = 0; k < kTeams; ++k) {
+      // neighbouring shares on different SMs
+      const long long i = static_cast<long long>(k) * gridDim.x + blockIdx.x;
+      const long long lo = quot * i + min(i, rem), hi = lo + quot + (i < rem ? 1 : 0);
+      if (threadIdx.x == 0) {
+        sh.lo[k] = lo;
+        sh.hi[k] = hi;
+      }
+      if (lo < hi && lo >= before && lo < before + mine) {  // the share begins in one of mine
+        long long at = before;
+        for (int q = s0; q < s1; ++q) {
+          const long long cost = seq_plan(ap, seq_span(ap.seqs, q, ap.T), q, group, R, TEAM).cost;
+          if (lo < at + cost) {
+            sh.seq[k] = q;
+            sh.start[k] = at;
+            break;
+          }
+          at += cost;
         }
-        before += cost;
       }
     }
     __syncthreads();
+    if (sh.lo[team] >= sh.hi[team]) return;
   }
-  const long long share_hi = sh.hi;
+  const long long share_hi = sh.hi[team];
   uint32_t it = 0;  // slabs this warp has taken through its ring
   bool ok = true;   // no wait has run out
-  long long x = sh.lo;  // first slab still to be looked at
-  int s = sh.seq, unit, chunk;
+  long long x = sh.lo[team];  // first slab still to be looked at
+  int s = sh.seq[team], unit, chunk;
   SeqSpan sp = seq_span(ap.seqs, s, ap.T);
-  SeqPlan plan = seq_plan(ap, sp, s, group, R);
+  SeqPlan plan = seq_plan(ap, sp, s, group, R, TEAM);
   {
-    const long long rel = x - sh.start;
+    const long long rel = x - sh.start[team];
     unit = static_cast<int>(rel / plan.slabs);
     const int in = static_cast<int>(rel % plan.slabs);
     chunk = (in + plan.step - 1) / plan.step;  // the first that begins here
@@ -277,7 +308,7 @@ __global__ void __launch_bounds__(kWarps * 32)
       ++s;  // x < share_hi <= total: there is another unit
       unit = chunk = 0;
       sp = seq_span(ap.seqs, s, ap.T);
-      plan = seq_plan(ap, sp, s, group, R);
+      plan = seq_plan(ap, sp, s, group, R, TEAM);
       continue;
     }
     const int tile = unit / ap.nkv, h = unit % ap.nkv;
@@ -291,7 +322,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     // ---- the ring's first slabs
     uint8_t* ring = smem + warp * (kStages * 2 * kPart);
     const int* bt = ap.seqs.block_tab + static_cast<long long>(s) * ap.seqs.max_pages;
-    const int first = lo + warp;
+    const int first = lo + tw;
     auto page_of = [&](int slab) { return slab < end ? bt[slab / (kPage / kSlab)] : 0; };
     auto good = [&](int page) { return page >= 0 && page < ap.kv_pages; };
     auto fetch = [&](int slab, int page, uint32_t n) {
@@ -311,9 +342,9 @@ __global__ void __launch_bounds__(kWarps * 32)
     };
     int pages[kStages];  // of the slabs from the current one on
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) pages[i] = page_of(first + i * kWarps);
+    for (int i = 0; i < kStages; ++i) pages[i] = page_of(first + i * TEAM);
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) fetch(first + i * kWarps, pages[i], it + i);
+    for (int i = 0; i < kStages - 1; ++i) fetch(first + i * TEAM, pages[i], it + i);
     auto scale_at = [&](const float* p, int page) {
       return p[static_cast<long long>(good(page) ? page : 0) * ap.nkv + h];
     };
@@ -404,27 +435,29 @@ __global__ void __launch_bounds__(kWarps * 32)
 
     float o[kMt][NT][4];
     float m[NT][2], l[NT][2];
+    float up[NT][2];  // kLift - m
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = -INFINITY;
+      up[nt][0] = up[nt][1] = kLift;
       l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
       for (int i = 0; i < kMt; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
     }
 
-    for (int slab = first; slab < end; slab += kWarps, ++it) {
-      fetch(slab + (kStages - 1) * kWarps, pages[kStages - 1], it + kStages - 1);
+    for (int slab = first; slab < end; slab += TEAM, ++it) {
+      fetch(slab + (kStages - 1) * TEAM, pages[kStages - 1], it + kStages - 1);
       const float ks = ks_next, vs = usable_vscale(vs_next);
       const int have = good(pages[0]) ? min(kSlab, sp.len - slab * kSlab) : 0;
 #pragma unroll
       for (int i = 0; i + 1 < kStages; ++i) pages[i] = pages[i + 1];
-      pages[kStages - 1] = page_of(slab + kStages * kWarps);
+      pages[kStages - 1] = page_of(slab + kStages * TEAM);
       ks_next = scale_at(ap.kscale, pages[0]);
       vs_next = scale_at(ap.vscale, pages[0]);
       if (!mbar_wait_warp(&sh.full[warp][it % kStages], (it / kStages) & 1)) {
         ok = false;
         for (int i = 1; i < kStages; ++i)  // nothing may still be on its way when the CTA ends
-          if (slab + i * kWarps < end)
+          if (slab + i * TEAM < end)
             mbar_wait_warp(&sh.full[warp][(it + i) % kStages], ((it + i) / kStages) & 1);
         break;
       }
@@ -479,6 +512,7 @@ __global__ void __launch_bounds__(kWarps * 32)
             if (big > m[nt][e]) {
               const float a = ex2_approx(m[nt][e] - big);
               m[nt][e] = big;
+              up[nt][e] = kLift - big;
               l[nt][e] *= a;
 #pragma unroll
               for (int i = 0; i < kMt; ++i) {
@@ -494,8 +528,7 @@ __global__ void __launch_bounds__(kWarps * 32)
         float p[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float ref = m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1];
-          p[e] = ex2_approx(c[nt][e] + (kLift - ref));
+          p[e] = ex2_approx(c[nt][e] + up[nt][e & 1]);
           l[nt][e & 1] = fmaf(p[e], ivs, l[nt][e & 1]);
         }
         pb[nt][0] = movmatrix_trans(cvt2_rn<__half>(make_float2(p[0], p[1])));
@@ -586,61 +619,68 @@ __global__ void __launch_bounds__(kWarps * 32)
           sh.l[warp][nt * 8 + 2 * t + e] = l[nt][e];
         }
       }
-    if (__syncthreads_or(!ok)) break;  // every slab has been read
-    float* obuf = reinterpret_cast<float*>(smem);
+    if constexpr (TEAM > 1) {
+      if (__syncthreads_or(!ok)) break;  // every slab has been read
+    } else {
+      if (!ok) break;
+      __syncwarp();
+    }
+    float* obuf = reinterpret_cast<float*>(smem + team * TEAM * (kStages * 2 * kPart));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = nt * 8 + 2 * t + e;
-        float big = sh.m[0][r];
+        float big = sh.m[team * TEAM][r];
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) big = fmaxf(big, sh.m[w][r]);
+        for (int w = 1; w < TEAM; ++w) big = fmaxf(big, sh.m[team * TEAM + w][r]);
         const float ref = big == -INFINITY ? 0.0f : big;
         const float a = ex2_approx(m[nt][e] - ref);
-        float* dst = obuf + (warp * R + r) * HD + 2 * kMt * g;
+        if (r >= rows) continue;
+        float* dst = obuf + (tw * R + r) * HD + 2 * kMt * g;
 #pragma unroll
         for (int i = 0; i < kMt / 2; ++i)
           *reinterpret_cast<float4*>(dst + 4 * i) = make_float4(
               o[2 * i][nt][e] * a, o[2 * i][nt][e + 2] * a, o[2 * i + 1][nt][e] * a, o[2 * i + 1][nt][e + 2] * a);
-        if (warp == 0 && g == 0) {
+        if (tw == 0 && g == 0) {
           float sum = 0.0f;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) sum += sh.l[w][r] * ex2_approx(sh.m[w][r] - ref);
-          sh.cm[r] = big;
-          sh.cl[r] = sum;
+          for (int w = 0; w < TEAM; ++w)
+            sum += sh.l[team * TEAM + w][r] * ex2_approx(sh.m[team * TEAM + w][r] - ref);
+          sh.cm[team][r] = big;
+          sh.cl[team][r] = sum;
         }
       }
-    __syncthreads();
-    auto joined = [&](int i) {  // four values of the CTA's O
+    team_sync();
+    auto joined = [&](int i) {  // four values of the team's O
       float4 v = reinterpret_cast<float4*>(obuf)[i];
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) {
+      for (int w = 1; w < TEAM; ++w) {
         const float4 y = reinterpret_cast<float4*>(obuf + w * R * HD)[i];
         v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
       }
       return v;
     };
 
-    // ---- the CTA's O, or the sum of the parts that it completes, and where it goes
+    // ---- the team's O, or the sum of the parts that it completes, and where it goes
     auto row_of = [&](int r) { return tile * R + r; };
     auto finish = [&](int i, float4 v) {  // four values of row i / (HD / 4)
       const int r = i / (HD / 4), row = row_of(r);
-      const float inv = sh.inv[r];
+      const float inv = sh.inv[team][r];
       store4(static_cast<T*>(ap.out) + (sp.t0 + row / group) * ap.ldo +
                  static_cast<long long>(h * group + row % group) * HD + 4 * (i % (HD / 4)),
              make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), ap.vec);
     };
     auto close_row = [&](int r, float ref, float sum) {
-      sh.inv[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
+      sh.inv[team][r] = sum == 0.0f ? 0.0f : 1.0f / sum;
       if (ap.lse)
         ap.lse[(sp.t0 + row_of(r) / group) * ap.nq + h * group + row_of(r) % group] =
             sum == 0.0f ? -INFINITY : (ref - kLift + log2f(sum)) * 0.69314718055994531f;
     };
     if (plan.chunks == 1) {
-      if (threadIdx.x < rows) close_row(threadIdx.x, sh.cm[threadIdx.x], sh.cl[threadIdx.x]);
-      __syncthreads();
-      for (int i = threadIdx.x; i < rows * (HD / 4); i += kWarps * 32) finish(i, joined(i));
+      if (tid < rows) close_row(tid, sh.cm[team][tid], sh.cl[team][tid]);
+      team_sync();
+      for (int i = tid; i < rows * (HD / 4); i += kTeamThreads) finish(i, joined(i));
     } else {
       const int groups = (plan.chunks + kJoin - 1) / kJoin;
       const long long u = (static_cast<long long>(s) * ap.tiles_max + tile) * ap.nkv + h;
@@ -648,22 +688,20 @@ __global__ void __launch_bounds__(kWarps * 32)
       float* parts = ap.parts + u * (ap.cap_parts + cap_groups) * ap.part_stride;
       int* arrived = ap.arrived + u * (cap_groups + 1);
       const int l_at = (ap.part_rows + 3) & ~3, o_at = 2 * l_at;
-      // counts an arrival of one of n; true for all threads of the CTA that is the last
+      // counts an arrival of one of n; true for all threads of the team that is the last
       auto arrive_last = [&](int* counter, int n) {
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-          sh.last = atomicAdd(counter, 1) == n - 1;
-          if (sh.last) *counter = 0;  // for the next launch
-          __threadfence();
+        team_sync();
+        if (tid == 0) {
+          sh.last[team] = arrive_count(counter) == n - 1;
+          if (sh.last[team]) *counter = 0;  // for the next launch
         }
-        __syncthreads();
-        return sh.last != 0;
+        team_sync();
+        return sh.last[team] != 0;
       };
       // reference, sum and weights of n parts from `from` on
       auto weigh = [&](const float* from, int n) {
-        if (threadIdx.x < rows) {
-          const int r = threadIdx.x;
+        if (tid < rows) {
+          const int r = tid;
           float pm[kJoin], pl[kJoin], big = -INFINITY, sum = 0.0f;
 #pragma unroll
           for (int k = 0; k < kJoin; ++k) {
@@ -675,13 +713,13 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
           for (int k = 0; k < kJoin; ++k) {
             const float w = ex2_approx(pm[k] - ref);
-            sh.w[k][r] = w;
+            sh.w[team][k][r] = w;
             sum = fmaf(w, pl[k], sum);
           }
-          sh.cm[r] = big;
-          sh.cl[r] = sum;
+          sh.cm[team][r] = big;
+          sh.cl[team][r] = sum;
         }
-        __syncthreads();
+        team_sync();
       };
       auto summed = [&](const float* from, int n, int i) {
         float4 y[kJoin], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -690,7 +728,7 @@ __global__ void __launch_bounds__(kWarps * 32)
           y[k] = k < n ? __ldcg(reinterpret_cast<const float4*>(from + k * ap.part_stride + o_at) + i) : v;
 #pragma unroll
         for (int k = 0; k < kJoin; ++k) {
-          const float a = sh.w[k][i / (HD / 4)];
+          const float a = sh.w[team][k][i / (HD / 4)];
           if (k < n)
             v = make_float4(fmaf(a, y[k].x, v.x), fmaf(a, y[k].y, v.y), fmaf(a, y[k].z, v.z),
                             fmaf(a, y[k].w, v.w));
@@ -698,11 +736,11 @@ __global__ void __launch_bounds__(kWarps * 32)
         return v;
       };
       float* mine = parts + chunk * ap.part_stride;
-      for (int i = threadIdx.x; i < rows * (HD / 4); i += kWarps * 32)
+      for (int i = tid; i < rows * (HD / 4); i += kTeamThreads)
         __stcg(reinterpret_cast<float4*>(mine + o_at) + i, joined(i));
-      if (threadIdx.x < rows) {
-        __stcg(mine + threadIdx.x, sh.cm[threadIdx.x]);
-        __stcg(mine + l_at + threadIdx.x, sh.cl[threadIdx.x]);
+      if (tid < rows) {
+        __stcg(mine + tid, sh.cm[team][tid]);
+        __stcg(mine + l_at + tid, sh.cl[team][tid]);
       }
       const int gr = chunk / kJoin, in_group = min(kJoin, plan.chunks - gr * kJoin);
       if (arrive_last(arrived + gr, in_group)) {
@@ -712,11 +750,11 @@ __global__ void __launch_bounds__(kWarps * 32)
         weigh(from, n);
         if (groups > 1) {
           float* to = parts + (ap.cap_parts + gr) * ap.part_stride;
-          for (int i = threadIdx.x; i < rows * (HD / 4); i += kWarps * 32)
+          for (int i = tid; i < rows * (HD / 4); i += kTeamThreads)
             __stcg(reinterpret_cast<float4*>(to + o_at) + i, summed(from, n, i));
-          if (threadIdx.x < rows) {
-            __stcg(to + threadIdx.x, sh.cm[threadIdx.x]);
-            __stcg(to + l_at + threadIdx.x, sh.cl[threadIdx.x]);
+          if (tid < rows) {
+            __stcg(to + tid, sh.cm[team][tid]);
+            __stcg(to + l_at + tid, sh.cl[team][tid]);
           }
           all_there = arrive_last(arrived + cap_groups, groups);
           if (all_there) {
@@ -726,15 +764,15 @@ __global__ void __launch_bounds__(kWarps * 32)
           }
         }
         if (all_there) {
-          if (threadIdx.x < rows) close_row(threadIdx.x, sh.cm[threadIdx.x], sh.cl[threadIdx.x]);
-          __syncthreads();
-          for (int i = threadIdx.x; i < rows * (HD / 4); i += kWarps * 32) finish(i, summed(from, n, i));
+          if (tid < rows) close_row(tid, sh.cm[team][tid], sh.cl[team][tid]);
+          team_sync();
+          for (int i = tid; i < rows * (HD / 4); i += kTeamThreads) finish(i, summed(from, n, i));
         }
       }
     }
     ++chunk;
-    fence_proxy_async_smem();  // O is overwritten by the next unit's copies
-    __syncthreads();
+    fence_proxy_async_smem();  // O is overwritten by the next chunk's copies
+    team_sync();
   }
   if (!ok && lane == 0 && ap.status) atomicOr(ap.status, kStatusTimeout);
 }
@@ -752,11 +790,12 @@ PartSizes part_sizes(int nq, int nkv, int hd, int max_q, int max_kv) {
   const long long rows = static_cast<long long>(max_q) * (nq / nkv);
   const int R = tile_rows(rows);
   p.tiles = static_cast<int>((rows + R - 1) / R);
-  const int slabs = std::max(1, (max_kv + kSlab - 1) / kSlab), step = chunk_slabs(slabs);
+  const int slabs = std::max(1, (max_kv + kSlab - 1) / kSlab), team = R == 8 ? 1 : kWarps;
+  const int step = chunk_slabs(slabs, team);
   p.parts = (slabs + step - 1) / step;
   // just past a change of the step, a shorter cache has more chunks
-  if (slabs >= kJoin * 16) p.parts = std::max(p.parts, kJoin);
-  if (slabs >= kMaxParts * 32) p.parts = kMaxParts;
+  if (slabs >= kJoin * (team == 1 ? 4 : 16)) p.parts = std::max(p.parts, kJoin);
+  if (slabs >= kMaxParts * (team == 1 ? 16 : 32)) p.parts = kMaxParts;
   p.groups = (p.parts + kJoin - 1) / kJoin;
   p.rows = static_cast<int>(std::min<long long>(R, rows));
   p.stride = 2 * ((p.rows + 3) & ~3) + p.rows * hd;
@@ -788,7 +827,7 @@ cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int ma
   int rc = make_tmap_nd(&tk, ap.kpool, false, 2, dims, stride, box, step, HD);
   if (!rc) rc = make_tmap_nd(&tv, ap.vpool, false, 2, dims, stride, box, step, HD);
   if (rc) return static_cast<cudaError_t>(rc);
-  auto kern = cache_attn_rows<T, HD, NT>;
+  auto kern = cache_attn_rows<T, HD, NT, NT == 1 ? 1 : kWarps>;
   static int resident[64] = {0};  // per instantiation and device
   int dev = 0;
   cudaGetDevice(&dev);
