@@ -90,8 +90,6 @@ struct CacheAttnParams {
 // vote instead of a maximum across lanes; kLift keeps the small p of a long
 // cache out of f16's subnormals and kLift + kSlack below its largest value.
 constexpr int kWarps = 4;
-constexpr int kStages = 4;
-constexpr int kSlab = 16;  // tokens
 constexpr float kLift = 8.0f, kSlack = 6.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -147,23 +145,23 @@ __device__ __forceinline__ void store4(T* p, float4 v, bool vec) {
   }
 }
 
-// Slabs of a chunk of a unit of `slabs` slabs.  Short units are cut fine, for
-// their latency: up to 16 chunks, joined in one step; longer ones so that a part
-// (2 (hd + 2) floats a row written and read) stays small next to its chunk's
-// 32 hd bytes a slab, up to 256 chunks, joined in two steps.
-// A team of four warps takes four slabs at a time, so its chunks start at 16.
-__host__ __device__ __forceinline__ int chunk_slabs(int slabs, int team) {
-  if (team == 1 && slabs <= kJoin * 4) return 4;
-  if (team == 1 && slabs <= kJoin * 8) return 8;
-  if (slabs <= (team == 1 ? kMaxParts : kJoin) * 16) return 16;
-  return slabs <= kMaxParts * 32 ? 32 : (slabs + kMaxParts - 1) / kMaxParts;
+// Tokens of a chunk of a unit of `tokens` tokens, a multiple of 32.  Short units
+// are cut fine, for their latency: up to 16 chunks, joined in one step; longer
+// ones so that a part (2 (hd + 2) floats a row written and read) stays small next
+// to its chunk's 2 hd bytes a token, up to 256 chunks, joined in two steps.
+// A team of four warps takes four slabs at a time, so its chunks start at 256.
+__host__ __device__ __forceinline__ int chunk_tokens(int tokens, int team) {
+  if (team == 1 && tokens <= kJoin * 64) return 64;
+  if (team == 1 && tokens <= kJoin * 128) return 128;
+  if (tokens <= (team == 1 ? kMaxParts : kJoin) * 256) return 256;
+  return tokens <= kMaxParts * 512 ? 512 : ((tokens - 1) / (kMaxParts * 32) + 1) * 32;
 }
 
 // Shared memory of the few-row kernel besides the ring.
-template <int R, int TEAM>
+template <int R, int TEAM, int STAGES>
 struct RowsShared {
   static constexpr int kTeams = kWarps / TEAM;
-  uint64_t full[kWarps][kStages];
+  uint64_t full[kWarps][STAGES];
   float m[kWarps][R], l[kWarps][R];  // the warps' references and sums
   float cm[kTeams][R], cl[kTeams][R];  // the teams'
   float w[kTeams][kJoin][R];         // weights of joined parts
@@ -190,11 +188,11 @@ struct SeqPlan {
   long long cost;  // slabs of all units
 };
 __device__ __forceinline__ SeqPlan seq_plan(const CacheAttnParams& ap, const SeqSpan& sp, int s,
-                                            int group, int R, int team) {
+                                            int group, int R, int team, int slab) {
   SeqPlan c;
   c.tiles = sp.ok ? (sp.n * group + R - 1) / R : 0;
-  c.slabs = max(1, (sp.len + kSlab - 1) / kSlab);  // an empty cache still owes its rows zeros
-  c.step = chunk_slabs(c.slabs, team);
+  c.slabs = max(1, (sp.len + slab - 1) / slab);  // an empty cache still owes its rows zeros
+  c.step = chunk_tokens(sp.len, team) / slab;
   c.chunks = (c.slabs + c.step - 1) / c.step;
   if (c.chunks > ap.cap_parts || static_cast<long long>(s + 1) * ap.tiles_max * ap.nkv > ap.cap_units) {
     c.step = c.slabs;  // no place for the parts
@@ -204,6 +202,15 @@ __device__ __forceinline__ SeqPlan seq_plan(const CacheAttnParams& ap, const Seq
   return c;
 }
 
+// Tokens of a slab: the more of them, the more independent work a warp has
+// between two waits and the fewer instructions a token, as far as the registers
+// reach (S^T takes 4 a 16 tokens and 8 rows).  The ring's bytes stay the same.
+template <int NT>
+struct Slab {
+  static constexpr int kTokens = NT <= 2 ? 32 : 16;
+  static constexpr int kStages = 64 / kTokens;
+};
+
 template <typename T, int HD, int NT, int TEAM>
 __global__ void __launch_bounds__(kWarps * 32)
     cache_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -211,10 +218,12 @@ __global__ void __launch_bounds__(kWarps * 32)
   constexpr int R = 8 * NT;          // rows of a tile
   constexpr int kKc = HD / 64;       // 16-byte units of K a thread reads a token
   constexpr int kMt = HD / 16;       // 16-dim blocks of O^T
+  constexpr int kSlab = Slab<NT>::kTokens, kStages = Slab<NT>::kStages;
+  constexpr int kMb = kSlab / 16;    // 16-token blocks of S^T
   constexpr int kPart = kSlab * HD;  // bytes of a slab's K (or V)
   extern __shared__ uint8_t smem_raw[];
   constexpr int kTeams = kWarps / TEAM, kTeamThreads = TEAM * 32;
-  __shared__ RowsShared<R, TEAM> sh;
+  __shared__ RowsShared<R, TEAM, kStages> sh;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -241,7 +250,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     for (int i = s0; i < s1; ++i) {
       const SeqSpan sp = seq_span(ap.seqs, i, ap.T);
       if (!sp.ok && blockIdx.x == 0 && ap.status) atomicOr(ap.status, kStatusBadShape);
-      mine += seq_plan(ap, sp, i, group, R, TEAM).cost;
+      mine += seq_plan(ap, sp, i, group, R, TEAM, kSlab).cost;
     }
     long long before = mine;  // inclusive scan
 #pragma unroll
@@ -272,7 +281,7 @@ __global__ void __launch_bounds__(kWarps * 32)
       if (lo < hi && lo >= before && lo < before + mine) {  // the share begins in one of mine
         long long at = before;
         for (int q = s0; q < s1; ++q) {
-          const long long cost = seq_plan(ap, seq_span(ap.seqs, q, ap.T), q, group, R, TEAM).cost;
+          const long long cost = seq_plan(ap, seq_span(ap.seqs, q, ap.T), q, group, R, TEAM, kSlab).cost;
           if (lo < at + cost) {
             sh.seq[k] = q;
             sh.start[k] = at;
@@ -291,7 +300,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   long long x = sh.lo[team];  // first slab still to be looked at
   int s = sh.seq[team], unit, chunk;
   SeqSpan sp = seq_span(ap.seqs, s, ap.T);
-  SeqPlan plan = seq_plan(ap, sp, s, group, R, TEAM);
+  SeqPlan plan = seq_plan(ap, sp, s, group, R, TEAM, kSlab);
   {
     const long long rel = x - sh.start[team];
     unit = static_cast<int>(rel / plan.slabs);
@@ -308,7 +317,7 @@ __global__ void __launch_bounds__(kWarps * 32)
       ++s;  // x < share_hi <= total: there is another unit
       unit = chunk = 0;
       sp = seq_span(ap.seqs, s, ap.T);
-      plan = seq_plan(ap, sp, s, group, R, TEAM);
+      plan = seq_plan(ap, sp, s, group, R, TEAM, kSlab);
       continue;
     }
     const int tile = unit / ap.nkv, h = unit % ap.nkv;
@@ -464,49 +473,69 @@ __global__ void __launch_bounds__(kWarps * 32)
       const uint32_t kb = smem_u32(ring) + it % kStages * (2 * kPart), vb = kb + kPart;
       const float lv = lg2_approx(vs), ivs = rcp_approx(vs);
 
-      float c[NT][4];
+      float c[kMb][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
+      for (int b = 0; b < kMb; ++b)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) c[b][nt][0] = c[b][nt][1] = c[b][nt][2] = c[b][nt][3] = 0.0f;
 #pragma unroll
       for (int i = 0; i < kKc; ++i) {
         const int u = (kKc * t + i) ^ (HD == 128 ? g & 7 : (g >> 1) & 3);
-        const uint4 ka = lds128(kb + g * HD + 16 * u), kc = lds128(kb + (g + 8) * HD + 16 * u);
-        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wc[4] = {kc.x, kc.y, kc.z, kc.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t a[4];
-          e4m3x4_f16x2(wa[j], a[0], a[2]);
-          e4m3x4_f16x2(wc[j], a[1], a[3]);
+        for (int b = 0; b < kMb; ++b) {
+          const uint4 ka = lds128(kb + (16 * b + g) * HD + 16 * u);
+          const uint4 kc = lds128(kb + (16 * b + g + 8) * HD + 16 * u);
+          const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wc[4] = {kc.x, kc.y, kc.z, kc.w};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816(c[nt], a, qf[nt][4 * i + j][0], qf[nt][4 * i + j][1]);
+          for (int j = 0; j < 4; ++j) {
+            uint32_t a[4];
+            e4m3x4_f16x2(wa[j], a[0], a[2]);
+            e4m3x4_f16x2(wc[j], a[1], a[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816(c[b][nt], a, qf[nt][4 * i + j][0], qf[nt][4 * i + j][1]);
+          }
         }
       }
 
-      // ---- softmax of tokens tok, tok + 8 (c[0..1], c[2..3]) for columns 2t, 2t + 1
+      // ---- softmax of tokens 16 b + g, + 8 (c[0..1], c[2..3]) for columns 2t, 2t + 1
       const bool partial = (slab + 1) * kSlab > all || have < kSlab;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float f[2] = {ks * fac[nt][0], ks * fac[nt][1]};
+#pragma unroll
+        for (int b = 0; b < kMb; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[b][nt][e] = fmaf(c[b][nt][e], f[e & 1], lv);
+      }
+      if (partial) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int b = 0; b < kMb; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int at = 16 * b + g + (e >> 1) * 8;
+              if (slab * kSlab + at >= lim[nt][e & 1] || at >= have) c[b][nt][e] = -INFINITY;
+            }
+      }
+      float top[NT][2];  // of this thread's tokens
       bool over = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c[nt][e] = fmaf(c[nt][e], ks * fac[nt][e & 1], lv);
-      if (partial) {
-        const int tok = slab * kSlab + g;
+        for (int e = 0; e < 2; ++e) {
+          top[nt][e] = fmaxf(c[0][nt][e], c[0][nt][e + 2]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (tok + (e >> 1) * 8 >= lim[nt][e & 1] || g + (e >> 1) * 8 >= have) c[nt][e] = -INFINITY;
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) over |= fmaxf(c[nt][e], c[nt][e + 2]) > m[nt][e] + kSlack;
+          for (int b = 1; b < kMb; ++b) top[nt][e] = fmaxf(top[nt][e], fmaxf(c[b][nt][e], c[b][nt][e + 2]));
+          over |= top[nt][e] > m[nt][e] + kSlack;
+        }
       if (__any_sync(0xFFFFFFFFu, over)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float big = fmaxf(c[nt][e], c[nt][e + 2]);
+            float big = top[nt][e];
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, w));
             if (big > m[nt][e]) {
@@ -522,88 +551,97 @@ __global__ void __launch_bounds__(kWarps * 32)
             }
           }
       }
-      uint32_t pb[NT][2];
+      uint32_t pb[kMb][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float p[4];
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[e] = ex2_approx(c[nt][e] + up[nt][e & 1]);
-          l[nt][e & 1] = fmaf(p[e], ivs, l[nt][e & 1]);
+        for (int b = 0; b < kMb; ++b) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            p[e] = ex2_approx(c[b][nt][e] + up[nt][e & 1]);
+            sum[e & 1] += p[e];
+          }
+          pb[b][nt][0] = movmatrix_trans(cvt2_rn<__half>(make_float2(p[0], p[1])));
+          pb[b][nt][1] = movmatrix_trans(cvt2_rn<__half>(make_float2(p[2], p[3])));
         }
-        pb[nt][0] = movmatrix_trans(cvt2_rn<__half>(make_float2(p[0], p[1])));
-        pb[nt][1] = movmatrix_trans(cvt2_rn<__half>(make_float2(p[2], p[3])));
+        l[nt][0] = fmaf(sum[0], ivs, l[nt][0]);
+        l[nt][1] = fmaf(sum[1], ivs, l[nt][1]);
       }
 
       // ---- O^T += V^T P^T: tokens 2t, 2t + 1, 2t + 8, 2t + 9 of dims 2 kMt g ..
-      uint32_t v[4][HD / 32];  // the four tokens' codes
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int row = 2 * t + (k & 1) + (k >> 1) * 8;
-        if constexpr (HD == 128) {
-          const uint4 d = lds128(vb + row * HD + 16 * (g ^ (row & 7)));
-          v[k][0] = d.x;
-          v[k][1] = d.y;
-          v[k][2] = d.z;
-          v[k][3] = d.w;
-        } else {
-          const uint32_t at = vb + row * HD + 16 * ((g >> 1) ^ ((row >> 1) & 3)) + 8 * (g & 1);
-          asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v[k][0]), "=r"(v[k][1]) : "r"(at));
-        }
-      }
-      if (partial) {
-        // What lies past the sequence's end is not used, whatever it holds.  And
-        // 0 . NaN is NaN: a NaN code that some rows do not see is taken out, and
-        // put into the results of the rows that do.
-        uint32_t nan[4];  // a bit for each of the thread's dims
-        bool any = false;
+      for (int b = 0; b < kMb; ++b) {
+        uint32_t v[4][HD / 32];  // the four tokens' codes
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          nan[k] = 0;
-          const bool in = 2 * t + (k & 1) + (k >> 1) * 8 < have;
+          const int row = 16 * b + 2 * t + (k & 1) + (k >> 1) * 8;
+          if constexpr (HD == 128) {
+            const uint4 d = lds128(vb + row * HD + 16 * (g ^ (row & 7)));
+            v[k][0] = d.x;
+            v[k][1] = d.y;
+            v[k][2] = d.z;
+            v[k][3] = d.w;
+          } else {
+            const uint32_t at = vb + row * HD + 16 * ((g >> 1) ^ ((row >> 1) & 3)) + 8 * (g & 1);
+            asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v[k][0]), "=r"(v[k][1]) : "r"(at));
+          }
+        }
+        if (partial) {
+          // What lies past the sequence's end is not used, whatever it holds.  And
+          // 0 . NaN is NaN: a NaN code that some rows do not see is taken out, and
+          // put into the results of the rows that do.
+          uint32_t nan[4];  // a bit for each of the thread's dims
+          bool any = false;
 #pragma unroll
-          for (int w = 0; w < HD / 32; ++w) {
-            if (!in) v[k][w] = 0;
+          for (int k = 0; k < 4; ++k) {
+            nan[k] = 0;
+            const bool in = 16 * b + 2 * t + (k & 1) + (k >> 1) * 8 < have;
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
-              if (((v[k][w] >> (8 * b)) & 0x7Fu) == 0x7Fu) {
-                nan[k] |= 1u << (4 * w + b);
-                v[k][w] &= ~(0xFFu << (8 * b));
+            for (int w = 0; w < HD / 32; ++w) {
+              if (!in) v[k][w] = 0;
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                if (((v[k][w] >> (8 * y)) & 0x7Fu) == 0x7Fu) {
+                  nan[k] |= 1u << (4 * w + y);
+                  v[k][w] &= ~(0xFFu << (8 * y));
+                }
+            }
+            any |= nan[k] != 0;
+          }
+          if (__any_sync(0xFFFFFFFFu, any)) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              for (int from = 0; from < 4; ++from) {
+                const uint32_t bits = __shfl_sync(0xFFFFFFFFu, nan[k], (lane & 28) + from);
+                const int at = 16 * b + 2 * from + (k & 1) + (k >> 1) * 8;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    if (slab * kSlab + at < lim[nt][e])
+#pragma unroll
+                      for (int i = 0; i < kMt; ++i) {
+                        if (bits >> (2 * i) & 1) o[i][nt][e] = NAN;
+                        if (bits >> (2 * i + 1) & 1) o[i][nt][e + 2] = NAN;
+                      }
               }
           }
-          any |= nan[k] != 0;
         }
-        if (__any_sync(0xFFFFFFFFu, any)) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            for (int from = 0; from < 4; ++from) {
-              const uint32_t bits = __shfl_sync(0xFFFFFFFFu, nan[k], (lane & 28) + from);
-              const int at = 2 * from + (k & 1) + (k >> 1) * 8;
+        for (int w = 0; w < HD / 32; ++w)
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t b01 = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140);
+            const uint32_t b23 = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
+            uint32_t a[4];
+            e4m3x4_f16x2(b01, a[0], a[1]);
+            e4m3x4_f16x2(b23, a[2], a[3]);
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                  if (slab * kSlab + at < lim[nt][e])
-#pragma unroll
-                    for (int i = 0; i < kMt; ++i) {
-                      if (bits >> (2 * i) & 1) o[i][nt][e] = NAN;
-                      if (bits >> (2 * i + 1) & 1) o[i][nt][e + 2] = NAN;
-                    }
-            }
-        }
+            for (int nt = 0; nt < NT; ++nt) mma16816(o[2 * w + half][nt], a, pb[b][nt][0], pb[b][nt][1]);
+          }
       }
-#pragma unroll
-      for (int w = 0; w < HD / 32; ++w)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t b01 = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140);
-          const uint32_t b23 = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
-          uint32_t a[4];
-          e4m3x4_f16x2(b01, a[0], a[1]);
-          e4m3x4_f16x2(b23, a[2], a[3]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816(o[2 * w + half][nt], a, pb[nt][0], pb[nt][1]);
-        }
       __syncwarp();  // the slot is refilled next
     }
 
@@ -790,12 +828,11 @@ PartSizes part_sizes(int nq, int nkv, int hd, int max_q, int max_kv) {
   const long long rows = static_cast<long long>(max_q) * (nq / nkv);
   const int R = tile_rows(rows);
   p.tiles = static_cast<int>((rows + R - 1) / R);
-  const int slabs = std::max(1, (max_kv + kSlab - 1) / kSlab), team = R == 8 ? 1 : kWarps;
-  const int step = chunk_slabs(slabs, team);
-  p.parts = (slabs + step - 1) / step;
+  const int tokens = std::max(1, max_kv), team = R == 8 ? 1 : kWarps;
+  p.parts = (tokens - 1) / chunk_tokens(tokens, team) + 1;
   // just past a change of the step, a shorter cache has more chunks
-  if (slabs >= kJoin * (team == 1 ? 4 : 16)) p.parts = std::max(p.parts, kJoin);
-  if (slabs >= kMaxParts * (team == 1 ? 16 : 32)) p.parts = kMaxParts;
+  if (tokens > kJoin * (team == 1 ? 64 : 256)) p.parts = std::max(p.parts, kJoin);
+  if (tokens > kMaxParts * 256) p.parts = kMaxParts;
   p.groups = (p.parts + kJoin - 1) / kJoin;
   p.rows = static_cast<int>(std::min<long long>(R, rows));
   p.stride = 2 * ((p.rows + 3) & ~3) + p.rows * hd;
@@ -814,7 +851,7 @@ int resident_ctas(K kern, size_t smem, cudaError_t* err) {
 
 template <typename T, int HD, int NT>
 cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int max_kv, cudaStream_t s) {
-  constexpr int R = 8 * NT;
+  constexpr int R = 8 * NT, kSlab = Slab<NT>::kTokens, kStages = Slab<NT>::kStages;
   // the ring holds the warps' O, 4 kWarps R HD bytes, at NT = 4; and 1 KB to align it
   constexpr int kSmem = kWarps * kStages * 2 * kSlab * HD + 1024;
   static_assert(kSmem - 1024 >= 4 * kWarps * R * HD, "the warps' O fits the ring");
