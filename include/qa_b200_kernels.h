@@ -171,13 +171,11 @@ int qa_k_kv_append(const void* q, long long ldq, const void* k, long long ldk, c
  * smaller or larger value gives the same results up to the order of sums.
  *
  * workspace: device memory, 16-byte aligned, of the size that
- * qa_k_cache_attention_workspace gives for these arguments (0: none is needed),
- * its first 2^20 bytes filled with zeros once before its first use; each call
- * leaves it fit for the next one, of whatever sizes, and two calls that may run
- * at the same time need one each.  With less of it, or NULL, some or all
- * sequences are not split over CTAs, which is slow for few long caches.  A
- * sequence's result does not depend on the others of the batch, as long as the
- * workspace has the size given.
+ * qa_k_cache_attention_workspace gives for these arguments (0: none is needed);
+ * what it holds does not matter, and two calls that may run at the same time
+ * need one each.  With less of it, or NULL, some or all sequences are not split
+ * over CTAs, which is slow for few long caches.  A sequence's result does not
+ * depend on the others of the batch, as long as the workspace has the size given.
  */
 int64_t qa_k_cache_attention_workspace(int nq, int nkv, int hd, int n_seqs, int max_q, int max_kv);
 int qa_k_cache_attention(const void* q, long long ldq, long long T, int nq, int nkv, int hd,

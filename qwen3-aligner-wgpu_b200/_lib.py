@@ -560,9 +560,8 @@ def cache_attention(q, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale,
     need = lib().qa_k_cache_attention_workspace(nq, nkv, hd, n, max_q, max_kv)
     ws = _workspaces.get((q.device, s)) if need else None
     if need and (ws is None or ws.numel() < need):
-        torch.cuda.synchronize(q.device)  # nobody uses the old one, and the new one is zeroed
-        ws = _workspaces[(q.device, s)] = torch.zeros(need, dtype=torch.uint8, device=q.device)
-        torch.cuda.synchronize(q.device)
+        torch.cuda.synchronize(q.device)  # nobody uses the old one
+        ws = _workspaces[(q.device, s)] = torch.empty(need, dtype=torch.uint8, device=q.device)
     check(lib().qa_k_cache_attention(
         q.data_ptr(), ldq, T, nq, nkv, hd, q_start.data_ptr(), kv_len.data_ptr(), n, max_q,
         max_kv, block_tab.data_ptr(), max_pages, kpool.data_ptr(), vpool.data_ptr(), pages,

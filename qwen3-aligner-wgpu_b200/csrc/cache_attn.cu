@@ -18,9 +18,7 @@ namespace {
 
 constexpr int kPage = 64;
 constexpr int kMaxCtasPerSm = 3;
-constexpr int kJoin = 16;                        // parts joined at a time
-constexpr int kMaxParts = kJoin * kJoin;         // parts of a unit
-constexpr long long kCounterBytes = 1ll << 20;   // the workspace's counters
+constexpr int kMaxParts = 1024;  // parts of a unit
 
 struct CacheAttnParams {
   const void* q;
@@ -37,8 +35,7 @@ struct CacheAttnParams {
   float* lse;
   int vec;      // q and out rows can be read and written 16 bytes at a time
   int tiles_max;       // tiles of a sequence of max_q tokens
-  int* arrived;        // workspace: parts that are there, a counter a group and one a unit
-  float* parts;        // workspace: a unit's parts and groups, part_stride floats each
+  float* parts;        // workspace: the units' parts, part_stride floats each
   long long cap_units; // units that have a place in the workspace
   int cap_parts;       // parts a unit has place for
   int part_rows, part_stride;
@@ -58,12 +55,12 @@ struct CacheAttnParams {
 //    teams that the GPU holds; a team takes the chunks that begin in its share,
 //    which it finds from kv_len and q_start itself.  A team is one warp for up to
 //    8 rows, so that nothing waits for anything else, and a CTA's four warps for
-//    more rows, whose parts are larger and take longer to join.
+//    more rows, whose parts are larger.
 //  - A unit of one chunk is finished where it is computed.  Otherwise each chunk
-//    leaves its part (m, l, O) in the workspace, and the team that completes a
-//    group of 16 parts joins them in order; with more than one group, the team
-//    that completes the last group joins the groups.  No second launch, no
-//    atomics on values, the same bits each time.
+//    leaves its part (m, l, O) in the workspace, and a second kernel joins a
+//    unit's parts in their order (joining them in this kernel, by whoever comes
+//    last, measured slower: one warp reads 512 parts of 7 rows in 50 us, at the
+//    very end).  No atomics, the same bits each time.
 //  - Each warp streams its own slabs through a private ring of kStages slabs
 //    (TMA, 128-byte swizzle; hd 64: 64-byte), without any CTA-wide barrier in
 //    the loop.
@@ -146,40 +143,29 @@ __device__ __forceinline__ void store4(T* p, float4 v, bool vec) {
 }
 
 // Tokens of a chunk of a unit of `tokens` tokens, a multiple of 32.  Short units
-// are cut fine, for their latency: up to 16 chunks, joined in one step; longer
-// ones so that a part (2 (hd + 2) floats a row written and read) stays small next
-// to its chunk's 2 hd bytes a token, up to 256 chunks, joined in two steps.
-// A team of four warps takes four slabs at a time, so its chunks start at 256.
+// are cut fine, for their latency; 256 tokens make a part (2 (hd + 2) floats a
+// row written and read) small next to its chunk (2 hd bytes a token).  A team of
+// four warps takes four slabs at a time and writes parts of more rows, so its
+// chunks start at 256.
 __host__ __device__ __forceinline__ int chunk_tokens(int tokens, int team) {
-  if (team == 1 && tokens <= kJoin * 64) return 64;
-  if (team == 1 && tokens <= kJoin * 128) return 128;
-  if (tokens <= (team == 1 ? kMaxParts : kJoin) * 256) return 256;
-  return tokens <= kMaxParts * 512 ? 512 : ((tokens - 1) / (kMaxParts * 32) + 1) * 32;
+  if (team == 1 && tokens <= 512) return 64;
+  if (team == 1 && tokens <= 2048) return 128;
+  return tokens <= kMaxParts * 256 ? 256 : ((tokens - 1) / (kMaxParts * 32) + 1) * 32;
 }
 
 // Shared memory of the few-row kernel besides the ring.
 template <int R, int TEAM, int STAGES>
 struct RowsShared {
   static constexpr int kTeams = kWarps / TEAM;
-  uint64_t full[kWarps][STAGES];
+  uint64_t full[kWarps][STAGES][2];  // K, V
   float m[kWarps][R], l[kWarps][R];  // the warps' references and sums
-  float cm[kTeams][R], cl[kTeams][R];  // the teams'
-  float w[kTeams][kJoin][R];         // weights of joined parts
+  float cm[R], cl[R];                // of the joined warps
   float inv[kTeams][R];              // 1 / sum
   long long scan[kWarps];
   long long lo[kTeams], hi[kTeams];  // the teams' shares of the slabs
   long long start[kTeams];           // first slab of the first sequence of the share
   int seq[kTeams];                   // that sequence
-  int last[kTeams];
 };
-
-// Counts an arrival; what this thread's warp or CTA wrote before its last
-// barrier is visible to who counts later.
-__device__ __forceinline__ int arrive_count(int* p) {
-  int old;
-  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(p) : "memory");
-  return old;
-}
 
 // What a sequence asks of the few-row kernel: tiles x K/V heads units of
 // `slabs` slabs, each in `chunks` chunks of `step` slabs.
@@ -202,6 +188,148 @@ __device__ __forceinline__ SeqPlan seq_plan(const CacheAttnParams& ap, const Seq
   return c;
 }
 
+// A team's share: the chunks that begin in it, as runs of one unit.
+template <int R, int TEAM, int SLAB>
+struct Walk {
+  long long x, hi;  // first slab still to be looked at, end of the share
+  int s, unit, chunk, run;  // the run: chunks [chunk, run) of a unit of sequence s
+  SeqSpan sp;
+  SeqPlan plan;
+
+  __device__ __forceinline__ void look(const CacheAttnParams& ap) {
+    sp = seq_span(ap.seqs, s, ap.T);
+    plan = seq_plan(ap, sp, s, ap.nq / ap.nkv, R, TEAM, SLAB);
+  }
+  // the share [lo, hi) begins in sequence `seq`, whose first slab is `start`
+  __device__ __forceinline__ void begin(const CacheAttnParams& ap, int seq, long long start, long long lo,
+                                        long long end) {
+    x = lo;
+    hi = end;
+    s = seq;
+    look(ap);
+    const long long rel = lo - start;
+    unit = static_cast<int>(rel / plan.slabs);
+    const int in = static_cast<int>(rel % plan.slabs);
+    run = (in + plan.step - 1) / plan.step;  // the first chunk that begins here
+    x += min(plan.slabs, run * plan.step) - in;
+  }
+  __device__ __forceinline__ bool next(const CacheAttnParams& ap) {
+    if (x >= hi) return false;
+    if (run == plan.chunks) {
+      run = 0;
+      ++unit;
+    }
+    while (unit >= plan.tiles * ap.nkv) {  // x < hi <= all slabs: there is another unit
+      ++s;
+      unit = run = 0;
+      look(ap);
+    }
+    chunk = run;
+    // a warp goes on to the end of its share in one run of its ring; a team's
+    // shared memory also joins its warps, chunk by chunk
+    run = chunk + 1;
+    if (TEAM == 1)
+      run = chunk + static_cast<int>(min(static_cast<long long>(plan.chunks - chunk), (hi - x - 1) / plan.step + 1));
+    x += min(plan.slabs, run * plan.step) - chunk * plan.step;
+    return true;
+  }
+};
+
+// A tile's rows of one sequence and K/V head.
+struct UnitAt {
+  int s, tile, h;
+  long long t0;  // the sequence's first row of q and out
+};
+
+__device__ __forceinline__ float* unit_parts(const CacheAttnParams& ap, const UnitAt& at) {
+  const long long u = (static_cast<long long>(at.s) * ap.tiles_max + at.tile) * ap.nkv + at.h;
+  return ap.parts + u * ap.cap_parts * ap.part_stride;
+}
+
+// Row `row` of a sequence is done: its lse; returns what its O is multiplied by.
+__device__ __forceinline__ float close_row(const CacheAttnParams& ap, const UnitAt& at, int row,
+                                           float big, float sum) {
+  const int group = ap.nq / ap.nkv;
+  if (ap.lse)
+    ap.lse[(at.t0 + row / group) * ap.nq + at.h * group + row % group] =
+        sum == 0.0f ? -INFINITY : (big - kLift + log2f(sum)) * 0.69314718055994531f;
+  return sum == 0.0f ? 0.0f : 1.0f / sum;
+}
+
+template <typename T, int HD>
+__device__ __forceinline__ void finish_row(const CacheAttnParams& ap, const UnitAt& at, int row, int dim,
+                                           float4 v, float inv) {
+  const int group = ap.nq / ap.nkv;
+  store4(static_cast<T*>(ap.out) + (at.t0 + row / group) * ap.ldo +
+             static_cast<long long>(at.h * group + row % group) * HD + dim,
+         make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), ap.vec);
+}
+
+// Joins the parts of the units of more than one chunk, a CTA a row: each of its
+// warps sums every kJoinWarps-th part (four dims a lane; hd 64: two parts at a
+// time), then the warps are summed, in an order that only the number of parts
+// sets.  Bound by latency: a part's row is one line of 4 hd bytes.
+constexpr int kJoinWarps = 8;
+
+template <typename T, int HD, int R, int TEAM, int SLAB>
+__global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const __grid_constant__ CacheAttnParams ap) {
+  constexpr int kLanes = HD / 4, kAtOnce = 32 / kLanes * kJoinWarps;  // lanes of a part, parts at once
+  __shared__ float s_red[kJoinWarps], s_sum[kJoinWarps];
+  __shared__ float4 s_o[kAtOnce][kLanes];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.y, s = blockIdx.x / ap.tiles_max, tile = blockIdx.x % ap.tiles_max, r = blockIdx.z;
+  pdl_wait();
+  pdl_trigger();
+  const int group = ap.nq / ap.nkv;
+  const SeqSpan sp = seq_span(ap.seqs, s, ap.T);
+  const SeqPlan plan = seq_plan(ap, sp, s, group, R, TEAM, SLAB);
+  if (plan.chunks == 1 || tile >= plan.tiles || tile * R + r >= sp.n * group) return;
+  const UnitAt at{s, tile, h, sp.t0};
+  const float* parts = unit_parts(ap, at);
+  const int l_at = (ap.part_rows + 3) & ~3, o_at = 2 * l_at + r * HD;
+  const int n = plan.chunks, first = threadIdx.x / kLanes, d = threadIdx.x % kLanes;
+  float big = -INFINITY;
+  for (int k = threadIdx.x; k < n; k += kJoinWarps * 32) big = fmaxf(big, parts[static_cast<long long>(k) * ap.part_stride + r]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+  if (lane == 0) s_red[warp] = big;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) big = fmaxf(big, s_red[w]);
+  const float ref = big == -INFINITY ? 0.0f : big;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float sum = 0.0f;
+#pragma unroll 8
+  for (int k = first; k < n; k += kAtOnce) {
+    const float* part = parts + static_cast<long long>(k) * ap.part_stride;
+    const float4 y = *reinterpret_cast<const float4*>(part + o_at + 4 * d);
+    const float a = ex2_approx(part[r] - ref);
+    sum = fmaf(a, part[l_at + r], sum);
+    v = make_float4(fmaf(a, y.x, v.x), fmaf(a, y.y, v.y), fmaf(a, y.z, v.z), fmaf(a, y.w, v.w));
+  }
+  s_o[first][d] = v;
+  // each part's sum once: from the first lane of its kLanes
+  if (d != 0) sum = 0.0f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  if (threadIdx.x < kLanes) {
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) sum += s_sum[w];
+    v = s_o[0][d];
+#pragma unroll
+    for (int k = 1; k < kAtOnce; ++k) {
+      const float4 y = s_o[k][d];
+      v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
+    }
+    const int row = tile * R + r;
+    if (d == 0) close_row(ap, at, row, big, sum);
+    finish_row<T, HD>(ap, at, row, 4 * d, v, sum == 0.0f ? 0.0f : 1.0f / sum);
+  }
+}
+
 // Tokens of a slab: the more of them, the more independent work a warp has
 // between two waits and the fewer instructions a token, as far as the registers
 // reach (S^T takes 4 a 16 tokens and 8 rows).  The ring's bytes stay the same.
@@ -212,9 +340,9 @@ struct Slab {
 };
 
 template <typename T, int HD, int NT, int TEAM>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     cache_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                    CacheAttnParams ap) {
+                    const __grid_constant__ CacheAttnParams ap) {
   constexpr int R = 8 * NT;          // rows of a tile
   constexpr int kKc = HD / 64;       // 16-byte units of K a thread reads a token
   constexpr int kMt = HD / 16;       // 16-dim blocks of O^T
@@ -236,7 +364,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
-    for (int i = 0; i < kWarps * kStages; ++i) mbar_init(&sh.full[0][0] + i, 1);
+    for (int i = 0; i < kWarps * kStages * 2; ++i) mbar_init(&sh.full[0][0][0] + i, 1);
     fence_barrier_init();
   }
   pdl_wait();
@@ -294,35 +422,16 @@ __global__ void __launch_bounds__(kWarps * 32)
     __syncthreads();
     if (sh.lo[team] >= sh.hi[team]) return;
   }
-  const long long share_hi = sh.hi[team];
+  Walk<R, TEAM, kSlab> walk;
+  walk.begin(ap, sh.seq[team], sh.start[team], sh.lo[team], sh.hi[team]);
   uint32_t it = 0;  // slabs this warp has taken through its ring
   bool ok = true;   // no wait has run out
-  long long x = sh.lo[team];  // first slab still to be looked at
-  int s = sh.seq[team], unit, chunk;
-  SeqSpan sp = seq_span(ap.seqs, s, ap.T);
-  SeqPlan plan = seq_plan(ap, sp, s, group, R, TEAM, kSlab);
-  {
-    const long long rel = x - sh.start[team];
-    unit = static_cast<int>(rel / plan.slabs);
-    const int in = static_cast<int>(rel % plan.slabs);
-    chunk = (in + plan.step - 1) / plan.step;  // the first that begins here
-    x += min(plan.slabs, chunk * plan.step) - in;
-  }
-  while (x < share_hi) {
-    if (chunk == plan.chunks) {
-      chunk = 0;
-      ++unit;
-    }
-    if (unit >= plan.tiles * ap.nkv) {
-      ++s;  // x < share_hi <= total: there is another unit
-      unit = chunk = 0;
-      sp = seq_span(ap.seqs, s, ap.T);
-      plan = seq_plan(ap, sp, s, group, R, TEAM, kSlab);
-      continue;
-    }
-    const int tile = unit / ap.nkv, h = unit % ap.nkv;
-    const int lo = chunk * plan.step, hi = min(plan.slabs, lo + plan.step);
-    x += hi - lo;
+  while (walk.next(ap)) {
+    const SeqSpan& sp = walk.sp;
+    const SeqPlan& plan = walk.plan;
+    const int s = walk.s, tile = walk.unit / ap.nkv, h = walk.unit % ap.nkv;
+    int chunk = walk.chunk;
+    const int run = walk.run, lo = chunk * plan.step, hi = min(plan.slabs, run * plan.step);
     const int rows = min(R, sp.n * group - tile * R);
     const int past = sp.len - sp.n;  // + i + 1: tokens seen by new token i
     const int seen = ap.causal ? min(sp.len, max(0, past + (tile * R + rows - 1) / group + 1)) : sp.len;
@@ -331,29 +440,31 @@ __global__ void __launch_bounds__(kWarps * 32)
     // ---- the ring's first slabs
     uint8_t* ring = smem + warp * (kStages * 2 * kPart);
     const int* bt = ap.seqs.block_tab + static_cast<long long>(s) * ap.seqs.max_pages;
-    const int first = lo + tw;
+    int slab = lo + tw;
     auto page_of = [&](int slab) { return slab < end ? bt[slab / (kPage / kSlab)] : 0; };
     auto good = [&](int page) { return page >= 0 && page < ap.kv_pages; };
-    auto fetch = [&](int slab, int page, uint32_t n) {
+    // K (v = 0) or V (v = 1) of a slab, the warp's n-th
+    auto fetch = [&](int slab, int page, uint32_t n, int v) {
       if (slab < end && lane == 0) {
-        uint64_t* bar = &sh.full[warp][n % kStages];
+        uint64_t* bar = &sh.full[warp][n % kStages][v];
         if (good(page)) {
           const int row = (page * ap.nkv + h) * kPage + slab % (kPage / kSlab) * kSlab;
-          uint8_t* dst = ring + n % kStages * (2 * kPart);
-          mbar_arrive_expect_tx(bar, 2 * kPart);
-          tma_load_2d(&tmK, bar, dst, 0, row);
-          tma_load_2d(&tmV, bar, dst + kPart, 0, row);
+          mbar_arrive_expect_tx(bar, kPart);
+          tma_load_2d(v ? &tmV : &tmK, bar, ring + n % kStages * (2 * kPart) + v * kPart, 0, row);
         } else {
           if (ap.status) atomicOr(ap.status, kStatusBadShape);
           mbar_arrive(bar);
         }
       }
     };
-    int pages[kStages];  // of the slabs from the current one on
+    int pages[kStages + 1];  // of the slabs from the current one on
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) pages[i] = page_of(first + i * TEAM);
+    for (int i = 0; i <= kStages; ++i) pages[i] = page_of(slab + i * TEAM);
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) fetch(first + i * TEAM, pages[i], it + i);
+    for (int i = 0; i < kStages; ++i) {
+      fetch(slab + i * TEAM, pages[i], it + i, 0);
+      fetch(slab + i * TEAM, pages[i], it + i, 1);
+    }
     auto scale_at = [&](const float* p, int page) {
       return p[static_cast<long long>(good(page) ? page : 0) * ap.nkv + h];
     };
@@ -442,6 +553,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     for (int nt = 0; nt < NT; ++nt) all = min(all, min(lim[nt][0], lim[nt][1]));
     all = __reduce_min_sync(0xFFFFFFFFu, all);
 
+    for (; chunk < run; ++chunk) {
     float o[kMt][NT][4];
     float m[NT][2], l[NT][2];
     float up[NT][2];  // kLift - m
@@ -454,20 +566,16 @@ __global__ void __launch_bounds__(kWarps * 32)
       for (int i = 0; i < kMt; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
     }
 
-    for (int slab = first; slab < end; slab += TEAM, ++it) {
-      fetch(slab + (kStages - 1) * TEAM, pages[kStages - 1], it + kStages - 1);
+    for (const int stop = min(end, (chunk + 1) * plan.step); slab < stop; slab += TEAM, ++it) {
       const float ks = ks_next, vs = usable_vscale(vs_next);
       const int have = good(pages[0]) ? min(kSlab, sp.len - slab * kSlab) : 0;
 #pragma unroll
-      for (int i = 0; i + 1 < kStages; ++i) pages[i] = pages[i + 1];
-      pages[kStages - 1] = page_of(slab + kStages * TEAM);
+      for (int i = 0; i < kStages; ++i) pages[i] = pages[i + 1];
+      pages[kStages] = page_of(slab + (kStages + 1) * TEAM);
       ks_next = scale_at(ap.kscale, pages[0]);
       vs_next = scale_at(ap.vscale, pages[0]);
-      if (!mbar_wait_warp(&sh.full[warp][it % kStages], (it / kStages) & 1)) {
+      if (!mbar_wait_warp(&sh.full[warp][it % kStages][0], (it / kStages) & 1)) {
         ok = false;
-        for (int i = 1; i < kStages; ++i)  // nothing may still be on its way when the CTA ends
-          if (slab + i * TEAM < end)
-            mbar_wait_warp(&sh.full[warp][(it + i) % kStages], ((it + i) / kStages) & 1);
         break;
       }
       const uint32_t kb = smem_u32(ring) + it % kStages * (2 * kPart), vb = kb + kPart;
@@ -497,6 +605,9 @@ __global__ void __launch_bounds__(kWarps * 32)
           }
         }
       }
+
+      __syncwarp();  // K has been read
+      fetch(slab + kStages * TEAM, pages[kStages - 1], it + kStages, 0);
 
       // ---- softmax of tokens 16 b + g, + 8 (c[0..1], c[2..3]) for columns 2t, 2t + 1
       const bool partial = (slab + 1) * kSlab > all || have < kSlab;
@@ -571,6 +682,10 @@ __global__ void __launch_bounds__(kWarps * 32)
       }
 
       // ---- O^T += V^T P^T: tokens 2t, 2t + 1, 2t + 8, 2t + 9 of dims 2 kMt g ..
+      if (!mbar_wait_warp(&sh.full[warp][it % kStages][1], (it / kStages) & 1)) {
+        ok = false;
+        break;
+      }
 #pragma unroll
       for (int b = 0; b < kMb; ++b) {
         uint32_t v[4][HD / 32];  // the four tokens' codes
@@ -642,176 +757,122 @@ __global__ void __launch_bounds__(kWarps * 32)
             for (int nt = 0; nt < NT; ++nt) mma16816(o[2 * w + half][nt], a, pb[b][nt][0], pb[b][nt][1]);
           }
       }
-      __syncwarp();  // the slot is refilled next
+      __syncwarp();  // V has been read
+      fetch(slab + kStages * TEAM, pages[kStages - 1], it + kStages, 1);
     }
 
-    // ---- join the warps: O [warp][row][dim] over the ring, scaled to one reference
+    if (!ok)  // a wait ran out: nothing may still be on its way when the CTA ends
+      for (uint32_t n = it; n <= it + kStages; ++n)
+        if (slab + static_cast<int>(n - it) * TEAM < end) {
+          mbar_wait_warp(&sh.full[warp][n % kStages][0], (n / kStages) & 1);
+          mbar_wait_warp(&sh.full[warp][n % kStages][1], (n / kStages) & 1);
+        }
+
+    // ---- the team's m, l and O
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) l[nt][e] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][e], w);
-        if (g == 0) {
+        if (TEAM > 1 && g == 0) {
           sh.m[warp][nt * 8 + 2 * t + e] = m[nt][e];
           sh.l[warp][nt * 8 + 2 * t + e] = l[nt][e];
         }
       }
+    float* obuf = reinterpret_cast<float*>(smem);  // [warp][row][dim] over the ring
     if constexpr (TEAM > 1) {
-      if (__syncthreads_or(!ok)) break;  // every slab has been read
-    } else {
-      if (!ok) break;
-      __syncwarp();
-    }
-    float* obuf = reinterpret_cast<float*>(smem + team * TEAM * (kStages * 2 * kPart));
+      if (__syncthreads_or(!ok)) goto done;  // every slab has been read
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = nt * 8 + 2 * t + e;
-        float big = sh.m[team * TEAM][r];
+        for (int e = 0; e < 2; ++e) {
+          const int r = nt * 8 + 2 * t + e;
+          if (r >= rows) continue;
+          float big = sh.m[0][r];
 #pragma unroll
-        for (int w = 1; w < TEAM; ++w) big = fmaxf(big, sh.m[team * TEAM + w][r]);
-        const float ref = big == -INFINITY ? 0.0f : big;
-        const float a = ex2_approx(m[nt][e] - ref);
-        if (r >= rows) continue;
-        float* dst = obuf + (tw * R + r) * HD + 2 * kMt * g;
+          for (int w = 1; w < TEAM; ++w) big = fmaxf(big, sh.m[w][r]);
+          const float ref = big == -INFINITY ? 0.0f : big;
+          const float a = ex2_approx(m[nt][e] - ref);
+          float* dst = obuf + (tw * R + r) * HD + 2 * kMt * g;
 #pragma unroll
-        for (int i = 0; i < kMt / 2; ++i)
-          *reinterpret_cast<float4*>(dst + 4 * i) = make_float4(
-              o[2 * i][nt][e] * a, o[2 * i][nt][e + 2] * a, o[2 * i + 1][nt][e] * a, o[2 * i + 1][nt][e + 2] * a);
-        if (tw == 0 && g == 0) {
-          float sum = 0.0f;
+          for (int i = 0; i < kMt / 2; ++i)
+            *reinterpret_cast<float4*>(dst + 4 * i) = make_float4(
+                o[2 * i][nt][e] * a, o[2 * i][nt][e + 2] * a, o[2 * i + 1][nt][e] * a, o[2 * i + 1][nt][e + 2] * a);
+          if (tw == 0 && g == 0) {
+            float sum = 0.0f;
 #pragma unroll
-          for (int w = 0; w < TEAM; ++w)
-            sum += sh.l[team * TEAM + w][r] * ex2_approx(sh.m[team * TEAM + w][r] - ref);
-          sh.cm[team][r] = big;
-          sh.cl[team][r] = sum;
+            for (int w = 0; w < TEAM; ++w) sum += sh.l[w][r] * ex2_approx(sh.m[w][r] - ref);
+            sh.cm[r] = big;
+            sh.cl[r] = sum;
+          }
         }
-      }
-    team_sync();
-    auto joined = [&](int i) {  // four values of the team's O
-      float4 v = reinterpret_cast<float4*>(obuf)[i];
+      __syncthreads();
+    } else {
+      if (!ok) goto done;
+    }
+    // calls put(row, dim, four values) for all of O, f32
+    auto each = [&](auto put) {
+      if constexpr (TEAM > 1) {
+        for (int i = tid; i < rows * (HD / 4); i += kTeamThreads) {
+          float4 v = reinterpret_cast<float4*>(obuf)[i];
 #pragma unroll
-      for (int w = 1; w < TEAM; ++w) {
-        const float4 y = reinterpret_cast<float4*>(obuf + w * R * HD)[i];
-        v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
+          for (int w = 1; w < TEAM; ++w) {
+            const float4 y = reinterpret_cast<float4*>(obuf + w * R * HD)[i];
+            v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
+          }
+          put(i / (HD / 4), 4 * (i % (HD / 4)), v);
+        }
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (nt * 8 + 2 * t + e < rows)
+#pragma unroll
+              for (int i = 0; i < kMt / 2; ++i)
+                put(nt * 8 + 2 * t + e, 2 * kMt * g + 4 * i,
+                    make_float4(o[2 * i][nt][e], o[2 * i][nt][e + 2], o[2 * i + 1][nt][e], o[2 * i + 1][nt][e + 2]));
       }
-      return v;
+    };
+    // calls put(row, m, l) for all rows
+    auto each_row = [&](auto put) {
+      if constexpr (TEAM > 1) {
+        if (tid < rows) put(tid, sh.cm[tid], sh.cl[tid]);
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (g == 0 && nt * 8 + 2 * t + e < rows) put(nt * 8 + 2 * t + e, m[nt][e], l[nt][e]);
+      }
     };
 
-    // ---- the team's O, or the sum of the parts that it completes, and where it goes
-    auto row_of = [&](int r) { return tile * R + r; };
-    auto finish = [&](int i, float4 v) {  // four values of row i / (HD / 4)
-      const int r = i / (HD / 4), row = row_of(r);
-      const float inv = sh.inv[team][r];
-      store4(static_cast<T*>(ap.out) + (sp.t0 + row / group) * ap.ldo +
-                 static_cast<long long>(h * group + row % group) * HD + 4 * (i % (HD / 4)),
-             make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), ap.vec);
-    };
-    auto close_row = [&](int r, float ref, float sum) {
-      sh.inv[team][r] = sum == 0.0f ? 0.0f : 1.0f / sum;
-      if (ap.lse)
-        ap.lse[(sp.t0 + row_of(r) / group) * ap.nq + h * group + row_of(r) % group] =
-            sum == 0.0f ? -INFINITY : (ref - kLift + log2f(sum)) * 0.69314718055994531f;
-    };
+    // ---- they are all there is, or a part
+    const UnitAt at{s, tile, h, sp.t0};
     if (plan.chunks == 1) {
-      if (tid < rows) close_row(tid, sh.cm[team][tid], sh.cl[team][tid]);
+      each_row([&](int r, float big, float sum) { sh.inv[team][r] = close_row(ap, at, tile * R + r, big, sum); });
       team_sync();
-      for (int i = tid; i < rows * (HD / 4); i += kTeamThreads) finish(i, joined(i));
+      each([&](int r, int dim, float4 v) { finish_row<T, HD>(ap, at, tile * R + r, dim, v, sh.inv[team][r]); });
+      team_sync();  // the sums are read before the next chunk's are written
     } else {
-      const int groups = (plan.chunks + kJoin - 1) / kJoin;
-      const long long u = (static_cast<long long>(s) * ap.tiles_max + tile) * ap.nkv + h;
-      const int cap_groups = (ap.cap_parts + kJoin - 1) / kJoin;
-      float* parts = ap.parts + u * (ap.cap_parts + cap_groups) * ap.part_stride;
-      int* arrived = ap.arrived + u * (cap_groups + 1);
-      const int l_at = (ap.part_rows + 3) & ~3, o_at = 2 * l_at;
-      // counts an arrival of one of n; true for all threads of the team that is the last
-      auto arrive_last = [&](int* counter, int n) {
-        team_sync();
-        if (tid == 0) {
-          sh.last[team] = arrive_count(counter) == n - 1;
-          if (sh.last[team]) *counter = 0;  // for the next launch
-        }
-        team_sync();
-        return sh.last[team] != 0;
-      };
-      // reference, sum and weights of n parts from `from` on
-      auto weigh = [&](const float* from, int n) {
-        if (tid < rows) {
-          const int r = tid;
-          float pm[kJoin], pl[kJoin], big = -INFINITY, sum = 0.0f;
-#pragma unroll
-          for (int k = 0; k < kJoin; ++k) {
-            pm[k] = k < n ? __ldcg(from + k * ap.part_stride + r) : -INFINITY;
-            pl[k] = k < n ? __ldcg(from + k * ap.part_stride + l_at + r) : 0.0f;
-            big = fmaxf(big, pm[k]);
-          }
-          const float ref = big == -INFINITY ? 0.0f : big;
-#pragma unroll
-          for (int k = 0; k < kJoin; ++k) {
-            const float w = ex2_approx(pm[k] - ref);
-            sh.w[team][k][r] = w;
-            sum = fmaf(w, pl[k], sum);
-          }
-          sh.cm[team][r] = big;
-          sh.cl[team][r] = sum;
-        }
-        team_sync();
-      };
-      auto summed = [&](const float* from, int n, int i) {
-        float4 y[kJoin], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int k = 0; k < kJoin; ++k)
-          y[k] = k < n ? __ldcg(reinterpret_cast<const float4*>(from + k * ap.part_stride + o_at) + i) : v;
-#pragma unroll
-        for (int k = 0; k < kJoin; ++k) {
-          const float a = sh.w[team][k][i / (HD / 4)];
-          if (k < n)
-            v = make_float4(fmaf(a, y[k].x, v.x), fmaf(a, y[k].y, v.y), fmaf(a, y[k].z, v.z),
-                            fmaf(a, y[k].w, v.w));
-        }
-        return v;
-      };
-      float* mine = parts + chunk * ap.part_stride;
-      for (int i = tid; i < rows * (HD / 4); i += kTeamThreads)
-        __stcg(reinterpret_cast<float4*>(mine + o_at) + i, joined(i));
-      if (tid < rows) {
-        __stcg(mine + tid, sh.cm[team][tid]);
-        __stcg(mine + l_at + tid, sh.cl[team][tid]);
-      }
-      const int gr = chunk / kJoin, in_group = min(kJoin, plan.chunks - gr * kJoin);
-      if (arrive_last(arrived + gr, in_group)) {
-        const float* from = parts + gr * kJoin * ap.part_stride;
-        int n = in_group;
-        bool all_there = true;
-        weigh(from, n);
-        if (groups > 1) {
-          float* to = parts + (ap.cap_parts + gr) * ap.part_stride;
-          for (int i = tid; i < rows * (HD / 4); i += kTeamThreads)
-            __stcg(reinterpret_cast<float4*>(to + o_at) + i, summed(from, n, i));
-          if (tid < rows) {
-            __stcg(to + tid, sh.cm[team][tid]);
-            __stcg(to + l_at + tid, sh.cl[team][tid]);
-          }
-          all_there = arrive_last(arrived + cap_groups, groups);
-          if (all_there) {
-            from = parts + ap.cap_parts * ap.part_stride;
-            n = groups;
-            weigh(from, n);
-          }
-        }
-        if (all_there) {
-          if (tid < rows) close_row(tid, sh.cm[team][tid], sh.cl[team][tid]);
-          team_sync();
-          for (int i = tid; i < rows * (HD / 4); i += kTeamThreads) finish(i, summed(from, n, i));
-        }
-      }
+      float* mine = unit_parts(ap, at) + chunk * ap.part_stride;
+      const int l_at = (ap.part_rows + 3) & ~3;
+      each([&](int r, int dim, float4 v) {
+        __stcg(reinterpret_cast<float4*>(mine + 2 * l_at + r * HD + dim), v);
+      });
+      each_row([&](int r, float big, float sum) {
+        __stcg(mine + r, big);
+        __stcg(mine + l_at + r, sum);
+      });
     }
-    ++chunk;
-    fence_proxy_async_smem();  // O is overwritten by the next chunk's copies
-    team_sync();
+    if constexpr (TEAM > 1) {
+      fence_proxy_async_smem();  // O is overwritten by the next chunk's copies
+      __syncthreads();
+    }
+    }
   }
+done:
   if (!ok && lane == 0 && ap.status) atomicOr(ap.status, kStatusTimeout);
 }
 
@@ -820,23 +881,23 @@ int tile_rows(long long rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <=
 
 // The workspace of a unit, for caches of up to max_kv tokens.
 struct PartSizes {
-  int tiles, parts, groups, rows, stride;
+  int tiles, parts, rows, stride;
   long long unit_bytes;
 };
 PartSizes part_sizes(int nq, int nkv, int hd, int max_q, int max_kv) {
   PartSizes p;
   const long long rows = static_cast<long long>(max_q) * (nq / nkv);
-  const int R = tile_rows(rows);
+  const int R = tile_rows(rows), team = R == 8 ? 1 : kWarps;
+  const int tokens = std::max(1, max_kv);
   p.tiles = static_cast<int>((rows + R - 1) / R);
-  const int tokens = std::max(1, max_kv), team = R == 8 ? 1 : kWarps;
   p.parts = (tokens - 1) / chunk_tokens(tokens, team) + 1;
   // just past a change of the step, a shorter cache has more chunks
-  if (tokens > kJoin * (team == 1 ? 64 : 256)) p.parts = std::max(p.parts, kJoin);
+  if (team == 1 && tokens > 512) p.parts = std::max(p.parts, 8);
+  if (team == 1 && tokens > 2048) p.parts = std::max(p.parts, 16);
   if (tokens > kMaxParts * 256) p.parts = kMaxParts;
-  p.groups = (p.parts + kJoin - 1) / kJoin;
   p.rows = static_cast<int>(std::min<long long>(R, rows));
   p.stride = 2 * ((p.rows + 3) & ~3) + p.rows * hd;
-  p.unit_bytes = 4ll * (p.parts + p.groups) * p.stride;
+  p.unit_bytes = 4ll * p.parts * p.stride;
   return p;
 }
 
@@ -864,7 +925,8 @@ cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int ma
   int rc = make_tmap_nd(&tk, ap.kpool, false, 2, dims, stride, box, step, HD);
   if (!rc) rc = make_tmap_nd(&tv, ap.vpool, false, 2, dims, stride, box, step, HD);
   if (rc) return static_cast<cudaError_t>(rc);
-  auto kern = cache_attn_rows<T, HD, NT, NT == 1 ? 1 : kWarps>;
+  constexpr int kTeam = NT == 1 ? 1 : kWarps;
+  auto kern = cache_attn_rows<T, HD, NT, kTeam>;
   static int resident[64] = {0};  // per instantiation and device
   int dev = 0;
   cudaGetDevice(&dev);
@@ -880,12 +942,16 @@ cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int ma
   ap.cap_parts = ps.parts;
   ap.part_rows = ps.rows;
   ap.part_stride = ps.stride;
-  if (ws && ws_bytes > kCounterBytes) {
-    ap.arrived = static_cast<int*>(ws);
-    ap.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kCounterBytes);
-    ap.cap_units = std::min((ws_bytes - kCounterBytes) / ps.unit_bytes, kCounterBytes / 4 / (ps.groups + 1));
+  ap.parts = static_cast<float*>(ws);
+  ap.cap_units = ws ? ws_bytes / ps.unit_bytes : 0;
+  cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kWarps * 32), kSmem, s, tk, tv, ap);
+  if (e == cudaSuccess && ps.parts > 1 && ap.cap_units > 0) {
+    const long long x = static_cast<long long>(ap.seqs.n_seqs) * ps.tiles;
+    if (x > 0x7FFFFFFFll || ap.nkv > 65535) return cudaErrorInvalidValue;
+    e = launch_pdl(cache_attn_join<T, HD, R, kTeam, kSlab>, dim3(static_cast<unsigned>(x), ap.nkv, ps.rows),
+                   dim3(kJoinWarps * 32), 0, s, ap);
   }
-  return launch_pdl(kern, dim3(grid), dim3(kWarps * 32), kSmem, s, tk, tv, ap);
+  return e;
 }
 
 template <typename T, int HD>
@@ -905,7 +971,7 @@ long long cache_attention_workspace(int nqh, int nkvh, int hd, int n_seqs, int m
   const PartSizes p = part_sizes(nqh, nkvh, hd, max_q, max_kv);
   if (p.parts == 1) return 0;
   const long long units = static_cast<long long>(n_seqs) * p.tiles * nkvh;
-  return std::min(kCounterBytes + units * p.unit_bytes, 1ll << 28);
+  return std::min(units * p.unit_bytes, 1ll << 30);
 }
 
 int cache_attention(const void* q, long long ldq, long long T, int nqh, int nkvh, int hd,

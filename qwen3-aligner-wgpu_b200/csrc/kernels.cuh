@@ -258,8 +258,7 @@ int kv_append(const void* q, long long ldq, const void* k, long long ldk, const 
 
 // Attention over the e4m3 cache (cache_attn.cu); lse [T][nqh] optional.
 // workspace: cache_attention_workspace() bytes (fewer, or null: some or all
-// long caches are not split), its first 2^20 zeroed once before its first use,
-// used by one launch at a time.
+// long caches are not split), used by one call at a time.
 int cache_attention(const void* q, long long ldq, long long T, int nqh, int nkvh, int hd,
                     const SeqMap& seqs, int max_q, int max_kv, const void* kpool, const void* vpool,
                     int kv_pages, const float* kscale, const float* vscale, float scale, bool causal,
