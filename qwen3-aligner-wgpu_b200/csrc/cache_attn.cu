@@ -299,13 +299,25 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const __grid_
   const float ref = big == -INFINITY ? 0.0f : big;
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float sum = 0.0f;
-#pragma unroll 8
-  for (int k = first; k < n; k += kAtOnce) {
-    const float* part = parts + static_cast<long long>(k) * ap.part_stride;
-    const float4 y = *reinterpret_cast<const float4*>(part + o_at + 4 * d);
-    const float a = ex2_approx(part[r] - ref);
-    sum = fmaf(a, part[l_at + r], sum);
-    v = make_float4(fmaf(a, y.x, v.x), fmaf(a, y.y, v.y), fmaf(a, y.z, v.z), fmaf(a, y.w, v.w));
+  constexpr int kBatch = 8;  // parts whose loads are in flight together
+  for (int k0 = first; k0 < n; k0 += kBatch * kAtOnce) {
+    float4 y[kBatch];
+    float pm[kBatch], pl[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int k = k0 + i * kAtOnce;
+      const float* part = parts + static_cast<long long>(min(k, n - 1)) * ap.part_stride;
+      y[i] = __ldcg(reinterpret_cast<const float4*>(part + o_at + 4 * d));
+      pm[i] = __ldcg(part + r);
+      pl[i] = __ldcg(part + l_at + r);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (k0 + i * kAtOnce < n) {
+        const float a = ex2_approx(pm[i] - ref);
+        sum = fmaf(a, pl[i], sum);
+        v = make_float4(fmaf(a, y[i].x, v.x), fmaf(a, y[i].y, v.y), fmaf(a, y[i].z, v.z), fmaf(a, y[i].w, v.w));
+      }
   }
   s_o[first][d] = v;
   // each part's sum once: from the first lane of its kLanes
