@@ -3,23 +3,24 @@
 // wq [N][K / 2] bytes, the even k of a pair in the low nibble.
 //
 // Built for few rows of x, where the weights' bytes are the bound (K / 2 a row
-// of W, each read once).  A warp takes 32 rows of W (two mma.sync M blocks) and
+// of W, each read once).  A warp takes 16 RB rows of W (RB mma.sync M blocks) and
 // walks K in steps of 128: a thread's 16 bytes of a W row are 32 weights, a
 // quad's four threads cover the step, and a load of eight rows keeps whole
-// 64-byte pieces in use; kAhead steps are on their way in registers.  The codes
-// become 16-bit integers by bit work (in the mantissa of a power of two) less the
-// zero, exactly; x is a 16-bit operand as it is; a group's sum is exact products
-// in f32 and is scaled in f32, so nothing is rounded before the output.
+// 64-byte pieces in use; 4 KB of steps, of the next rows too, are on their way
+// in registers.  The codes become 16-bit integers by bit work (in the mantissa of
+// a power of two) less the zero, exactly; x is a 16-bit operand as it is; a
+// group's sum is exact products in f32 and is scaled in f32, so nothing is
+// rounded before the output.
 //
 // The order of k inside a step is free as long as both operands agree.  A word's
 // nibbles leave the bit work as the pairs (0,4) (1,5) (2,6) (3,7); x is put in
-// that order when the CTA copies it into shared memory, as the 16 bytes that a
-// thread needs for a word.  x stays there for all rows that the CTA takes, if it
-// fits; a longer K goes through in chunks.
+// that order in shared memory, as the 16 bytes that a thread needs for a word.
+// x stays there for all rows that the CTA takes, if it fits; a longer K goes
+// through in chunks.
 //
-// With few rows of W a CTA's eight warps share 32 rows and split K, and their
-// sums are joined in shared memory in warp order; with many each warp has rows
-// of its own.  No atomics, the same bits each time.
+// With few rows of W a CTA's eight warps share rows and split K, and their sums
+// are joined in shared memory in warp order; with many each warp has rows of its
+// own.  No atomics, the same bits each time.
 #include <algorithm>
 #include <type_traits>
 
@@ -32,10 +33,16 @@ namespace qa {
 namespace {
 
 constexpr int kStep = 128;   // k of a step
-constexpr int kRows = 32;    // rows of W a warp
 constexpr int kWarps = 8;
-constexpr int kAhead = 2;    // steps of W on their way
 constexpr int kXBytes = 96 * 1024;  // most of x in shared memory: two CTAs an SM
+
+// For 8 NT tokens: M blocks a warp takes (more share each operand of x, as far as
+// the registers reach) and steps of W in registers, one in use and the others on
+// their way: 4 or 3 KB a warp.
+template <int NT>
+struct Form {
+  static constexpr int kRb = NT == 1 ? 2 : 1, kRows = 16 * kRb, kAhead = NT == 1 ? 3 : 4;
+};
 
 struct W4Params {
   const void* x;
@@ -80,6 +87,7 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
 template <typename T>
 struct Zero {  // base + zero, twice
   uint32_t lo, hi;
+  __device__ __forceinline__ Zero() : Zero(8u) {}
   __device__ __forceinline__ explicit Zero(uint32_t z) {
     if constexpr (H16Traits<T>::kBf16) {
       lo = hi = (0x4300u | z) * 0x10001u;
@@ -131,9 +139,9 @@ __device__ __forceinline__ void weights8(uint32_t w, const Zero<T>& z, const Bit
 // GPS: groups of a step, 1, 2 or 4 (group 128, 64, 32).  FAST: rows of x and W can
 // be read 16 bytes at a time, a step's scales and zeros at once, and K is whole
 // steps.
-template <typename T, int NT, int GPS, bool FAST>
+template <typename T, int NT, int GPS, bool ZEROS, bool FAST>
 __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(const __grid_constant__ W4Params wp) {
-  constexpr int kTok = 8 * NT;
+  constexpr int kTok = 8 * NT, kRb = Form<NT>::kRb, kRows = Form<NT>::kRows, kAhead = Form<NT>::kAhead;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int m0 = blockIdx.y * kTok, toks = min(kTok, wp.M - m0);
@@ -149,115 +157,185 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
   pdl_wait();
   pdl_trigger();
 
-  // steps [l0, l0 + chunk) of every slice; a thread has one unit and token
-  auto stage = [&](int l0) {
-    const int c = threadIdx.x % 16;
-    for (int m = threadIdx.x / 16; m < toks; m += kWarps * 2) {
-      const T* row = static_cast<const T*>(wp.x) + (m0 + m) * wp.ldx + 32 * (c & 3) + 8 * (c >> 2);
-      uint8_t* to = smem + m * kTokBytes + 16 * (c ^ 4 * (m & 1));
-      for (int sl = 0; sl < wp.slices; ++sl) {
-        const int n = min(wp.chunk, wp.per - l0), st0 = sl * wp.per + l0;
-#pragma unroll 4
-        for (int i = 0; i < n; ++i) {
-          const int k = (st0 + i) * kStep;
-          uint4 d = make_uint4(0, 0, 0, 0);  // past K
-          if (FAST ? st0 + i < steps : k + 32 * (c & 3) + 8 * (c >> 2) < wp.K) {
-            if (FAST || wp.vec_x) {
-              d = __ldg(reinterpret_cast<const uint4*>(row + k));
-            } else {
-              T* e = reinterpret_cast<T*>(&d);
+  // ---- W, its scales and zeros: `flat` counts this warp's steps over all its tiles
+  const int first = slice * wp.per, own = min(wp.per, steps - first);  // own may be < 1
+  const int row_step = gridDim.x * tiles * kRows, all_rows = wp.N;
+  const int row_first = (blockIdx.x * tiles + warp / wp.slices) * kRows;
+  using Packed = std::conditional_t<GPS == 4, uint64_t, uint32_t>;  // a step's scales of a row
+  struct Ahead {
+    uint4 w[2 * kRb];
+    Packed s;
+    uint32_t z;
+  };
+  const uint8_t* wr[2 * kRb];  // rows g, g + 8, .. of the tile being fetched; past N the last row
+  long long sr = 0;            // where lane t's row (one of the quad's) has its scales
+  auto at_tile = [&](int row0) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j) e[j] = row[k + j];
-            }
+    for (int r = 0; r < 2 * kRb; ++r)
+      wr[r] = wp.wq + static_cast<long long>(min(row0 + g + 8 * r, all_rows - 1)) * wp.ldw + 16 * t;
+    sr = static_cast<long long>(min(row0 + g + 8 * (t % (2 * kRb)), all_rows - 1)) * groups;
+  };
+  int f_row = row_first, f_step = first;  // to be fetched next
+  at_tile(f_row);
+  auto fetch = [&](Ahead& a) {
+    const int st = f_step;
+    if constexpr (FAST) {
+#pragma unroll
+      for (int r = 0; r < 2 * kRb; ++r) a.w[r] = __ldg(reinterpret_cast<const uint4*>(wr[r] + st * (kStep / 2)));
+      const T* sp = static_cast<const T*>(wp.scales) + sr + st * GPS;
+      if constexpr (GPS == 1) a.s = *reinterpret_cast<const uint16_t*>(sp);
+      else a.s = *reinterpret_cast<const Packed*>(sp);
+      if constexpr (ZEROS) {
+        const uint8_t* zp = wp.zeros + sr + st * GPS;
+        a.z = GPS == 1 ? *zp : GPS == 2 ? *reinterpret_cast<const uint16_t*>(zp) : *reinterpret_cast<const uint32_t*>(zp);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 2 * kRb; ++r) {
+        const uint8_t* p = wr[r] + st * (kStep / 2);
+        a.w[r] = make_uint4(0, 0, 0, 0);
+        if (st * kStep + 32 * t < wp.K) {
+          if (wp.vec_w) {
+            a.w[r] = __ldg(reinterpret_cast<const uint4*>(p));
+          } else {
+            uint8_t* b = reinterpret_cast<uint8_t*>(&a.w[r]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) b[i] = p[i];
           }
-          // (0 1)(2 3)(4 5)(6 7) -> (0 4)(1 5)(2 6)(3 7)
-          *reinterpret_cast<uint4*>(to + sl * slice_bytes + i * step_bytes) =
-              make_uint4(__byte_perm(d.x, d.z, 0x5410), __byte_perm(d.x, d.z, 0x7632),
-                         __byte_perm(d.y, d.w, 0x5410), __byte_perm(d.y, d.w, 0x7632));
         }
       }
+      a.s = 0;
+      a.z = 0;
+#pragma unroll
+      for (int q = 0; q < GPS; ++q)
+        if (st * GPS + q < groups) {
+          a.s |= static_cast<Packed>(static_cast<const uint16_t*>(wp.scales)[sr + st * GPS + q]) << (16 * q);
+          if (ZEROS) a.z |= static_cast<uint32_t>(wp.zeros[sr + st * GPS + q]) << (8 * q);
+        }
     }
+    if (++f_step == first + own) {
+      f_step = first;
+      f_row += row_step;  // past N: the last row again, which nobody uses
+      at_tile(min(f_row, all_rows - 1));
+    }
+  };
+  Ahead ring[kAhead];
+  if (own > 0)
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) fetch(ring[i]);
+
+  // ---- x: steps [l0, l0 + chunk) of every slice.  A thread has one unit of one
+  // token, and with few tokens every `apart`-th step
+  const int apart = max(1, 2 * kWarps / toks), x_m = threadIdx.x / 16 % toks, x_from = threadIdx.x / 16 / toks;
+  auto stage = [&](int l0) {
+    const int c = threadIdx.x % 16;
+    auto each = [&](auto f) {  // f(place, token, k) for the thread's units
+      if (x_from < apart)
+        for (int sl = 0; sl < wp.slices; ++sl) {
+          const int n = min(wp.chunk, wp.per - l0), st0 = sl * wp.per + l0;
+          uint8_t* to = smem + sl * slice_bytes + x_m * kTokBytes + 16 * (c ^ 4 * (x_m & 1));
+#pragma unroll 2
+          for (int i = x_from; i < n; i += apart)
+            f(to + i * step_bytes, x_m, (st0 + i) * kStep + 32 * (c & 3) + 8 * (c >> 2));
+        }
+    };
+    if (FAST || wp.vec_x) {
+      each([&](uint8_t* to, int m, int k) {  // zeros past K
+        const T* src = static_cast<const T*>(wp.x) + (m0 + m) * wp.ldx;
+        cp_async16(smem_u32(to), k < wp.K ? src + k : src, k < wp.K ? 16 : 0);
+      });
+      cp_async_commit();
+      cp_async_wait_all();
+    } else {
+      each([&](uint8_t* to, int m, int k) {
+        const T* src = static_cast<const T*>(wp.x) + (m0 + m) * wp.ldx + k;
+        T* e = reinterpret_cast<T*>(to);
+        for (int j = 0; j < 8; ++j) e[j] = k < wp.K ? src[j] : f2h<T>(0.0f);
+      });
+    }
+    // (0 1)(2 3)(4 5)(6 7) -> (0 4)(1 5)(2 6)(3 7)
+    each([&](uint8_t* to, int, int) {
+      const uint4 d = *reinterpret_cast<const uint4*>(to);
+      *reinterpret_cast<uint4*>(to) = make_uint4(__byte_perm(d.x, d.z, 0x5410), __byte_perm(d.x, d.z, 0x7632),
+                                                 __byte_perm(d.y, d.w, 0x5410), __byte_perm(d.y, d.w, 0x7632));
+    });
   };
 
   const bool once = wp.chunk >= wp.per;  // x stays for all rows
-  const int first = slice * wp.per, own = min(wp.per, steps - first);  // own may be < 1
-  const uint8_t* xs = smem + slice * slice_bytes + g * kTokBytes + 16 * t;
-  const int even = 64 * (g & 1), odd = -even;  // of the words w
-  const int all_tiles = (wp.N + kRows - 1) / kRows;
+  // where this lane's token has its even and odd words; columns past the tokens
+  // take the last one's x, and nobody reads their sums
+  const uint8_t *x_even[NT], *x_odd[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int m = min(8 * nt + g, toks - 1);
+    x_even[nt] = smem + slice * slice_bytes + m * kTokBytes + 16 * t + 64 * (m & 1);
+    x_odd[nt] = smem + slice * slice_bytes + m * kTokBytes + 16 * t - 64 * (m & 1);
+  }
   bool staged = false;
-  for (int tile0 = blockIdx.x * tiles; tile0 < all_tiles; tile0 += gridDim.x * tiles) {
-    const int row0 = (tile0 + warp / wp.slices) * kRows;
-    // rows g, g + 8 of the two blocks; past N the last row is read and not stored
-    const uint8_t* wr[4];
+  int slot = 0;  // of the ring
+  for (int row_cta = blockIdx.x * tiles * kRows; row_cta < all_rows; row_cta += row_step) {
+    const int row0 = row_cta + warp / wp.slices * kRows;
+    float acc[kRb][NT][4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) wr[r] = wp.wq + min(row0 + g + 8 * r, wp.N - 1) * wp.ldw + 16 * t;
-    // lane t fetches the scales and zeros of the quad's row g + 8 t
-    const long long sr = static_cast<long long>(min(row0 + g + 8 * t, wp.N - 1)) * groups;
-    const T* srow = static_cast<const T*>(wp.scales) + sr;
-    const uint8_t* zrow = wp.zeros ? wp.zeros + sr : nullptr;
-    auto load_w = [&](int r, int step) {
-      if constexpr (FAST) step = min(step, steps - 1);  // past the end: nobody uses it
-      const uint8_t* p = wr[r] + step * (kStep / 2);
-      if constexpr (FAST) return __ldg(reinterpret_cast<const uint4*>(p));
-      uint4 d = make_uint4(0, 0, 0, 0);
-      if (step * kStep + 32 * t < wp.K) {
-        if (wp.vec_w) {
-          d = __ldg(reinterpret_cast<const uint4*>(p));
-        } else {
-          uint8_t* b = reinterpret_cast<uint8_t*>(&d);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) b[i] = p[i];
-        }
-      }
-      return d;
-    };
-    using Packed = std::conditional_t<GPS == 4, uint64_t, uint32_t>;  // a step's scales of a row
-    auto load_s = [&](int step) {
-      if constexpr (FAST) step = min(step, steps - 1);
-      const T* p = srow + step * GPS;
-      Packed d = 0;
-      if constexpr (FAST) {
-        if constexpr (GPS == 1) d = *reinterpret_cast<const uint16_t*>(p);
-        else d = *reinterpret_cast<const Packed*>(p);
-      } else {
-#pragma unroll
-        for (int q = 0; q < GPS; ++q)
-          if (step * GPS + q < groups)
-            d |= static_cast<Packed>(reinterpret_cast<const uint16_t*>(p)[q]) << (16 * q);
-      }
-      return d;
-    };
-    auto load_z = [&](int step) {
-      uint32_t d = 0x08080808u;
-      if (zrow) {
-        if constexpr (FAST) step = min(step, steps - 1);
-        const uint8_t* p = zrow + step * GPS;
-        if constexpr (FAST) {
-          d = GPS == 1 ? *p : GPS == 2 ? *reinterpret_cast<const uint16_t*>(p) : *reinterpret_cast<const uint32_t*>(p);
-        } else {
-          d = 0;
-#pragma unroll
-          for (int q = 0; q < GPS; ++q)
-            if (step * GPS + q < groups) d |= static_cast<uint32_t>(p[q]) << (8 * q);
-        }
-      }
-      return d;
-    };
-    uint4 ring[kAhead][4];
-    Packed ring_s[kAhead];
-    uint32_t ring_z[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) ring[i][r] = load_w(r, first + i);
-      ring_s[i] = load_s(first + i);
-      ring_z[i] = load_z(first + i);
-    }
-    float acc[2][NT][4];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < kRb; ++b)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) acc[b][nt][0] = acc[b][nt][1] = acc[b][nt][2] = acc[b][nt][3] = 0.0f;
+
+    // one step, with what `a` brought; then a's place is filled again
+    auto take = [&](Ahead& a, int at) {
+      Zero<T> zr[2 * kRb] = {};
+      if constexpr (ZEROS) {
+#pragma unroll
+        for (int r = 0; r < 2 * kRb; ++r)  // a lane's 32 weights lie in one group
+          zr[r] = Zero<T>(__shfl_sync(0xFFFFFFFFu, a.z, (lane & 28) + r) >> (8 * (t * GPS / 4)) & 0xFFu);
+      }
+      float c[GPS][kRb][NT][4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t k[2 * kRb][4];
+#pragma unroll
+        for (int r = 0; r < 2 * kRb; ++r) {
+          const uint32_t word = w == 0 ? a.w[r].x : w == 1 ? a.w[r].y : w == 2 ? a.w[r].z : a.w[r].w;
+          weights8<T>(word, zr[r], bits, k[r]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint4 x = *reinterpret_cast<const uint4*>((w & 1 ? x_odd[nt] : x_even[nt]) + at + 64 * w);
+#pragma unroll
+          for (int q = 0; q < GPS; ++q) {
+            // with several groups in the step, x of the other groups' lanes is left
+            // out: a code times 0 is 0
+            const bool in = GPS == 1 || t * GPS / 4 == q;
+            const uint32_t x0 = in ? x.x : 0u, x1 = in ? x.y : 0u, x2 = in ? x.z : 0u, x3 = in ? x.w : 0u;
+#pragma unroll
+            for (int b = 0; b < kRb; ++b) {
+              const uint32_t a0[4] = {k[2 * b][0], k[2 * b + 1][0], k[2 * b][1], k[2 * b + 1][1]};
+              const uint32_t a1[4] = {k[2 * b][2], k[2 * b + 1][2], k[2 * b][3], k[2 * b + 1][3]};
+              if (w == 0)
+                mma_16816<T, true>(c[q][b][nt], a0, x0, x1);
+              else
+                mma_16816<T, false>(c[q][b][nt], a0, x0, x1);
+              mma_16816<T, false>(c[q][b][nt], a1, x2, x3);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 2 * kRb; ++r) {
+        const Packed four = __shfl_sync(0xFFFFFFFFu, a.s, (lane & 28) + r);
+#pragma unroll
+        for (int q = 0; q < GPS; ++q) {
+          const uint16_t h = static_cast<uint16_t>(four >> (16 * q));
+          const float sc = h2f<T>(*reinterpret_cast<const T*>(&h));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              acc[r / 2][nt][2 * (r & 1) + e] = fmaf(sc, c[q][r / 2][nt][2 * (r & 1) + e], acc[r / 2][nt][2 * (r & 1) + e]);
+        }
+      }
+      fetch(a);
+    };
 
     int li = 0;  // step of the slice
     for (int l0 = 0; l0 < wp.per; l0 += wp.chunk) {
@@ -267,76 +345,16 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
         __syncthreads();
         staged = once;
       }
-      for (const int stop = min(own, l0 + wp.chunk); li < stop; li += kAhead) {
+      const int stop = min(own, l0 + wp.chunk);
+      while (li < stop) {
+        // the ring goes on over tiles, its place in the loop's unrolled body does not
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const int st = first + li + i;
-          uint4 wv[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            wv[r] = ring[i][r];
-            ring[i][r] = load_w(r, st + kAhead);
+        for (int i = 0; i < kAhead; ++i)
+          if (slot == i && li < stop) {
+            take(ring[i], (li - l0) * step_bytes);
+            ++li;
+            slot = (i + 1) % kAhead;
           }
-          const Packed sv = ring_s[i];
-          const uint32_t zv = ring_z[i];
-          ring_s[i] = load_s(st + kAhead);
-          ring_z[i] = load_z(st + kAhead);
-          if (li + i >= own) continue;
-          float sc[4][GPS];
-          Zero<T> zr[4] = {Zero<T>(8u), Zero<T>(8u), Zero<T>(8u), Zero<T>(8u)};
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const Packed four = __shfl_sync(0xFFFFFFFFu, sv, (lane & 28) + r);
-#pragma unroll
-            for (int q = 0; q < GPS; ++q) {
-              const uint16_t bits = static_cast<uint16_t>(four >> (16 * q));
-              sc[r][q] = h2f<T>(*reinterpret_cast<const T*>(&bits));
-            }
-            // a lane's 32 weights lie in one group
-            if (wp.zeros) zr[r] = Zero<T>(__shfl_sync(0xFFFFFFFFu, zv, (lane & 28) + r) >> (8 * (t * GPS / 4)) & 0xFFu);
-          }
-          float c[GPS][2][NT][4];
-          const uint8_t* xst = xs + (li + i - l0) * step_bytes;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            uint32_t a[4][4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const uint32_t word = w == 0 ? wv[r].x : w == 1 ? wv[r].y : w == 2 ? wv[r].z : wv[r].w;
-              weights8<T>(word, zr[r], bits, a[r]);
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              uint4 x = make_uint4(0, 0, 0, 0);
-              if (8 * nt + g < toks) x = *reinterpret_cast<const uint4*>(xst + 8 * nt * kTokBytes + 64 * w + (w & 1 ? odd : even));
-#pragma unroll
-              for (int q = 0; q < GPS; ++q) {
-                // with several groups in the step, x of the other groups' lanes is
-                // left out: a code times 0 is 0
-                const bool in = GPS == 1 || t * GPS / 4 == q;
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                  const uint32_t a0[4] = {a[2 * b][0], a[2 * b + 1][0], a[2 * b][1], a[2 * b + 1][1]};
-                  const uint32_t a1[4] = {a[2 * b][2], a[2 * b + 1][2], a[2 * b][3], a[2 * b + 1][3]};
-                  if (w == 0)
-                    mma_16816<T, true>(c[q][b][nt], a0, in ? x.x : 0u, in ? x.y : 0u);
-                  else
-                    mma_16816<T, false>(c[q][b][nt], a0, in ? x.x : 0u, in ? x.y : 0u);
-                  mma_16816<T, false>(c[q][b][nt], a1, in ? x.z : 0u, in ? x.w : 0u);
-                }
-              }
-            }
-          }
-#pragma unroll
-          for (int q = 0; q < GPS; ++q)
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  acc[b][nt][e] = fmaf(sc[2 * b + (e >> 1)][q], c[q][b][nt][e], acc[b][nt][e]);
-        }
       }
     }
     // ---- sums [warp][token][row], joined over the slices in their order; eight
@@ -344,7 +362,7 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
     constexpr int kSums = kTok * kRows;
     float* mine = red + warp * kSums;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < kRb; ++b)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -388,30 +406,30 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
       __syncthreads();
       for (int i = threadIdx.x; i < tiles * (kSums / 8); i += kWarps * 32) {
         const int tile = i / (kSums / 8);
-        put(red + tile * wp.slices * kSums, i % (kSums / 8), (tile0 + tile) * kRows);
+        put(red + tile * wp.slices * kSums, i % (kSums / 8), row_cta + tile * kRows);
       }
       __syncthreads();
     }
   }
 }
 
-template <typename T, int NT, int GPS, bool FAST>
+template <typename T, int NT, int GPS, bool ZEROS, bool FAST>
 cudaError_t launch(W4Params wp, cudaStream_t s) {
-  constexpr int kRed = kWarps * 8 * NT * kRows * 4;
+  constexpr int kRows = Form<NT>::kRows, kRed = kWarps * 8 * NT * kRows * 4;
+  constexpr int kCtas = GPS * NT <= 2 ? 2 : 1;  // an SM
   const int toks = std::min(8 * NT, wp.M), step_bytes = toks * 2 * kStep;
-  const int steps = (wp.K + kStep - 1) / kStep, tiles = (wp.N + kRows - 1) / kRows;
-  const int y = (wp.M + 8 * NT - 1) / (8 * NT);
-  if (y > 65535) return cudaErrorInvalidValue;
-  // split K until there are about 16 warps an SM, while each has a step
+  const int steps = (wp.K + kStep - 1) / kStep, tiles = (wp.N - 1) / kRows + 1;
+  const int y = (wp.M - 1) / (8 * NT) + 1;
+  if (y > 65535 || wp.N > 0x40000000) return cudaErrorInvalidValue;
+  // split K until every SM has its warps, while each has a step
   wp.slices = 1;
-  while (wp.slices < kWarps && static_cast<long long>(tiles) * y * wp.slices < 16ll * device_sm_count() &&
+  while (wp.slices < kWarps && static_cast<long long>(tiles) * y * wp.slices < kCtas * kWarps * device_sm_count() &&
          2 * wp.slices <= steps)
     wp.slices *= 2;
   wp.per = (steps + wp.slices - 1) / wp.slices;
-  wp.chunk = std::max(kAhead, (kXBytes - kRed) / (step_bytes * wp.slices) / kAhead * kAhead);
-  wp.chunk = std::min(wp.chunk, wp.per);
+  wp.chunk = std::min(wp.per, std::max(1, (kXBytes - kRed) / (step_bytes * wp.slices)));
   const int smem = wp.slices * wp.chunk * step_bytes + kRed;
-  auto k = w4_kernel<T, NT, GPS, FAST>;
+  auto k = w4_kernel<T, NT, GPS, ZEROS, FAST>;
   static int set[64] = {0};  // per instantiation and device
   int dev = 0;
   cudaGetDevice(&dev);
@@ -421,7 +439,7 @@ cudaError_t launch(W4Params wp, cudaStream_t s) {
     set[dev & 63] = smem;
   }
   const int per = kWarps / wp.slices;
-  const int grid = std::min((tiles + per - 1) / per, std::max(1, (GPS * NT <= 2 ? 2 : 1) * device_sm_count() / y));
+  const int grid = std::min((tiles + per - 1) / per, std::max(1, kCtas * device_sm_count() / y));
   return launch_pdl(k, dim3(grid, y), dim3(kWarps * 32), smem, s, wp);
 }
 
@@ -429,7 +447,8 @@ template <typename T, int NT, int GPS>
 cudaError_t launch_form(const W4Params& wp, cudaStream_t s) {
   const bool fast = wp.vec_x && wp.vec_w && wp.K % kStep == 0 && reinterpret_cast<uintptr_t>(wp.scales) % 8 == 0 &&
                     reinterpret_cast<uintptr_t>(wp.zeros) % 4 == 0;
-  return fast ? launch<T, NT, GPS, true>(wp, s) : launch<T, NT, GPS, false>(wp, s);
+  if (wp.zeros) return fast ? launch<T, NT, GPS, true, true>(wp, s) : launch<T, NT, GPS, true, false>(wp, s);
+  return fast ? launch<T, NT, GPS, false, true>(wp, s) : launch<T, NT, GPS, false, false>(wp, s);
 }
 
 template <typename T, int NT>
