@@ -18,9 +18,9 @@
 // x stays there for all rows that the CTA takes, if it fits; a longer K goes
 // through in chunks.
 //
-// With few rows of W a CTA's eight warps share rows and split K, and their sums
-// are joined in shared memory in warp order; with many each warp has rows of its
-// own.  No atomics, the same bits each time.
+// With few rows of W a cluster of 2, 4 or 8 CTAs shares rows and splits K (so that
+// a CTA needs its part of x only), and the sums are joined through distributed
+// shared memory in the CTAs' order.  No atomics, the same bits each time.
 #include <algorithm>
 #include <type_traits>
 
@@ -56,9 +56,9 @@ struct W4Params {
   void* out;
   long long ldo;
   int vec_x, vec_w;  // rows of x / W can be read 16 bytes at a time
-  int slices;        // warps that share rows of W: 1, 2, 4 or 8
+  int slices;        // CTAs of a cluster, which share rows of W: 1, 2, 4 or 8
   int per;           // steps of a slice
-  int chunk;         // steps of every slice that have x in shared memory at a time
+  int chunk;         // steps of the slice that have x in shared memory at a time
   int vec_o;         // eight adjacent outputs can be written at once
 };
 
@@ -136,6 +136,13 @@ __device__ __forceinline__ void weights8(uint32_t w, const Zero<T>& z, const Bit
   }
 }
 
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
 // GPS: groups of a step, 1, 2 or 4 (group 128, 64, 32).  FAST: rows of x and W can
 // be read 16 bytes at a time, a step's scales and zeros at once, and K is whole
 // steps.
@@ -146,21 +153,22 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int m0 = blockIdx.y * kTok, toks = min(kTok, wp.M - m0);
   const int steps = (wp.K + kStep - 1) / kStep, groups = wp.K / wp.group;
-  const int slice = warp % wp.slices, tiles = kWarps / wp.slices;
-  // x: [slice][step][token][16 units of 16 bytes: word w of lane t at 4 w + t, odd
+  const int slice = wp.slices > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int cta = blockIdx.x / wp.slices, ctas = gridDim.x / wp.slices;
+  // x: [step][token][16 units of 16 bytes: word w of lane t at 4 w + t, odd
   // tokens with w ^ 1], so that an access of eight lanes (two tokens, four units)
   // meets 32 different banks; then the warps' sums
   constexpr int kTokBytes = 2 * kStep;
-  const int step_bytes = toks * kTokBytes, slice_bytes = wp.chunk * step_bytes;
-  float* red = reinterpret_cast<float*>(smem + wp.slices * slice_bytes);
+  const int step_bytes = toks * kTokBytes;
+  float* red = reinterpret_cast<float*>(smem + wp.chunk * step_bytes);
   const Bits<T> bits;
   pdl_wait();
   pdl_trigger();
 
   // ---- W, its scales and zeros: `flat` counts this warp's steps over all its tiles
   const int first = slice * wp.per, own = min(wp.per, steps - first);  // own may be < 1
-  const int row_step = gridDim.x * tiles * kRows, all_rows = wp.N;
-  const int row_first = (blockIdx.x * tiles + warp / wp.slices) * kRows;
+  const int row_step = ctas * kWarps * kRows, all_rows = wp.N;
+  const int row_first = (cta * kWarps + warp) * kRows;
   using Packed = std::conditional_t<GPS == 4, uint64_t, uint32_t>;  // a step's scales of a row
   struct Ahead {
     uint4 w[2 * kRb];
@@ -224,20 +232,18 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) fetch(ring[i]);
 
-  // ---- x: steps [l0, l0 + chunk) of every slice.  A thread has one unit of one
+  // ---- x: steps [l0, l0 + chunk) of the slice.  A thread has one unit of one
   // token, and with few tokens every `apart`-th step
   const int apart = max(1, 2 * kWarps / toks), x_m = threadIdx.x / 16 % toks, x_from = threadIdx.x / 16 / toks;
   auto stage = [&](int l0) {
     const int c = threadIdx.x % 16;
     auto each = [&](auto f) {  // f(place, token, k) for the thread's units
-      if (x_from < apart)
-        for (int sl = 0; sl < wp.slices; ++sl) {
-          const int n = min(wp.chunk, wp.per - l0), st0 = sl * wp.per + l0;
-          uint8_t* to = smem + sl * slice_bytes + x_m * kTokBytes + 16 * (c ^ 4 * (x_m & 1));
+      if (x_from >= apart) return;
+      uint8_t* to = smem + x_m * kTokBytes + 16 * (c ^ 4 * (x_m & 1));
+      const int n = min(wp.chunk, wp.per - l0);
 #pragma unroll 2
-          for (int i = x_from; i < n; i += apart)
-            f(to + i * step_bytes, x_m, (st0 + i) * kStep + 32 * (c & 3) + 8 * (c >> 2));
-        }
+      for (int i = x_from; i < n; i += apart)
+        f(to + i * step_bytes, x_m, (first + l0 + i) * kStep + 32 * (c & 3) + 8 * (c >> 2));
     };
     if (FAST || wp.vec_x) {
       each([&](uint8_t* to, int m, int k) {  // zeros past K
@@ -268,13 +274,12 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int m = min(8 * nt + g, toks - 1);
-    x_even[nt] = smem + slice * slice_bytes + m * kTokBytes + 16 * t + 64 * (m & 1);
-    x_odd[nt] = smem + slice * slice_bytes + m * kTokBytes + 16 * t - 64 * (m & 1);
+    x_even[nt] = smem + m * kTokBytes + 16 * t + 64 * (m & 1);
+    x_odd[nt] = smem + m * kTokBytes + 16 * t - 64 * (m & 1);
   }
   bool staged = false;
   int slot = 0;  // of the ring
-  for (int row_cta = blockIdx.x * tiles * kRows; row_cta < all_rows; row_cta += row_step) {
-    const int row0 = row_cta + warp / wp.slices * kRows;
+  for (int row_cta = cta * kWarps * kRows; row_cta < all_rows; row_cta += row_step) {
     float acc[kRb][NT][4];
 #pragma unroll
     for (int b = 0; b < kRb; ++b)
@@ -357,9 +362,8 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
           }
       }
     }
-    // ---- sums [warp][token][row], joined over the slices in their order; eight
-    // rows of a token are a unit of the output
-    constexpr int kSums = kTok * kRows;
+    // ---- sums [warp][token][row]; eight rows of a token are a unit of the output
+    constexpr int kSums = kTok * kRows, kUnits = kSums / 8;
     float* mine = red + warp * kSums;
 #pragma unroll
     for (int b = 0; b < kRb; ++b)
@@ -368,21 +372,7 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           mine[(8 * nt + 2 * t + (e & 1)) * kRows + 16 * b + g + (e >> 1) * 8] = acc[b][nt][e];
-    auto put = [&](const float* from, int unit, int row) {  // unit of a tile that begins at row `row`
-      const int m = unit / (kRows / 8), n = row + unit % (kRows / 8) * 8;
-      if (m >= toks || n >= wp.N) return;
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) *reinterpret_cast<float4*>(v + 4 * j) = *reinterpret_cast<const float4*>(from + unit * 8 + 4 * j);
-      for (int w = 1; w < wp.slices; ++w)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float4 y = *reinterpret_cast<const float4*>(from + w * kSums + unit * 8 + 4 * j);
-          v[4 * j] += y.x;
-          v[4 * j + 1] += y.y;
-          v[4 * j + 2] += y.z;
-          v[4 * j + 3] += y.w;
-        }
+    auto put = [&](float (&v)[8], int m, int n) {
       T* to = static_cast<T*>(wp.out) + (m0 + m) * wp.ldo + n;
       if (wp.bias)
 #pragma unroll
@@ -400,15 +390,38 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
     if (wp.slices == 1) {
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < kSums / 8 / 32; ++i) put(mine, lane + 32 * i, row0);
+      for (int i = 0; i < kUnits; i += 32) {
+        const int u = i + lane, m = u / (kRows / 8), n = row_cta + warp * kRows + u % (kRows / 8) * 8;
+        if (m < toks && n < all_rows) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) *reinterpret_cast<float4*>(v + 4 * j) = *reinterpret_cast<const float4*>(mine + 8 * u + 4 * j);
+          put(v, m, n);
+        }
+      }
       __syncwarp();
     } else {
-      __syncthreads();
-      for (int i = threadIdx.x; i < tiles * (kSums / 8); i += kWarps * 32) {
-        const int tile = i / (kSums / 8);
-        put(red + tile * wp.slices * kSums, i % (kSums / 8), row_cta + tile * kRows);
+      cluster_sync();  // the cluster's sums are there; each CTA joins its share of the units
+      for (int i = slice * (kWarps * 32) + threadIdx.x; i < kWarps * kUnits; i += wp.slices * (kWarps * 32)) {
+        const int u = i % kUnits, m = u / (kRows / 8), n = row_cta + i / kUnits * kRows + u % (kRows / 8) * 8;
+        if (m >= toks || n >= all_rows) continue;
+        const uint32_t at = smem_u32(red + 8 * i);
+        float v[8] = {};
+        for (int r = 0; r < wp.slices; ++r) {
+          const uint32_t from = mapa_shared(at, r);
+          const float4 y = ld_cluster_f32x4(from), z = ld_cluster_f32x4(from + 16);
+          v[0] += y.x;
+          v[1] += y.y;
+          v[2] += y.z;
+          v[3] += y.w;
+          v[4] += z.x;
+          v[5] += z.y;
+          v[6] += z.z;
+          v[7] += z.w;
+        }
+        put(v, m, n);
       }
-      __syncthreads();
+      cluster_sync();  // read before they are written again, or the CTA ends
     }
   }
 }
@@ -421,14 +434,15 @@ cudaError_t launch(W4Params wp, cudaStream_t s) {
   const int steps = (wp.K + kStep - 1) / kStep, tiles = (wp.N - 1) / kRows + 1;
   const int y = (wp.M - 1) / (8 * NT) + 1;
   if (y > 65535 || wp.N > 0x40000000) return cudaErrorInvalidValue;
-  // split K until every SM has its warps, while each has a step
+  // split K until the GPU is full, while each CTA has a step
+  const int groups = (tiles - 1) / kWarps + 1;
   wp.slices = 1;
-  while (wp.slices < kWarps && static_cast<long long>(tiles) * y * wp.slices < kCtas * kWarps * device_sm_count() &&
+  while (wp.slices < 8 && static_cast<long long>(groups) * y * wp.slices < kCtas * device_sm_count() &&
          2 * wp.slices <= steps)
     wp.slices *= 2;
   wp.per = (steps + wp.slices - 1) / wp.slices;
-  wp.chunk = std::min(wp.per, std::max(1, (kXBytes - kRed) / (step_bytes * wp.slices)));
-  const int smem = wp.slices * wp.chunk * step_bytes + kRed;
+  wp.chunk = std::min(wp.per, std::max(1, (kXBytes - kRed) / step_bytes));
+  const int smem = wp.chunk * step_bytes + kRed;
   auto k = w4_kernel<T, NT, GPS, ZEROS, FAST>;
   static int set[64] = {0};  // per instantiation and device
   int dev = 0;
@@ -438,9 +452,21 @@ cudaError_t launch(W4Params wp, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     set[dev & 63] = smem;
   }
-  const int per = kWarps / wp.slices;
-  const int grid = std::min((tiles + per - 1) / per, std::max(1, kCtas * device_sm_count() / y));
-  return launch_pdl(k, dim3(grid, y), dim3(kWarps * 32), smem, s, wp);
+  const int ctas = std::min(groups, std::max(1, kCtas * device_sm_count() / (y * wp.slices)));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas * wp.slices, y);
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = wp.slices;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = wp.slices > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, k, wp);
 }
 
 template <typename T, int NT, int GPS>
