@@ -12,6 +12,10 @@
 // group's sum is exact products in f32 and is scaled in f32, so nothing is
 // rounded before the output.
 //
+// A word (8 weights) of all lanes lies in one group: of a step's 128 k a lane has
+// 16 bytes in a row with groups of 128, 8 bytes in each of two groups of 64, 4 in
+// each of four groups of 32.
+//
 // The order of k inside a step is free as long as both operands agree.  A word's
 // nibbles leave the bit work as the pairs (0,4) (1,5) (2,6) (3,7); x is put in
 // that order in shared memory, as the 16 bytes that a thread needs for a word.
@@ -41,7 +45,7 @@ constexpr int kXBytes = 96 * 1024;  // most of x in shared memory: two CTAs an S
 // their way: 4 or 3 KB a warp.
 template <int NT>
 struct Form {
-  static constexpr int kRb = NT == 1 ? 2 : 1, kRows = 16 * kRb, kAhead = NT == 1 ? 3 : 4;
+  static constexpr int kRb = NT == 1 ? 2 : 1, kRows = 16 * kRb, kAhead = 3, kCtas = 2;
 };
 
 struct W4Params {
@@ -146,8 +150,15 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t a) {
 // GPS: groups of a step, 1, 2 or 4 (group 128, 64, 32).  FAST: rows of x and W can
 // be read 16 bytes at a time, a step's scales and zeros at once, and K is whole
 // steps.
+
+// First k, in its step, of word w of lane t.
+template <int GPS>
+__device__ __forceinline__ int word_k(int w, int t) {
+  return GPS == 1 ? 32 * t + 8 * w : GPS == 2 ? 64 * (w >> 1) + 16 * t + 8 * (w & 1) : 32 * w + 8 * t;
+}
+
 template <typename T, int NT, int GPS, bool ZEROS, bool FAST>
-__global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(const __grid_constant__ W4Params wp) {
+__global__ void __launch_bounds__(kWarps * 32, Form<NT>::kCtas) w4_kernel(const __grid_constant__ W4Params wp) {
   constexpr int kTok = 8 * NT, kRb = Form<NT>::kRb, kRows = Form<NT>::kRows, kAhead = Form<NT>::kAhead;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -180,7 +191,7 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
   auto at_tile = [&](int row0) {
 #pragma unroll
     for (int r = 0; r < 2 * kRb; ++r)
-      wr[r] = wp.wq + static_cast<long long>(min(row0 + g + 8 * r, all_rows - 1)) * wp.ldw + 16 * t;
+      wr[r] = wp.wq + static_cast<long long>(min(row0 + g + 8 * r, all_rows - 1)) * wp.ldw + word_k<GPS>(0, t) / 2;
     sr = static_cast<long long>(min(row0 + g + 8 * (t % (2 * kRb)), all_rows - 1)) * groups;
   };
   int f_row = row_first, f_step = first;  // to be fetched next
@@ -189,7 +200,18 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
     const int st = f_step;
     if constexpr (FAST) {
 #pragma unroll
-      for (int r = 0; r < 2 * kRb; ++r) a.w[r] = __ldg(reinterpret_cast<const uint4*>(wr[r] + st * (kStep / 2)));
+      for (int r = 0; r < 2 * kRb; ++r) {
+        const uint8_t* p = wr[r] + st * (kStep / 2);
+        if constexpr (GPS == 1) {
+          a.w[r] = __ldg(reinterpret_cast<const uint4*>(p));
+        } else if constexpr (GPS == 2) {
+          const uint2 lo = __ldg(reinterpret_cast<const uint2*>(p)), hi = __ldg(reinterpret_cast<const uint2*>(p + 32));
+          a.w[r] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        } else {
+          a.w[r] = make_uint4(__ldg(reinterpret_cast<const uint32_t*>(p)), __ldg(reinterpret_cast<const uint32_t*>(p + 16)),
+                              __ldg(reinterpret_cast<const uint32_t*>(p + 32)), __ldg(reinterpret_cast<const uint32_t*>(p + 48)));
+        }
+      }
       const T* sp = static_cast<const T*>(wp.scales) + sr + st * GPS;
       if constexpr (GPS == 1) a.s = *reinterpret_cast<const uint16_t*>(sp);
       else a.s = *reinterpret_cast<const Packed*>(sp);
@@ -200,16 +222,13 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
     } else {
 #pragma unroll
       for (int r = 0; r < 2 * kRb; ++r) {
-        const uint8_t* p = wr[r] + st * (kStep / 2);
-        a.w[r] = make_uint4(0, 0, 0, 0);
-        if (st * kStep + 32 * t < wp.K) {
-          if (wp.vec_w) {
-            a.w[r] = __ldg(reinterpret_cast<const uint4*>(p));
-          } else {
-            uint8_t* b = reinterpret_cast<uint8_t*>(&a.w[r]);
+        uint8_t* b = reinterpret_cast<uint8_t*>(&a.w[r]);
+        const uint8_t* p = wr[r] + st * (kStep / 2) - word_k<GPS>(0, t) / 2;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) b[i] = p[i];
-          }
+        for (int w = 0; w < 4; ++w) {
+          const int k = word_k<GPS>(w, t);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) b[4 * w + i] = st * kStep + k < wp.K ? p[k / 2 + i] : 0;
         }
       }
       a.s = 0;
@@ -243,7 +262,7 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
       const int n = min(wp.chunk, wp.per - l0);
 #pragma unroll 2
       for (int i = x_from; i < n; i += apart)
-        f(to + i * step_bytes, x_m, (first + l0 + i) * kStep + 32 * (c & 3) + 8 * (c >> 2));
+        f(to + i * step_bytes, x_m, (first + l0 + i) * kStep + word_k<GPS>(c >> 2, c & 3));
     };
     if (FAST || wp.vec_x) {
       each([&](uint8_t* to, int m, int k) {  // zeros past K
@@ -288,55 +307,42 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
 
     // one step, with what `a` brought; then a's place is filled again
     auto take = [&](Ahead& a, int at) {
-      Zero<T> zr[2 * kRb] = {};
-      if constexpr (ZEROS) {
-#pragma unroll
-        for (int r = 0; r < 2 * kRb; ++r)  // a lane's 32 weights lie in one group
-          zr[r] = Zero<T>(__shfl_sync(0xFFFFFFFFu, a.z, (lane & 28) + r) >> (8 * (t * GPS / 4)) & 0xFFu);
-      }
-      float c[GPS][kRb][NT][4];
+      float c[kRb][NT][4];
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
+        const int q = w * GPS / 4;  // the word's group
+        const bool opens = w % (4 / GPS) == 0, closes = (w + 1) % (4 / GPS) == 0;
         uint32_t k[2 * kRb][4];
 #pragma unroll
         for (int r = 0; r < 2 * kRb; ++r) {
+          Zero<T> zero;
+          if constexpr (ZEROS) zero = Zero<T>(__shfl_sync(0xFFFFFFFFu, a.z, (lane & 28) + r) >> (8 * q) & 0xFFu);
           const uint32_t word = w == 0 ? a.w[r].x : w == 1 ? a.w[r].y : w == 2 ? a.w[r].z : a.w[r].w;
-          weights8<T>(word, zr[r], bits, k[r]);
+          weights8<T>(word, zero, bits, k[r]);
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const uint4 x = *reinterpret_cast<const uint4*>((w & 1 ? x_odd[nt] : x_even[nt]) + at + 64 * w);
 #pragma unroll
-          for (int q = 0; q < GPS; ++q) {
-            // with several groups in the step, x of the other groups' lanes is left
-            // out: a code times 0 is 0
-            const bool in = GPS == 1 || t * GPS / 4 == q;
-            const uint32_t x0 = in ? x.x : 0u, x1 = in ? x.y : 0u, x2 = in ? x.z : 0u, x3 = in ? x.w : 0u;
-#pragma unroll
-            for (int b = 0; b < kRb; ++b) {
-              const uint32_t a0[4] = {k[2 * b][0], k[2 * b + 1][0], k[2 * b][1], k[2 * b + 1][1]};
-              const uint32_t a1[4] = {k[2 * b][2], k[2 * b + 1][2], k[2 * b][3], k[2 * b + 1][3]};
-              if (w == 0)
-                mma_16816<T, true>(c[q][b][nt], a0, x0, x1);
-              else
-                mma_16816<T, false>(c[q][b][nt], a0, x0, x1);
-              mma_16816<T, false>(c[q][b][nt], a1, x2, x3);
-            }
+          for (int b = 0; b < kRb; ++b) {
+            const uint32_t a0[4] = {k[2 * b][0], k[2 * b + 1][0], k[2 * b][1], k[2 * b + 1][1]};
+            const uint32_t a1[4] = {k[2 * b][2], k[2 * b + 1][2], k[2 * b][3], k[2 * b + 1][3]};
+            if (opens)
+              mma_16816<T, true>(c[b][nt], a0, x.x, x.y);
+            else
+              mma_16816<T, false>(c[b][nt], a0, x.x, x.y);
+            mma_16816<T, false>(c[b][nt], a1, x.z, x.w);
           }
         }
-      }
+        if (!closes) continue;
 #pragma unroll
-      for (int r = 0; r < 2 * kRb; ++r) {
-        const Packed four = __shfl_sync(0xFFFFFFFFu, a.s, (lane & 28) + r);
-#pragma unroll
-        for (int q = 0; q < GPS; ++q) {
-          const uint16_t h = static_cast<uint16_t>(four >> (16 * q));
+        for (int r = 0; r < 2 * kRb; ++r) {
+          const uint16_t h = static_cast<uint16_t>(__shfl_sync(0xFFFFFFFFu, a.s, (lane & 28) + r) >> (16 * q));
           const float sc = h2f<T>(*reinterpret_cast<const T*>(&h));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-              acc[r / 2][nt][2 * (r & 1) + e] = fmaf(sc, c[q][r / 2][nt][2 * (r & 1) + e], acc[r / 2][nt][2 * (r & 1) + e]);
+            for (int e = 2 * (r & 1); e < 2 * (r & 1) + 2; ++e) acc[r / 2][nt][e] = fmaf(sc, c[r / 2][nt][e], acc[r / 2][nt][e]);
         }
       }
       fetch(a);
@@ -429,7 +435,7 @@ __global__ void __launch_bounds__(kWarps * 32, GPS * NT <= 2 ? 2 : 1) w4_kernel(
 template <typename T, int NT, int GPS, bool ZEROS, bool FAST>
 cudaError_t launch(W4Params wp, cudaStream_t s) {
   constexpr int kRows = Form<NT>::kRows, kRed = kWarps * 8 * NT * kRows * 4;
-  constexpr int kCtas = GPS * NT <= 2 ? 2 : 1;  // an SM
+  constexpr int kCtas = Form<NT>::kCtas;
   const int toks = std::min(8 * NT, wp.M), step_bytes = toks * 2 * kStep;
   const int steps = (wp.K + kStep - 1) / kStep, tiles = (wp.N - 1) / kRows + 1;
   const int y = (wp.M - 1) / (8 * NT) + 1;
