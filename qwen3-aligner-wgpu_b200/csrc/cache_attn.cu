@@ -7,40 +7,13 @@
 // lse = log sum_c exp(s_c); a row that sees nothing gets 0 and -inf.
 #include <algorithm>
 
+#include "cache_attn.cuh"
 #include "gemm_tc.cuh"
-#include "kernels.cuh"
-#include "sm100.cuh"
 #include "tma_host.h"
 
 namespace qa {
 
 namespace {
-
-constexpr int kPage = 64;
-constexpr int kMaxCtasPerSm = 3;
-constexpr int kMaxParts = 1024;  // parts of a unit
-
-struct CacheAttnParams {
-  const void* q;
-  long long ldq, T;
-  int nq, nkv;
-  SeqMap seqs;
-  const uint8_t *kpool, *vpool;
-  int kv_pages;
-  const float *kscale, *vscale;
-  float scale;
-  int causal;
-  void* out;
-  long long ldo;
-  float* lse;
-  int vec;      // q and out rows can be read and written 16 bytes at a time
-  int tiles_max;       // tiles of a sequence of max_q tokens
-  float* parts;        // workspace: the units' parts, part_stride floats each
-  long long cap_units; // units that have a place in the workspace
-  int cap_parts;       // parts a unit has place for
-  int part_rows, part_stride;
-  unsigned* status;
-};
 
 // ------------------------------------------------------------ few query rows
 // A query row is one (new token, head of the K/V head's group); row r of a
@@ -79,16 +52,12 @@ struct CacheAttnParams {
 // power of two that brings its largest component to [2^14, 2^15): what falls
 // into f16's subnormals lies 2^-39 below that.  P is rounded to f16.
 //
-// Softmax in base 2 with x = s log2(e): the running reference M of a row is
-// over x + log2(vscale), so the page's scale goes into the exponent and P . V
-// needs no scaling:  p = 2^(x + log2 vscale + kLift - M),  O = sum p vcode,
-// l = sum p / vscale,  out = O / l.  M moves only when a value exceeds it by
-// 2^kSlack (any reference gives the same quotient), so a slab usually needs one
-// vote instead of a maximum across lanes; kLift keeps the small p of a long
-// cache out of f16's subnormals and kLift + kSlack below its largest value.
+// As M moves rarely, a slab usually needs one vote instead of a maximum across
+// lanes.
+constexpr int kMaxCtasPerSm = 3;
+constexpr int kMaxParts = 1024;  // parts of a unit
+
 constexpr int kWarps = 4;
-constexpr float kLift = 8.0f, kSlack = 6.0f;
-constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
@@ -106,40 +75,10 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   return d;
 }
 
-// Four e4m3 codes (low byte first) as two f16x2; NaN codes stay NaN.
-__device__ __forceinline__ void e4m3x4_f16x2(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
-      "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-      : "=r"(lo), "=r"(hi) : "r"(w));
-}
-__device__ __forceinline__ float lg2_approx(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
-}
-
-// Base-2 logarithm and reciprocal of a page's V scale; a scale of 0 (a page of
-// zeros written by someone else) counts as 2^-100.
-__device__ __forceinline__ float usable_vscale(float v) { return fmaxf(v, 7.8886090522101181e-31f); }
-
-// Four output values of a row.
-template <typename T>
-__device__ __forceinline__ void store4(T* p, float4 v, bool vec) {
-  const uint32_t a = cvt2_rn<T>(make_float2(v.x, v.y)), b = cvt2_rn<T>(make_float2(v.z, v.w));
-  if (vec) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(a, b);
-  } else {
-    const uint32_t w[2] = {a, b};
-    const T* e = reinterpret_cast<const T*>(w);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = e[i];
-  }
 }
 
 // Tokens of a chunk of a unit of `tokens` tokens, a multiple of 32.  Short units
@@ -235,112 +174,15 @@ struct Walk {
   }
 };
 
-// A tile's rows of one sequence and K/V head.
-struct UnitAt {
-  int s, tile, h;
-  long long t0;  // the sequence's first row of q and out
+// The parts that this kernel leaves, for the join.
+template <int R, int TEAM, int SLAB>
+struct RowsPlan {
+  static constexpr int kRows = R;
+  __device__ static int parts(const CacheAttnParams& ap, const SeqSpan& sp, int s, int) {
+    const int n = seq_plan(ap, sp, s, ap.nq / ap.nkv, R, TEAM, SLAB).chunks;
+    return n > 1 ? n : 0;
+  }
 };
-
-__device__ __forceinline__ float* unit_parts(const CacheAttnParams& ap, const UnitAt& at) {
-  const long long u = (static_cast<long long>(at.s) * ap.tiles_max + at.tile) * ap.nkv + at.h;
-  return ap.parts + u * ap.cap_parts * ap.part_stride;
-}
-
-// Row `row` of a sequence is done: its lse; returns what its O is multiplied by.
-__device__ __forceinline__ float close_row(const CacheAttnParams& ap, const UnitAt& at, int row,
-                                           float big, float sum) {
-  const int group = ap.nq / ap.nkv;
-  if (ap.lse)
-    ap.lse[(at.t0 + row / group) * ap.nq + at.h * group + row % group] =
-        sum == 0.0f ? -INFINITY : (big - kLift + log2f(sum)) * 0.69314718055994531f;
-  return sum == 0.0f ? 0.0f : 1.0f / sum;
-}
-
-template <typename T, int HD>
-__device__ __forceinline__ void finish_row(const CacheAttnParams& ap, const UnitAt& at, int row, int dim,
-                                           float4 v, float inv) {
-  const int group = ap.nq / ap.nkv;
-  store4(static_cast<T*>(ap.out) + (at.t0 + row / group) * ap.ldo +
-             static_cast<long long>(at.h * group + row % group) * HD + dim,
-         make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), ap.vec);
-}
-
-// Joins the parts of the units of more than one chunk, a CTA a row: each of its
-// warps sums every kJoinWarps-th part (four dims a lane; hd 64: two parts at a
-// time), then the warps are summed, in an order that only the number of parts
-// sets.  Bound by latency: a part's row is one line of 4 hd bytes.
-constexpr int kJoinWarps = 8;
-
-template <typename T, int HD, int R, int TEAM, int SLAB>
-__global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const __grid_constant__ CacheAttnParams ap) {
-  constexpr int kLanes = HD / 4, kAtOnce = 32 / kLanes * kJoinWarps;  // lanes of a part, parts at once
-  __shared__ float s_red[kJoinWarps], s_sum[kJoinWarps];
-  __shared__ float4 s_o[kAtOnce][kLanes];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.y, s = blockIdx.x / ap.tiles_max, tile = blockIdx.x % ap.tiles_max, r = blockIdx.z;
-  pdl_wait();
-  pdl_trigger();
-  const int group = ap.nq / ap.nkv;
-  const SeqSpan sp = seq_span(ap.seqs, s, ap.T);
-  const SeqPlan plan = seq_plan(ap, sp, s, group, R, TEAM, SLAB);
-  if (plan.chunks == 1 || tile >= plan.tiles || tile * R + r >= sp.n * group) return;
-  const UnitAt at{s, tile, h, sp.t0};
-  const float* parts = unit_parts(ap, at);
-  const int l_at = (ap.part_rows + 3) & ~3, o_at = 2 * l_at + r * HD;
-  const int n = plan.chunks, first = threadIdx.x / kLanes, d = threadIdx.x % kLanes;
-  float big = -INFINITY;
-  for (int k = threadIdx.x; k < n; k += kJoinWarps * 32) big = fmaxf(big, parts[static_cast<long long>(k) * ap.part_stride + r]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
-  if (lane == 0) s_red[warp] = big;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) big = fmaxf(big, s_red[w]);
-  const float ref = big == -INFINITY ? 0.0f : big;
-  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float sum = 0.0f;
-  constexpr int kBatch = 8;  // parts whose loads are in flight together
-  for (int k0 = first; k0 < n; k0 += kBatch * kAtOnce) {
-    float4 y[kBatch];
-    float pm[kBatch], pl[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int k = k0 + i * kAtOnce;
-      const float* part = parts + static_cast<long long>(min(k, n - 1)) * ap.part_stride;
-      y[i] = __ldcg(reinterpret_cast<const float4*>(part + o_at + 4 * d));
-      pm[i] = __ldcg(part + r);
-      pl[i] = __ldcg(part + l_at + r);
-    }
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-      if (k0 + i * kAtOnce < n) {
-        const float a = ex2_approx(pm[i] - ref);
-        sum = fmaf(a, pl[i], sum);
-        v = make_float4(fmaf(a, y[i].x, v.x), fmaf(a, y[i].y, v.y), fmaf(a, y[i].z, v.z), fmaf(a, y[i].w, v.w));
-      }
-  }
-  s_o[first][d] = v;
-  // each part's sum once: from the first lane of its kLanes
-  if (d != 0) sum = 0.0f;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-  if (lane == 0) s_sum[warp] = sum;
-  __syncthreads();
-  if (threadIdx.x < kLanes) {
-    sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) sum += s_sum[w];
-    v = s_o[0][d];
-#pragma unroll
-    for (int k = 1; k < kAtOnce; ++k) {
-      const float4 y = s_o[k][d];
-      v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
-    }
-    const int row = tile * R + r;
-    if (d == 0) close_row(ap, at, row, big, sum);
-    finish_row<T, HD>(ap, at, row, 4 * d, v, sum == 0.0f ? 0.0f : 1.0f / sum);
-  }
-}
 
 // Tokens of a slab: the more of them, the more independent work a warp has
 // between two waits and the fewer instructions a token, as far as the registers
@@ -889,7 +731,7 @@ done:
 }
 
 // Rows of a tile of the few-row kernel for sequences of up to `rows` rows.
-int tile_rows(long long rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 24 ? 24 : 32; }
+int tile_rows(long long rows) { return rows <= 8 ? 8 : 16; }
 
 // The workspace of a unit, for caches of up to max_kv tokens.
 struct PartSizes {
@@ -960,7 +802,7 @@ cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int ma
   if (e == cudaSuccess && ps.parts > 1 && ap.cap_units > 0) {
     const long long x = static_cast<long long>(ap.seqs.n_seqs) * ps.tiles;
     if (x > 0x7FFFFFFFll || ap.nkv > 65535) return cudaErrorInvalidValue;
-    e = launch_pdl(cache_attn_join<T, HD, R, kTeam, kSlab>, dim3(static_cast<unsigned>(x), ap.nkv, ps.rows),
+    e = launch_pdl(cache_attn_join<T, HD, RowsPlan<R, kTeam, kSlab>>, dim3(static_cast<unsigned>(x), ap.nkv, ps.rows),
                    dim3(kJoinWarps * 32), 0, s, ap);
   }
   return e;
@@ -968,22 +810,37 @@ cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int ma
 
 template <typename T, int HD>
 cudaError_t launch_any(const CacheAttnParams& ap, void* ws, long long ws_bytes, int max_kv, cudaStream_t s) {
-  switch (tile_rows(static_cast<long long>(ap.seqs.max_q) * (ap.nq / ap.nkv))) {
-    case 8: return launch_rows<T, HD, 1>(ap, ws, ws_bytes, max_kv, s);
-    case 16: return launch_rows<T, HD, 2>(ap, ws, ws_bytes, max_kv, s);
-    case 24: return launch_rows<T, HD, 3>(ap, ws, ws_bytes, max_kv, s);
-    default: return launch_rows<T, HD, 4>(ap, ws, ws_bytes, max_kv, s);
-  }
+  if (tile_rows(static_cast<long long>(ap.seqs.max_q) * (ap.nq / ap.nkv)) == 8)
+    return launch_rows<T, HD, 1>(ap, ws, ws_bytes, max_kv, s);
+  return launch_rows<T, HD, 2>(ap, ws, ws_bytes, max_kv, s);
 }
+
+// Rows of a K/V head and sequence up to which the few-row kernel is used.
+constexpr int kFewRows = 16;
 
 }  // namespace
 
-long long cache_attention_workspace(int nqh, int nkvh, int hd, int n_seqs, int max_q, int max_kv) {
-  if (nkvh <= 0 || nqh < nkvh || n_seqs <= 0 || max_q <= 0) return 0;
+long long cache_rows_workspace(int nqh, int nkvh, int hd, int n_seqs, int max_q, int max_kv) {
   const PartSizes p = part_sizes(nqh, nkvh, hd, max_q, max_kv);
   if (p.parts == 1) return 0;
-  const long long units = static_cast<long long>(n_seqs) * p.tiles * nkvh;
-  return std::min(units * p.unit_bytes, 1ll << 30);
+  return static_cast<long long>(n_seqs) * p.tiles * nkvh * p.unit_bytes;
+}
+
+int cache_attention_rows(const CacheAttnParams& ap, int hd, bool bf16, int max_kv, void* ws,
+                         long long ws_bytes, cudaStream_t s) {
+  if (bf16)
+    return hd == 128 ? launch_any<__nv_bfloat16, 128>(ap, ws, ws_bytes, max_kv, s)
+                     : launch_any<__nv_bfloat16, 64>(ap, ws, ws_bytes, max_kv, s);
+  return hd == 128 ? launch_any<__half, 128>(ap, ws, ws_bytes, max_kv, s)
+                   : launch_any<__half, 64>(ap, ws, ws_bytes, max_kv, s);
+}
+
+long long cache_attention_workspace(int nqh, int nkvh, int hd, int n_seqs, int max_q, int max_kv) {
+  if (nkvh <= 0 || nqh < nkvh || n_seqs <= 0 || max_q <= 0) return 0;
+  const bool few = static_cast<long long>(max_q) * (nqh / nkvh) <= kFewRows;
+  const long long bytes = few ? cache_rows_workspace(nqh, nkvh, hd, n_seqs, max_q, max_kv)
+                              : cache_tiles_workspace(nqh, nkvh, hd, n_seqs, max_q, max_kv);
+  return std::min(bytes, 1ll << 30);
 }
 
 int cache_attention(const void* q, long long ldq, long long T, int nqh, int nkvh, int hd,
@@ -1013,14 +870,10 @@ int cache_attention(const void* q, long long ldq, long long T, int nqh, int nkvh
   ap.status = status;
   ap.vec = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 == 0) &&
            ((ldq | ldo) % 8 == 0);
-  cudaError_t e;
-  if (bf16)
-    e = hd == 128 ? launch_any<__nv_bfloat16, 128>(ap, workspace, workspace_bytes, max_kv, s)
-                  : launch_any<__nv_bfloat16, 64>(ap, workspace, workspace_bytes, max_kv, s);
-  else
-    e = hd == 128 ? launch_any<__half, 128>(ap, workspace, workspace_bytes, max_kv, s)
-                  : launch_any<__half, 64>(ap, workspace, workspace_bytes, max_kv, s);
-  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+  const bool few = static_cast<long long>(max_q) * (nqh / nkvh) <= kFewRows;
+  const int rc = few ? cache_attention_rows(ap, hd, bf16, max_kv, workspace, workspace_bytes, s)
+                     : cache_attention_tiles(ap, hd, bf16, max_kv, workspace, workspace_bytes, s);
+  return rc ? rc : (int)cudaGetLastError();
 }
 
 }  // namespace qa

@@ -1,0 +1,195 @@
+// What the two kernels of cache_attention share: its parameters, the codes'
+// conversion, where results go, and the kernel that joins the parts of a sequence.
+#pragma once
+
+#include "kernels.cuh"
+#include "sm100.cuh"
+
+namespace qa {
+
+struct CacheAttnParams {
+  const void* q;
+  long long ldq, T;
+  int nq, nkv;
+  SeqMap seqs;
+  const uint8_t *kpool, *vpool;
+  int kv_pages;
+  const float *kscale, *vscale;
+  float scale;
+  int causal;
+  void* out;
+  long long ldo;
+  float* lse;
+  int vec;      // q and out rows can be read and written 16 bytes at a time
+  int tiles_max;       // tiles of a sequence of max_q tokens
+  float* parts;        // workspace: the units' parts, part_stride floats each
+  long long cap_units; // units that have a place in the workspace
+  int cap_parts;       // parts a unit has place for
+  int part_rows, part_stride;
+  unsigned* status;
+};
+
+namespace {
+
+constexpr int kPage = 64;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Softmax in base 2 with x = s log2(e): the running reference M of a row is over
+// x + log2(vscale), so the page's scale goes into the exponent and P . V needs no
+// scaling:  p = 2^(x + log2 vscale + kLift - M),  O = sum p vcode,
+// l = sum p / vscale,  out = O / l.  M moves only when a value exceeds it by
+// 2^kSlack (any reference gives the same quotient); kLift keeps the small p of a
+// long cache out of f16's subnormals, and 2^(kLift + kSlack) is below its largest
+// value.
+constexpr float kLift = 8.0f, kSlack = 6.0f;
+
+
+// Four e4m3 codes (low byte first) as two f16x2; NaN codes stay NaN.
+__device__ __forceinline__ void e4m3x4_f16x2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Base-2 logarithm and reciprocal of a page's V scale; a scale of 0 (a page of
+// zeros written by someone else) counts as 2^-100.
+__device__ __forceinline__ float usable_vscale(float v) { return fmaxf(v, 7.8886090522101181e-31f); }
+
+// Four output values of a row.
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float4 v, bool vec) {
+  const uint32_t a = cvt2_rn<T>(make_float2(v.x, v.y)), b = cvt2_rn<T>(make_float2(v.z, v.w));
+  if (vec) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(a, b);
+  } else {
+    const uint32_t w[2] = {a, b};
+    const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = e[i];
+  }
+}
+
+// A tile's rows of one sequence and K/V head.
+struct UnitAt {
+  int s, tile, h;
+  long long t0;  // the sequence's first row of q and out
+};
+
+__device__ __forceinline__ float* unit_parts(const CacheAttnParams& ap, const UnitAt& at) {
+  const long long u = (static_cast<long long>(at.s) * ap.tiles_max + at.tile) * ap.nkv + at.h;
+  return ap.parts + u * ap.cap_parts * ap.part_stride;
+}
+
+// Row `row` of a sequence is done: its lse; returns what its O is multiplied by.
+__device__ __forceinline__ float close_row(const CacheAttnParams& ap, const UnitAt& at, int row,
+                                           float big, float sum) {
+  const int group = ap.nq / ap.nkv;
+  if (ap.lse)
+    ap.lse[(at.t0 + row / group) * ap.nq + at.h * group + row % group] =
+        sum == 0.0f ? -INFINITY : (big - kLift + log2f(sum)) * 0.69314718055994531f;
+  return sum == 0.0f ? 0.0f : 1.0f / sum;
+}
+
+template <typename T, int HD>
+__device__ __forceinline__ void finish_row(const CacheAttnParams& ap, const UnitAt& at, int row, int dim,
+                                           float4 v, float inv) {
+  const int group = ap.nq / ap.nkv;
+  store4(static_cast<T*>(ap.out) + (at.t0 + row / group) * ap.ldo +
+             static_cast<long long>(at.h * group + row % group) * HD + dim,
+         make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), ap.vec);
+}
+
+// Joins the parts of the units that left any (Plan::parts), a CTA a row: each of its
+// warps sums every kJoinWarps-th part (four dims a lane; hd 64: two parts at a
+// time), then the warps are summed, in an order that only the number of parts
+// sets.  Bound by latency: a part's row is one line of 4 hd bytes.
+constexpr int kJoinWarps = 8;
+
+template <typename T, int HD, typename Plan>
+__global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const __grid_constant__ CacheAttnParams ap) {
+  constexpr int kLanes = HD / 4, kAtOnce = 32 / kLanes * kJoinWarps;  // lanes of a part, parts at once
+  __shared__ float s_red[kJoinWarps], s_sum[kJoinWarps];
+  __shared__ float4 s_o[kAtOnce][kLanes];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.y, s = blockIdx.x / ap.tiles_max, tile = blockIdx.x % ap.tiles_max, r = blockIdx.z;
+  pdl_wait();
+  pdl_trigger();
+  const int group = ap.nq / ap.nkv;
+  const SeqSpan sp = seq_span(ap.seqs, s, ap.T);
+  if (!sp.ok || tile * Plan::kRows + r >= sp.n * group) return;
+  const int n = Plan::parts(ap, sp, s, tile);
+  if (n == 0) return;
+  const UnitAt at{s, tile, h, sp.t0};
+  const float* parts = unit_parts(ap, at);
+  const int l_at = (ap.part_rows + 3) & ~3, o_at = 2 * l_at + r * HD;
+  const int first = threadIdx.x / kLanes, d = threadIdx.x % kLanes;
+  float big = -INFINITY;
+  for (int k = threadIdx.x; k < n; k += kJoinWarps * 32) big = fmaxf(big, parts[static_cast<long long>(k) * ap.part_stride + r]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+  if (lane == 0) s_red[warp] = big;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) big = fmaxf(big, s_red[w]);
+  const float ref = big == -INFINITY ? 0.0f : big;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float sum = 0.0f;
+  constexpr int kBatch = 8;  // parts whose loads are in flight together
+  for (int k0 = first; k0 < n; k0 += kBatch * kAtOnce) {
+    float4 y[kBatch];
+    float pm[kBatch], pl[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int k = k0 + i * kAtOnce;
+      const float* part = parts + static_cast<long long>(min(k, n - 1)) * ap.part_stride;
+      y[i] = __ldcg(reinterpret_cast<const float4*>(part + o_at + 4 * d));
+      pm[i] = __ldcg(part + r);
+      pl[i] = __ldcg(part + l_at + r);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (k0 + i * kAtOnce < n) {
+        const float a = ex2_approx(pm[i] - ref);
+        sum = fmaf(a, pl[i], sum);
+        v = make_float4(fmaf(a, y[i].x, v.x), fmaf(a, y[i].y, v.y), fmaf(a, y[i].z, v.z), fmaf(a, y[i].w, v.w));
+      }
+  }
+  s_o[first][d] = v;
+  // each part's sum once: from the first lane of its kLanes
+  if (d != 0) sum = 0.0f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  if (threadIdx.x < kLanes) {
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) sum += s_sum[w];
+    v = s_o[0][d];
+#pragma unroll
+    for (int k = 1; k < kAtOnce; ++k) {
+      const float4 y = s_o[k][d];
+      v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
+    }
+    const int row = tile * Plan::kRows + r;
+    if (d == 0) close_row(ap, at, row, big, sum);
+    finish_row<T, HD>(ap, at, row, 4 * d, v, sum == 0.0f ? 0.0f : 1.0f / sum);
+  }
+}
+
+}  // namespace
+
+// The two kernels' launches, and the workspace that each asks for.
+int cache_attention_rows(const CacheAttnParams& ap, int hd, bool bf16, int max_kv, void* ws,
+                         long long ws_bytes, cudaStream_t s);
+int cache_attention_tiles(const CacheAttnParams& ap, int hd, bool bf16, int max_kv, void* ws,
+                          long long ws_bytes, cudaStream_t s);
+long long cache_rows_workspace(int nqh, int nkvh, int hd, int n_seqs, int max_q, int max_kv);
+long long cache_tiles_workspace(int nqh, int nkvh, int hd, int n_seqs, int max_q, int max_kv);
+
+}  // namespace qa

@@ -1,0 +1,824 @@
+// Attention over the 8-bit paged cache for many query rows, on the tcgen05 tensor
+// cores (the formulas: cache_attn.cu; the softmax's references: cache_attn.cuh).
+//
+// A unit is one K/V head of one sequence and up to 256 rows (row r is new token
+// r / group, head r % group), two M = 128 tiles; its key tiles hold 128 cached
+// tokens.  The kernel is persistent, one CTA an SM, and has two streams of
+//   S_h = Q K^T (M 128, N 128, K hd),  softmax,  O_h += P V (N hd, K 128 keys)
+// so that one stream's products run while the other one's softmax does:
+//  - a unit of more than 128 rows: a stream for each tile, sharing every key tile;
+//  - otherwise: both streams have the same tile, one the even key tiles and one
+//    the odd ones, each with its own reference, sum and O, which the join puts
+//    together (half the time a key tile, which is what bounds few rows: a stream
+//    alone takes longer over 128 keys than the SM's share of the memory does).
+//
+//   warps 0-3    queries to f16 (bf16 ones scaled by a power of two per row:
+//                exact) and K, V codes to f16 (exact) in shared memory, 128-byte
+//                swizzled; a thread has its 128 bytes of the next key tile's K and
+//                V on their way while it converts this one's;
+//   warp 4       tensor memory and the MMAs;
+//   warps 5-12   softmax of the streams, one row a thread, and the results.
+//
+// Tokens past a sequence's end become zeros.  0 . NaN is NaN: in key tiles that
+// some rows see only part of, NaN codes of V are taken out, and the softmax threads
+// put NaN into the results of the rows that do see them.
+//
+// TMEM: S_h (P_h over it) at 128 h, O_h at 256 + 128 h.
+#include <algorithm>
+
+#include "cache_attn.cuh"
+#include "gemm_tc.cuh"
+
+namespace qa {
+
+namespace {
+
+constexpr int kRows = 128;      // of an MMA tile
+constexpr int kUnitRows = 256;
+constexpr int kKeys = 128;
+constexpr int kConvWarps = 4, kSoftWarps = 8;
+constexpr int kConv = kConvWarps * 32;
+constexpr int kThreads = (kConvWarps + 1 + kSoftWarps) * 32;
+constexpr uint32_t kHalf = kRows * 128;  // 64 f16 columns of a tile
+constexpr uint32_t kTmemCols = 512;
+constexpr int kMinStep = 8;    // key tiles of a chunk, at least
+constexpr int kMaxChunks = 16;
+constexpr uint32_t kStage = 4096;  // per softmax warp: 32 rows of 64 output columns
+
+// Key tiles of a chunk of a sequence with `keys` key tiles and `tiles` units a
+// head: enough chunks to fill the GPU from one sequence, as few as that takes.
+__host__ __device__ __forceinline__ int chunk_step(int keys, int tiles) {
+  const int want = kMaxChunks / tiles > 1 ? kMaxChunks / tiles : 1;
+  const int step = (keys + want - 1) / want;
+  return step > kMinStep ? step : kMinStep;
+}
+
+struct TilePlan {
+  int tiles, step;
+};
+__device__ __forceinline__ TilePlan tile_plan(const CacheAttnParams& ap, const SeqSpan& sp) {
+  const int group = ap.nq / ap.nkv;
+  TilePlan p;
+  p.tiles = sp.ok ? (sp.n * group + kUnitRows - 1) / kUnitRows : 0;
+  p.step = chunk_step(max(1, (sp.len + kKeys - 1) / kKeys), max(1, p.tiles));
+  return p;
+}
+
+// One unit's tile of rows.
+struct Unit {
+  int rows, seen;    // rows; tokens that its last row sees
+  int keys;          // key tiles, at least one: a row that sees nothing still gets zeros
+  int step, chunks;  // key tiles of a chunk, chunks
+  bool pair;         // two tiles of rows, or no place for parts: streams are tiles
+};
+__device__ __forceinline__ Unit unit_of(const CacheAttnParams& ap, const SeqSpan& sp, const TilePlan& p,
+                                        int s, int tile) {
+  const int group = ap.nq / ap.nkv;
+  Unit u;
+  u.rows = min(kUnitRows, sp.n * group - tile * kUnitRows);
+  const int last = (tile * kUnitRows + u.rows - 1) / group;
+  u.seen = ap.causal ? min(sp.len, max(0, sp.len - sp.n + last + 1)) : sp.len;
+  u.keys = max(1, (u.seen + kKeys - 1) / kKeys);
+  u.step = p.step;
+  u.chunks = (u.keys + u.step - 1) / u.step;
+  u.pair = u.rows > kRows;
+  if ((u.pair ? u.chunks : 2 * u.chunks) > ap.cap_parts ||
+      static_cast<long long>(s + 1) * ap.tiles_max * ap.nkv > ap.cap_units) {
+    u.pair = true;
+    u.chunks = 1;
+    u.step = u.keys;
+  }
+  return u;
+}
+
+// The parts that this kernel leaves, for the join.
+struct TilesPlan {
+  static constexpr int kRows = kUnitRows;
+  __device__ static int parts(const CacheAttnParams& ap, const SeqSpan& sp, int s, int tile) {
+    const Unit u = unit_of(ap, sp, tile_plan(ap, sp), s, tile);
+    return u.pair ? (u.chunks > 1 ? u.chunks : 0) : 2 * u.chunks;
+  }
+};
+
+// One piece of work: a chunk of a unit.
+struct Item {
+  int s, tile, h, chunk;
+  int k0, cnt;  // its key tiles
+};
+
+// A CTA's share: the chunks that begin in it.
+struct TileWalk {
+  long long x, hi;  // first key tile (of all units' laid end to end) not looked at, end of the share
+  Item it;
+  SeqSpan sp;
+  TilePlan plan;
+  Unit u;
+
+  __device__ __forceinline__ void look(const CacheAttnParams& ap) {
+    sp = seq_span(ap.seqs, it.s, ap.T);
+    plan = tile_plan(ap, sp);
+  }
+  __device__ __forceinline__ void begin(const CacheAttnParams& ap, int seq, long long start, long long lo,
+                                        long long end) {
+    x = lo;
+    hi = end;
+    it = Item{seq, 0, 0, 0, 0, 0};
+    look(ap);
+    long long rel = lo - start;
+    for (;; ++it.tile) {  // the share begins in this sequence: its units hold it
+      u = unit_of(ap, sp, plan, it.s, it.tile);
+      const long long c = static_cast<long long>(u.keys) * ap.nkv;
+      if (rel < c) break;
+      rel -= c;
+    }
+    it.h = static_cast<int>(rel / u.keys);
+    const int in = static_cast<int>(rel % u.keys);
+    it.chunk = (in + u.step - 1) / u.step - 1;
+    x += min(u.keys, (it.chunk + 1) * u.step) - in;
+  }
+  __device__ __forceinline__ bool next(const CacheAttnParams& ap) {
+    if (x >= hi) return false;
+    if (++it.chunk == u.chunks) {
+      it.chunk = 0;
+      if (++it.h == ap.nkv) {
+        it.h = 0;
+        ++it.tile;
+        while (it.tile >= plan.tiles) {  // x < hi <= all key tiles: there is another unit
+          ++it.s;
+          it.tile = 0;
+          look(ap);
+        }
+        u = unit_of(ap, sp, plan, it.s, it.tile);
+      }
+    }
+    it.k0 = it.chunk * u.step;
+    it.cnt = min(u.step, u.keys - it.k0);
+    x += it.cnt;
+    return true;
+  }
+};
+
+// A piece of work as the warps read it, from shared memory.
+struct Work {
+  long long t0;      // the sequence's first row of q and out
+  const int* bt;     // its pages
+  float* parts;      // where this chunk's (first) part goes; null: results are final
+  int s, tile, h;
+  int row0, rows;    // the unit's first row in the sequence, its rows
+  int len, past;     // cached tokens; past + i + 1 of them are seen by new token i when causal
+  int seen, all;     // tokens seen by the last row, by every row
+  int k0, cnt;       // key tiles
+  bool pair;
+  // jobs of stream h, and the key tile (of the item) of its k-th
+  __device__ __forceinline__ int jobs(int st) const {
+    return pair ? (st == 0 || rows > kRows ? cnt : 0) : (cnt + 1 - st) / 2;
+  }
+  __device__ __forceinline__ int key_tile(int st, int k) const { return pair ? k : 2 * k + st; }
+  // whether stream st is the last to use a key tile
+  __device__ __forceinline__ bool last_user(int st) const { return !pair || st == 1 || rows <= kRows; }
+};
+constexpr int kBatch = 4;  // pieces of work described at a time
+
+__device__ __forceinline__ Work work_of(const CacheAttnParams& ap, const TileWalk& walk) {
+  const int group = ap.nq / ap.nkv;
+  const Item& it = walk.it;
+  const Unit& u = walk.u;
+  Work w;
+  w.t0 = walk.sp.t0;
+  w.bt = ap.seqs.block_tab + static_cast<long long>(it.s) * ap.seqs.max_pages;
+  w.s = it.s;
+  w.tile = it.tile;
+  w.h = it.h;
+  w.row0 = it.tile * kUnitRows;
+  w.rows = u.rows;
+  w.len = walk.sp.len;
+  w.past = walk.sp.len - walk.sp.n;
+  w.seen = u.seen;
+  w.all = ap.causal ? min(w.len, max(0, w.past + w.row0 / group + 1)) : w.len;
+  w.k0 = it.k0;
+  w.cnt = it.cnt;
+  w.pair = u.pair;
+  w.parts = u.pair && u.chunks == 1
+                ? nullptr
+                : unit_parts(ap, UnitAt{it.s, it.tile, it.h, w.t0}) +
+                      (u.pair ? it.chunk : 2 * it.chunk) * static_cast<long long>(ap.part_stride);
+  return w;
+}
+
+template <int HD>
+struct Mem {
+  static constexpr uint32_t kTile = kHalf * (HD / 64);  // Q, K or V
+  static constexpr size_t kSmem = 6 * kTile + kSoftWarps * kStage + 2 * kUnitRows * 4 + 512 + kBatch * sizeof(Work);
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_constant__ CacheAttnParams ap) {
+  constexpr uint32_t kTile = Mem<HD>::kTile;
+  constexpr int kCpr = HD / 16;           // 16-byte units of codes a row
+  constexpr int kIter = kRows * kCpr / kConv;  // units of a tile a conversion thread
+  extern __shared__ __align__(1024) uint8_t smem[];  // no room to align it by hand
+  static_assert(Mem<HD>::kSmem <= 232448, "shared memory of a CTA");
+  uint8_t* sQ = smem;              // [tile]
+  uint8_t* sK = sQ + 2 * kTile;    // [slot]
+  uint8_t* sV = sK + 2 * kTile;    // [slot]
+  uint8_t* stage = sV + 2 * kTile; // [softmax warp]
+  float* s_undo = reinterpret_cast<float*>(stage + kSoftWarps * kStage);  // [item & 1][row]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_undo + 2 * kUnitRows);
+  uint64_t* q_full = bars + 0;   // [item & 1] queries and their factors are there
+  uint64_t* q_free = bars + 2;   // the item's last S is done
+  uint64_t* k_full = bars + 4;   // [slot]
+  uint64_t* k_empty = bars + 6;
+  uint64_t* v_full = bars + 8;
+  uint64_t* v_empty = bars + 10;
+  uint64_t* s_full = bars + 12;  // [stream] S computed
+  uint64_t* p_full = bars + 14;  // [stream] P written over S
+  uint64_t* o_ready = bars + 16; // [stream] P V done
+  uint64_t* o_free = bars + 18;  // [stream] O read
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 20);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tslot + 1);
+  long long* share = reinterpret_cast<long long*>(bars + 22);  // lo, hi, start, sequence
+  long long* scan = share + 4;                                 // [warp]
+  int* staged = reinterpret_cast<int*>(scan + kThreads / 32);  // pieces of work described
+  Work* work = reinterpret_cast<Work*>(bars + 64);             // [kBatch]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = ap.nq / ap.nkv, n_seqs = ap.seqs.n_seqs;
+  if (smem_u32(smem) & 1023u) {  // the swizzled tiles would not be where the MMA looks for them
+    if (threadIdx.x == 0 && ap.status) atomicOr(ap.status, kStatusTimeout);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], kConv);
+      mbar_init(&k_full[i], kConv);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], kConv);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], kRows);
+      mbar_init(&o_ready[i], 1);
+      mbar_init(&o_free[i], kRows);
+    }
+    mbar_init(q_free, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == kConvWarps) tmem_alloc(tslot, kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tslot;
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- this CTA's share: thread i adds up sequences [i c, (i + 1) c)
+  bool any;
+  {
+    const int c = (n_seqs + kThreads - 1) / kThreads;
+    const int s0 = min(n_seqs, static_cast<int>(threadIdx.x) * c), s1 = min(n_seqs, s0 + c);
+    auto cost_of = [&](int s) {
+      const SeqSpan sp = seq_span(ap.seqs, s, ap.T);
+      const TilePlan p = tile_plan(ap, sp);
+      long long sum = 0;
+      for (int t = 0; t < p.tiles; ++t) sum += unit_of(ap, sp, p, s, t).keys;
+      return sum * ap.nkv;
+    };
+    long long mine = 0;
+    for (int s = s0; s < s1; ++s) {
+      mine += cost_of(s);
+      if (blockIdx.x == 0 && ap.status && !seq_span(ap.seqs, s, ap.T).ok) atomicOr(ap.status, kStatusBadShape);
+    }
+    long long before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xFFFFFFFFu, before, o);
+      if (lane >= o) before += y;
+    }
+    if (lane == 31) scan[warp] = before;
+    __syncthreads();
+    long long total = 0;
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    before -= mine;
+    const long long quot = total / gridDim.x, rem = total % gridDim.x, b = blockIdx.x;
+    const long long lo = quot * b + min(b, rem), hi = lo + quot + (b < rem ? 1 : 0);
+    any = lo < hi;
+    if (any && lo >= before && lo < before + mine) {
+      share[0] = lo;
+      share[1] = hi;
+      long long at = before;
+      for (int s = s0; s < s1; ++s) {
+        const long long cost = cost_of(s);
+        if (lo < at + cost) {
+          share[2] = at;
+          share[3] = s;
+          break;
+        }
+        at += cost;
+      }
+    }
+    __syncthreads();
+  }
+  auto fail = [&]() {
+    *abort_flag = 1;
+    if (ap.status) atomicOr(ap.status, kStatusTimeout);
+  };
+  // bounded wait taken by a whole warp, warp-uniform result
+  auto wait = [&](uint64_t* bar, uint32_t par) -> bool {
+    return __all_sync(0xFFFFFFFFu, !*abort_flag && mbar_wait(bar, par & 1u));
+  };
+  auto good = [&](int page) { return page >= 0 && page < ap.kv_pages; };
+  TileWalk walk;  // thread 0's
+  if (threadIdx.x == 0 && any) walk.begin(ap, static_cast<int>(share[3]), share[2], share[0], share[1]);
+  bool ok = true;
+  uint32_t n_it = 0;  // pieces of work before this one
+  uint32_t g = 0;     // key tiles before this one
+  uint32_t uses0 = 0, uses1 = 0, jobs0 = 0, jobs1 = 0;  // of the streams
+  for (;;) {
+    if (threadIdx.x == 0) {
+      int n = 0;
+      while (any && n < kBatch && walk.next(ap)) work[n++] = work_of(ap, walk);
+      *staged = n;
+    }
+    __syncthreads();
+    const int n_work = *staged;
+    if (n_work == 0 || *abort_flag) break;
+  if (warp < kConvWarps) {
+    // ================================================ conversion
+    const int tid = threadIdx.x;
+    const int row0 = tid / kCpr, c = tid % kCpr;  // rows row0 + i kConv / kCpr, unit c of each
+    constexpr int kRowStep = kConv / kCpr;
+    // the two 16-byte halves of a converted unit, f16 dims 16 c .. 16 c + 15 of row r
+    auto put = [&](uint8_t* tile, int r, uint4 lo, uint4 hi) {
+      uint8_t* base = tile + (c >> 2) * kHalf + r * 128;
+      const int u = 2 * (c & 3), sw = r & 7;
+      // lanes of the two halves store their pieces in opposite order: different banks
+      const bool flip = (c >> 2) & 1;
+      *reinterpret_cast<uint4*>(base + 16 * ((u + flip) ^ sw)) = flip ? hi : lo;
+      *reinterpret_cast<uint4*>(base + 16 * ((u + !flip) ^ sw)) = flip ? lo : hi;
+    };
+    for (int wi = 0; ok && wi < n_work; ++wi) {
+      const Work& it = work[wi];
+      const int seen = it.seen, all = it.all, h_kv = it.h;
+      // ---- codes of a key tile, on their way
+      auto load = [&](const uint8_t* pool, int kt, uint4 (&d)[kIter]) {
+        const int key0 = kt * kKeys;
+        int page[2];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          page[p] = key0 + p * kPage < seen ? it.bt[kt * 2 + p] : -1;
+          if (!good(page[p]) && key0 + p * kPage < seen && tid == 0 && ap.status) atomicOr(ap.status, kStatusBadShape);
+        }
+#pragma unroll
+        for (int i = 0; i < kIter; ++i) {
+          const int r = row0 + i * kRowStep, p = i >= kIter / 2;
+          d[i] = make_uint4(0, 0, 0, 0);
+          if (key0 + r < seen && good(page[p]))
+            d[i] = __ldg(reinterpret_cast<const uint4*>(
+                pool + ((static_cast<long long>(page[p]) * ap.nkv + h_kv) * kPage + (r & 63)) * HD + 16 * c));
+        }
+      };
+      auto store = [&](uint8_t* tile, uint4 (&d)[kIter]) {
+#pragma unroll
+        for (int i = 0; i < kIter; ++i) {
+          uint4 lo, hi;
+          e4m3x4_f16x2(d[i].x, lo.x, lo.y);
+          e4m3x4_f16x2(d[i].y, lo.z, lo.w);
+          e4m3x4_f16x2(d[i].z, hi.x, hi.y);
+          e4m3x4_f16x2(d[i].w, hi.z, hi.w);
+          put(tile, row0 + i * kRowStep, lo, hi);
+        }
+      };
+      uint4 dk[kIter], dv[kIter];
+      load(ap.kpool, it.k0, dk);
+      load(ap.vpool, it.k0, dv);
+      // ---- queries
+      if (n_it > 0 && !wait(q_free, n_it - 1)) {
+        ok = false;
+        break;
+      }
+      float* undo_of = s_undo + (n_it & 1) * kUnitRows;
+      const int tiles = it.rows > kRows ? 2 : 1;
+      for (int r = row0; r < tiles * kRows; r += kRowStep) {
+        uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        if (r < it.rows) {
+          const int row = it.row0 + r;
+          const T* src = static_cast<const T*>(ap.q) + (it.t0 + row / group) * ap.ldq +
+                         static_cast<long long>(h_kv * group + row % group) * HD + 16 * c;
+          if (ap.vec) {
+            raw[0] = reinterpret_cast<const uint4*>(src)[0];
+            raw[1] = reinterpret_cast<const uint4*>(src)[1];
+          } else {
+            T* e = reinterpret_cast<T*>(raw);
+            for (int k = 0; k < 16; ++k) e[k] = src[k];
+          }
+        }
+        float undo = 1.0f;
+        uint32_t* w = reinterpret_cast<uint32_t*>(raw);
+        if constexpr (H16Traits<T>::kBf16) {
+          const T* e = reinterpret_cast<const T*>(raw);
+          float big = 0.0f, shift = 1.0f;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) big = fmaxf(big, fabsf(h2f<T>(e[k])));
+#pragma unroll
+          for (int o = kCpr / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+          const int ex = (__float_as_int(big) >> 23) - 127;  // 2^ex <= big
+          if (big > 0.0f && ex < 128) {
+            const int up = min(14 - ex, 126);
+            shift = __int_as_float((up + 127) << 23);
+            undo = __int_as_float((127 - up) << 23);
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const T* e2 = reinterpret_cast<const T*>(&w[k]);
+            w[k] = cvt2_rn<__half>(make_float2(h2f<T>(e2[0]) * shift, h2f<T>(e2[1]) * shift));
+          }
+        }
+        if (ap.scale < 0.0f)  // the softmax takes a positive scale
+#pragma unroll
+          for (int k = 0; k < 8; ++k) w[k] ^= 0x80008000u;
+        put(sQ + (r / kRows) * kTile, r % kRows, raw[0], raw[1]);
+        if (c == 0) undo_of[r] = undo;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&q_full[n_it & 1]);
+      // ---- key tiles
+      for (int j = 0; j < it.cnt; ++j, ++g) {
+        const int slot = g & 1, kt = it.k0 + j;
+        if (!wait(&k_empty[slot], (g >> 1) + 1)) {
+          ok = false;
+          break;
+        }
+        store(sK + slot * kTile, dk);
+        if (j + 1 < it.cnt) load(ap.kpool, kt + 1, dk);
+        fence_proxy_async_smem();
+        mbar_arrive(&k_full[slot]);
+        if ((kt + 1) * kKeys > all) {
+#pragma unroll
+          for (int i = 0; i < kIter; ++i) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(&dv[i]);
+            if (kt * kKeys + row0 + i * kRowStep >= all)
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                  if (((w[y] >> (8 * b)) & 0x7Fu) == 0x7Fu) w[y] &= ~(0xFFu << (8 * b));
+          }
+        }
+        if (!wait(&v_empty[slot], (g >> 1) + 1)) {
+          ok = false;
+          break;
+        }
+        store(sV + slot * kTile, dv);
+        if (j + 1 < it.cnt) load(ap.vpool, kt + 1, dv);
+        fence_proxy_async_smem();
+        mbar_arrive(&v_full[slot]);
+      }
+      ++n_it;
+    }
+  } else if (warp == kConvWarps) {
+    // ================================================ MMA (the warp together, one lane elected)
+    const uint32_t idS = f16_instr_desc(kRows, kKeys, false);
+    const uint32_t idPV = f16_instr_desc(kRows, HD, false) | (1u << 16);  // V MN-major
+    const uint32_t qa = smem_u32(sQ), ka = smem_u32(sK), va = smem_u32(sV);
+    for (int wi = 0; ok && wi < n_work; ++wi) {
+      const Work& it = work[wi];
+      const int nj[2] = {it.jobs(0), it.jobs(1)};
+      const bool pair = it.pair;
+      if (!wait(&q_full[n_it & 1], n_it >> 1)) {
+        ok = false;
+        break;
+      }
+      int left = nj[0] + nj[1];  // S products to be issued
+      // S of stream h's k-th job
+      auto issue_s = [&](int h, int k) -> bool {
+        const uint32_t kt = g + it.key_tile(h, k);
+        if (!wait(&k_full[kt & 1], kt >> 1)) return false;
+        tc_fence_after();
+        const uint64_t dq = sw128_kmajor_desc(qa + (pair ? h * kTile : 0));
+        const uint64_t dk = sw128_kmajor_desc(ka + (kt & 1) * kTile);
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * (kHalf >> 4) + (ks & 3) * 2;
+          mma_f16_e(tbase + h * 128, dq + off, dk + off, idS, ks > 0 ? 1u : 0u);
+        }
+        mma_commit_e(&s_full[h]);
+        if (it.last_user(h)) mma_commit_e(&k_empty[kt & 1]);
+        if (--left == 0) mma_commit_e(q_free);
+        return true;
+      };
+      for (int h = 0; h < 2 && ok; ++h)
+        if (nj[h] > 0) ok = issue_s(h, 0);
+      for (int k = 0; ok && k < max(nj[0], nj[1]); ++k)
+        for (int h = 0; h < 2 && ok; ++h) {
+          if (k >= nj[h]) continue;
+          const uint32_t uses = h ? uses1 : uses0;
+          if (k == 0 && uses > 0 && !wait(&o_free[h], uses - 1)) {
+            ok = false;
+            break;
+          }
+          const uint32_t kt = g + it.key_tile(h, k);
+          if (!wait(&p_full[h], h ? jobs1 : jobs0) || !wait(&v_full[kt & 1], kt >> 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t tp = tbase + h * 128;
+          const uint64_t dv = sw128_mn_desc(va + (kt & 1) * kTile, kHalf, 1024);
+#pragma unroll
+          for (int ks = 0; ks < kKeys / 16; ++ks)
+            mma_f16_ts_e(tbase + 256 + h * 128, tp + (ks >> 2) * 64 + (ks & 3) * 8, dv + ks * 128, idPV,
+                         (k > 0 || ks > 0) ? 1u : 0u);
+          mma_commit_e(&o_ready[h]);
+          if (it.last_user(h)) mma_commit_e(&v_empty[kt & 1]);
+          ++(h ? jobs1 : jobs0);
+          if (k + 1 < nj[h]) ok = issue_s(h, k + 1);
+        }
+      uses0 += nj[0] > 0;
+      uses1 += nj[1] > 0;
+      g += it.cnt;
+      ++n_it;
+    }
+  } else {
+    // ================================================ softmax and results: stream h, row r
+    const int sw = warp - kConvWarps - 1, h = sw / 4, quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t tS = tbase + h * 128 + lane_off, tO = tbase + 256 + h * 128 + lane_off;
+    uint8_t* st = stage + sw * kStage;
+    const float scale = fmaxf(fabsf(ap.scale) * kLog2e, 1.1754944e-38f);  // 0 would lose the masks
+    uint32_t& jobs = jobs0;
+    for (int wi = 0; ok && wi < n_work; ++wi) {
+      const Work& it = work[wi];
+      const int nj = it.jobs(h);
+      const int ur = it.pair ? h * kRows + r : r;  // the unit's row
+      const int row = it.row0 + ur, tok = row / group;
+      const bool valid = ur < it.rows;
+      if (it.pair && h == 1 && it.rows <= kRows) {  // no such tile
+        ++n_it;
+        continue;
+      }
+      const int lim = !valid ? 0 : ap.causal ? max(0, min(it.len, it.past + tok + 1)) : it.len;  // tokens it sees
+      const int h_kv = it.h;
+      float m = -INFINITY, l = 0.0f;
+      uint32_t nan[HD / 32] = {};  // results that a seen NaN code of V spoils
+      float kf = 0.0f;
+      if (nj > 0) {
+        if (!wait(&q_full[n_it & 1], n_it >> 1)) {
+          ok = false;
+          break;
+        }
+        kf = s_undo[(n_it & 1) * kUnitRows + ur] * scale;
+      }
+      ++n_it;
+      // scales of a key tile's pages
+      float ks_n[2], vs_n[2];
+      bool on_n[2];
+      auto scales = [&](int kt) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int page = kt * kKeys + p * kPage < it.seen ? it.bt[2 * kt + p] : -1;
+          on_n[p] = good(page);
+          const long long at = static_cast<long long>(on_n[p] ? page : 0) * ap.nkv + h_kv;
+          ks_n[p] = ap.kscale[at];
+          vs_n[p] = ap.vscale[at];
+        }
+      };
+      if (nj > 0) scales(it.k0 + it.key_tile(h, 0));
+      for (int k = 0; k < nj; ++k, ++jobs) {
+        const int kt = it.k0 + it.key_tile(h, k);
+        float f[2], lv[2], ivs[2];
+        int n_see[2];  // of the two pages' tokens
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const float vs = usable_vscale(vs_n[p]);
+          f[p] = ks_n[p] * kf;
+          lv[p] = lg2_approx(vs);
+          ivs[p] = rcp_approx(vs);
+          n_see[p] = on_n[p] ? lim - kt * kKeys - p * kPage : 0;
+        }
+        if (k + 1 < nj) scales(it.k0 + it.key_tile(h, k + 1));
+        if (!wait(&s_full[h], jobs)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t x[64];
+        auto fetch = [&](int p) {
+          tmem_ld_x64(tS + p * 64, x);
+          if (n_see[p] < 64)
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (i >= n_see[p]) x[i] = __float_as_uint(-INFINITY);
+        };
+        float top = -INFINITY;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          fetch(p);
+          float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 64; ++i) t4[i & 3] = fmaxf(t4[i & 3], __uint_as_float(x[i]));
+          const float t = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+          top = fmaxf(top, fmaf(t, f[p], lv[p]));
+        }
+        const bool grow = top > m + kSlack;
+        float alpha = 1.0f;
+        if (grow) {
+          alpha = ex2_approx(m - top);  // 0 the first time
+          m = top;
+          l *= alpha;
+        }
+        if (k > 0 && __any_sync(0xFFFFFFFFu, grow)) {
+          if (!wait(&o_ready[h], jobs - 1)) {  // the last P V is done
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll 1
+          for (int q = 0; q < HD / 32; ++q) {
+            float o[32];
+            tmem_ld32(tO + q * 32, o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= alpha;
+            tmem_st32(tO + q * 32, o);
+          }
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int p = 1 - q;  // page 1 first: its scores are in x
+          if (q == 1) fetch(p);
+          const float up = lv[p] + (kLift - ref);
+          float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          uint32_t w[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float p0 = ex2_approx(fmaf(__uint_as_float(x[2 * e]), f[p], up));
+            const float p1 = ex2_approx(fmaf(__uint_as_float(x[2 * e + 1]), f[p], up));
+            s4[e & 3] += p0 + p1;
+            w[e] = cvt2_rn<__half>(make_float2(p0, p1));
+          }
+          l = fmaf((s4[0] + s4[1]) + (s4[2] + s4[3]), ivs[p], l);
+          tmem_st_x32(tS + p * 64, w);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[h]);
+        // ---- NaN codes of V that only some rows see
+        if ((kt + 1) * kKeys > it.all) {
+          const int from = max(it.all, kt * kKeys), to = min(it.seen, (kt + 1) * kKeys);
+          for (int key0 = from; key0 < to; key0 += 32 / kCpr) {
+            // the warp looks at 32 / kCpr tokens at a time, a unit a lane
+            const int key = key0 + lane / kCpr;
+            uint32_t bits = 0;
+            const int page = key < to ? it.bt[key / kPage] : -1;
+            if (good(page)) {
+              const uint4 d = __ldg(reinterpret_cast<const uint4*>(
+                  ap.vpool + ((static_cast<long long>(page) * ap.nkv + h_kv) * kPage + (key & 63)) * HD +
+                  16 * (lane % kCpr)));
+              const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+              for (int y = 0; y < 16; ++y)
+                if (((w[y / 4] >> (8 * (y % 4))) & 0x7Fu) == 0x7Fu) bits |= 1u << y;
+            }
+            if (!__any_sync(0xFFFFFFFFu, bits != 0)) continue;
+#pragma unroll 1
+            for (int from_lane = 0; from_lane < 32; ++from_lane) {
+              const uint32_t b = __shfl_sync(0xFFFFFFFFu, bits, from_lane);
+              const int its_key = __shfl_sync(0xFFFFFFFFu, key, from_lane), unit = from_lane % kCpr;
+              if (b && its_key < lim)
+#pragma unroll
+                for (int y = 0; y < HD / 32; ++y)
+                  if (y == unit / 2) nan[y] |= b << (16 * (unit & 1));
+            }
+          }
+        }
+      }
+      if (!ok) break;
+      if (nj > 0 && !wait(&o_ready[h], jobs - 1)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      // ---- the row's result, or its part
+      const UnitAt at{it.s, it.tile, h_kv, it.t0};
+      float inv = 1.0f;
+      float* part = it.parts;
+      if (part) {
+        const int l_at = (ap.part_rows + 3) & ~3;
+        if (!it.pair) part += h * static_cast<long long>(ap.part_stride);
+        if (valid) {
+          __stcg(part + ur, m);
+          __stcg(part + l_at + ur, l);
+        }
+        part += 2 * l_at + ur * HD;
+      } else if (valid) {
+        inv = close_row(ap, at, row, m, l);
+      }
+      T* dst = static_cast<T*>(ap.out) + (it.t0 + tok) * ap.ldo + static_cast<long long>(h_kv * group + row % group) * HD;
+#pragma unroll
+      for (int q = 0; q < HD / 32; ++q) {
+        float o[32];
+        if (nj > 0) {
+          tmem_ld32(tO + q * 32, o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+        }
+        if (nan[q])
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (nan[q] >> e & 1) o[e] = NAN;
+        if (part) {
+          if (valid)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              __stcg(reinterpret_cast<float4*>(part + q * 32) + e,
+                     make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
+        } else if (ap.vec) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = cvt2_rn<T>(make_float2(o[2 * e] * inv, o[2 * e + 1] * inv));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            stage_unit(st, (q & 1) * 4 + e, make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]));
+          if (q & 1) flush_rows<T>(st, valid ? dst : nullptr, (q - 1) * 32, q * 32);
+        } else if (valid) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) dst[q * 32 + e] = f2h<T>(o[e] * inv);
+        }
+      }
+      if (nj > 0) {
+        tc_fence_before();
+        mbar_arrive(&o_free[h]);
+      }
+    }
+  }
+    if (!ok && lane == 0) fail();
+    __syncthreads();  // the descriptions have been read
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kConvWarps) {
+    tc_fence_after();
+    tmem_dealloc(tbase, kTmemCols);
+  }
+}
+
+struct PartSizes {
+  int tiles, parts, rows, stride;
+  long long unit_bytes;
+};
+PartSizes part_sizes(int nq, int nkv, int hd, int max_q, int max_kv) {
+  PartSizes p;
+  const long long rows = static_cast<long long>(max_q) * (nq / nkv);
+  p.tiles = static_cast<int>((rows + kUnitRows - 1) / kUnitRows);
+  const int keys = std::max(1, (max_kv + kKeys - 1) / kKeys);
+  p.parts = 2 * std::min(kMaxChunks, (keys + kMinStep - 1) / kMinStep);
+  p.rows = static_cast<int>(std::min<long long>(kUnitRows, rows));
+  p.stride = 2 * ((p.rows + 3) & ~3) + p.rows * hd;
+  p.unit_bytes = 4ll * p.parts * p.stride;
+  return p;
+}
+
+template <typename T, int HD>
+cudaError_t launch(CacheAttnParams ap, int max_kv, void* ws, long long ws_bytes, cudaStream_t s) {
+  const PartSizes ps = part_sizes(ap.nq, ap.nkv, HD, ap.seqs.max_q, max_kv);
+  ap.tiles_max = ps.tiles;
+  ap.cap_parts = ps.parts;
+  ap.part_rows = ps.rows;
+  ap.part_stride = ps.stride;
+  ap.parts = static_cast<float*>(ws);
+  ap.cap_units = ws ? ws_bytes / ps.unit_bytes : 0;
+  auto k = cache_attn_tiles<T, HD>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Mem<HD>::kSmem);
+  if (e == cudaSuccess) e = launch_pdl(k, dim3(device_sm_count()), dim3(kThreads), Mem<HD>::kSmem, s, ap);
+  if (e == cudaSuccess && ap.cap_units > 0) {
+    const long long x = static_cast<long long>(ap.seqs.n_seqs) * ps.tiles;
+    if (x > 0x7FFFFFFFll || ap.nkv > 65535) return cudaErrorInvalidValue;
+    e = launch_pdl(cache_attn_join<T, HD, TilesPlan>, dim3(static_cast<unsigned>(x), ap.nkv, ps.rows),
+                   dim3(kJoinWarps * 32), 0, s, ap);
+  }
+  return e;
+}
+
+}  // namespace
+
+long long cache_tiles_workspace(int nqh, int nkvh, int hd, int n_seqs, int max_q, int max_kv) {
+  const PartSizes p = part_sizes(nqh, nkvh, hd, max_q, max_kv);
+  return static_cast<long long>(n_seqs) * p.tiles * nkvh * p.unit_bytes;
+}
+
+int cache_attention_tiles(const CacheAttnParams& ap, int hd, bool bf16, int max_kv, void* ws,
+                          long long ws_bytes, cudaStream_t s) {
+  if (bf16)
+    return hd == 128 ? launch<__nv_bfloat16, 128>(ap, max_kv, ws, ws_bytes, s)
+                     : launch<__nv_bfloat16, 64>(ap, max_kv, ws, ws_bytes, s);
+  return hd == 128 ? launch<__half, 128>(ap, max_kv, ws, ws_bytes, s)
+                   : launch<__half, 64>(ap, max_kv, ws, ws_bytes, s);
+}
+
+}  // namespace qa
