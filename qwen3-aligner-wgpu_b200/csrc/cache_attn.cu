@@ -800,10 +800,7 @@ cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int ma
   ap.cap_units = ws ? ws_bytes / ps.unit_bytes : 0;
   cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kWarps * 32), kSmem, s, tk, tv, ap);
   if (e == cudaSuccess && ps.parts > 1 && ap.cap_units > 0) {
-    const long long x = static_cast<long long>(ap.seqs.n_seqs) * ps.tiles;
-    if (x > 0x7FFFFFFFll || ap.nkv > 65535) return cudaErrorInvalidValue;
-    e = launch_pdl(cache_attn_join<T, HD, RowsPlan<R, kTeam, kSlab>>, dim3(static_cast<unsigned>(x), ap.nkv, ps.rows),
-                   dim3(kJoinWarps * 32), 0, s, ap);
+    e = launch_join<T, HD, RowsPlan<R, kTeam, kSlab>>(ap, s);
   }
   return e;
 }

@@ -104,82 +104,104 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& ap, const Unit
          make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), ap.vec);
 }
 
-// Joins the parts of the units that left any (Plan::parts), a CTA a row: each of its
-// warps sums every kJoinWarps-th part (four dims a lane; hd 64: two parts at a
-// time), then the warps are summed, in an order that only the number of parts
-// sets.  Bound by latency: a part's row is one line of 4 hd bytes.
+// Joins the parts of the units that left any (Plan::parts), four dims of a row a
+// lane (hd 64: two parts a warp at a time).  Up to kFewParts a warp sums a row
+// alone and a CTA takes eight rows; beyond, a CTA's warps share the row, each
+// summing every eighth part, and are then summed in turn.  Which of the two, and
+// so the order of the sum, goes by the number of parts alone.  Bound by latency: a
+// part's row is one line of 4 hd bytes.
 constexpr int kJoinWarps = 8;
+constexpr int kFewParts = 32;
 
+// grid: (sequences x tiles, K/V heads, rows, or rows / 8 when no unit has more than
+// kFewParts)
 template <typename T, int HD, typename Plan>
 __global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const __grid_constant__ CacheAttnParams ap) {
-  constexpr int kLanes = HD / 4, kAtOnce = 32 / kLanes * kJoinWarps;  // lanes of a part, parts at once
-  __shared__ float s_red[kJoinWarps], s_sum[kJoinWarps];
-  __shared__ float4 s_o[kAtOnce][kLanes];
+  constexpr int kLanes = HD / 4, kPer = 32 / kLanes;  // lanes of a part, parts of a warp at once
+  __shared__ float s_l[kJoinWarps];
+  __shared__ float4 s_o[kJoinWarps][kLanes];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.y, s = blockIdx.x / ap.tiles_max, tile = blockIdx.x % ap.tiles_max, r = blockIdx.z;
+  const int h = blockIdx.y, s = blockIdx.x / ap.tiles_max, tile = blockIdx.x % ap.tiles_max;
   pdl_wait();
   pdl_trigger();
   const int group = ap.nq / ap.nkv;
   const SeqSpan sp = seq_span(ap.seqs, s, ap.T);
-  if (!sp.ok || tile * Plan::kRows + r >= sp.n * group) return;
+  if (!sp.ok) return;
+  const int rows = min(Plan::kRows, sp.n * group - tile * Plan::kRows);
+  if (rows <= 0) return;
   const int n = Plan::parts(ap, sp, s, tile);
   if (n == 0) return;
+  const bool alone = n <= kFewParts, eight = ap.cap_parts <= kFewParts;  // eight rows a CTA
+  int r = eight ? 8 * blockIdx.z : blockIdx.z;
+  if (alone) {
+    if (r % 8) return;
+    r += warp;
+  }
+  if (r >= rows) return;  // the CTA's warps end together, or work alone
   const UnitAt at{s, tile, h, sp.t0};
   const float* parts = unit_parts(ap, at);
   const int l_at = (ap.part_rows + 3) & ~3, o_at = 2 * l_at + r * HD;
-  const int first = threadIdx.x / kLanes, d = threadIdx.x % kLanes;
+  const int first = (alone ? 0 : warp * kPer) + lane / kLanes, step = alone ? kPer : kPer * kJoinWarps;
+  const int d = lane % kLanes;
   float big = -INFINITY;
-  for (int k = threadIdx.x; k < n; k += kJoinWarps * 32) big = fmaxf(big, parts[static_cast<long long>(k) * ap.part_stride + r]);
+  for (int k = lane; k < n; k += 32) big = fmaxf(big, __ldcg(parts + static_cast<long long>(k) * ap.part_stride + r));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
-  if (lane == 0) s_red[warp] = big;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) big = fmaxf(big, s_red[w]);
   const float ref = big == -INFINITY ? 0.0f : big;
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float sum = 0.0f;
   constexpr int kBatch = 8;  // parts whose loads are in flight together
-  for (int k0 = first; k0 < n; k0 += kBatch * kAtOnce) {
+  for (int k0 = first; k0 < n; k0 += kBatch * step) {
     float4 y[kBatch];
     float pm[kBatch], pl[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int k = k0 + i * kAtOnce;
-      const float* part = parts + static_cast<long long>(min(k, n - 1)) * ap.part_stride;
+      const float* part = parts + static_cast<long long>(min(k0 + i * step, n - 1)) * ap.part_stride;
       y[i] = __ldcg(reinterpret_cast<const float4*>(part + o_at + 4 * d));
       pm[i] = __ldcg(part + r);
       pl[i] = __ldcg(part + l_at + r);
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
-      if (k0 + i * kAtOnce < n) {
+      if (k0 + i * step < n) {
         const float a = ex2_approx(pm[i] - ref);
         sum = fmaf(a, pl[i], sum);
         v = make_float4(fmaf(a, y[i].x, v.x), fmaf(a, y[i].y, v.y), fmaf(a, y[i].z, v.z), fmaf(a, y[i].w, v.w));
       }
   }
-  s_o[first][d] = v;
-  // each part's sum once: from the first lane of its kLanes
-  if (d != 0) sum = 0.0f;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-  if (lane == 0) s_sum[warp] = sum;
-  __syncthreads();
-  if (threadIdx.x < kLanes) {
-    sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) sum += s_sum[w];
+  if constexpr (kPer == 2) {
+    sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
+    v = make_float4(v.x + __shfl_xor_sync(0xFFFFFFFFu, v.x, 16), v.y + __shfl_xor_sync(0xFFFFFFFFu, v.y, 16),
+                    v.z + __shfl_xor_sync(0xFFFFFFFFu, v.z, 16), v.w + __shfl_xor_sync(0xFFFFFFFFu, v.w, 16));
+  }
+  if (!alone) {
+    if (lane < kLanes) s_o[warp][d] = v;
+    if (lane == 0) s_l[warp] = sum;
+    __syncthreads();
+    if (warp > 0) return;
     v = s_o[0][d];
+    sum = s_l[0];
 #pragma unroll
-    for (int k = 1; k < kAtOnce; ++k) {
-      const float4 y = s_o[k][d];
+    for (int w = 1; w < kJoinWarps; ++w) {
+      const float4 y = s_o[w][d];
       v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
+      sum += s_l[w];
     }
+  }
+  if (lane < kLanes) {
     const int row = tile * Plan::kRows + r;
     if (d == 0) close_row(ap, at, row, big, sum);
     finish_row<T, HD>(ap, at, row, 4 * d, v, sum == 0.0f ? 0.0f : 1.0f / sum);
   }
+}
+
+template <typename T, int HD, typename Plan>
+cudaError_t launch_join(const CacheAttnParams& ap, cudaStream_t s) {
+  const long long x = static_cast<long long>(ap.seqs.n_seqs) * ap.tiles_max;
+  if (x > 0x7FFFFFFFll || ap.nkv > 65535) return cudaErrorInvalidValue;
+  const int z = ap.cap_parts <= kFewParts ? (ap.part_rows + 7) / 8 : ap.part_rows;
+  return launch_pdl(cache_attn_join<T, HD, Plan>, dim3(static_cast<unsigned>(x), ap.nkv, z), dim3(kJoinWarps * 32), 0,
+                    s, ap);
 }
 
 }  // namespace

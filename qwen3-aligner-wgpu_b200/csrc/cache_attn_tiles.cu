@@ -13,11 +13,11 @@
 //    alone takes longer over 128 keys than the SM's share of the memory does).
 //
 //   warps 0-3    queries to f16 (bf16 ones scaled by a power of two per row:
-//                exact) and K, V codes to f16 (exact) in shared memory, 128-byte
-//                swizzled; a thread has its 128 bytes of the next key tile's K and
-//                V on their way while it converts this one's;
+//                exact) and K, V codes to f16 (exact), from the ring of codes to
+//                the operands' tiles in shared memory, 128-byte swizzled;
 //   warp 4       tensor memory and the MMAs;
-//   warps 5-12   softmax of the streams, one row a thread, and the results.
+//   warp 5       TMA: K and V pages (8 KB of codes) into the ring, four ahead;
+//   warps 6-13   softmax of the streams, one row a thread, and the results.
 //
 // Tokens past a sequence's end become zeros.  0 . NaN is NaN: in key tiles that
 // some rows see only part of, NaN codes of V are taken out, and the softmax threads
@@ -28,6 +28,7 @@
 
 #include "cache_attn.cuh"
 #include "gemm_tc.cuh"
+#include "tma_host.h"
 
 namespace qa {
 
@@ -38,12 +39,12 @@ constexpr int kUnitRows = 256;
 constexpr int kKeys = 128;
 constexpr int kConvWarps = 4, kSoftWarps = 8;
 constexpr int kConv = kConvWarps * 32;
-constexpr int kThreads = (kConvWarps + 1 + kSoftWarps) * 32;
+constexpr int kThreads = (kConvWarps + 2 + kSoftWarps) * 32;
+constexpr int kRing = 4;       // pages of codes
 constexpr uint32_t kHalf = kRows * 128;  // 64 f16 columns of a tile
 constexpr uint32_t kTmemCols = 512;
 constexpr int kMinStep = 8;    // key tiles of a chunk, at least
 constexpr int kMaxChunks = 16;
-constexpr uint32_t kStage = 4096;  // per softmax warp: 32 rows of 64 output columns
 
 // Key tiles of a chunk of a sequence with `keys` key tiles and `tiles` units a
 // head: enough chunks to fill the GPU from one sequence, as few as that takes.
@@ -205,24 +206,41 @@ __device__ __forceinline__ Work work_of(const CacheAttnParams& ap, const TileWal
   return w;
 }
 
+// Store 16 consecutive 32-bit columns of this warp's 32 TMEM lanes (no wait).
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&w)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]), "r"(w[9]),
+      "r"(w[10]), "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
+      : "memory");
+}
+
+// 0x80 in each byte of w that is a NaN code.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) {
+  return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+}
+
 template <int HD>
 struct Mem {
   static constexpr uint32_t kTile = kHalf * (HD / 64);  // Q, K or V
-  static constexpr size_t kSmem = 6 * kTile + kSoftWarps * kStage + 2 * kUnitRows * 4 + 512 + kBatch * sizeof(Work);
+  static constexpr size_t kSmem = 6 * kTile + kRing * kPage * HD + 2 * kUnitRows * 4 + 512 + kBatch * sizeof(Work);
 };
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_constant__ CacheAttnParams ap) {
+__global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_constant__ CUtensorMap tmK,
+                                                                const __grid_constant__ CUtensorMap tmV,
+                                                                const __grid_constant__ CacheAttnParams ap) {
   constexpr uint32_t kTile = Mem<HD>::kTile;
   constexpr int kCpr = HD / 16;           // 16-byte units of codes a row
-  constexpr int kIter = kRows * kCpr / kConv;  // units of a tile a conversion thread
+  constexpr uint32_t kPageBytes = kPage * HD;
   extern __shared__ __align__(1024) uint8_t smem[];  // no room to align it by hand
   static_assert(Mem<HD>::kSmem <= 232448, "shared memory of a CTA");
   uint8_t* sQ = smem;              // [tile]
   uint8_t* sK = sQ + 2 * kTile;    // [slot]
   uint8_t* sV = sK + 2 * kTile;    // [slot]
-  uint8_t* stage = sV + 2 * kTile; // [softmax warp]
-  float* s_undo = reinterpret_cast<float*>(stage + kSoftWarps * kStage);  // [item & 1][row]
+  uint8_t* ring = sV + 2 * kTile;  // [slot] a page of codes
+  float* s_undo = reinterpret_cast<float*>(ring + kRing * kPageBytes);  // [item & 1][row]
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_undo + 2 * kUnitRows);
   uint64_t* q_full = bars + 0;   // [item & 1] queries and their factors are there
   uint64_t* q_free = bars + 2;   // the item's last S is done
@@ -234,9 +252,12 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
   uint64_t* p_full = bars + 14;  // [stream] P written over S
   uint64_t* o_ready = bars + 16; // [stream] P V done
   uint64_t* o_free = bars + 18;  // [stream] O read
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 20);
+  uint64_t* r_full = bars + 20;  // [ring slot]
+  uint64_t* r_empty = bars + 24;
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 28);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tslot + 1);
-  long long* share = reinterpret_cast<long long*>(bars + 22);  // lo, hi, start, sequence
+  int* r_ok = reinterpret_cast<int*>(bars + 29);               // [ring slot] the page was loaded
+  long long* share = reinterpret_cast<long long*>(bars + 31);  // lo, hi, start, sequence
   long long* scan = share + 4;                                 // [warp]
   int* staged = reinterpret_cast<int*>(scan + kThreads / 32);  // pieces of work described
   Work* work = reinterpret_cast<Work*>(bars + 64);             // [kBatch]
@@ -259,7 +280,13 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
       mbar_init(&o_ready[i], 1);
       mbar_init(&o_free[i], kRows);
     }
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&r_full[i], 1);
+      mbar_init(&r_empty[i], kConvWarps);
+    }
     mbar_init(q_free, 1);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -335,6 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
   bool ok = true;
   uint32_t n_it = 0;  // pieces of work before this one
   uint32_t g = 0;     // key tiles before this one
+  uint32_t pages = 0;  // of codes before this one
   uint32_t uses0 = 0, uses1 = 0, jobs0 = 0, jobs1 = 0;  // of the streams
   for (;;) {
     if (threadIdx.x == 0) {
@@ -348,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
   if (warp < kConvWarps) {
     // ================================================ conversion
     const int tid = threadIdx.x;
-    const int row0 = tid / kCpr, c = tid % kCpr;  // rows row0 + i kConv / kCpr, unit c of each
+    const int row0 = tid / kCpr, c = tid % kCpr;  // rows row0 + i kRowStep, unit c of each
     constexpr int kRowStep = kConv / kCpr;
     // the two 16-byte halves of a converted unit, f16 dims 16 c .. 16 c + 15 of row r
     auto put = [&](uint8_t* tile, int r, uint4 lo, uint4 hi) {
@@ -362,38 +390,39 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
     for (int wi = 0; ok && wi < n_work; ++wi) {
       const Work& it = work[wi];
       const int seen = it.seen, all = it.all, h_kv = it.h;
-      // ---- codes of a key tile, on their way
-      auto load = [&](const uint8_t* pool, int kt, uint4 (&d)[kIter]) {
-        const int key0 = kt * kKeys;
-        int page[2];
+      // a key tile's two pages from the ring to a tile
+      // (the loops over pages are not unrolled, here and in the softmax: the roles' code
+      // together has to stay in the instruction cache)
+      auto convert = [&](uint8_t* tile, int key0, bool v) -> bool {
+#pragma unroll 1
+        for (int p = 0; p < 2; ++p, ++pages) {
+          const int slot = pages % kRing;
+          if (!wait(&r_full[slot], pages / kRing)) return false;
+          const bool on = r_ok[slot];
+          const uint8_t* from = ring + slot * kPageBytes;
+          const bool edge = key0 + (p + 1) * kPage > seen, some = v && key0 + (p + 1) * kPage > all;
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          page[p] = key0 + p * kPage < seen ? it.bt[kt * 2 + p] : -1;
-          if (!good(page[p]) && key0 + p * kPage < seen && tid == 0 && ap.status) atomicOr(ap.status, kStatusBadShape);
-        }
+          for (int i = 0; i < kPage / kRowStep; ++i) {
+            const int r = row0 + i * kRowStep, key = key0 + p * kPage + r;
+            uint4 d = *reinterpret_cast<const uint4*>(from + r * HD + 16 * (c ^ (HD == 128 ? r & 7 : (r >> 1) & 3)));
+            if (!on || (edge && key >= seen)) d = make_uint4(0, 0, 0, 0);
+            if (some && key >= all) {
+              uint32_t* w = reinterpret_cast<uint32_t*>(&d);
 #pragma unroll
-        for (int i = 0; i < kIter; ++i) {
-          const int r = row0 + i * kRowStep, p = i >= kIter / 2;
-          d[i] = make_uint4(0, 0, 0, 0);
-          if (key0 + r < seen && good(page[p]))
-            d[i] = __ldg(reinterpret_cast<const uint4*>(
-                pool + ((static_cast<long long>(page[p]) * ap.nkv + h_kv) * kPage + (r & 63)) * HD + 16 * c));
+              for (int y = 0; y < 4; ++y) w[y] &= ~((nan_codes(w[y]) >> 7) * 0xFFu);
+            }
+            uint4 lo, hi;
+            e4m3x4_f16x2(d.x, lo.x, lo.y);
+            e4m3x4_f16x2(d.y, lo.z, lo.w);
+            e4m3x4_f16x2(d.z, hi.x, hi.y);
+            e4m3x4_f16x2(d.w, hi.z, hi.w);
+            put(tile, p * kPage + r, lo, hi);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&r_empty[slot]);
         }
+        return true;
       };
-      auto store = [&](uint8_t* tile, uint4 (&d)[kIter]) {
-#pragma unroll
-        for (int i = 0; i < kIter; ++i) {
-          uint4 lo, hi;
-          e4m3x4_f16x2(d[i].x, lo.x, lo.y);
-          e4m3x4_f16x2(d[i].y, lo.z, lo.w);
-          e4m3x4_f16x2(d[i].z, hi.x, hi.y);
-          e4m3x4_f16x2(d[i].w, hi.z, hi.w);
-          put(tile, row0 + i * kRowStep, lo, hi);
-        }
-      };
-      uint4 dk[kIter], dv[kIter];
-      load(ap.kpool, it.k0, dk);
-      load(ap.vpool, it.k0, dv);
       // ---- queries
       if (n_it > 0 && !wait(q_free, n_it - 1)) {
         ok = false;
@@ -445,36 +474,18 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
       fence_proxy_async_smem();
       mbar_arrive(&q_full[n_it & 1]);
       // ---- key tiles
-      for (int j = 0; j < it.cnt; ++j, ++g) {
-        const int slot = g & 1, kt = it.k0 + j;
-        if (!wait(&k_empty[slot], (g >> 1) + 1)) {
-          ok = false;
-          break;
-        }
-        store(sK + slot * kTile, dk);
-        if (j + 1 < it.cnt) load(ap.kpool, kt + 1, dk);
-        fence_proxy_async_smem();
-        mbar_arrive(&k_full[slot]);
-        if ((kt + 1) * kKeys > all) {
-#pragma unroll
-          for (int i = 0; i < kIter; ++i) {
-            uint32_t* w = reinterpret_cast<uint32_t*>(&dv[i]);
-            if (kt * kKeys + row0 + i * kRowStep >= all)
-#pragma unroll
-              for (int y = 0; y < 4; ++y)
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-                  if (((w[y] >> (8 * b)) & 0x7Fu) == 0x7Fu) w[y] &= ~(0xFFu << (8 * b));
+      for (int j = 0; ok && j < it.cnt; ++j, ++g) {
+        const int slot = g & 1;
+#pragma unroll 1
+        for (int v = 0; v < 2; ++v) {
+          if (!wait((v ? v_empty : k_empty) + slot, (g >> 1) + 1) ||
+              !convert((v ? sV : sK) + slot * kTile, (it.k0 + j) * kKeys, v)) {
+            ok = false;
+            break;
           }
+          fence_proxy_async_smem();
+          mbar_arrive((v ? v_full : k_full) + slot);
         }
-        if (!wait(&v_empty[slot], (g >> 1) + 1)) {
-          ok = false;
-          break;
-        }
-        store(sV + slot * kTile, dv);
-        if (j + 1 < it.cnt) load(ap.vpool, kt + 1, dv);
-        fence_proxy_async_smem();
-        mbar_arrive(&v_full[slot]);
       }
       ++n_it;
     }
@@ -485,13 +496,13 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
     const uint32_t qa = smem_u32(sQ), ka = smem_u32(sK), va = smem_u32(sV);
     for (int wi = 0; ok && wi < n_work; ++wi) {
       const Work& it = work[wi];
-      const int nj[2] = {it.jobs(0), it.jobs(1)};
+      const int nj0 = it.jobs(0), nj1 = it.jobs(1);
       const bool pair = it.pair;
       if (!wait(&q_full[n_it & 1], n_it >> 1)) {
         ok = false;
         break;
       }
-      int left = nj[0] + nj[1];  // S products to be issued
+      int left = nj0 + nj1;  // S products to be issued
       // S of stream h's k-th job
       auto issue_s = [&](int h, int k) -> bool {
         const uint32_t kt = g + it.key_tile(h, k);
@@ -509,11 +520,14 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
         if (--left == 0) mma_commit_e(q_free);
         return true;
       };
+#pragma unroll 1
       for (int h = 0; h < 2 && ok; ++h)
-        if (nj[h] > 0) ok = issue_s(h, 0);
-      for (int k = 0; ok && k < max(nj[0], nj[1]); ++k)
+        if ((h ? nj1 : nj0) > 0) ok = issue_s(h, 0);
+      for (int k = 0; ok && k < max(nj0, nj1); ++k)
+#pragma unroll 1
         for (int h = 0; h < 2 && ok; ++h) {
-          if (k >= nj[h]) continue;
+          const int nj = h ? nj1 : nj0;
+          if (k >= nj) continue;
           const uint32_t uses = h ? uses1 : uses0;
           if (k == 0 && uses > 0 && !wait(&o_free[h], uses - 1)) {
             ok = false;
@@ -534,20 +548,55 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
           mma_commit_e(&o_ready[h]);
           if (it.last_user(h)) mma_commit_e(&v_empty[kt & 1]);
           ++(h ? jobs1 : jobs0);
-          if (k + 1 < nj[h]) ok = issue_s(h, k + 1);
+          if (k + 1 < nj) ok = issue_s(h, k + 1);
         }
-      uses0 += nj[0] > 0;
-      uses1 += nj[1] > 0;
+      uses0 += nj0 > 0;
+      uses1 += nj1 > 0;
       g += it.cnt;
+      ++n_it;
+    }
+  } else if (warp == kConvWarps + 1) {
+    // ================================================ TMA
+    for (int wi = 0; ok && wi < n_work; ++wi) {
+      const Work& it = work[wi];
+      int next[2] = {0, 0};  // page ids, read a key tile ahead
+      auto look = [&](int kt) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) next[p] = kt * kKeys + p * kPage < it.seen ? it.bt[2 * kt + p] : -2;
+      };
+      look(it.k0);
+      for (int j = 0; ok && j < it.cnt; ++j) {
+        const int now[2] = {next[0], next[1]};
+        if (j + 1 < it.cnt) look(it.k0 + j + 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i, ++pages) {  // K, K, V, V
+          const int slot = pages % kRing, page = now[i & 1];
+          if (!wait(&r_empty[slot], pages / kRing + 1)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) {
+            r_ok[slot] = good(page);
+            if (good(page)) {
+              mbar_arrive_expect_tx(&r_full[slot], kPageBytes);
+              tma_load_2d(i < 2 ? &tmK : &tmV, &r_full[slot], ring + slot * kPageBytes, 0,
+                          (page * ap.nkv + it.h) * kPage);
+            } else {
+              if (page != -2 && ap.status) atomicOr(ap.status, kStatusBadShape);
+              mbar_arrive(&r_full[slot]);
+            }
+          }
+          __syncwarp();
+        }
+      }
       ++n_it;
     }
   } else {
     // ================================================ softmax and results: stream h, row r
-    const int sw = warp - kConvWarps - 1, h = sw / 4, quarter = warp & 3;
+    const int h = (warp - kConvWarps - 2) / 4, quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tbase + h * 128 + lane_off, tO = tbase + 256 + h * 128 + lane_off;
-    uint8_t* st = stage + sw * kStage;
     const float scale = fmaxf(fabsf(ap.scale) * kLog2e, 1.1754944e-38f);  // 0 would lose the masks
     uint32_t& jobs = jobs0;
     for (int wi = 0; ok && wi < n_work; ++wi) {
@@ -563,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
       const int lim = !valid ? 0 : ap.causal ? max(0, min(it.len, it.past + tok + 1)) : it.len;  // tokens it sees
       const int h_kv = it.h;
       float m = -INFINITY, l = 0.0f;
-      uint32_t nan[HD / 32] = {};  // results that a seen NaN code of V spoils
+      uint32_t nan[4] = {0, 0, 0, 0};  // results that a seen NaN code of V spoils
       float kf = 0.0f;
       if (nj > 0) {
         if (!wait(&q_full[n_it & 1], n_it >> 1)) {
@@ -605,23 +654,21 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
           break;
         }
         tc_fence_after();
-        uint32_t x[64];
-        auto fetch = [&](int p) {
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int p = 0; p < 2; ++p) {
+          uint32_t x[64];
           tmem_ld_x64(tS + p * 64, x);
-          if (n_see[p] < 64)
+          const int see = p ? n_see[1] : n_see[0];
+          if (see < 64)
 #pragma unroll
             for (int i = 0; i < 64; ++i)
-              if (i >= n_see[p]) x[i] = __float_as_uint(-INFINITY);
-        };
-        float top = -INFINITY;
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          fetch(p);
+              if (i >= see) x[i] = __float_as_uint(-INFINITY);
           float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int i = 0; i < 64; ++i) t4[i & 3] = fmaxf(t4[i & 3], __uint_as_float(x[i]));
           const float t = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-          top = fmaxf(top, fmaf(t, f[p], lv[p]));
+          top = fmaxf(top, fmaf(t, p ? f[1] : f[0], p ? lv[1] : lv[0]));
         }
         const bool grow = top > m + kSlack;
         float alpha = 1.0f;
@@ -646,22 +693,28 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
+        // 32 scores at a time; a page's P (32 columns) goes over scores already read
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          const int p = q >> 1, half = q & 1;
+          uint32_t x[32], w[16];
+          tmem_ld_x32(tS + q * 32, x);
+          const int see = (p ? n_see[1] : n_see[0]) - 32 * half;
+          if (see < 32)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int p = 1 - q;  // page 1 first: its scores are in x
-          if (q == 1) fetch(p);
-          const float up = lv[p] + (kLift - ref);
+            for (int i = 0; i < 32; ++i)
+              if (i >= see) x[i] = __float_as_uint(-INFINITY);
+          const float up = (p ? lv[1] : lv[0]) + (kLift - ref), fp = p ? f[1] : f[0];
           float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          uint32_t w[32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float p0 = ex2_approx(fmaf(__uint_as_float(x[2 * e]), f[p], up));
-            const float p1 = ex2_approx(fmaf(__uint_as_float(x[2 * e + 1]), f[p], up));
+          for (int e = 0; e < 16; ++e) {
+            const float p0 = ex2_approx(fmaf(__uint_as_float(x[2 * e]), fp, up));
+            const float p1 = ex2_approx(fmaf(__uint_as_float(x[2 * e + 1]), fp, up));
             s4[e & 3] += p0 + p1;
             w[e] = cvt2_rn<__half>(make_float2(p0, p1));
           }
-          l = fmaf((s4[0] + s4[1]) + (s4[2] + s4[3]), ivs[p], l);
-          tmem_st_x32(tS + p * 64, w);
+          l = fmaf((s4[0] + s4[1]) + (s4[2] + s4[3]), p ? ivs[1] : ivs[0], l);
+          tmem_st_x16(tS + p * 64 + half * 16, w);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -678,10 +731,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
               const uint4 d = __ldg(reinterpret_cast<const uint4*>(
                   ap.vpool + ((static_cast<long long>(page) * ap.nkv + h_kv) * kPage + (key & 63)) * HD +
                   16 * (lane % kCpr)));
-              const uint32_t w[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-              for (int y = 0; y < 16; ++y)
-                if (((w[y / 4] >> (8 * (y % 4))) & 0x7Fu) == 0x7Fu) bits |= 1u << y;
+              auto four = [](uint32_t w) {  // the NaN codes of a word, a bit each
+                const uint32_t n = nan_codes(w) >> 7;
+                return (n & 1u) | (n >> 7 & 2u) | (n >> 14 & 4u) | (n >> 21 & 8u);
+              };
+              bits = four(d.x) | four(d.y) << 4 | four(d.z) << 8 | four(d.w) << 12;
             }
             if (!__any_sync(0xFFFFFFFFu, bits != 0)) continue;
 #pragma unroll 1
@@ -690,7 +744,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
               const int its_key = __shfl_sync(0xFFFFFFFFu, key, from_lane), unit = from_lane % kCpr;
               if (b && its_key < lim)
 #pragma unroll
-                for (int y = 0; y < HD / 32; ++y)
+                for (int y = 0; y < 4; ++y)
                   if (y == unit / 2) nan[y] |= b << (16 * (unit & 1));
             }
           }
@@ -718,7 +772,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
         inv = close_row(ap, at, row, m, l);
       }
       T* dst = static_cast<T*>(ap.out) + (it.t0 + tok) * ap.ldo + static_cast<long long>(h_kv * group + row % group) * HD;
-#pragma unroll
+#pragma unroll 1
       for (int q = 0; q < HD / 32; ++q) {
         float o[32];
         if (nj > 0) {
@@ -727,24 +781,25 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0.0f;
         }
-        if (nan[q])
+        const uint32_t bad = q == 0 ? nan[0] : q == 1 ? nan[1] : q == 2 ? nan[2] : nan[3];
+        if (bad)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if (nan[q] >> e & 1) o[e] = NAN;
+            if (bad >> e & 1) o[e] = NAN;
         if (part) {
           if (valid)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               __stcg(reinterpret_cast<float4*>(part + q * 32) + e,
                      make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
-        } else if (ap.vec) {
-          uint32_t w[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) w[e] = cvt2_rn<T>(make_float2(o[2 * e] * inv, o[2 * e + 1] * inv));
+        } else if (valid && ap.vec) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            stage_unit(st, (q & 1) * 4 + e, make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]));
-          if (q & 1) flush_rows<T>(st, valid ? dst : nullptr, (q - 1) * 32, q * 32);
+            *reinterpret_cast<uint4*>(dst + q * 32 + 8 * e) =
+                make_uint4(cvt2_rn<T>(make_float2(o[8 * e] * inv, o[8 * e + 1] * inv)),
+                           cvt2_rn<T>(make_float2(o[8 * e + 2] * inv, o[8 * e + 3] * inv)),
+                           cvt2_rn<T>(make_float2(o[8 * e + 4] * inv, o[8 * e + 5] * inv)),
+                           cvt2_rn<T>(make_float2(o[8 * e + 6] * inv, o[8 * e + 7] * inv)));
         } else if (valid) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) dst[q * 32 + e] = f2h<T>(o[e] * inv);
@@ -758,6 +813,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
   }
     if (!ok && lane == 0) fail();
     __syncthreads();  // the descriptions have been read
+    if (*abort_flag && warp == kConvWarps + 1)  // no copy may be on its way when the CTA ends
+      for (uint32_t n = pages > kRing ? pages - kRing : 0; n < pages; ++n)
+        mbar_wait_warp(&r_full[n % kRing], (n / kRing) & 1);
   }
 
   tc_fence_before();
@@ -793,14 +851,20 @@ cudaError_t launch(CacheAttnParams ap, int max_kv, void* ws, long long ws_bytes,
   ap.part_stride = ps.stride;
   ap.parts = static_cast<float*>(ws);
   ap.cap_units = ws ? ws_bytes / ps.unit_bytes : 0;
+  CUtensorMap tk, tv;
+  const long long rows = static_cast<long long>(ap.kv_pages) * ap.nkv * kPage;
+  if (rows > 0x7FFFFFFFll) return cudaErrorInvalidValue;  // TMA row coordinates
+  // codes in pairs, as 16-bit elements
+  const long long dims[2] = {HD / 2, rows}, stride[1] = {HD};
+  const int box[2] = {HD / 2, kPage}, step[2] = {1, 1};
+  int rc = make_tmap_nd(&tk, ap.kpool, false, 2, dims, stride, box, step, HD);
+  if (!rc) rc = make_tmap_nd(&tv, ap.vpool, false, 2, dims, stride, box, step, HD);
+  if (rc) return static_cast<cudaError_t>(rc);
   auto k = cache_attn_tiles<T, HD>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Mem<HD>::kSmem);
-  if (e == cudaSuccess) e = launch_pdl(k, dim3(device_sm_count()), dim3(kThreads), Mem<HD>::kSmem, s, ap);
+  if (e == cudaSuccess) e = launch_pdl(k, dim3(device_sm_count()), dim3(kThreads), Mem<HD>::kSmem, s, tk, tv, ap);
   if (e == cudaSuccess && ap.cap_units > 0) {
-    const long long x = static_cast<long long>(ap.seqs.n_seqs) * ps.tiles;
-    if (x > 0x7FFFFFFFll || ap.nkv > 65535) return cudaErrorInvalidValue;
-    e = launch_pdl(cache_attn_join<T, HD, TilesPlan>, dim3(static_cast<unsigned>(x), ap.nkv, ps.rows),
-                   dim3(kJoinWarps * 32), 0, s, ap);
+    e = launch_join<T, HD, TilesPlan>(ap, s);
   }
   return e;
 }
