@@ -178,6 +178,7 @@ struct Walk {
 template <int R, int TEAM, int SLAB>
 struct RowsPlan {
   static constexpr int kRows = R;
+  static constexpr bool kAlone = false;
   __device__ static int parts(const CacheAttnParams& ap, const SeqSpan& sp, int s, int) {
     const int n = seq_plan(ap, sp, s, ap.nq / ap.nkv, R, TEAM, SLAB).chunks;
     return n > 1 ? n : 0;

@@ -105,16 +105,13 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& ap, const Unit
 }
 
 // Joins the parts of the units that left any (Plan::parts), four dims of a row a
-// lane (hd 64: two parts a warp at a time).  Up to kFewParts a warp sums a row
-// alone and a CTA takes eight rows; beyond, a CTA's warps share the row, each
-// summing every eighth part, and are then summed in turn.  Which of the two, and
-// so the order of the sum, goes by the number of parts alone.  Bound by latency: a
-// part's row is one line of 4 hd bytes.
+// lane (hd 64: two parts a warp at a time).  Few rows of many parts (the few-row
+// kernel's): a CTA's warps share a row, each summing every eighth part, and are
+// then summed in turn.  Many rows of few parts (kAlone): a warp a row.  Bound by
+// latency: a part's row is one line of 4 hd bytes.
 constexpr int kJoinWarps = 8;
-constexpr int kFewParts = 32;
 
-// grid: (sequences x tiles, K/V heads, rows, or rows / 8 when no unit has more than
-// kFewParts)
+// grid: (sequences x tiles, K/V heads, rows, or rows / 8)
 template <typename T, int HD, typename Plan>
 __global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const __grid_constant__ CacheAttnParams ap) {
   constexpr int kLanes = HD / 4, kPer = 32 / kLanes;  // lanes of a part, parts of a warp at once
@@ -131,12 +128,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const __grid_
   if (rows <= 0) return;
   const int n = Plan::parts(ap, sp, s, tile);
   if (n == 0) return;
-  const bool alone = n <= kFewParts, eight = ap.cap_parts <= kFewParts;  // eight rows a CTA
-  int r = eight ? 8 * blockIdx.z : blockIdx.z;
-  if (alone) {
-    if (r % 8) return;
-    r += warp;
-  }
+  constexpr bool alone = Plan::kAlone;
+  const int r = alone ? kJoinWarps * blockIdx.z + warp : blockIdx.z;
   if (r >= rows) return;  // the CTA's warps end together, or work alone
   const UnitAt at{s, tile, h, sp.t0};
   const float* parts = unit_parts(ap, at);
@@ -144,9 +137,17 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const __grid_
   const int first = (alone ? 0 : warp * kPer) + lane / kLanes, step = alone ? kPer : kPer * kJoinWarps;
   const int d = lane % kLanes;
   float big = -INFINITY;
-  for (int k = lane; k < n; k += 32) big = fmaxf(big, __ldcg(parts + static_cast<long long>(k) * ap.part_stride + r));
+  for (int k = alone ? lane : threadIdx.x; k < n; k += alone ? 32 : 32 * kJoinWarps)
+    big = fmaxf(big, __ldcg(parts + static_cast<long long>(k) * ap.part_stride + r));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+  if constexpr (!alone) {
+    if (lane == 0) s_l[warp] = big;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) big = fmaxf(big, s_l[w]);
+    __syncthreads();
+  }
   const float ref = big == -INFINITY ? 0.0f : big;
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float sum = 0.0f;
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const __grid_
     v = make_float4(v.x + __shfl_xor_sync(0xFFFFFFFFu, v.x, 16), v.y + __shfl_xor_sync(0xFFFFFFFFu, v.y, 16),
                     v.z + __shfl_xor_sync(0xFFFFFFFFu, v.z, 16), v.w + __shfl_xor_sync(0xFFFFFFFFu, v.w, 16));
   }
-  if (!alone) {
+  if constexpr (!alone) {
     if (lane < kLanes) s_o[warp][d] = v;
     if (lane == 0) s_l[warp] = sum;
     __syncthreads();
@@ -199,7 +200,7 @@ template <typename T, int HD, typename Plan>
 cudaError_t launch_join(const CacheAttnParams& ap, cudaStream_t s) {
   const long long x = static_cast<long long>(ap.seqs.n_seqs) * ap.tiles_max;
   if (x > 0x7FFFFFFFll || ap.nkv > 65535) return cudaErrorInvalidValue;
-  const int z = ap.cap_parts <= kFewParts ? (ap.part_rows + 7) / 8 : ap.part_rows;
+  const int z = Plan::kAlone ? (ap.part_rows + kJoinWarps - 1) / kJoinWarps : ap.part_rows;
   return launch_pdl(cache_attn_join<T, HD, Plan>, dim3(static_cast<unsigned>(x), ap.nkv, z), dim3(kJoinWarps * 32), 0,
                     s, ap);
 }

@@ -95,6 +95,7 @@ __device__ __forceinline__ Unit unit_of(const CacheAttnParams& ap, const SeqSpan
 // The parts that this kernel leaves, for the join.
 struct TilesPlan {
   static constexpr int kRows = kUnitRows;
+  static constexpr bool kAlone = true;
   __device__ static int parts(const CacheAttnParams& ap, const SeqSpan& sp, int s, int tile) {
     const Unit u = unit_of(ap, sp, tile_plan(ap, sp), s, tile);
     return u.pair ? (u.chunks > 1 ? u.chunks : 0) : 2 * u.chunks;
@@ -375,18 +376,19 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
     if (n_work == 0 || *abort_flag) break;
   if (warp < kConvWarps) {
     // ================================================ conversion
-    const int tid = threadIdx.x;
-    const int row0 = tid / kCpr, c = tid % kCpr;  // rows row0 + i kRowStep, unit c of each
+    // A thread has unit c of the rows row0 + i kRowStep.  hd 128: neighbouring rows'
+    // lanes 0-3 and 4-7 take opposite halves of their rows, so that the eight lanes
+    // of a 16-byte access meet different banks when they read codes and when they
+    // write f16 (whose units are XORed with the row's low bits).
     constexpr int kRowStep = kConv / kCpr;
-    // the two 16-byte halves of a converted unit, f16 dims 16 c .. 16 c + 15 of row r
-    auto put = [&](uint8_t* tile, int r, uint4 lo, uint4 hi) {
-      uint8_t* base = tile + (c >> 2) * kHalf + r * 128;
-      const int u = 2 * (c & 3), sw = r & 7;
-      // lanes of the two halves store their pieces in opposite order: different banks
-      const bool flip = (c >> 2) & 1;
-      *reinterpret_cast<uint4*>(base + 16 * ((u + flip) ^ sw)) = flip ? hi : lo;
-      *reinterpret_cast<uint4*>(base + 16 * ((u + !flip) ^ sw)) = flip ? lo : hi;
-    };
+    const int c = HD == 128 ? (lane & 3) + 4 * ((lane >> 2 ^ lane >> 3) & 1) : lane & 3;
+    const int row0 = HD == 128 ? warp * 4 + (lane >> 4) * 2 + (lane >> 2 & 1) : warp * 8 + (lane >> 2);
+    const uint32_t from0 = row0 * HD + 16 * (c ^ (HD == 128 ? row0 & 7 : (row0 >> 1) & 3));
+    // f16 dims 16 c .. 16 c + 15 of row0, as two units; row0 + i kRowStep has the
+    // same low bits
+    const uint32_t to0 = (c >> 2) * kHalf + row0 * 128 + 16 * ((2 * (c & 3)) ^ (row0 & 7));
+    const uint32_t to1 = (c >> 2) * kHalf + row0 * 128 + 16 * ((2 * (c & 3) + 1) ^ (row0 & 7));
+    static_assert(kRowStep % 8 == 0, "rows of a thread have the same low bits");
     for (int wi = 0; ok && wi < n_work; ++wi) {
       const Work& it = work[wi];
       const int seen = it.seen, all = it.all, h_kv = it.h;
@@ -400,23 +402,32 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
           if (!wait(&r_full[slot], pages / kRing)) return false;
           const bool on = r_ok[slot];
           const uint8_t* from = ring + slot * kPageBytes;
-          const bool edge = key0 + (p + 1) * kPage > seen, some = v && key0 + (p + 1) * kPage > all;
+          uint4 d[kPage / kRowStep];
+#pragma unroll
+          for (int i = 0; i < kPage / kRowStep; ++i)
+            d[i] = *reinterpret_cast<const uint4*>(from + from0 + i * (kRowStep * HD));
+          if (!on || key0 + (p + 1) * kPage > seen || (v && key0 + (p + 1) * kPage > all)) {
+#pragma unroll
+            for (int i = 0; i < kPage / kRowStep; ++i) {
+              const int key = key0 + p * kPage + row0 + i * kRowStep;
+              uint32_t* w = reinterpret_cast<uint32_t*>(&d[i]);
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                if (v && key >= all) w[y] &= ~((nan_codes(w[y]) >> 7) * 0xFFu);
+                if (!on || key >= seen) w[y] = 0;
+              }
+            }
+          }
+          uint8_t* to = tile + p * kPage * 128;
 #pragma unroll
           for (int i = 0; i < kPage / kRowStep; ++i) {
-            const int r = row0 + i * kRowStep, key = key0 + p * kPage + r;
-            uint4 d = *reinterpret_cast<const uint4*>(from + r * HD + 16 * (c ^ (HD == 128 ? r & 7 : (r >> 1) & 3)));
-            if (!on || (edge && key >= seen)) d = make_uint4(0, 0, 0, 0);
-            if (some && key >= all) {
-              uint32_t* w = reinterpret_cast<uint32_t*>(&d);
-#pragma unroll
-              for (int y = 0; y < 4; ++y) w[y] &= ~((nan_codes(w[y]) >> 7) * 0xFFu);
-            }
             uint4 lo, hi;
-            e4m3x4_f16x2(d.x, lo.x, lo.y);
-            e4m3x4_f16x2(d.y, lo.z, lo.w);
-            e4m3x4_f16x2(d.z, hi.x, hi.y);
-            e4m3x4_f16x2(d.w, hi.z, hi.w);
-            put(tile, p * kPage + r, lo, hi);
+            e4m3x4_f16x2(d[i].x, lo.x, lo.y);
+            e4m3x4_f16x2(d[i].y, lo.z, lo.w);
+            e4m3x4_f16x2(d[i].z, hi.x, hi.y);
+            e4m3x4_f16x2(d[i].w, hi.z, hi.w);
+            *reinterpret_cast<uint4*>(to + to0 + i * (kRowStep * 128)) = lo;
+            *reinterpret_cast<uint4*>(to + to1 + i * (kRowStep * 128)) = hi;
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&r_empty[slot]);
@@ -452,7 +463,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
 #pragma unroll
           for (int k = 0; k < 16; ++k) big = fmaxf(big, fabsf(h2f<T>(e[k])));
 #pragma unroll
-          for (int o = kCpr / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+          for (int o = 1; o < 4; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+          if (HD == 128) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 8));
           const int ex = (__float_as_int(big) >> 23) - 127;  // 2^ex <= big
           if (big > 0.0f && ex < 128) {
             const int up = min(14 - ex, 126);
@@ -468,7 +480,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
         if (ap.scale < 0.0f)  // the softmax takes a positive scale
 #pragma unroll
           for (int k = 0; k < 8; ++k) w[k] ^= 0x80008000u;
-        put(sQ + (r / kRows) * kTile, r % kRows, raw[0], raw[1]);
+        uint8_t* to = sQ + (r / kRows) * kTile + (r % kRows - row0) * 128;
+        *reinterpret_cast<uint4*>(to + to0) = raw[0];
+        *reinterpret_cast<uint4*>(to + to1) = raw[1];
         if (c == 0) undo_of[r] = undo;
       }
       fence_proxy_async_smem();
@@ -654,21 +668,23 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
           break;
         }
         tc_fence_after();
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int p = 0; p < 2; ++p) {
-          uint32_t x[64];
+        uint32_t x[64];
+        auto fetch = [&](int p) {
           tmem_ld_x64(tS + p * 64, x);
-          const int see = p ? n_see[1] : n_see[0];
-          if (see < 64)
+          if (n_see[p] < 64)
 #pragma unroll
             for (int i = 0; i < 64; ++i)
-              if (i >= see) x[i] = __float_as_uint(-INFINITY);
+              if (i >= n_see[p]) x[i] = __float_as_uint(-INFINITY);
+        };
+        float top = -INFINITY;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          fetch(p);
           float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int i = 0; i < 64; ++i) t4[i & 3] = fmaxf(t4[i & 3], __uint_as_float(x[i]));
           const float t = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-          top = fmaxf(top, fmaf(t, p ? f[1] : f[0], p ? lv[1] : lv[0]));
+          top = fmaxf(top, fmaf(t, f[p], lv[p]));
         }
         const bool grow = top > m + kSlack;
         float alpha = 1.0f;
@@ -693,28 +709,26 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
-        // 32 scores at a time; a page's P (32 columns) goes over scores already read
-#pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          const int p = q >> 1, half = q & 1;
-          uint32_t x[32], w[16];
-          tmem_ld_x32(tS + q * 32, x);
-          const int see = (p ? n_see[1] : n_see[0]) - 32 * half;
-          if (see < 32)
+        // page 1 first: its scores are in x; a page's P (32 columns) goes over its scores
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i >= see) x[i] = __float_as_uint(-INFINITY);
-          const float up = (p ? lv[1] : lv[0]) + (kLift - ref), fp = p ? f[1] : f[0];
+        for (int q = 0; q < 2; ++q) {
+          const int p = 1 - q;
+          if (q == 1) fetch(p);
+          const float up = lv[p] + (kLift - ref);
           float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float p0 = ex2_approx(fmaf(__uint_as_float(x[2 * e]), fp, up));
-            const float p1 = ex2_approx(fmaf(__uint_as_float(x[2 * e + 1]), fp, up));
-            s4[e & 3] += p0 + p1;
-            w[e] = cvt2_rn<__half>(make_float2(p0, p1));
+          for (int half = 0; half < 2; ++half) {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float p0 = ex2_approx(fmaf(__uint_as_float(x[32 * half + 2 * e]), f[p], up));
+              const float p1 = ex2_approx(fmaf(__uint_as_float(x[32 * half + 2 * e + 1]), f[p], up));
+              s4[e & 3] += p0 + p1;
+              w[e] = cvt2_rn<__half>(make_float2(p0, p1));
+            }
+            tmem_st_x16(tS + p * 64 + half * 16, w);
           }
-          l = fmaf((s4[0] + s4[1]) + (s4[2] + s4[3]), p ? ivs[1] : ivs[0], l);
-          tmem_st_x16(tS + p * 64 + half * 16, w);
+          l = fmaf((s4[0] + s4[1]) + (s4[2] + s4[3]), ivs[p], l);
         }
         tmem_wait_st();
         tc_fence_before();
