@@ -157,10 +157,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const __grid_
     float pm[kBatch], pl[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const float* part = parts + static_cast<long long>(min(k0 + i * step, n - 1)) * ap.part_stride;
-      y[i] = __ldcg(reinterpret_cast<const float4*>(part + o_at + 4 * d));
-      pm[i] = __ldcg(part + r);
-      pl[i] = __ldcg(part + l_at + r);
+      const float* part = parts + static_cast<long long>(k0 + i * step) * ap.part_stride;
+      y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      pm[i] = pl[i] = 0.0f;
+      if (k0 + i * step < n) {
+        y[i] = __ldcg(reinterpret_cast<const float4*>(part + o_at + 4 * d));
+        pm[i] = __ldcg(part + r);
+        pl[i] = __ldcg(part + l_at + r);
+      }
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)

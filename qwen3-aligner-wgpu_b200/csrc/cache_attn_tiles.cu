@@ -41,6 +41,7 @@ constexpr int kConvWarps = 4, kSoftWarps = 8;
 constexpr int kConv = kConvWarps * 32;
 constexpr int kThreads = (kConvWarps + 2 + kSoftWarps) * 32;
 constexpr int kRing = 4;       // pages of codes
+constexpr int kScales = 4;     // key tiles whose pages' scales are there
 constexpr uint32_t kHalf = kRows * 128;  // 64 f16 columns of a tile
 constexpr uint32_t kTmemCols = 512;
 constexpr int kMinStep = 8;    // key tiles of a chunk, at least
@@ -176,10 +177,10 @@ struct Work {
     return pair ? (st == 0 || rows > kRows ? cnt : 0) : (cnt + 1 - st) / 2;
   }
   __device__ __forceinline__ int key_tile(int st, int k) const { return pair ? k : 2 * k + st; }
-  // whether stream st is the last to use a key tile
-  __device__ __forceinline__ bool last_user(int st) const { return !pair || st == 1 || rows <= kRows; }
+  // whether stream st is the last to use a key tile that streams share
+  __device__ __forceinline__ bool last_user(int st) const { return st == 1 || rows <= kRows; }
 };
-constexpr int kBatch = 4;  // pieces of work described at a time
+constexpr int kBatch = 2;  // pieces of work described at a time
 
 __device__ __forceinline__ Work work_of(const CacheAttnParams& ap, const TileWalk& walk) {
   const int group = ap.nq / ap.nkv;
@@ -225,7 +226,8 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t w) {
 template <int HD>
 struct Mem {
   static constexpr uint32_t kTile = kHalf * (HD / 64);  // Q, K or V
-  static constexpr size_t kSmem = 6 * kTile + kRing * kPage * HD + 2 * kUnitRows * 4 + 512 + kBatch * sizeof(Work);
+  static constexpr size_t kSmem = 6 * kTile + kRing * kPage * HD + 2 * kUnitRows * 4 + 512 +
+                                  kScales * 2 * sizeof(float4) + kBatch * sizeof(Work);
 };
 
 template <typename T, int HD>
@@ -255,15 +257,18 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
   uint64_t* o_free = bars + 18;  // [stream] O read
   uint64_t* r_full = bars + 20;  // [ring slot]
   uint64_t* r_empty = bars + 24;
+  uint64_t* sc_full = bars + 50;  // [key tile % kScales] scales are there
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 28);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tslot + 1);
   int* r_ok = reinterpret_cast<int*>(bars + 29);               // [ring slot] the page was loaded
   long long* share = reinterpret_cast<long long*>(bars + 31);  // lo, hi, start, sequence
   long long* scan = share + 4;                                 // [warp]
   int* staged = reinterpret_cast<int*>(scan + kThreads / 32);  // pieces of work described
-  Work* work = reinterpret_cast<Work*>(bars + 64);             // [kBatch]
+  // a page's K scale, log2 and reciprocal of its V scale, 1 if it is there
+  float4* sc = reinterpret_cast<float4*>(bars + 64);           // [kScales][2]
+  Work* work = reinterpret_cast<Work*>(sc + kScales * 2);      // [kBatch]
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int group = ap.nq / ap.nkv, n_seqs = ap.seqs.n_seqs;
   if (smem_u32(smem) & 1023u) {  // the swizzled tiles would not be where the MMA looks for them
     if (threadIdx.x == 0 && ap.status) atomicOr(ap.status, kStatusTimeout);
@@ -285,6 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
       mbar_init(&r_full[i], 1);
       mbar_init(&r_empty[i], kConvWarps);
     }
+    for (int i = 0; i < kScales; ++i) mbar_init(&sc_full[i], 1);
     mbar_init(q_free, 1);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -295,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tbase = *tslot;
+  const uint32_t tbase = __shfl_sync(0xFFFFFFFFu, *tslot, 0);
   pdl_wait();
   pdl_trigger();
 
@@ -355,8 +361,12 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
   };
   // bounded wait taken by a whole warp, warp-uniform result
   auto wait = [&](uint64_t* bar, uint32_t par) -> bool {
+    if (__all_sync(0xFFFFFFFFu, mbar_try_wait(smem_u32(bar), par & 1u))) return true;
     return __all_sync(0xFFFFFFFFu, !*abort_flag && mbar_wait(bar, par & 1u));
   };
+  // a value that is the same in all lanes, known as such to the compiler: operands
+  // of the MMAs are then made in uniform registers
+  auto same = [](int v) { return __shfl_sync(0xFFFFFFFFu, v, 0); };
   auto good = [&](int page) { return page >= 0 && page < ap.kv_pages; };
   TileWalk walk;  // thread 0's
   if (threadIdx.x == 0 && any) walk.begin(ap, static_cast<int>(share[3]), share[2], share[0], share[1]);
@@ -434,56 +444,80 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
         }
         return true;
       };
-      // ---- queries
+      // ---- queries: the first rows are on their way while the last item's products end
+      const int rows_up = it.rows > kRows ? 2 * kRows : kRows;
+      int tok = (it.row0 + row0) / group, head = (it.row0 + row0) % group;  // of the row to be read
+      const int tok_step = kRowStep / group, head_step = kRowStep % group;
+      constexpr int kTogether = 8;  // rows whose loads are in flight together
+      uint4 raw[kTogether][2];
+      auto load_q = [&](int r0) {
+#pragma unroll
+        for (int i = 0; i < kTogether; ++i) {
+          raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
+          if (r0 + i * kRowStep < it.rows) {
+            const T* src = static_cast<const T*>(ap.q) + (it.t0 + tok) * ap.ldq + (h_kv * group + head) * HD + 16 * c;
+            if (ap.vec) {
+              raw[i][0] = reinterpret_cast<const uint4*>(src)[0];
+              raw[i][1] = reinterpret_cast<const uint4*>(src)[1];
+            } else {
+              T* e = reinterpret_cast<T*>(raw[i]);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) e[k] = src[k];
+            }
+          }
+          tok += tok_step;
+          head += head_step;
+          if (head >= group) {
+            head -= group;
+            ++tok;
+          }
+        }
+      };
+      load_q(row0);
       if (n_it > 0 && !wait(q_free, n_it - 1)) {
         ok = false;
         break;
       }
       float* undo_of = s_undo + (n_it & 1) * kUnitRows;
-      const int tiles = it.rows > kRows ? 2 : 1;
-      for (int r = row0; r < tiles * kRows; r += kRowStep) {
-        uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-        if (r < it.rows) {
-          const int row = it.row0 + r;
-          const T* src = static_cast<const T*>(ap.q) + (it.t0 + row / group) * ap.ldq +
-                         static_cast<long long>(h_kv * group + row % group) * HD + 16 * c;
-          if (ap.vec) {
-            raw[0] = reinterpret_cast<const uint4*>(src)[0];
-            raw[1] = reinterpret_cast<const uint4*>(src)[1];
-          } else {
-            T* e = reinterpret_cast<T*>(raw);
-            for (int k = 0; k < 16; ++k) e[k] = src[k];
+#pragma unroll 1
+      for (int r0 = row0; r0 < rows_up; r0 += kTogether * kRowStep) {
+        if (r0 != row0) load_q(r0);
+#pragma unroll
+        for (int i = 0; i < kTogether; ++i) {
+          const int r = r0 + i * kRowStep;
+          float undo = 1.0f;
+          uint32_t* w = reinterpret_cast<uint32_t*>(raw[i]);
+          if constexpr (H16Traits<T>::kBf16) {
+            float shift = 1.0f;
+            // the largest magnitude, in pairs: of two finite bf16 the larger bits are
+            // the larger magnitude, and those of infinities and NaN are larger still
+            uint32_t top = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = __vmaxu2(top, w[k] & 0x7FFF7FFFu);
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            if (HD == 128) top = __vmaxu2(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+            const int ex = static_cast<int>(max(top & 0xFFFFu, top >> 16) >> 7) - 127;  // 2^ex <= it
+            if (top && ex < 128) {
+              const int up = min(14 - ex, 126);
+              shift = __int_as_float((up + 127) << 23);
+              undo = __int_as_float((127 - up) << 23);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              w[k] = cvt2_rn<__half>(
+                  make_float2(__uint_as_float(w[k] << 16) * shift, __uint_as_float(w[k] & 0xFFFF0000u) * shift));
+            }
           }
+          if (ap.scale < 0.0f)  // the softmax takes a positive scale
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] ^= 0x80008000u;
+          if (r >= rows_up) break;
+          uint8_t* to = sQ + (r / kRows) * kTile + (r % kRows - row0) * 128;
+          *reinterpret_cast<uint4*>(to + to0) = raw[i][0];
+          *reinterpret_cast<uint4*>(to + to1) = raw[i][1];
+          if (c == 0) undo_of[r] = undo;
         }
-        float undo = 1.0f;
-        uint32_t* w = reinterpret_cast<uint32_t*>(raw);
-        if constexpr (H16Traits<T>::kBf16) {
-          const T* e = reinterpret_cast<const T*>(raw);
-          float big = 0.0f, shift = 1.0f;
-#pragma unroll
-          for (int k = 0; k < 16; ++k) big = fmaxf(big, fabsf(h2f<T>(e[k])));
-#pragma unroll
-          for (int o = 1; o < 4; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
-          if (HD == 128) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 8));
-          const int ex = (__float_as_int(big) >> 23) - 127;  // 2^ex <= big
-          if (big > 0.0f && ex < 128) {
-            const int up = min(14 - ex, 126);
-            shift = __int_as_float((up + 127) << 23);
-            undo = __int_as_float((127 - up) << 23);
-          }
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const T* e2 = reinterpret_cast<const T*>(&w[k]);
-            w[k] = cvt2_rn<__half>(make_float2(h2f<T>(e2[0]) * shift, h2f<T>(e2[1]) * shift));
-          }
-        }
-        if (ap.scale < 0.0f)  // the softmax takes a positive scale
-#pragma unroll
-          for (int k = 0; k < 8; ++k) w[k] ^= 0x80008000u;
-        uint8_t* to = sQ + (r / kRows) * kTile + (r % kRows - row0) * 128;
-        *reinterpret_cast<uint4*>(to + to0) = raw[0];
-        *reinterpret_cast<uint4*>(to + to1) = raw[1];
-        if (c == 0) undo_of[r] = undo;
       }
       fence_proxy_async_smem();
       mbar_arrive(&q_full[n_it & 1]);
@@ -510,8 +544,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
     const uint32_t qa = smem_u32(sQ), ka = smem_u32(sK), va = smem_u32(sV);
     for (int wi = 0; ok && wi < n_work; ++wi) {
       const Work& it = work[wi];
-      const int nj0 = it.jobs(0), nj1 = it.jobs(1);
-      const bool pair = it.pair;
+      const int nj0 = same(it.jobs(0)), nj1 = same(it.jobs(1)), cnt = same(it.cnt);
+      const bool pair = same(it.pair);
+      const uint32_t last = same(it.last_user(0)) ? 0 : 1;  // stream that frees a shared key tile
+      const uint64_t dq0 = sw128_kmajor_desc(qa), dq1 = sw128_kmajor_desc(pair ? qa + kTile : qa);
       if (!wait(&q_full[n_it & 1], n_it >> 1)) {
         ok = false;
         break;
@@ -519,54 +555,44 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
       int left = nj0 + nj1;  // S products to be issued
       // S of stream h's k-th job
       auto issue_s = [&](int h, int k) -> bool {
-        const uint32_t kt = g + it.key_tile(h, k);
+        const uint32_t kt = g + (pair ? k : 2 * k + h);
         if (!wait(&k_full[kt & 1], kt >> 1)) return false;
         tc_fence_after();
-        const uint64_t dq = sw128_kmajor_desc(qa + (pair ? h * kTile : 0));
-        const uint64_t dk = sw128_kmajor_desc(ka + (kt & 1) * kTile);
+        const uint64_t dq = h ? dq1 : dq0, dk = sw128_kmajor_desc(ka + (kt & 1) * kTile);
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks) {
           const uint32_t off = (ks >> 2) * (kHalf >> 4) + (ks & 3) * 2;
           mma_f16_e(tbase + h * 128, dq + off, dk + off, idS, ks > 0 ? 1u : 0u);
         }
         mma_commit_e(&s_full[h]);
-        if (it.last_user(h)) mma_commit_e(&k_empty[kt & 1]);
+        if (!pair || h == last) mma_commit_e(&k_empty[kt & 1]);
         if (--left == 0) mma_commit_e(q_free);
         return true;
       };
-#pragma unroll 1
-      for (int h = 0; h < 2 && ok; ++h)
-        if ((h ? nj1 : nj0) > 0) ok = issue_s(h, 0);
-      for (int k = 0; ok && k < max(nj0, nj1); ++k)
-#pragma unroll 1
-        for (int h = 0; h < 2 && ok; ++h) {
-          const int nj = h ? nj1 : nj0;
-          if (k >= nj) continue;
-          const uint32_t uses = h ? uses1 : uses0;
-          if (k == 0 && uses > 0 && !wait(&o_free[h], uses - 1)) {
-            ok = false;
-            break;
-          }
-          const uint32_t kt = g + it.key_tile(h, k);
-          if (!wait(&p_full[h], h ? jobs1 : jobs0) || !wait(&v_full[kt & 1], kt >> 1)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t tp = tbase + h * 128;
-          const uint64_t dv = sw128_mn_desc(va + (kt & 1) * kTile, kHalf, 1024);
+      // P V of stream h's k-th job, then S of its next
+      auto step = [&](int h, int k, int nj, uint32_t uses, uint32_t& jobs) -> bool {
+        if (k >= nj) return true;
+        if (k == 0 && uses > 0 && !wait(&o_free[h], uses - 1)) return false;
+        const uint32_t kt = g + (pair ? k : 2 * k + h);
+        if (!wait(&v_full[kt & 1], kt >> 1) || !wait(&p_full[h], jobs)) return false;
+        tc_fence_after();
+        const uint64_t dv = sw128_mn_desc(va + (kt & 1) * kTile, kHalf, 1024);
 #pragma unroll
-          for (int ks = 0; ks < kKeys / 16; ++ks)
-            mma_f16_ts_e(tbase + 256 + h * 128, tp + (ks >> 2) * 64 + (ks & 3) * 8, dv + ks * 128, idPV,
-                         (k > 0 || ks > 0) ? 1u : 0u);
-          mma_commit_e(&o_ready[h]);
-          if (it.last_user(h)) mma_commit_e(&v_empty[kt & 1]);
-          ++(h ? jobs1 : jobs0);
-          if (k + 1 < nj) ok = issue_s(h, k + 1);
-        }
+        for (int ks = 0; ks < kKeys / 16; ++ks)
+          mma_f16_ts_e(tbase + 256 + h * 128, tbase + h * 128 + (ks >> 2) * 64 + (ks & 3) * 8, dv + ks * 128, idPV,
+                       (k > 0 || ks > 0) ? 1u : 0u);
+        mma_commit_e(&o_ready[h]);
+        if (!pair || h == last) mma_commit_e(&v_empty[kt & 1]);
+        ++jobs;
+        return k + 1 >= nj || issue_s(h, k + 1);
+      };
+      if (nj0 > 0) ok = issue_s(0, 0);
+      if (ok && nj1 > 0) ok = issue_s(1, 0);
+      for (int k = 0; ok && k < max(nj0, nj1); ++k)
+        ok = step(0, k, nj0, uses0, jobs0) && step(1, k, nj1, uses1, jobs1);
       uses0 += nj0 > 0;
       uses1 += nj1 > 0;
-      g += it.cnt;
+      g += cnt;
       ++n_it;
     }
   } else if (warp == kConvWarps + 1) {
@@ -582,12 +608,29 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
       for (int j = 0; ok && j < it.cnt; ++j) {
         const int now[2] = {next[0], next[1]};
         if (j + 1 < it.cnt) look(it.k0 + j + 1);
+        float ks = 0.0f, vs = 1.0f;  // lanes 0 and 1: of their pages
+        if (lane < 2 && good(now[lane & 1])) {
+          const long long at = static_cast<long long>(now[lane & 1]) * ap.nkv + it.h;
+          ks = ap.kscale[at];
+          vs = usable_vscale(ap.vscale[at]);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i, ++pages) {  // K, K, V, V
           const int slot = pages % kRing, page = now[i & 1];
           if (!wait(&r_empty[slot], pages / kRing + 1)) {
             ok = false;
             break;
+          }
+          if (i == 1) {
+            // Four key tiles back, the softmax is done with this place: the page before
+            // this one needed the ring's last K page converted, and with it the V
+            // tile before that, whose slot was free only after the P V product two
+            // tiles further back.
+            if (lane < 2)
+              sc[(g % kScales) * 2 + lane] = make_float4(ks, lg2_approx(vs), rcp_approx(vs), good(now[lane & 1]) ? 1.0f : 0.0f);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sc_full[g % kScales]);
+            ++g;
           }
           if (lane == 0) {
             r_ok[slot] = good(page);
@@ -611,22 +654,53 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tbase + h * 128 + lane_off, tO = tbase + 256 + h * 128 + lane_off;
-    const float scale = fmaxf(fabsf(ap.scale) * kLog2e, 1.1754944e-38f);  // 0 would lose the masks
+    constexpr float kTiny = 1.1754944e-38f;  // a factor of 0 would lose the masks (0 . -inf is NaN)
+    const float scale = fabsf(ap.scale) * kLog2e;
     uint32_t& jobs = jobs0;
     for (int wi = 0; ok && wi < n_work; ++wi) {
       const Work& it = work[wi];
+      // Dims 32 quarter .. of the results (all of them: any bit, quarter -1) that NaN
+      // codes of V of tokens [from, to) below lim spoil.  The warp looks at 32 / kCpr
+      // tokens at a time, a unit of 16 dims a lane.
+      auto nan_dims = [&](int from, int to, int lim, int quarter) {
+        uint32_t mask = 0;
+#pragma unroll 1
+        for (int key0 = from; key0 < to; key0 += 32 / kCpr) {
+          const int key = key0 + lane / kCpr, page = key < to ? it.bt[key / kPage] : -1;
+          uint32_t bits = 0;
+          if (good(page)) {
+            const uint4 d = __ldg(reinterpret_cast<const uint4*>(
+                ap.vpool + ((static_cast<long long>(page) * ap.nkv + it.h) * kPage + (key & 63)) * HD +
+                16 * (lane % kCpr)));
+            auto four = [](uint32_t w) {  // the NaN codes of a word, a bit each
+              const uint32_t n = nan_codes(w) >> 7;
+              return (n & 1u) | (n >> 7 & 2u) | (n >> 14 & 4u) | (n >> 21 & 8u);
+            };
+            bits = four(d.x) | four(d.y) << 4 | four(d.z) << 8 | four(d.w) << 12;
+          }
+          if (!__any_sync(0xFFFFFFFFu, bits != 0)) continue;
+#pragma unroll 1
+          for (int l2 = 0; l2 < 32; ++l2) {
+            const uint32_t b = __shfl_sync(0xFFFFFFFFu, bits, l2);
+            const int its_key = __shfl_sync(0xFFFFFFFFu, key, l2), unit = l2 % kCpr;
+            if (its_key < lim && (quarter < 0 || unit / 2 == quarter)) mask |= b << (16 * (unit & 1));
+          }
+        }
+        return mask;
+      };
       const int nj = it.jobs(h);
       const int ur = it.pair ? h * kRows + r : r;  // the unit's row
       const int row = it.row0 + ur, tok = row / group;
       const bool valid = ur < it.rows;
       if (it.pair && h == 1 && it.rows <= kRows) {  // no such tile
         ++n_it;
+        g += it.cnt;
         continue;
       }
       const int lim = !valid ? 0 : ap.causal ? max(0, min(it.len, it.past + tok + 1)) : it.len;  // tokens it sees
       const int h_kv = it.h;
       float m = -INFINITY, l = 0.0f;
-      uint32_t nan[4] = {0, 0, 0, 0};  // results that a seen NaN code of V spoils
+      bool spoiled = false;  // some results, by a NaN code of V that was taken out
       float kf = 0.0f;
       if (nj > 0) {
         if (!wait(&q_full[n_it & 1], n_it >> 1)) {
@@ -636,33 +710,14 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
         kf = s_undo[(n_it & 1) * kUnitRows + ur] * scale;
       }
       ++n_it;
-      // scales of a key tile's pages
-      float ks_n[2], vs_n[2];
-      bool on_n[2];
-      auto scales = [&](int kt) {
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const int page = kt * kKeys + p * kPage < it.seen ? it.bt[2 * kt + p] : -1;
-          on_n[p] = good(page);
-          const long long at = static_cast<long long>(on_n[p] ? page : 0) * ap.nkv + h_kv;
-          ks_n[p] = ap.kscale[at];
-          vs_n[p] = ap.vscale[at];
-        }
-      };
-      if (nj > 0) scales(it.k0 + it.key_tile(h, 0));
       for (int k = 0; k < nj; ++k, ++jobs) {
         const int kt = it.k0 + it.key_tile(h, k);
-        float f[2], lv[2], ivs[2];
-        int n_see[2];  // of the two pages' tokens
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const float vs = usable_vscale(vs_n[p]);
-          f[p] = ks_n[p] * kf;
-          lv[p] = lg2_approx(vs);
-          ivs[p] = rcp_approx(vs);
-          n_see[p] = on_n[p] ? lim - kt * kKeys - p * kPage : 0;
+        const uint32_t place = g + it.key_tile(h, k);
+        if (!wait(&sc_full[place % kScales], place / kScales)) {
+          ok = false;
+          break;
         }
-        if (k + 1 < nj) scales(it.k0 + it.key_tile(h, k + 1));
+        const float4* pg = sc + (place % kScales) * 2;
         if (!wait(&s_full[h], jobs)) {
           ok = false;
           break;
@@ -671,10 +726,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
         uint32_t x[64];
         auto fetch = [&](int p) {
           tmem_ld_x64(tS + p * 64, x);
-          if (n_see[p] < 64)
+          const int see = pg[p].w != 0.0f ? lim - kt * kKeys - p * kPage : 0;
+          if (see < 64)
 #pragma unroll
             for (int i = 0; i < 64; ++i)
-              if (i >= n_see[p]) x[i] = __float_as_uint(-INFINITY);
+              if (i >= see) x[i] = __float_as_uint(-INFINITY);
         };
         float top = -INFINITY;
 #pragma unroll
@@ -684,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
 #pragma unroll
           for (int i = 0; i < 64; ++i) t4[i & 3] = fmaxf(t4[i & 3], __uint_as_float(x[i]));
           const float t = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-          top = fmaxf(top, fmaf(t, f[p], lv[p]));
+          top = fmaxf(top, fmaf(t, fmaxf(pg[p].x * kf, kTiny), pg[p].y));
         }
         const bool grow = top > m + kSlack;
         float alpha = 1.0f;
@@ -714,55 +770,29 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
         for (int q = 0; q < 2; ++q) {
           const int p = 1 - q;
           if (q == 1) fetch(p);
-          const float up = lv[p] + (kLift - ref);
+          const float4 of = pg[p];
+          const float up = of.y + (kLift - ref), fp = fmaxf(of.x * kf, kTiny);
           float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float p0 = ex2_approx(fmaf(__uint_as_float(x[32 * half + 2 * e]), f[p], up));
-              const float p1 = ex2_approx(fmaf(__uint_as_float(x[32 * half + 2 * e + 1]), f[p], up));
+              const float p0 = ex2_approx(fmaf(__uint_as_float(x[32 * half + 2 * e]), fp, up));
+              const float p1 = ex2_approx(fmaf(__uint_as_float(x[32 * half + 2 * e + 1]), fp, up));
               s4[e & 3] += p0 + p1;
               w[e] = cvt2_rn<__half>(make_float2(p0, p1));
             }
             tmem_st_x16(tS + p * 64 + half * 16, w);
           }
-          l = fmaf((s4[0] + s4[1]) + (s4[2] + s4[3]), ivs[p], l);
+          l = fmaf((s4[0] + s4[1]) + (s4[2] + s4[3]), of.z, l);
         }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&p_full[h]);
         // ---- NaN codes of V that only some rows see
-        if ((kt + 1) * kKeys > it.all) {
-          const int from = max(it.all, kt * kKeys), to = min(it.seen, (kt + 1) * kKeys);
-          for (int key0 = from; key0 < to; key0 += 32 / kCpr) {
-            // the warp looks at 32 / kCpr tokens at a time, a unit a lane
-            const int key = key0 + lane / kCpr;
-            uint32_t bits = 0;
-            const int page = key < to ? it.bt[key / kPage] : -1;
-            if (good(page)) {
-              const uint4 d = __ldg(reinterpret_cast<const uint4*>(
-                  ap.vpool + ((static_cast<long long>(page) * ap.nkv + h_kv) * kPage + (key & 63)) * HD +
-                  16 * (lane % kCpr)));
-              auto four = [](uint32_t w) {  // the NaN codes of a word, a bit each
-                const uint32_t n = nan_codes(w) >> 7;
-                return (n & 1u) | (n >> 7 & 2u) | (n >> 14 & 4u) | (n >> 21 & 8u);
-              };
-              bits = four(d.x) | four(d.y) << 4 | four(d.z) << 8 | four(d.w) << 12;
-            }
-            if (!__any_sync(0xFFFFFFFFu, bits != 0)) continue;
-#pragma unroll 1
-            for (int from_lane = 0; from_lane < 32; ++from_lane) {
-              const uint32_t b = __shfl_sync(0xFFFFFFFFu, bits, from_lane);
-              const int its_key = __shfl_sync(0xFFFFFFFFu, key, from_lane), unit = from_lane % kCpr;
-              if (b && its_key < lim)
-#pragma unroll
-                for (int y = 0; y < 4; ++y)
-                  if (y == unit / 2) nan[y] |= b << (16 * (unit & 1));
-            }
-          }
-        }
+        if ((kt + 1) * kKeys > it.all)
+          spoiled |= nan_dims(max(it.all, kt * kKeys), min(it.seen, (kt + 1) * kKeys), lim, -1) != 0;
       }
       if (!ok) break;
       if (nj > 0 && !wait(&o_ready[h], jobs - 1)) {
@@ -795,11 +825,19 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0.0f;
         }
-        const uint32_t bad = q == 0 ? nan[0] : q == 1 ? nan[1] : q == 2 ? nan[2] : nan[3];
-        if (bad)
+        if (__any_sync(0xFFFFFFFFu, spoiled)) {
+          // this chunk's tokens of the stream, which the warp has seen to hold some
+          uint32_t bad = 0;
+#pragma unroll 1
+          for (int k = 0; k < nj; ++k) {
+            const int kt = it.k0 + it.key_tile(h, k);
+            if ((kt + 1) * kKeys > it.all)
+              bad |= nan_dims(max(it.all, kt * kKeys), min(it.seen, (kt + 1) * kKeys), lim, q);
+          }
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (bad >> e & 1) o[e] = NAN;
+        }
         if (part) {
           if (valid)
 #pragma unroll
@@ -823,6 +861,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
         tc_fence_before();
         mbar_arrive(&o_free[h]);
       }
+      g += it.cnt;
     }
   }
     if (!ok && lane == 0) fail();
