@@ -2,6 +2,8 @@
 // conversion, where results go, and the kernel that joins the parts of a sequence.
 #pragma once
 
+#include <algorithm>
+
 #include "kernels.cuh"
 #include "sm100.cuh"
 
@@ -113,7 +115,7 @@ constexpr int kJoinWarps = 8;
 
 // grid: (sequences x tiles, K/V heads, rows, or rows / 8)
 template <typename T, int HD, typename Plan>
-__global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const __grid_constant__ CacheAttnParams ap) {
+__global__ void __launch_bounds__(kJoinWarps * 32, Plan::kAlone ? 4 : 2) cache_attn_join(const __grid_constant__ CacheAttnParams ap) {
   constexpr int kLanes = HD / 4, kPer = 32 / kLanes;  // lanes of a part, parts of a warp at once
   __shared__ float s_l[kJoinWarps];
   __shared__ float4 s_o[kJoinWarps][kLanes];
@@ -129,11 +131,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const __grid_
   const int n = Plan::parts(ap, sp, s, tile);
   if (n == 0) return;
   constexpr bool alone = Plan::kAlone;
-  const int r = alone ? kJoinWarps * blockIdx.z + warp : blockIdx.z;
-  if (r >= rows) return;  // the CTA's warps end together, or work alone
   const UnitAt at{s, tile, h, sp.t0};
   const float* parts = unit_parts(ap, at);
-  const int l_at = (ap.part_rows + 3) & ~3, o_at = 2 * l_at + r * HD;
+  const int l_at = (ap.part_rows + 3) & ~3;
+  // the CTA's warps share row blockIdx.z, or take rows of their own
+  for (int r = alone ? kJoinWarps * blockIdx.z + warp : blockIdx.z; r < rows; r += (alone ? kJoinWarps : 1) * gridDim.z) {
+  const int o_at = 2 * l_at + r * HD;
   const int first = (alone ? 0 : warp * kPer) + lane / kLanes, step = alone ? kPer : kPer * kJoinWarps;
   const int d = lane % kLanes;
   float big = -INFINITY;
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const __grid_
   const float ref = big == -INFINITY ? 0.0f : big;
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float sum = 0.0f;
-  constexpr int kBatch = 8;  // parts whose loads are in flight together
+  constexpr int kBatch = alone ? 4 : 8;  // parts whose loads are in flight together
   for (int k0 = first; k0 < n; k0 += kBatch * step) {
     float4 y[kBatch];
     float pm[kBatch], pl[kBatch];
@@ -198,13 +201,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_attn_join(const __grid_
     if (d == 0) close_row(ap, at, row, big, sum);
     finish_row<T, HD>(ap, at, row, 4 * d, v, sum == 0.0f ? 0.0f : 1.0f / sum);
   }
+  }
 }
 
 template <typename T, int HD, typename Plan>
 cudaError_t launch_join(const CacheAttnParams& ap, cudaStream_t s) {
   const long long x = static_cast<long long>(ap.seqs.n_seqs) * ap.tiles_max;
   if (x > 0x7FFFFFFFll || ap.nkv > 65535) return cudaErrorInvalidValue;
-  const int z = Plan::kAlone ? (ap.part_rows + kJoinWarps - 1) / kJoinWarps : ap.part_rows;
+  const int z = Plan::kAlone ? std::min((ap.part_rows - 1) / kJoinWarps + 1, 8) : ap.part_rows;
   return launch_pdl(cache_attn_join<T, HD, Plan>, dim3(static_cast<unsigned>(x), ap.nkv, z), dim3(kJoinWarps * 32), 0,
                     s, ap);
 }

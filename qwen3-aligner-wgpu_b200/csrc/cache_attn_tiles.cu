@@ -227,7 +227,7 @@ template <int HD>
 struct Mem {
   static constexpr uint32_t kTile = kHalf * (HD / 64);  // Q, K or V
   static constexpr size_t kSmem = 6 * kTile + kRing * kPage * HD + 2 * kUnitRows * 4 + 512 +
-                                  kScales * 2 * sizeof(float4) + kBatch * sizeof(Work);
+                                  kScales * 2 * sizeof(float4) + kBatch * sizeof(Work) + sizeof(TileWalk);
 };
 
 template <typename T, int HD>
@@ -368,7 +368,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
   // of the MMAs are then made in uniform registers
   auto same = [](int v) { return __shfl_sync(0xFFFFFFFFu, v, 0); };
   auto good = [&](int page) { return page >= 0 && page < ap.kv_pages; };
-  TileWalk walk;  // thread 0's
+  // thread 0's, in shared memory: it would take registers of every thread otherwise
+  TileWalk& walk = *reinterpret_cast<TileWalk*>(work + kBatch);
   if (threadIdx.x == 0 && any) walk.begin(ap, static_cast<int>(share[3]), share[2], share[0], share[1]);
   bool ok = true;
   uint32_t n_it = 0;  // pieces of work before this one
@@ -444,26 +445,30 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
         }
         return true;
       };
-      // ---- queries: the first rows are on their way while the last item's products end
+      // ---- queries: copied to where their f16 values go (16 bits either way), all on
+      // their way at once, then bf16 converted in place.  Short loops: code that runs
+      // once a piece of work comes from beyond the instruction cache.
+      if (n_it > 0 && !wait(q_free, n_it - 1)) {
+        ok = false;
+        break;
+      }
       const int rows_up = it.rows > kRows ? 2 * kRows : kRows;
-      int tok = (it.row0 + row0) / group, head = (it.row0 + row0) % group;  // of the row to be read
-      const int tok_step = kRowStep / group, head_step = kRowStep % group;
-      constexpr int kTogether = 8;  // rows whose loads are in flight together
-      uint4 raw[kTogether][2];
-      auto load_q = [&](int r0) {
-#pragma unroll
-        for (int i = 0; i < kTogether; ++i) {
-          raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
-          if (r0 + i * kRowStep < it.rows) {
-            const T* src = static_cast<const T*>(ap.q) + (it.t0 + tok) * ap.ldq + (h_kv * group + head) * HD + 16 * c;
-            if (ap.vec) {
-              raw[i][0] = reinterpret_cast<const uint4*>(src)[0];
-              raw[i][1] = reinterpret_cast<const uint4*>(src)[1];
-            } else {
-              T* e = reinterpret_cast<T*>(raw[i]);
-#pragma unroll
-              for (int k = 0; k < 16; ++k) e[k] = src[k];
-            }
+      auto q_at = [&](int r, uint32_t unit) { return sQ + (r / kRows) * kTile + (r % kRows - row0) * 128 + unit; };
+      {
+        int tok = (it.row0 + row0) / group, head = (it.row0 + row0) % group;  // of the row to be read
+        const int tok_step = kRowStep / group, head_step = kRowStep % group;
+#pragma unroll 1
+        for (int r = row0; r < rows_up; r += kRowStep) {
+          const bool in = r < it.rows;
+          const T* src = static_cast<const T*>(ap.q);
+          if (in) src += (it.t0 + tok) * ap.ldq + (h_kv * group + head) * HD + 16 * c;
+          if (ap.vec) {
+            cp_async16(smem_u32(q_at(r, to0)), src, in ? 16 : 0);
+            cp_async16(smem_u32(q_at(r, to1)), src + (in ? 8 : 0), in ? 16 : 0);
+          } else {
+#pragma unroll 1
+            for (int k = 0; k < 16; ++k)
+              reinterpret_cast<T*>(q_at(r, k < 8 ? to0 : to1))[k % 8] = in ? src[k] : f2h<T>(0.0f);
           }
           tok += tok_step;
           head += head_step;
@@ -472,21 +477,17 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
             ++tok;
           }
         }
-      };
-      load_q(row0);
-      if (n_it > 0 && !wait(q_free, n_it - 1)) {
-        ok = false;
-        break;
+        cp_async_commit();
+        cp_async_wait_all();
       }
       float* undo_of = s_undo + (n_it & 1) * kUnitRows;
-#pragma unroll 1
-      for (int r0 = row0; r0 < rows_up; r0 += kTogether * kRowStep) {
-        if (r0 != row0) load_q(r0);
-#pragma unroll
-        for (int i = 0; i < kTogether; ++i) {
-          const int r = r0 + i * kRowStep;
-          float undo = 1.0f;
-          uint32_t* w = reinterpret_cast<uint32_t*>(raw[i]);
+      const bool flip = ap.scale < 0.0f;  // the softmax takes a positive scale
+#pragma unroll 2
+      for (int r = row0; r < rows_up; r += kRowStep) {
+        float undo = 1.0f;
+        if (H16Traits<T>::kBf16 || flip) {
+          uint4 raw[2] = {*reinterpret_cast<const uint4*>(q_at(r, to0)), *reinterpret_cast<const uint4*>(q_at(r, to1))};
+          uint32_t* w = reinterpret_cast<uint32_t*>(raw);
           if constexpr (H16Traits<T>::kBf16) {
             float shift = 1.0f;
             // the largest magnitude, in pairs: of two finite bf16 the larger bits are
@@ -504,20 +505,17 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
               undo = __int_as_float((127 - up) << 23);
             }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
+            for (int k = 0; k < 8; ++k)
               w[k] = cvt2_rn<__half>(
                   make_float2(__uint_as_float(w[k] << 16) * shift, __uint_as_float(w[k] & 0xFFFF0000u) * shift));
-            }
           }
-          if (ap.scale < 0.0f)  // the softmax takes a positive scale
+          if (flip)
 #pragma unroll
             for (int k = 0; k < 8; ++k) w[k] ^= 0x80008000u;
-          if (r >= rows_up) break;
-          uint8_t* to = sQ + (r / kRows) * kTile + (r % kRows - row0) * 128;
-          *reinterpret_cast<uint4*>(to + to0) = raw[i][0];
-          *reinterpret_cast<uint4*>(to + to1) = raw[i][1];
-          if (c == 0) undo_of[r] = undo;
+          *reinterpret_cast<uint4*>(q_at(r, to0)) = raw[0];
+          *reinterpret_cast<uint4*>(q_at(r, to1)) = raw[1];
         }
+        if (c == 0) undo_of[r] = undo;
       }
       fence_proxy_async_smem();
       mbar_arrive(&q_full[n_it & 1]);
