@@ -197,6 +197,15 @@ int qa_k_w4_linear(const void* x, long long ldx, int M, int K, const uint8_t* wq
                    int N, int group, const void* scales, const uint8_t* zeros, const float* bias,
                    void* out, long long ldo, int bf16, void* stream);
 
+/*
+ * The same three calls with their arguments in the same order in an array, but for
+ * the one float (pointers as integers): for callers through an interpreter, where
+ * passing 36 arguments one by one takes longer than the kernel.
+ */
+int qa_k_kv_append_v(const long long* args, float eps);
+int qa_k_cache_attention_v(const long long* args, float scale);
+int qa_k_w4_linear_v(const long long* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -62,7 +63,8 @@ EXPORTED = [
     "qa_local_head_enabled", "qa_local_head_refine",
     "qa_k_gemm", "qa_k_conv3x3s2", "qa_k_causal_attention", "qa_k_window_attention",
     "qa_k_conv1", "qa_k_gemm_qkv_rope", "qa_k_kv_append", "qa_k_cache_attention",
-    "qa_k_cache_attention_workspace", "qa_k_w4_linear",
+    "qa_k_cache_attention_workspace", "qa_k_w4_linear", "qa_k_kv_append_v",
+    "qa_k_cache_attention_v", "qa_k_w4_linear_v",
 ]
 
 c_void_p = ctypes.c_void_p
@@ -205,6 +207,9 @@ def _declare(L: ctypes.CDLL) -> None:
     L.qa_k_cache_attention_workspace.restype = ctypes.c_int64
     L.qa_k_w4_linear.argtypes = [c_void_p, c_ll, c_int, c_int, c_void_p, c_ll, c_int, c_int,
                                  c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_int, c_void_p]
+    L.qa_k_kv_append_v.argtypes = [ctypes.c_char_p, ctypes.c_float]
+    L.qa_k_cache_attention_v.argtypes = [ctypes.c_char_p, ctypes.c_float]
+    L.qa_k_w4_linear_v.argtypes = [ctypes.c_char_p]
     if hasattr(L, "qa_open"):
         L.qa_open.argtypes = [c_int, c_int, ctypes.POINTER(c_void_p)]
         L.qa_load.argtypes = [c_void_p, c_void_p, c_int, c_void_p]
@@ -389,66 +394,94 @@ def gemm_qkv_rope(A, B, q_out, pos_of, clip_of, block_tab, kc, vc, cos_t, sin_t,
 
 
 # ---------------------------------------------------------------- growing sessions
+# A decoding step calls these once a layer, so their checks read each attribute of a
+# tensor once and build a message only when something is wrong, and the arguments go
+# to the library as one array (qa_k_*_v).
+_pack35, _pack27, _pack15 = (struct.Struct(f"{n}q").pack for n in (35, 27, 15))
 
-def _need(ok, what) -> None:
-    if not ok:
+_F16 = _BF16 = _F32 = _I32 = _U8 = _E4M3 = None
+
+
+def _types():
+    global _F16, _BF16, _F32, _I32, _U8, _E4M3
+    import torch
+    _F16, _BF16, _F32, _I32, _U8, _E4M3 = (torch.float16, torch.bfloat16, torch.float32, torch.int32,
+                                           torch.uint8, torch.float8_e4m3fn)
+    return _F16
+
+
+def _rows(t, T, width, dt, name) -> int:
+    """Row stride of t, which is [T, width] of 16-bit `dt` with adjacent columns."""
+    if t.shape == (T, width) and t.dtype is dt:
+        ld, one = t.stride()
+        if T < 2:
+            ld = width
+        if (one == 1 or width == 1) and ld >= width:
+            return ld
+    raise ValueError(f"{name}: [{T}, {width}] of {dt} with adjacent columns")
+
+
+def _flat(t, shape, dt, what) -> None:
+    """t is a contiguous tensor of that shape and type."""
+    if t.dtype is not dt or t.shape != shape or not t.is_contiguous():
         raise ValueError(what)
 
 
-def _rows16(t, width, T, dtype, name) -> int:
-    """Row stride of t, which is [T, width] of 16-bit `dtype` with adjacent columns."""
-    ld = t.stride(0) if T > 1 else width
-    _need(t.dim() == 2 and t.shape[0] == T and t.shape[1] == width and t.dtype == dtype
-          and (t.stride(1) == 1 or width == 1) and ld >= width,
-          f"{name}: [{T}, {width}] of {dtype} with adjacent columns")
-    return ld
-
-
-def _on_device(*tensors) -> None:
-    dev = tensors[0].device
-    _need(all(t is None or (t.is_cuda and t.device == dev) for t in tensors),
-          "all tensors on one CUDA device")
-
-
-def _seq_args(T, q_start, kv_len, block_tab, kpool, vpool, max_q) -> tuple:
+def _seq_args(q_start, kv_len, block_tab, kpool, vpool, max_q) -> tuple:
     """Shapes of the sequence maps and pools; (n_seqs, max_pages, pages, nkv, hd)."""
-    import torch
-    i32 = torch.int32
-    _need(q_start.dtype == i32 and kv_len.dtype == i32 and block_tab.dtype == i32
-          and q_start.is_contiguous() and kv_len.is_contiguous() and block_tab.is_contiguous()
-          and q_start.dim() == 1 and kv_len.dim() == 1 and block_tab.dim() == 2
-          and q_start.shape[0] == kv_len.shape[0] + 1 == block_tab.shape[0] + 1
-          and block_tab.shape[1] > 0,
-          "q_start int32 [n + 1], kv_len int32 [n], block_tab int32 [n, max_pages], contiguous")
+    if (kv_len.dim() != 1 or block_tab.dim() != 2 or kpool.dim() != 4):
+        raise ValueError("kv_len [n], block_tab [n, max_pages], pools [pages, heads, 64, hd]")
+    n = kv_len.shape[0]
+    bt = block_tab.shape
+    what = "q_start int32 [n + 1], kv_len int32 [n], block_tab int32 [n, max_pages], contiguous"
+    _flat(q_start, (n + 1,), _I32, what)
+    _flat(kv_len, (n,), _I32, what)
+    _flat(block_tab, (n, bt[1]), _I32, what)
     ps = kpool.shape
-    _need(len(ps) == 4 and ps == vpool.shape and ps[2] == 64 and ps[3] in (64, 128)
-          and ps[0] > 0 and ps[1] > 0 and kpool.dtype == vpool.dtype
-          and kpool.is_contiguous() and vpool.is_contiguous(),
-          "kpool / vpool [pages, heads, 64, 64 or 128], contiguous, of one type")
-    _need(max_q >= 0, "max_q >= 0")
-    return kv_len.shape[0], block_tab.shape[1], ps[0], ps[1], ps[3]
+    pages, nkv, page, hd = ps
+    if (page != 64 or (hd != 64 and hd != 128) or pages == 0 or nkv == 0 or bt[1] == 0
+            or vpool.shape != ps or vpool.dtype is not kpool.dtype
+            or not kpool.is_contiguous() or not vpool.is_contiguous()):
+        raise ValueError("kpool / vpool [pages, heads, 64, 64 or 128], contiguous, of one type, and max_pages > 0")
+    if max_q < 0:
+        raise ValueError("max_q >= 0")
+    return n, bt[1], pages, nkv, hd
 
 
 def check_sequences(T, q_start, kv_len, block_tab, pages, max_q, appending) -> None:
     """Host-side range checks of the sequence maps (copies them to the host;
     ValueError on failure): what the kernels would otherwise report in *status."""
     import torch
+
+    def need(ok, what):
+        if not ok:
+            raise ValueError(what)
+
     qs, kl, bt = q_start.cpu().long(), kv_len.cpu().long(), block_tab.cpu().long()
     n = qs.diff()
     if n.numel() == 0:
         return
-    _need(int(qs[0]) >= 0 and int(n.min()) >= 0 and int(qs[-1]) <= T, "q_start out of range")
-    _need(int(n.max()) <= max_q, "a sequence has more than max_q new tokens")
-    _need(int(kl.min()) >= 0 and int(kl.max()) <= 64 * bt.shape[1], "kv_len out of range")
-    _need(not appending or bool((kl >= n).all()), "kv_len counts the new tokens")
+    need(int(qs[0]) >= 0 and int(n.min()) >= 0 and int(qs[-1]) <= T, "q_start out of range")
+    need(int(n.max()) <= max_q, "a sequence has more than max_q new tokens")
+    need(int(kl.min()) >= 0 and int(kl.max()) <= 64 * bt.shape[1], "kv_len out of range")
+    need(not appending or bool((kl >= n).all()), "kv_len counts the new tokens")
     used = torch.arange(bt.shape[1])[None] < ((kl + 63) // 64)[:, None]
     ids = bt[used]
-    _need(ids.numel() == 0 or (int(ids.min()) >= 0 and int(ids.max()) < pages),
-          "block_tab names a page outside the pools")
+    need(ids.numel() == 0 or (int(ids.min()) >= 0 and int(ids.max()) < pages),
+         "block_tab names a page outside the pools")
     if appending:
         first = ((kl - n) // 64)[:, None]
         written = bt[used & (torch.arange(bt.shape[1])[None] >= first) & (n > 0)[:, None]]
-        _need(written.unique().numel() == written.numel(), "two sequences append to one page")
+        need(written.unique().numel() == written.numel(), "two sequences append to one page")
+
+
+def _stream(dev, stream):
+    import torch
+    return torch.cuda.current_stream(dev).cuda_stream if stream is None else stream
+
+
+def _elsewhere():
+    raise ValueError("all tensors on one CUDA device")
 
 
 def kv_append(q, k, v, q_out, q_start, kv_len, block_tab, kpool, vpool, *, max_q, kscale=None,
@@ -466,62 +499,95 @@ def kv_append(q, k, v, q_out, q_start, kv_len, block_tab, kpool, vpool, *, max_q
     to the host to check them; without it, what is malformed sets bit 2 of
     `status` (int32 [1]) and is skipped.
     """
-    import torch
-    T, dt = q.shape[0], q.dtype
-    n, max_pages, pages, nkv, hd = _seq_args(T, q_start, kv_len, block_tab, kpool, vpool, max_q)
-    _need(dt in (torch.float16, torch.bfloat16), "q, k and v are float16 or bfloat16")
-    width = q.shape[1] if q.dim() == 2 else 0
+    if _F16 is None:
+        _types()
+    n, max_pages, pages, nkv, hd = _seq_args(q_start, kv_len, block_tab, kpool, vpool, max_q)
+    dt = q.dtype
+    if q.dim() != 2 or (dt is not _F16 and dt is not _BF16):
+        raise ValueError("q [T, heads * hd] float16 or bfloat16")
+    T, width = q.shape
     nq = width // hd
-    _need(nq > 0 and nq % nkv == 0, "q has a multiple of the cache's heads")
-    ldq, ldqo = _rows16(q, nq * hd, T, dt, "q"), _rows16(q_out, nq * hd, T, dt, "q_out")
-    ldk, ldv = _rows16(k, nkv * hd, T, dt, "k"), _rows16(v, nkv * hd, T, dt, "v")
-    f32 = torch.float32
-    if kscale is None:
-        _need(vscale is None and kpool.dtype == dt, "pools of q's type, or e4m3 with both scales")
+    if nq == 0 or nq % nkv or nq * hd != width:
+        raise ValueError("q has a multiple of the cache's heads")
+    kw = nkv * hd
+    ldq, ldqo = _rows(q, T, width, dt, "q"), _rows(q_out, T, width, dt, "q_out")
+    ldk, ldv = _rows(k, T, kw, dt, "k"), _rows(v, T, kw, dt, "v")
+    dev = q.get_device()
+    if dev < 0 or not (k.get_device() == v.get_device() == q_out.get_device() == q_start.get_device()
+                       == kv_len.get_device() == block_tab.get_device() == kpool.get_device()
+                       == vpool.get_device() == dev):
+        here = False
     else:
-        _need(vscale is not None and kpool.dtype == torch.float8_e4m3fn
-              and all(x.dtype == f32 and x.is_contiguous() and tuple(x.shape) == (pages, nkv)
-                      for x in (kscale, vscale)),
-              "e4m3 pools with kscale and vscale f32 [pages, heads]")
+        here = True
+    ks = vs = cs = sn = ps = ax = gq = gk = st = 0
+    if kscale is None:
+        if vscale is not None or kpool.dtype is not dt:
+            raise ValueError("pools of q's type, or e4m3 with both scales")
+    else:
+        if vscale is None or kpool.dtype is not _E4M3:
+            raise ValueError("e4m3 pools with kscale and vscale f32 [pages, heads]")
+        _flat(kscale, (pages, nkv), _F32, "kscale f32 [pages, heads]")
+        _flat(vscale, (pages, nkv), _F32, "vscale f32 [pages, heads]")
+        ks, vs = kscale.data_ptr(), vscale.data_ptr()
+        here = here and kscale.get_device() == dev and vscale.get_device() == dev
     rows, axes, stride = 0, 1, 0
     if cos is not None:
+        if sin is None or cos.dim() != 2 or cos.shape[0] == 0:
+            raise ValueError("cos and sin f32 [rows, hd / 2]")
         rows = cos.shape[0]
-        _need(sin is not None and rows > 0
-              and all(x.dtype == f32 and x.is_contiguous() and tuple(x.shape) == (rows, hd // 2)
-                      for x in (cos, sin)), "cos and sin f32 [rows, hd / 2]")
+        _flat(cos, (rows, hd // 2), _F32, "cos f32 [rows, hd / 2]")
+        _flat(sin, (rows, hd // 2), _F32, "sin f32 [rows, hd / 2]")
+        cs, sn = cos.data_ptr(), sin.data_ptr()
+        here = here and cos.get_device() == dev and sin.get_device() == dev
         if pos is not None:
-            _need(pos.dtype == torch.int32 and pos.dim() in (1, 2) and pos.shape[-1] == T
-                  and (T < 2 or pos.stride(-1) == 1), "pos int32 [T] or [axes, T]")
-            if pos.dim() == 2:
+            d = pos.dim()
+            if (pos.dtype is not _I32 or d not in (1, 2) or pos.shape[-1] != T
+                    or (T > 1 and pos.stride(-1) != 1)):
+                raise ValueError("pos int32 [T] or [axes, T]")
+            if d == 2:
                 axes, stride = pos.shape[0], pos.stride(0)
-            _need(1 <= axes <= 4, "one to four axes")
-            _need(axes == 1 or (axis_of is not None and axis_of.dtype == torch.int32
-                                and axis_of.is_contiguous() and tuple(axis_of.shape) == (hd // 2,)),
-                  "axis_of int32 [hd / 2] for several axes")
-    else:
-        _need(sin is None and pos is None, "sin and pos go with cos")
+            if not 1 <= axes <= 4:
+                raise ValueError("one to four axes")
+            ps = pos.data_ptr()
+            here = here and pos.get_device() == dev
+            if axes > 1:
+                if axis_of is None:
+                    raise ValueError("axis_of int32 [hd / 2] for several axes")
+                _flat(axis_of, (hd // 2,), _I32, "axis_of int32 [hd / 2]")
+                ax = axis_of.data_ptr()
+                here = here and axis_of.get_device() == dev
+    elif sin is not None or pos is not None:
+        raise ValueError("sin and pos go with cos")
     if qn is not None or kn is not None:
-        _need(qn is not None and kn is not None
-              and all(x.dtype == f32 and x.is_contiguous() and tuple(x.shape) == (hd,)
-                      for x in (qn, kn)), "qn and kn f32 [hd]")
+        if qn is None or kn is None:
+            raise ValueError("qn and kn go together")
+        _flat(qn, (hd,), _F32, "qn f32 [hd]")
+        _flat(kn, (hd,), _F32, "kn f32 [hd]")
+        gq, gk = qn.data_ptr(), kn.data_ptr()
+        here = here and qn.get_device() == dev and kn.get_device() == dev
+    if status is not None:
+        st = status.data_ptr()
+        here = here and status.get_device() == dev
     if validate:
         check_sequences(T, q_start, kv_len, block_tab, pages, max_q, True)
         if axes > 1:
             a = axis_of.cpu()
-            _need(int(a.min()) >= 0 and int(a.max()) < axes, "axis_of out of range")
-        if pos is not None and T:
-            _need(int(pos.min()) >= 0 and int(pos.max()) < rows, "pos outside the tables")
-        elif cos is not None and n:
-            _need(int(kv_len.max()) <= rows, "kv_len outside the tables")
-    _on_device(q, k, v, q_out, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale, cos, sin,
-               pos, axis_of, qn, kn, status)
-    s = stream if stream is not None else torch.cuda.current_stream(q.device).cuda_stream
-    check(lib().qa_k_kv_append(
-        q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
-        q_out.data_ptr(), ldqo, T, nq, nkv, hd, q_start.data_ptr(), kv_len.data_ptr(),
-        n, max_q, block_tab.data_ptr(), max_pages, kpool.data_ptr(), vpool.data_ptr(), pages,
-        ptr(kscale), ptr(vscale), ptr(cos), ptr(sin), rows, ptr(pos), stride, axes, ptr(axis_of),
-        ptr(qn), ptr(kn), eps, 1 if dt == torch.bfloat16 else 0, ptr(status), s))
+            if int(a.min()) < 0 or int(a.max()) >= axes:
+                raise ValueError("axis_of out of range")
+        if pos is not None:
+            if T and (int(pos.min()) < 0 or int(pos.max()) >= rows):
+                raise ValueError("pos outside the tables")
+        elif cos is not None and n and int(kv_len.max()) > rows:
+            raise ValueError("kv_len outside the tables")
+    if not here:
+        _elsewhere()
+    rc = _fn_kv_append()(_pack35(
+        q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, q_out.data_ptr(), ldqo, T, nq, nkv,
+        hd, q_start.data_ptr(), kv_len.data_ptr(), n, max_q, block_tab.data_ptr(), max_pages,
+        kpool.data_ptr(), vpool.data_ptr(), pages, ks, vs, cs, sn, rows, ps, stride, axes, ax, gq, gk,
+        1 if dt is _BF16 else 0, st, _stream(dev, stream)), eps)
+    if rc:
+        check(rc)
 
 
 _workspaces: dict = {}  # (device, stream) -> the attention's workspace
@@ -535,39 +601,62 @@ def cache_attention(q, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale,
     q and out [T, nq * hd] 16-bit; the maps, pools and scales as for kv_append;
     lse f32 [T, nq] optional; scale defaults to 1 / sqrt(hd).  max_q and max_kv
     bound the sequences' new and cached tokens.  `validate` copies the maps to
-    the host to check them.  A workspace is kept for each stream and
-    grows with the sizes seen (outside of graph capture).
+    the host to check them.  A workspace is kept for each stream and grows with
+    the sizes seen (outside of graph capture).
     """
-    import torch
-    T, dt = q.shape[0], q.dtype
-    n, max_pages, pages, nkv, hd = _seq_args(T, q_start, kv_len, block_tab, kpool, vpool, max_q)
-    _need(dt in (torch.float16, torch.bfloat16), "q and out are float16 or bfloat16")
-    f32 = torch.float32
-    _need(kpool.dtype == torch.float8_e4m3fn and kscale.dtype == f32 and vscale.dtype == f32
-          and kscale.shape == vscale.shape == (pages, nkv) and kscale.is_contiguous()
-          and vscale.is_contiguous(), "e4m3 pools with kscale and vscale f32 [pages, heads]")
-    nq = q.shape[1] // hd if q.dim() == 2 else 0
-    _need(nq > 0 and nq % nkv == 0, "q has a multiple of the cache's heads")
-    ldq, ldo = _rows16(q, nq * hd, T, dt, "q"), _rows16(out, nq * hd, T, dt, "out")
-    _need(lse is None or (lse.dtype == f32 and lse.is_contiguous() and lse.shape == (T, nq)),
-          "lse f32 [T, heads]")
-    _need(max_kv >= 0, "max_kv >= 0")
+    if _F16 is None:
+        _types()
+    n, max_pages, pages, nkv, hd = _seq_args(q_start, kv_len, block_tab, kpool, vpool, max_q)
+    dt = q.dtype
+    if q.dim() != 2 or (dt is not _F16 and dt is not _BF16):
+        raise ValueError("q [T, heads * hd] float16 or bfloat16")
+    if kpool.dtype is not _E4M3:
+        raise ValueError("e4m3 pools")
+    _flat(kscale, (pages, nkv), _F32, "kscale f32 [pages, heads]")
+    _flat(vscale, (pages, nkv), _F32, "vscale f32 [pages, heads]")
+    T, width = q.shape
+    nq = width // hd
+    if nq == 0 or nq % nkv or nq * hd != width:
+        raise ValueError("q has a multiple of the cache's heads")
+    ldq, ldo = _rows(q, T, width, dt, "q"), _rows(out, T, width, dt, "out")
+    if max_kv < 0:
+        raise ValueError("max_kv >= 0")
+    ls = st = 0
+    dev = q.get_device()
+    here = dev >= 0 and (out.get_device() == q_start.get_device() == kv_len.get_device()
+                         == block_tab.get_device() == kpool.get_device() == vpool.get_device()
+                         == kscale.get_device() == vscale.get_device() == dev)
+    if lse is not None:
+        _flat(lse, (T, nq), _F32, "lse f32 [T, heads]")
+        ls = lse.data_ptr()
+        here = here and lse.get_device() == dev
+    if status is not None:
+        st = status.data_ptr()
+        here = here and status.get_device() == dev
     if validate:
         check_sequences(T, q_start, kv_len, block_tab, pages, max_q, False)
-        _need(n == 0 or int(kv_len.max()) <= max_kv, "a cache is longer than max_kv")
-    _on_device(q, out, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale, lse, status)
-    s = stream if stream is not None else torch.cuda.current_stream(q.device).cuda_stream
-    need = lib().qa_k_cache_attention_workspace(nq, nkv, hd, n, max_q, max_kv)
-    ws = _workspaces.get((q.device, s)) if need else None
-    if need and (ws is None or ws.numel() < need):
-        torch.cuda.synchronize(q.device)  # nobody uses the old one
-        ws = _workspaces[(q.device, s)] = torch.empty(need, dtype=torch.uint8, device=q.device)
-    check(lib().qa_k_cache_attention(
+        if n and int(kv_len.max()) > max_kv:
+            raise ValueError("a cache is longer than max_kv")
+    if not here:
+        _elsewhere()
+    s = _stream(dev, stream)
+    call, size = _fn_cache_attention()
+    need = size(nq, nkv, hd, n, max_q, max_kv)
+    ws = 0
+    if need:
+        buf = _workspaces.get((dev, s))
+        if buf is None or buf.numel() < need:
+            import torch
+            torch.cuda.synchronize(dev)  # nobody uses the old one
+            buf = _workspaces[(dev, s)] = torch.empty(need, dtype=_U8, device=q.device)
+        ws = buf.data_ptr()
+    rc = call(_pack27(
         q.data_ptr(), ldq, T, nq, nkv, hd, q_start.data_ptr(), kv_len.data_ptr(), n, max_q,
         max_kv, block_tab.data_ptr(), max_pages, kpool.data_ptr(), vpool.data_ptr(), pages,
-        kscale.data_ptr(), vscale.data_ptr(), hd ** -0.5 if scale is None else scale,
-        1 if causal else 0, out.data_ptr(), ldo, ptr(lse), ptr(ws), need,
-        1 if dt == torch.bfloat16 else 0, ptr(status), s))
+        kscale.data_ptr(), vscale.data_ptr(), 1 if causal else 0, out.data_ptr(), ldo, ls, ws, need,
+        1 if dt is _BF16 else 0, st, s), hd ** -0.5 if scale is None else scale)
+    if rc:
+        check(rc)
 
 
 def w4_linear(x, wq, scales, out, *, zeros=None, bias=None, stream=None):
@@ -577,24 +666,56 @@ def w4_linear(x, wq, scales, out, *, zeros=None, bias=None, stream=None):
     group 32, 64 or 128 (told by the shapes); zeros uint8 like scales (None: 8);
     bias f32 [N].
     """
-    import torch
+    if _F16 is None:
+        _types()
     dt = x.dtype
-    _need(dt in (torch.float16, torch.bfloat16) and x.dim() == 2, "x [M, K] float16 or bfloat16")
+    if x.dim() != 2 or wq.dim() != 2 or scales.dim() != 2 or (dt is not _F16 and dt is not _BF16):
+        raise ValueError("x [M, K] float16 or bfloat16, wq [N, K / 2], scales [N, K / group]")
     M, K = x.shape
-    _need(wq.dim() == 2 and wq.dtype == torch.uint8 and 2 * wq.shape[1] == K
-          and wq.stride(1) == 1 and wq.stride(0) >= wq.shape[1], "wq uint8 [N, K / 2]")
-    N = wq.shape[0]
-    _need(scales.dim() == 2 and scales.dtype == dt and scales.shape[0] == N
-          and scales.is_contiguous() and scales.shape[1] > 0, "scales [N, K / group] of x's type")
-    group = K // scales.shape[1]
-    _need(group in (32, 64, 128) and group * scales.shape[1] == K, "group 32, 64 or 128")
-    _need(zeros is None or (zeros.dtype == torch.uint8 and zeros.shape == scales.shape
-                            and zeros.is_contiguous()), "zeros uint8 [N, K / group]")
-    _need(bias is None or (bias.dtype == torch.float32 and bias.shape == (N,)
-                           and bias.is_contiguous()), "bias f32 [N]")
-    ldx, ldo = _rows16(x, K, M, dt, "x"), _rows16(out, N, M, dt, "out")
-    _on_device(x, wq, scales, out, zeros, bias)
-    s = stream if stream is not None else torch.cuda.current_stream(x.device).cuda_stream
-    check(lib().qa_k_w4_linear(
-        x.data_ptr(), ldx, M, K, wq.data_ptr(), wq.stride(0), N, group, scales.data_ptr(),
-        ptr(zeros), ptr(bias), out.data_ptr(), ldo, 1 if dt == torch.bfloat16 else 0, s))
+    N, half = wq.shape
+    ldw, one = wq.stride()
+    if N < 2:
+        ldw = half
+    if wq.dtype is not _U8 or 2 * half != K or (one != 1 and half > 1) or ldw < half:
+        raise ValueError("wq uint8 [N, K / 2]")
+    groups = scales.shape[1]
+    _flat(scales, (N, groups), dt, "scales [N, K / group] of x's type")
+    group = K // groups if groups else 0
+    if group not in (32, 64, 128) or group * groups != K:
+        raise ValueError("group 32, 64 or 128")
+    ldx, ldo = _rows(x, M, K, dt, "x"), _rows(out, M, N, dt, "out")
+    dev = x.get_device()
+    here = dev >= 0 and wq.get_device() == scales.get_device() == out.get_device() == dev
+    z = b = 0
+    if zeros is not None:
+        _flat(zeros, (N, groups), _U8, "zeros uint8 [N, K / group]")
+        z = zeros.data_ptr()
+        here = here and zeros.get_device() == dev
+    if bias is not None:
+        _flat(bias, (N,), _F32, "bias f32 [N]")
+        b = bias.data_ptr()
+        here = here and bias.get_device() == dev
+    if not here:
+        _elsewhere()
+    rc = _fn_w4_linear()(_pack15(
+        x.data_ptr(), ldx, M, K, wq.data_ptr(), ldw, N, group, scales.data_ptr(), z, b,
+        out.data_ptr(), ldo, 1 if dt is _BF16 else 0, _stream(dev, stream)))
+    if rc:
+        check(rc)
+
+
+# The C functions, looked up once: lib() takes a lock.
+_fns: dict = {}
+
+
+def _fn_kv_append():
+    return _fns.get("append") or _fns.setdefault("append", lib().qa_k_kv_append_v)
+
+
+def _fn_cache_attention():
+    return _fns.get("attend") or _fns.setdefault(
+        "attend", (lib().qa_k_cache_attention_v, lib().qa_k_cache_attention_workspace))
+
+
+def _fn_w4_linear():
+    return _fns.get("w4") or _fns.setdefault("w4", lib().qa_k_w4_linear_v)

@@ -197,3 +197,43 @@ extern "C" int qa_k_w4_linear(const void* x, long long ldx, int M, int K, const 
                            bf16 != 0, static_cast<cudaStream_t>(stream));
   return rc == 0 ? QA_OK : QA_ERR_CUDA;
 }
+
+namespace {
+
+template <typename T>
+T* as_ptr(long long v) {
+  return reinterpret_cast<T*>(static_cast<uintptr_t>(v));
+}
+
+}  // namespace
+
+extern "C" int qa_k_kv_append_v(const long long* a, float eps) {
+  if (!a) return QA_ERR_ARG;
+  return qa_k_kv_append(as_ptr<void>(a[0]), a[1], as_ptr<void>(a[2]), a[3], as_ptr<void>(a[4]), a[5],
+                        as_ptr<void>(a[6]), a[7], a[8], (int)a[9], (int)a[10], (int)a[11],
+                        as_ptr<int>(a[12]), as_ptr<int>(a[13]), (int)a[14], (int)a[15],
+                        as_ptr<int>(a[16]), (int)a[17], as_ptr<void>(a[18]), as_ptr<void>(a[19]),
+                        (int)a[20], as_ptr<float>(a[21]), as_ptr<float>(a[22]), as_ptr<float>(a[23]),
+                        as_ptr<float>(a[24]), (int)a[25], as_ptr<int>(a[26]), a[27], (int)a[28],
+                        as_ptr<int>(a[29]), as_ptr<float>(a[30]), as_ptr<float>(a[31]), eps,
+                        (int)a[32], as_ptr<unsigned>(a[33]), as_ptr<void>(a[34]));
+}
+
+extern "C" int qa_k_cache_attention_v(const long long* a, float scale) {
+  if (!a) return QA_ERR_ARG;
+  return qa_k_cache_attention(as_ptr<void>(a[0]), a[1], a[2], (int)a[3], (int)a[4], (int)a[5],
+                              as_ptr<int>(a[6]), as_ptr<int>(a[7]), (int)a[8], (int)a[9], (int)a[10],
+                              as_ptr<int>(a[11]), (int)a[12], as_ptr<void>(a[13]),
+                              as_ptr<void>(a[14]), (int)a[15], as_ptr<float>(a[16]),
+                              as_ptr<float>(a[17]), scale, (int)a[18], as_ptr<void>(a[19]), a[20],
+                              as_ptr<float>(a[21]), as_ptr<void>(a[22]), a[23], (int)a[24],
+                              as_ptr<unsigned>(a[25]), as_ptr<void>(a[26]));
+}
+
+extern "C" int qa_k_w4_linear_v(const long long* a) {
+  if (!a) return QA_ERR_ARG;
+  return qa_k_w4_linear(as_ptr<void>(a[0]), a[1], (int)a[2], (int)a[3], as_ptr<uint8_t>(a[4]), a[5],
+                        (int)a[6], (int)a[7], as_ptr<void>(a[8]), as_ptr<uint8_t>(a[9]),
+                        as_ptr<float>(a[10]), as_ptr<void>(a[11]), a[12], (int)a[13],
+                        as_ptr<void>(a[14]));
+}
