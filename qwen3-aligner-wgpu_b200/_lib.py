@@ -602,7 +602,8 @@ def cache_attention(q, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale,
     lse f32 [T, nq] optional; scale defaults to 1 / sqrt(hd).  max_q and max_kv
     bound the sequences' new and cached tokens.  `validate` copies the maps to
     the host to check them.  A workspace is kept for each stream and grows with
-    the sizes seen (outside of graph capture).
+    the sizes seen; under graph capture it comes from the graph's own pool, so that
+    a graph neither shares it with later calls nor outlives it.
     """
     if _F16 is None:
         _types()
@@ -644,11 +645,14 @@ def cache_attention(q, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale,
     need = size(nq, nkv, hd, n, max_q, max_kv)
     ws = 0
     if need:
-        buf = _workspaces.get((dev, s))
-        if buf is None or buf.numel() < need:
-            import torch
-            torch.cuda.synchronize(dev)  # nobody uses the old one
-            buf = _workspaces[(dev, s)] = torch.empty(need, dtype=_U8, device=q.device)
+        import torch
+        if torch.cuda.is_current_stream_capturing():
+            buf = torch.empty(need, dtype=_U8, device=q.device)  # the graph's own
+        else:
+            buf = _workspaces.get((dev, s))
+            if buf is None or buf.numel() < need:
+                torch.cuda.synchronize(dev)  # nobody uses the old one
+                buf = _workspaces[(dev, s)] = torch.empty(need, dtype=_U8, device=q.device)
         ws = buf.data_ptr()
     rc = call(_pack27(
         q.data_ptr(), ldq, T, nq, nkv, hd, q_start.data_ptr(), kv_len.data_ptr(), n, max_q,
