@@ -17,11 +17,14 @@
 // where a code becomes subnormal.  A page's scale never shrinks while the page
 // fills; the token in slot 0 starts it afresh, whatever a former user left.
 //
-// One CTA per (sequence, page the append touches, K/V head) holds the page's
-// new keys and values in registers between the maximum and the codes, so every
-// input is read once and nothing is written twice; it also rotates the group's
-// query heads for the same tokens, with the same cos / sin rows.  A page and
-// head belongs to one CTA: no atomics, the same bits every time.
+// A CTA takes one (sequence, page the append touches, K/V head) and some of the
+// group's query heads, which turn by the same cos / sin rows; the first of a
+// group's CTAs also takes the keys and values.  Each thread copies what it will
+// use itself into shared memory (cp.async), all of it before the first use, so
+// that the loads in flight cost no registers and no barrier; the new keys stay in
+// registers between the page's maximum and the codes.  Every input is read once,
+// nothing is written twice, a page and head belongs to one CTA: no atomics, the
+// same bits every time.
 #include <cuda_fp8.h>
 
 #include "kernels.cuh"
@@ -32,8 +35,8 @@ namespace qa {
 namespace {
 
 constexpr int kPage = 64;
-constexpr int kThreads = 256;
-constexpr float kE4m3Max = 448.0f;
+constexpr int kThreads = 256;                    // at most
+constexpr uint32_t kStage = 72 * 1024;           // staged by a CTA: three CTAs an SM
 
 struct AppendParams {
   const void *q, *k, *v;
@@ -42,8 +45,12 @@ struct AppendParams {
   long long T;
   int group;  // query heads per K/V head
   int nkv;
+  int heads;          // query heads of a CTA
+  int head_ctas;      // CTAs that share a group's query heads
+  int ctas;           // nkv * head_ctas, for one run of tokens
+  int rounds;         // in which a CTA goes through its tokens
   SeqMap seqs;
-  int pages_per_seq;  // grid.x = n_seqs * pages_per_seq
+  int runs_per_seq;   // CTAs along a sequence's new tokens, at most
   void *kpool, *vpool;
   int kv_pages;
   float *kscale, *vscale;
@@ -86,6 +93,12 @@ __device__ __forceinline__ uint4 narrow8(const float* f) {
                     cvt2_rn<T>(make_float2(f[4], f[5])), cvt2_rn<T>(make_float2(f[6], f[7])));
 }
 
+__device__ __forceinline__ void load_f8(const float* p, float* f) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    reinterpret_cast<float4*>(f)[i] = reinterpret_cast<const float4*>(p)[i];
+}
+
 // Least power of two s >= 2^-64 with m <= 448 s (m finite, >= 0).  448 is
 // 1.75 * 2^8, so the exponent follows from m's own and one comparison.
 __device__ __forceinline__ float page_scale(float m) {
@@ -112,9 +125,9 @@ __device__ __forceinline__ uint2 codes8(const float* f, float inv) {
   return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 
-// Codes of a page's first `rows` rows, multiplied by ratio < 1.
+// The first `bytes` codes of a page, multiplied by ratio < 1.
 __device__ __forceinline__ void rescale_rows(uint8_t* page, int bytes, float ratio) {
-  for (int i = threadIdx.x * 16; i < bytes; i += kThreads * 16) {
+  for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16) {
     uint4 d = *reinterpret_cast<uint4*>(page + i);
     __nv_fp8x2_storage_t* c = reinterpret_cast<__nv_fp8x2_storage_t*>(&d);
 #pragma unroll
@@ -129,46 +142,94 @@ __device__ __forceinline__ void rescale_rows(uint8_t* page, int bytes, float rat
   }
 }
 
+// Tokens of a CTA.  A page's scales need all of its new tokens in one place; the
+// 16-bit cache has none, and takes what one round of threads covers.
+template <int HD, bool B8>
+constexpr int tokens() {
+  return B8 ? kPage : kThreads / (HD / 16);
+}
+
 template <typename T, int HD, bool B8>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(AppendParams ap) {
+__global__ void __launch_bounds__(kThreads, B8 ? (HD == 128 ? 2 : 3) : 4)
+    kv_append_kernel(AppendParams ap) {
   constexpr int kHalf = HD / 2;
-  constexpr int kLanes = HD / 16;             // lanes of a row: 8 dims of each half per lane
-  constexpr int kAtOnce = kThreads / kLanes;  // rows at once
-  constexpr int kRounds = kPage / kAtOnce;
+  constexpr int kLanes = HD / 16;  // of a token: 8 dims of each half per lane
+  constexpr int kTokens = tokens<HD, B8>();
+  constexpr int kRounds = kTokens * kLanes / kThreads;  // at most
+  extern __shared__ __align__(16) uint4 stage[];  // [slot][round][half][thread]
   __shared__ float s_max[2][kThreads / 32];
 
   pdl_wait();
   pdl_trigger();
-  const int s = blockIdx.x / ap.pages_per_seq, j = blockIdx.x % ap.pages_per_seq;
-  const int h = blockIdx.y;
+  // heads first: CTAs that run together read neighbouring columns of the same rows
+  const int y = blockIdx.x % ap.ctas, x = blockIdx.x / ap.ctas;
+  const int s = x / ap.runs_per_seq, j = x % ap.runs_per_seq;
+  const int h = y / ap.head_ctas, g0 = y % ap.head_ctas * ap.heads;
+  const int heads = min(ap.heads, ap.group - g0);
   const SeqSpan sp = seq_span(ap.seqs, s, ap.T);
   if (!sp.ok || sp.n > sp.len) {
-    if (j == 0 && h == 0 && threadIdx.x == 0 && ap.status) atomicOr(ap.status, kStatusBadShape);
+    if (j == 0 && y == 0 && threadIdx.x == 0 && ap.status) atomicOr(ap.status, kStatusBadShape);
     return;
   }
   const int c0 = sp.len - sp.n;       // cache index of the first new token
-  const int pg = c0 / kPage + j;      // page of the sequence
-  const int lo = max(c0, pg * kPage), hi = min(sp.len, (pg + 1) * kPage);  // cache indices
+  const int run = c0 / kTokens + j;
+  const int lo = max(c0, run * kTokens), hi = min(sp.len, (run + 1) * kTokens);  // cache indices
   if (lo >= hi) return;
-  const int page = ap.seqs.block_tab[static_cast<long long>(s) * ap.seqs.max_pages + pg];
-  const bool page_ok = page >= 0 && page < ap.kv_pages;
-  bool bad = !page_ok;
 
+  const int rows = blockDim.x / kLanes;  // tokens of a round
   const int row = threadIdx.x / kLanes, d0 = (threadIdx.x % kLanes) * 8;
-  const bool vec = ap.vec;
-  int ax[8];
+  const int warp_row = threadIdx.x / 32 * (32 / kLanes);
+  const bool vec = ap.vec, with_kv = g0 == 0;
+  const long long col = static_cast<long long>(h * ap.group + g0) * HD + d0;
+
+  // slots: the query heads, then k, then v
+  auto staged = [&](int slot, int r, int half) {
+    return stage + ((slot * ap.rounds + r) * 2 + half) * blockDim.x + threadIdx.x;
+  };
+  auto fetch = [&](int slot, int r, const T* p) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) ax[i] = ap.rope.n_axes > 1 ? ap.rope.axis_of[d0 + i] & 3 : 0;
+    for (int i = 0; i < 2; ++i) {
+      if (vec)
+        cp_async16(smem_u32(staged(slot, r, i)), p + i * kHalf, 16);
+      else
+        *staged(slot, r, i) = load8(p + i * kHalf, false);
+    }
+  };
+  for (int r = 0; r < ap.rounds; ++r) {
+    const int c = lo + r * rows + row;
+    if (c < hi) {
+      const long long t = sp.t0 + (c - c0);
+      if (with_kv) {
+        fetch(heads, r, static_cast<const T*>(ap.k) + t * ap.ldk + h * HD + d0);
+        fetch(heads + 1, r, static_cast<const T*>(ap.v) + t * ap.ldv + h * HD + d0);
+      }
+      const T* qr = static_cast<const T*>(ap.q) + t * ap.ldq + col;
+      for (int g = 0; g < heads; ++g) fetch(g, r, qr + g * HD);
+    }
+    cp_async_commit();
+  }
+
+  bool bad = false, page_ok = true;
+  int page = 0;
+  if (with_kv) {
+    page = ap.seqs.block_tab[static_cast<long long>(s) * ap.seqs.max_pages + lo / kPage];
+    page_ok = page >= 0 && page < ap.kv_pages;
+    bad = !page_ok;
+  }
+  uint32_t axes = 0;  // 2 bits for each of this lane's frequencies
+  if (ap.rope.n_axes > 1)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) axes |= (ap.rope.axis_of[d0 + i] & 3) << (2 * i);
 
   float kx[B8 ? kRounds : 1][16];
-  uint4 vx[B8 ? kRounds : 1][2];
   float kmax = 0.0f, vmax = 0.0f;
+  // Whole warps leave, so that the shuffles below always have theirs.
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
+    if (r >= ap.rounds || lo + r * rows + warp_row >= hi) break;
     const int rr = B8 ? r : 0;
-    const int c = lo + r * kAtOnce + row;
+    const int c = lo + r * rows + row;
     const bool on = c < hi;
-    // lanes without a token follow along with the last one's, for the shuffles
     const long long t = sp.t0 + (min(c, hi - 1) - c0);
     float cs[8], sn[8];
     if (ap.rope.cos_t) {
@@ -183,22 +244,24 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(AppendParams ap) {
           bad = true;
           p[a] = 0;
         }
-      if (ap.rope.n_axes > 1) {
+      load_f8(ap.rope.cos_t + static_cast<long long>(p[0]) * kHalf + d0, cs);
+      load_f8(ap.rope.sin_t + static_cast<long long>(p[0]) * kHalf + d0, sn);
+      // Another axis's row as a whole, only where its position differs: single
+      // elements would cost the load unit a pass per token each.
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int pi = ax[i] == 0 ? p[0] : ax[i] == 1 ? p[1] : ax[i] == 2 ? p[2] : p[3];
-          const long long at = static_cast<long long>(pi) * kHalf + d0 + i;
-          cs[i] = ap.rope.cos_t[at];
-          sn[i] = ap.rope.sin_t[at];
-        }
-      } else {
-        const long long at = static_cast<long long>(p[0]) * kHalf + d0;
+      for (int a = 1; a < 4; ++a)
+        if (a < ap.rope.n_axes && p[a] != p[0]) {
+          const long long at = static_cast<long long>(p[a]) * kHalf + d0;
+          float c2[8], s2[8];
+          load_f8(ap.rope.cos_t + at, c2);
+          load_f8(ap.rope.sin_t + at, s2);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          reinterpret_cast<float4*>(cs)[i] = reinterpret_cast<const float4*>(ap.rope.cos_t + at)[i];
-          reinterpret_cast<float4*>(sn)[i] = reinterpret_cast<const float4*>(ap.rope.sin_t + at)[i];
+          for (int i = 0; i < 8; ++i)
+            if ((axes >> (2 * i) & 3) == a) {
+              cs[i] = c2[i];
+              sn[i] = s2[i];
+            }
         }
-      }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -206,11 +269,10 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(AppendParams ap) {
         sn[i] = 0.0f;
       }
     }
-    // a row's 16 values of this lane: normalised, rotated
-    auto turn = [&](uint4 a, uint4 b, const float* gain, float* y) {
-      float x[16];
-      widen8<T>(a, x);
-      widen8<T>(b, x + 8);
+    // a head's 16 values of this lane: normalised, rotated
+    auto turn = [&](int slot, const float* gain, float* x) {
+      widen8<T>(*staged(slot, r, 0), x);
+      widen8<T>(*staged(slot, r, 1), x + 8);
       if (gain) {
         float ss = 0.0f;
 #pragma unroll
@@ -226,52 +288,53 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(AppendParams ap) {
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        y[i] = x[i] * cs[i] - x[8 + i] * sn[i];
-        y[8 + i] = x[8 + i] * cs[i] + x[i] * sn[i];
+        const float a = x[i], b = x[8 + i];
+        x[i] = a * cs[i] - b * sn[i];
+        x[8 + i] = b * cs[i] + a * sn[i];
       }
     };
-    const T* kr = static_cast<const T*>(ap.k) + t * ap.ldk + h * HD + d0;
-    const T* vr = static_cast<const T*>(ap.v) + t * ap.ldv + h * HD + d0;
-    const uint4 ka = load8(kr, vec), kb = load8(kr + kHalf, vec);
-    vx[rr][0] = load8(vr, vec);
-    vx[rr][1] = load8(vr + kHalf, vec);
-    turn(ka, kb, ap.kn, kx[rr]);
-    if constexpr (B8) {
-      if (on) {
-        float vf[16];
-        widen8<T>(vx[rr][0], vf);
-        widen8<T>(vx[rr][1], vf + 8);
+    if (r + 1 < ap.rounds)
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRounds - 1) : "memory");
+    else
+      cp_async_wait_all();
+    if (with_kv) {  // uniform in the CTA
+      turn(heads, ap.kn, kx[rr]);
+      if constexpr (B8) {
+        if (on) {
+          float vf[16];
+          widen8<T>(*staged(heads + 1, r, 0), vf);
+          widen8<T>(*staged(heads + 1, r, 1), vf + 8);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          kmax = fmaxf(kmax, finite_abs(kx[rr][i]));
-          vmax = fmaxf(vmax, finite_abs(vf[i]));
+          for (int i = 0; i < 16; ++i) {
+            kmax = fmaxf(kmax, finite_abs(kx[rr][i]));
+            vmax = fmaxf(vmax, finite_abs(vf[i]));
+          }
         }
+      } else if (on && page_ok) {
+        const long long at =
+            ((static_cast<long long>(page) * ap.nkv + h) * kPage + c % kPage) * HD + d0;
+        T* kd = static_cast<T*>(ap.kpool) + at;
+        T* vd = static_cast<T*>(ap.vpool) + at;
+        store8(kd, narrow8<T>(kx[rr]), true);
+        store8(kd + kHalf, narrow8<T>(kx[rr] + 8), true);
+        store8(vd, *staged(heads + 1, r, 0), true);
+        store8(vd + kHalf, *staged(heads + 1, r, 1), true);
       }
-    } else if (on && page_ok) {
-      const long long at = ((static_cast<long long>(page) * ap.nkv + h) * kPage + c % kPage) * HD + d0;
-      T* kd = static_cast<T*>(ap.kpool) + at;
-      T* vd = static_cast<T*>(ap.vpool) + at;
-      store8(kd, narrow8<T>(kx[rr]), true);
-      store8(kd + kHalf, narrow8<T>(kx[rr] + 8), true);
-      store8(vd, vx[rr][0], true);
-      store8(vd + kHalf, vx[rr][1], true);
     }
-#pragma unroll 2
-    for (int g = 0; g < ap.group; ++g) {
-      const long long col = static_cast<long long>(h * ap.group + g) * HD + d0;
-      const T* qr = static_cast<const T*>(ap.q) + t * ap.ldq + col;
-      const uint4 qa = load8(qr, vec), qb = load8(qr + kHalf, vec);
-      float y[16];
-      turn(qa, qb, ap.qn, y);
+    T* qd = static_cast<T*>(ap.q_out) + t * ap.ldqo + col;
+#pragma unroll 1
+    for (int g = 0; g < heads; ++g) {
+      float z[16];
+      turn(g, ap.qn, z);
       if (on) {
-        T* qd = static_cast<T*>(ap.q_out) + t * ap.ldqo + col;
-        store8(qd, narrow8<T>(y), vec);
-        store8(qd + kHalf, narrow8<T>(y + 8), vec);
+        store8(qd + g * HD, narrow8<T>(z), vec);
+        store8(qd + g * HD + kHalf, narrow8<T>(z + 8), vec);
       }
     }
   }
   if (bad && ap.status) atomicOr(ap.status, kStatusBadShape);
   if constexpr (B8) {
+    if (!with_kv || !page_ok) return;  // uniform in the CTA
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       kmax = fmaxf(kmax, __shfl_xor_sync(0xFFFFFFFFu, kmax, o));
@@ -281,13 +344,11 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(AppendParams ap) {
       s_max[0][threadIdx.x / 32] = kmax;
       s_max[1][threadIdx.x / 32] = vmax;
     }
-    if (!page_ok) return;
     const long long ph = static_cast<long long>(page) * ap.nkv + h;
     const int a = lo % kPage;  // rows of the page that were there before
     const float kold = a ? ap.kscale[ph] : 0.0f, vold = a ? ap.vscale[ph] : 0.0f;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) {
+    for (int i = 0; i < static_cast<int>(blockDim.x) / 32; ++i) {
       kmax = fmaxf(kmax, s_max[0][i]);
       vmax = fmaxf(vmax, s_max[1][i]);
     }
@@ -303,11 +364,11 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(AppendParams ap) {
     const float kinv = 1.0f / ks, vinv = 1.0f / vs;  // exact: powers of two
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
-      const int c = lo + r * kAtOnce + row;
-      if (c < hi) {
+      const int c = lo + r * rows + row;
+      if (r < ap.rounds && c < hi) {
         float vf[16];
-        widen8<T>(vx[r][0], vf);
-        widen8<T>(vx[r][1], vf + 8);
+        widen8<T>(*staged(heads + 1, r, 0), vf);
+        widen8<T>(*staged(heads + 1, r, 1), vf + 8);
         const int at = c % kPage * HD + d0;
         *reinterpret_cast<uint2*>(kp + at) = codes8(kx[r], kinv);
         *reinterpret_cast<uint2*>(kp + at + kHalf) = codes8(kx[r] + 8, kinv);
@@ -318,10 +379,33 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(AppendParams ap) {
   }
 }
 
-template <typename T, int HD>
-cudaError_t launch(const AppendParams& ap, dim3 grid, bool b8, cudaStream_t s) {
-  return b8 ? launch_pdl(kv_append_kernel<T, HD, true>, grid, dim3(kThreads), 0, s, ap)
-            : launch_pdl(kv_append_kernel<T, HD, false>, grid, dim3(kThreads), 0, s, ap);
+template <typename T, int HD, bool B8>
+cudaError_t launch(AppendParams& ap, cudaStream_t s) {
+  constexpr int kTokens = tokens<HD, B8>();
+  ap.runs_per_seq = (ap.seqs.max_q + 2 * kTokens - 2) / kTokens;  // from a run's last slot on
+  const int work = min(ap.seqs.max_q, kTokens) * (HD / 16);
+  const int threads = min(kThreads, (work + 31) / 32 * 32);
+  ap.rounds = (work + threads - 1) / threads;
+  const uint32_t slot = ap.rounds * 2 * threads * 16;
+  const int most = kStage / slot - 2;
+  ap.head_ctas = (ap.group + most - 1) / most;
+  ap.heads = (ap.group + ap.head_ctas - 1) / ap.head_ctas;
+  ap.ctas = ap.nkv * ap.head_ctas;
+  const long long ctas = static_cast<long long>(ap.seqs.n_seqs) * ap.runs_per_seq * ap.ctas;
+  if (ctas > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+  const uint32_t bytes = (ap.heads + 2) * slot;
+  if (bytes > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kv_append_kernel<T, HD, B8>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, kStage);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_pdl(kv_append_kernel<T, HD, B8>, dim3(static_cast<unsigned>(ctas)),
+                    dim3(threads), bytes, s, ap);
+}
+template <typename T>
+cudaError_t launch(AppendParams& ap, int hd, bool b8, cudaStream_t s) {
+  if (hd == 128) return b8 ? launch<T, 128, true>(ap, s) : launch<T, 128, false>(ap, s);
+  return b8 ? launch<T, 64, true>(ap, s) : launch<T, 64, false>(ap, s);
 }
 
 }  // namespace
@@ -346,7 +430,6 @@ int kv_append(const void* q, long long ldq, const void* k, long long ldk, const 
   ap.nkv = nkvh;
   ap.seqs = seqs;
   ap.seqs.max_q = max_q;
-  ap.pages_per_seq = (max_q + 2 * kPage - 2) / kPage;  // a run of max_q tokens from slot 63 on
   ap.kpool = kv.k;
   ap.vpool = kv.v;
   ap.kv_pages = kv_pages;
@@ -360,16 +443,8 @@ int kv_append(const void* q, long long ldq, const void* k, long long ldk, const 
              reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(q_out)) % 16 == 0) &&
            ((ldq | ldk | ldv | ldqo) % 8 == 0);
   ap.status = status;
-  const long long gx = static_cast<long long>(seqs.n_seqs) * ap.pages_per_seq;
-  if (gx > 0x7FFFFFFFll || nkvh > 65535) return (int)cudaErrorInvalidValue;
-  const dim3 grid(static_cast<unsigned>(gx), nkvh);
-  cudaError_t e;
-  if (bf16)
-    e = hd == 128 ? launch<__nv_bfloat16, 128>(ap, grid, kscale != nullptr, s)
-                  : launch<__nv_bfloat16, 64>(ap, grid, kscale != nullptr, s);
-  else
-    e = hd == 128 ? launch<__half, 128>(ap, grid, kscale != nullptr, s)
-                  : launch<__half, 64>(ap, grid, kscale != nullptr, s);
+  const cudaError_t e = bf16 ? launch<__nv_bfloat16>(ap, hd, kscale != nullptr, s)
+                             : launch<__half>(ap, hd, kscale != nullptr, s);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
