@@ -6,6 +6,7 @@
 //   s_c = scale kscale[page(c)] (q . kcode_c),  out = sum_c softmax(s)_c vscale[page(c)] vcode_c,
 // lse = log sum_c exp(s_c); a row that sees nothing gets 0 and -inf.
 #include <algorithm>
+#include <atomic>
 
 #include "cache_attn.cuh"
 #include "gemm_tc.cuh"
@@ -81,12 +82,19 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
   return v;
 }
 
-// Tokens of a chunk of a unit of `tokens` tokens, a multiple of 32.  Short units
-// are cut fine, for their latency; 256 tokens make a part (2 (hd + 2) floats a
-// row written and read) small next to its chunk (2 hd bytes a token).  A team of
-// four warps takes four slabs at a time and writes parts of more rows, so its
-// chunks start at 256.
+// Warps of a team: four (a CTA) for more than 8 rows, and for caches of which none
+// is long, as far as the caller knows (max_kv).
+constexpr int kShort = 512;
+__host__ __device__ __forceinline__ constexpr int team_warps(int R, int max_kv) {
+  return R > 8 || max_kv <= kShort ? kWarps : 1;
+}
+
+// Tokens of a chunk of a unit of `tokens` tokens, a multiple of 32.  256 tokens make
+// a part (2 (hd + 2) floats a row written and read) small next to its chunk (2 hd
+// bytes a token).  Single warps cut short units finer, for their latency; a team's
+// four warps join a short one in shared memory, without a part.
 __host__ __device__ __forceinline__ int chunk_tokens(int tokens, int team) {
+  if (team > 1 && tokens <= kShort) return kShort;
   if (team == 1 && tokens <= 512) return 64;
   if (team == 1 && tokens <= 2048) return 128;
   return tokens <= kMaxParts * 256 ? 256 : ((tokens - 1) / (kMaxParts * 32) + 1) * 32;
@@ -187,12 +195,8 @@ struct RowsPlan {
 
 // Tokens of a slab: the more of them, the more independent work a warp has
 // between two waits and the fewer instructions a token, as far as the registers
-// reach (S^T takes 4 a 16 tokens and 8 rows).  The ring's bytes stay the same.
-template <int NT>
-struct Slab {
-  static constexpr int kTokens = NT <= 2 ? 32 : 16;
-  static constexpr int kStages = 64 / kTokens;
-};
+// reach (S^T takes 4 a 16 tokens and 8 rows).
+constexpr int kSlab = 32, kStages = 2;
 
 template <typename T, int HD, int NT, int TEAM>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
@@ -201,7 +205,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
   constexpr int R = 8 * NT;          // rows of a tile
   constexpr int kKc = HD / 64;       // 16-byte units of K a thread reads a token
   constexpr int kMt = HD / 16;       // 16-dim blocks of O^T
-  constexpr int kSlab = Slab<NT>::kTokens, kStages = Slab<NT>::kStages;
   constexpr int kMb = kSlab / 16;    // 16-token blocks of S^T
   constexpr int kPart = kSlab * HD;  // bytes of a slab's K (or V)
   extern __shared__ uint8_t smem_raw[];
@@ -742,7 +745,7 @@ struct PartSizes {
 PartSizes part_sizes(int nq, int nkv, int hd, int max_q, int max_kv) {
   PartSizes p;
   const long long rows = static_cast<long long>(max_q) * (nq / nkv);
-  const int R = tile_rows(rows), team = R == 8 ? 1 : kWarps;
+  const int R = tile_rows(rows), team = team_warps(R, max_kv);
   const int tokens = std::max(1, max_kv);
   p.tiles = static_cast<int>((rows + R - 1) / R);
   p.parts = (tokens - 1) / chunk_tokens(tokens, team) + 1;
@@ -765,10 +768,10 @@ int resident_ctas(K kern, size_t smem, cudaError_t* err) {
   return std::min(per, kMaxCtasPerSm) * device_sm_count();
 }
 
-template <typename T, int HD, int NT>
+template <typename T, int HD, int NT, int TEAM>
 cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int max_kv, cudaStream_t s) {
-  constexpr int R = 8 * NT, kSlab = Slab<NT>::kTokens, kStages = Slab<NT>::kStages;
-  // the ring holds the warps' O, 4 kWarps R HD bytes, at NT = 4; and 1 KB to align it
+  constexpr int R = 8 * NT;
+  // the ring, which also takes the warps' O, 4 kWarps R HD bytes; and 1 KB to align it
   constexpr int kSmem = kWarps * kStages * 2 * kSlab * HD + 1024;
   static_assert(kSmem - 1024 >= 4 * kWarps * R * HD, "the warps' O fits the ring");
   CUtensorMap tk, tv;
@@ -780,9 +783,8 @@ cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int ma
   int rc = make_tmap_nd(&tk, ap.kpool, false, 2, dims, stride, box, step, HD);
   if (!rc) rc = make_tmap_nd(&tv, ap.vpool, false, 2, dims, stride, box, step, HD);
   if (rc) return static_cast<cudaError_t>(rc);
-  constexpr int kTeam = NT == 1 ? 1 : kWarps;
-  auto kern = cache_attn_rows<T, HD, NT, kTeam>;
-  static int resident[64] = {0};  // per instantiation and device
+  auto kern = cache_attn_rows<T, HD, NT, TEAM>;
+  static std::atomic<int> resident[64];  // per instantiation and device
   int dev = 0;
   cudaGetDevice(&dev);
   int grid = resident[dev & 63];
@@ -799,9 +801,12 @@ cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int ma
   ap.part_stride = ps.stride;
   ap.parts = static_cast<float*>(ws);
   ap.cap_units = ws ? ws_bytes / ps.unit_bytes : 0;
+  // no more CTAs than chunks, as far as max_kv tells
+  const long long chunks = static_cast<long long>(ap.seqs.n_seqs) * ps.tiles * ap.nkv * ps.parts;
+  grid = static_cast<int>(std::min<long long>(grid, (chunks * TEAM + kWarps - 1) / kWarps));
   cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kWarps * 32), kSmem, s, tk, tv, ap);
   if (e == cudaSuccess && ps.parts > 1 && ap.cap_units > 0) {
-    e = launch_join<T, HD, RowsPlan<R, kTeam, kSlab>>(ap, s);
+    e = launch_join<T, HD, RowsPlan<R, TEAM, kSlab>>(ap, s);
   }
   return e;
 }
@@ -809,8 +814,9 @@ cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int ma
 template <typename T, int HD>
 cudaError_t launch_any(const CacheAttnParams& ap, void* ws, long long ws_bytes, int max_kv, cudaStream_t s) {
   if (tile_rows(static_cast<long long>(ap.seqs.max_q) * (ap.nq / ap.nkv)) == 8)
-    return launch_rows<T, HD, 1>(ap, ws, ws_bytes, max_kv, s);
-  return launch_rows<T, HD, 2>(ap, ws, ws_bytes, max_kv, s);
+    return team_warps(8, max_kv) == 1 ? launch_rows<T, HD, 1, 1>(ap, ws, ws_bytes, max_kv, s)
+                                      : launch_rows<T, HD, 1, kWarps>(ap, ws, ws_bytes, max_kv, s);
+  return launch_rows<T, HD, 2, kWarps>(ap, ws, ws_bytes, max_kv, s);
 }
 
 // Rows of a K/V head and sequence up to which the few-row kernel is used.

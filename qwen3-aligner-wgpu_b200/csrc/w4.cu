@@ -26,6 +26,7 @@
 // a CTA needs its part of x only), and the sums are joined through distributed
 // shared memory in the CTAs' order.  No atomics, the same bits each time.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "gemm_tc.cuh"
@@ -450,13 +451,13 @@ cudaError_t launch(W4Params wp, cudaStream_t s) {
   wp.chunk = std::min(wp.per, std::max(1, (kXBytes - kRed) / step_bytes));
   const int smem = wp.chunk * step_bytes + kRed;
   auto k = w4_kernel<T, NT, GPS, ZEROS, FAST>;
-  static int set[64] = {0};  // per instantiation and device
+  static std::atomic<bool> set[64];  // per instantiation and device
   int dev = 0;
   cudaGetDevice(&dev);
-  if (set[dev & 63] < smem) {
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (dev >= 64 || !set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kXBytes);
     if (e != cudaSuccess) return e;
-    set[dev & 63] = smem;
+    if (dev < 64) set[dev] = true;
   }
   const int ctas = std::min(groups, std::max(1, kCtas * device_sm_count() / (y * wp.slices)));
   cudaLaunchConfig_t cfg = {};
