@@ -183,10 +183,10 @@ struct Walk {
 };
 
 // The parts that this kernel leaves, for the join.
-template <int R, int TEAM, int SLAB>
+template <int R, int TEAM, int SLAB, bool ALONE>
 struct RowsPlan {
   static constexpr int kRows = R;
-  static constexpr bool kAlone = false;
+  static constexpr bool kAlone = ALONE;
   __device__ static int parts(const CacheAttnParams& ap, const SeqSpan& sp, int s, int) {
     const int n = seq_plan(ap, sp, s, ap.nq / ap.nkv, R, TEAM, SLAB).chunks;
     return n > 1 ? n : 0;
@@ -735,7 +735,7 @@ done:
 }
 
 // Rows of a tile of the few-row kernel for sequences of up to `rows` rows.
-int tile_rows(long long rows) { return rows <= 8 ? 8 : 16; }
+int tile_rows(long long rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 24; }
 
 // The workspace of a unit, for caches of up to max_kv tokens.
 struct PartSizes {
@@ -806,21 +806,25 @@ cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int ma
   grid = static_cast<int>(std::min<long long>(grid, (chunks * TEAM + kWarps - 1) / kWarps));
   cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kWarps * 32), kSmem, s, tk, tv, ap);
   if (e == cudaSuccess && ps.parts > 1 && ap.cap_units > 0) {
-    e = launch_join<T, HD, RowsPlan<R, TEAM, kSlab>>(ap, s);
+    constexpr bool kMany = R > 8;  // rows enough for a warp each
+    e = kMany && ps.parts <= kJoinAlone ? launch_join<T, HD, RowsPlan<R, TEAM, kSlab, kMany>>(ap, s)
+                                        : launch_join<T, HD, RowsPlan<R, TEAM, kSlab, false>>(ap, s);
   }
   return e;
 }
 
 template <typename T, int HD>
 cudaError_t launch_any(const CacheAttnParams& ap, void* ws, long long ws_bytes, int max_kv, cudaStream_t s) {
-  if (tile_rows(static_cast<long long>(ap.seqs.max_q) * (ap.nq / ap.nkv)) == 8)
+  const int R = tile_rows(static_cast<long long>(ap.seqs.max_q) * (ap.nq / ap.nkv));
+  if (R == 24) return launch_rows<T, HD, 3, kWarps>(ap, ws, ws_bytes, max_kv, s);
+  if (R == 8)
     return team_warps(8, max_kv) == 1 ? launch_rows<T, HD, 1, 1>(ap, ws, ws_bytes, max_kv, s)
                                       : launch_rows<T, HD, 1, kWarps>(ap, ws, ws_bytes, max_kv, s);
   return launch_rows<T, HD, 2, kWarps>(ap, ws, ws_bytes, max_kv, s);
 }
 
 // Rows of a K/V head and sequence up to which the few-row kernel is used.
-constexpr int kFewRows = 16;
+constexpr int kFewRows = 24;
 
 }  // namespace
 
