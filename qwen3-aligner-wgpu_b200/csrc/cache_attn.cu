@@ -25,11 +25,10 @@ namespace {
 // is that every SM reads all the time, bytes in flight and instructions a byte.
 //  - A unit's cached tokens are cut into chunks by the unit's own length alone
 //    (so a sequence's result does not depend on the batch it is in).  The slabs
-//    of 16 tokens of all units, laid end to end, are shared out evenly over the
-//    teams that the GPU holds; a team takes the chunks that begin in its share,
-//    which it finds from kv_len and q_start itself.  A team is one warp for up to
-//    8 rows, so that nothing waits for anything else, and a CTA's four warps for
-//    more rows, whose parts are larger.
+//    of 32 tokens of all units, laid end to end, are shared out evenly over the
+//    CTAs that the GPU holds; a CTA takes the chunks that begin in its share,
+//    which it finds from kv_len and q_start itself.  Its four warps take every
+//    fourth slab of a chunk and are joined in shared memory.
 //  - A unit of one chunk is finished where it is computed.  Otherwise each chunk
 //    leaves its part (m, l, O) in the workspace, and a second kernel joins a
 //    unit's parts in their order (joining them in this kernel, by whoever comes
@@ -82,36 +81,30 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
   return v;
 }
 
-// Warps of a team: four (a CTA) for more than 8 rows, and for caches of which none
-// is long, as far as the caller knows (max_kv).
-constexpr int kShort = 512;
-__host__ __device__ __forceinline__ constexpr int team_warps(int R, int max_kv) {
-  return R > 8 || max_kv <= kShort ? kWarps : 1;
-}
-
-// Tokens of a chunk of a unit of `tokens` tokens, a multiple of 32.  256 tokens make
-// a part (2 (hd + 2) floats a row written and read) small next to its chunk (2 hd
-// bytes a token).  Single warps cut short units finer, for their latency; a team's
-// four warps join a short one in shared memory, without a part.
-__host__ __device__ __forceinline__ int chunk_tokens(int tokens, int team) {
-  if (team > 1 && tokens <= kShort) return kShort;
-  if (team == 1 && tokens <= 512) return 64;
-  if (team == 1 && tokens <= 2048) return 128;
-  return tokens <= kMaxParts * 256 ? 256 : ((tokens - 1) / (kMaxParts * 32) + 1) * 32;
+// Tokens of a chunk of a unit of `tokens` tokens, a multiple of 32.  A short unit is
+// one chunk, which needs no part and no second kernel (one row, 16/8 heads of 128,
+// against 64- and 128-token chunks of single warps that are joined afterwards: 64
+// sessions of 512 tokens 29 against 39 us, one of 128 tokens 10 against 14, of 1024
+// the same).  Longer ones: 768 tokens keep the parts few and the shares even (two
+// sessions of 131,000 tokens: 46 us, 49 with 512, 60 with 256; 16 of 5000 with 24
+// rows: 55, 59 and 77; one of 8192 with 24 rows: 39, 27 and 29).
+constexpr int kShort = 1024, kChunk = 768;
+__host__ __device__ __forceinline__ int chunk_tokens(int tokens) {
+  if (tokens <= kShort) return kShort;
+  return tokens <= kMaxParts * kChunk ? kChunk : ((tokens - 1) / (kMaxParts * 32) + 1) * 32;
 }
 
 // Shared memory of the few-row kernel besides the ring.
-template <int R, int TEAM, int STAGES>
+template <int R, int STAGES>
 struct RowsShared {
-  static constexpr int kTeams = kWarps / TEAM;
   uint64_t full[kWarps][STAGES][2];  // K, V
   float m[kWarps][R], l[kWarps][R];  // the warps' references and sums
   float cm[R], cl[R];                // of the joined warps
-  float inv[kTeams][R];              // 1 / sum
+  float inv[R];                      // 1 / sum
   long long scan[kWarps];
-  long long lo[kTeams], hi[kTeams];  // the teams' shares of the slabs
-  long long start[kTeams];           // first slab of the first sequence of the share
-  int seq[kTeams];                   // that sequence
+  long long lo, hi;                  // the CTA's share of the slabs
+  long long start;                   // first slab of the first sequence of the share
+  int seq;                           // that sequence
 };
 
 // What a sequence asks of the few-row kernel: tiles x K/V heads units of
@@ -121,11 +114,11 @@ struct SeqPlan {
   long long cost;  // slabs of all units
 };
 __device__ __forceinline__ SeqPlan seq_plan(const CacheAttnParams& ap, const SeqSpan& sp, int s,
-                                            int group, int R, int team, int slab) {
+                                            int group, int R, int slab) {
   SeqPlan c;
   c.tiles = sp.ok ? (sp.n * group + R - 1) / R : 0;
   c.slabs = max(1, (sp.len + slab - 1) / slab);  // an empty cache still owes its rows zeros
-  c.step = chunk_tokens(sp.len, team) / slab;
+  c.step = chunk_tokens(sp.len) / slab;
   c.chunks = (c.slabs + c.step - 1) / c.step;
   if (c.chunks > ap.cap_parts || static_cast<long long>(s + 1) * ap.tiles_max * ap.nkv > ap.cap_units) {
     c.step = c.slabs;  // no place for the parts
@@ -135,8 +128,8 @@ __device__ __forceinline__ SeqPlan seq_plan(const CacheAttnParams& ap, const Seq
   return c;
 }
 
-// A team's share: the chunks that begin in it, as runs of one unit.
-template <int R, int TEAM, int SLAB>
+// A CTA's share: the chunks that begin in it.
+template <int R, int SLAB>
 struct Walk {
   long long x, hi;  // first slab still to be looked at, end of the share
   int s, unit, chunk, run;  // the run: chunks [chunk, run) of a unit of sequence s
@@ -145,7 +138,7 @@ struct Walk {
 
   __device__ __forceinline__ void look(const CacheAttnParams& ap) {
     sp = seq_span(ap.seqs, s, ap.T);
-    plan = seq_plan(ap, sp, s, ap.nq / ap.nkv, R, TEAM, SLAB);
+    plan = seq_plan(ap, sp, s, ap.nq / ap.nkv, R, SLAB);
   }
   // the share [lo, hi) begins in sequence `seq`, whose first slab is `start`
   __device__ __forceinline__ void begin(const CacheAttnParams& ap, int seq, long long start, long long lo,
@@ -172,23 +165,19 @@ struct Walk {
       look(ap);
     }
     chunk = run;
-    // a warp goes on to the end of its share in one run of its ring; a team's
-    // shared memory also joins its warps, chunk by chunk
-    run = chunk + 1;
-    if (TEAM == 1)
-      run = chunk + static_cast<int>(min(static_cast<long long>(plan.chunks - chunk), (hi - x - 1) / plan.step + 1));
+    run = chunk + 1;  // shared memory joins the warps chunk by chunk
     x += min(plan.slabs, run * plan.step) - chunk * plan.step;
     return true;
   }
 };
 
 // The parts that this kernel leaves, for the join.
-template <int R, int TEAM, int SLAB, bool ALONE>
+template <int R, int SLAB, bool ALONE>
 struct RowsPlan {
   static constexpr int kRows = R;
   static constexpr bool kAlone = ALONE;
   __device__ static int parts(const CacheAttnParams& ap, const SeqSpan& sp, int s, int) {
-    const int n = seq_plan(ap, sp, s, ap.nq / ap.nkv, R, TEAM, SLAB).chunks;
+    const int n = seq_plan(ap, sp, s, ap.nq / ap.nkv, R, SLAB).chunks;
     return n > 1 ? n : 0;
   }
 };
@@ -198,7 +187,7 @@ struct RowsPlan {
 // reach (S^T takes 4 a 16 tokens and 8 rows).
 constexpr int kSlab = 32, kStages = 2;
 
-template <typename T, int HD, int NT, int TEAM>
+template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     cache_attn_rows(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ CacheAttnParams ap) {
@@ -208,16 +197,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
   constexpr int kMb = kSlab / 16;    // 16-token blocks of S^T
   constexpr int kPart = kSlab * HD;  // bytes of a slab's K (or V)
   extern __shared__ uint8_t smem_raw[];
-  constexpr int kTeams = kWarps / TEAM, kTeamThreads = TEAM * 32;
-  __shared__ RowsShared<R, TEAM, kStages> sh;
+  __shared__ RowsShared<R, kStages> sh;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int team = warp / TEAM, tw = warp % TEAM, tid = threadIdx.x % kTeamThreads;
-  auto team_sync = [] {
-    if constexpr (TEAM == 1) __syncwarp();
-    else __syncthreads();
-  };
+  const int tid = threadIdx.x;
   const int group = ap.nq / ap.nkv, n_seqs = ap.seqs.n_seqs;
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmK);
@@ -236,7 +220,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     for (int i = s0; i < s1; ++i) {
       const SeqSpan sp = seq_span(ap.seqs, i, ap.T);
       if (!sp.ok && blockIdx.x == 0 && ap.status) atomicOr(ap.status, kStatusBadShape);
-      mine += seq_plan(ap, sp, i, group, R, TEAM, kSlab).cost;
+      mine += seq_plan(ap, sp, i, group, R, kSlab).cost;
     }
     long long before = mine;  // inclusive scan
 #pragma unroll
@@ -253,35 +237,29 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       total += sh.scan[w];
     }
     before -= mine;
-    const long long n_teams = static_cast<long long>(gridDim.x) * kTeams;
-    const long long quot = total / n_teams, rem = total % n_teams;
-#pragma unroll
-    for (int k = 0; k < kTeams; ++k) {
-      // neighbouring shares on different SMs
-      const long long i = static_cast<long long>(k) * gridDim.x + blockIdx.x;
-      const long long lo = quot * i + min(i, rem), hi = lo + quot + (i < rem ? 1 : 0);
-      if (threadIdx.x == 0) {
-        sh.lo[k] = lo;
-        sh.hi[k] = hi;
-      }
-      if (lo < hi && lo >= before && lo < before + mine) {  // the share begins in one of mine
-        long long at = before;
-        for (int q = s0; q < s1; ++q) {
-          const long long cost = seq_plan(ap, seq_span(ap.seqs, q, ap.T), q, group, R, TEAM, kSlab).cost;
-          if (lo < at + cost) {
-            sh.seq[k] = q;
-            sh.start[k] = at;
-            break;
-          }
-          at += cost;
+    const long long quot = total / gridDim.x, rem = total % gridDim.x, i = blockIdx.x;
+    const long long lo = quot * i + min(i, rem), hi = lo + quot + (i < rem ? 1 : 0);
+    if (threadIdx.x == 0) {
+      sh.lo = lo;
+      sh.hi = hi;
+    }
+    if (lo < hi && lo >= before && lo < before + mine) {  // the share begins in one of mine
+      long long at = before;
+      for (int q = s0; q < s1; ++q) {
+        const long long cost = seq_plan(ap, seq_span(ap.seqs, q, ap.T), q, group, R, kSlab).cost;
+        if (lo < at + cost) {
+          sh.seq = q;
+          sh.start = at;
+          break;
         }
+        at += cost;
       }
     }
     __syncthreads();
-    if (sh.lo[team] >= sh.hi[team]) return;
+    if (sh.lo >= sh.hi) return;
   }
-  Walk<R, TEAM, kSlab> walk;
-  walk.begin(ap, sh.seq[team], sh.start[team], sh.lo[team], sh.hi[team]);
+  Walk<R, kSlab> walk;
+  walk.begin(ap, sh.seq, sh.start, sh.lo, sh.hi);
   uint32_t it = 0;  // slabs this warp has taken through its ring
   bool ok = true;   // no wait has run out
   while (walk.next(ap)) {
@@ -298,7 +276,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     // ---- the ring's first slabs
     uint8_t* ring = smem + warp * (kStages * 2 * kPart);
     const int* bt = ap.seqs.block_tab + static_cast<long long>(s) * ap.seqs.max_pages;
-    int slab = lo + tw;
+    int slab = lo + warp;
     auto page_of = [&](int slab) { return slab < end ? bt[slab / (kPage / kSlab)] : 0; };
     auto good = [&](int page) { return page >= 0 && page < ap.kv_pages; };
     // K (v = 0) or V (v = 1) of a slab, the warp's n-th
@@ -317,11 +295,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     };
     int pages[kStages + 1];  // of the slabs from the current one on
 #pragma unroll
-    for (int i = 0; i <= kStages; ++i) pages[i] = page_of(slab + i * TEAM);
+    for (int i = 0; i <= kStages; ++i) pages[i] = page_of(slab + i * kWarps);
 #pragma unroll
     for (int i = 0; i < kStages; ++i) {
-      fetch(slab + i * TEAM, pages[i], it + i, 0);
-      fetch(slab + i * TEAM, pages[i], it + i, 1);
+      fetch(slab + i * kWarps, pages[i], it + i, 0);
+      fetch(slab + i * kWarps, pages[i], it + i, 1);
     }
     auto scale_at = [&](const float* p, int page) {
       return p[static_cast<long long>(good(page) ? page : 0) * ap.nkv + h];
@@ -424,12 +402,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       for (int i = 0; i < kMt; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
     }
 
-    for (const int stop = min(end, (chunk + 1) * plan.step); slab < stop; slab += TEAM, ++it) {
+    for (const int stop = min(end, (chunk + 1) * plan.step); slab < stop; slab += kWarps, ++it) {
       const float ks = ks_next, vs = usable_vscale(vs_next);
       const int have = good(pages[0]) ? min(kSlab, sp.len - slab * kSlab) : 0;
 #pragma unroll
       for (int i = 0; i < kStages; ++i) pages[i] = pages[i + 1];
-      pages[kStages] = page_of(slab + (kStages + 1) * TEAM);
+      pages[kStages] = page_of(slab + (kStages + 1) * kWarps);
       ks_next = scale_at(ap.kscale, pages[0]);
       vs_next = scale_at(ap.vscale, pages[0]);
       if (!mbar_wait_warp(&sh.full[warp][it % kStages][0], (it / kStages) & 1)) {
@@ -465,7 +443,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       }
 
       __syncwarp();  // K has been read
-      fetch(slab + kStages * TEAM, pages[kStages - 1], it + kStages, 0);
+      fetch(slab + kStages * kWarps, pages[kStages - 1], it + kStages, 0);
 
       // ---- softmax of tokens 16 b + g, + 8 (c[0..1], c[2..3]) for columns 2t, 2t + 1
       const bool partial = (slab + 1) * kSlab > all || have < kSlab;
@@ -616,30 +594,30 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
           }
       }
       __syncwarp();  // V has been read
-      fetch(slab + kStages * TEAM, pages[kStages - 1], it + kStages, 1);
+      fetch(slab + kStages * kWarps, pages[kStages - 1], it + kStages, 1);
     }
 
     if (!ok)  // a wait ran out: nothing may still be on its way when the CTA ends
       for (uint32_t n = it; n <= it + kStages; ++n)
-        if (slab + static_cast<int>(n - it) * TEAM < end) {
+        if (slab + static_cast<int>(n - it) * kWarps < end) {
           mbar_wait_warp(&sh.full[warp][n % kStages][0], (n / kStages) & 1);
           mbar_wait_warp(&sh.full[warp][n % kStages][1], (n / kStages) & 1);
         }
 
-    // ---- the team's m, l and O
+    // ---- the warps' m, l and O
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) l[nt][e] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][e], w);
-        if (TEAM > 1 && g == 0) {
+        if (g == 0) {
           sh.m[warp][nt * 8 + 2 * t + e] = m[nt][e];
           sh.l[warp][nt * 8 + 2 * t + e] = l[nt][e];
         }
       }
     float* obuf = reinterpret_cast<float*>(smem);  // [warp][row][dim] over the ring
-    if constexpr (TEAM > 1) {
+    {
       if (__syncthreads_or(!ok)) goto done;  // every slab has been read
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -649,70 +627,50 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
           if (r >= rows) continue;
           float big = sh.m[0][r];
 #pragma unroll
-          for (int w = 1; w < TEAM; ++w) big = fmaxf(big, sh.m[w][r]);
+          for (int w = 1; w < kWarps; ++w) big = fmaxf(big, sh.m[w][r]);
           const float ref = big == -INFINITY ? 0.0f : big;
           const float a = ex2_approx(m[nt][e] - ref);
-          float* dst = obuf + (tw * R + r) * HD + 2 * kMt * g;
+          float* dst = obuf + (warp * R + r) * HD + 2 * kMt * g;
 #pragma unroll
           for (int i = 0; i < kMt / 2; ++i)
             *reinterpret_cast<float4*>(dst + 4 * i) = make_float4(
                 o[2 * i][nt][e] * a, o[2 * i][nt][e + 2] * a, o[2 * i + 1][nt][e] * a, o[2 * i + 1][nt][e + 2] * a);
-          if (tw == 0 && g == 0) {
+          if (warp == 0 && g == 0) {
             float sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < TEAM; ++w) sum += sh.l[w][r] * ex2_approx(sh.m[w][r] - ref);
+            for (int w = 0; w < kWarps; ++w) sum += sh.l[w][r] * ex2_approx(sh.m[w][r] - ref);
             sh.cm[r] = big;
             sh.cl[r] = sum;
           }
         }
       __syncthreads();
-    } else {
-      if (!ok) goto done;
     }
     // calls put(row, dim, four values) for all of O, f32
     auto each = [&](auto put) {
-      if constexpr (TEAM > 1) {
-        for (int i = tid; i < rows * (HD / 4); i += kTeamThreads) {
+      {
+        for (int i = tid; i < rows * (HD / 4); i += kWarps * 32) {
           float4 v = reinterpret_cast<float4*>(obuf)[i];
 #pragma unroll
-          for (int w = 1; w < TEAM; ++w) {
+          for (int w = 1; w < kWarps; ++w) {
             const float4 y = reinterpret_cast<float4*>(obuf + w * R * HD)[i];
             v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
           }
           put(i / (HD / 4), 4 * (i % (HD / 4)), v);
         }
-      } else {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (nt * 8 + 2 * t + e < rows)
-#pragma unroll
-              for (int i = 0; i < kMt / 2; ++i)
-                put(nt * 8 + 2 * t + e, 2 * kMt * g + 4 * i,
-                    make_float4(o[2 * i][nt][e], o[2 * i][nt][e + 2], o[2 * i + 1][nt][e], o[2 * i + 1][nt][e + 2]));
       }
     };
     // calls put(row, m, l) for all rows
     auto each_row = [&](auto put) {
-      if constexpr (TEAM > 1) {
-        if (tid < rows) put(tid, sh.cm[tid], sh.cl[tid]);
-      } else {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (g == 0 && nt * 8 + 2 * t + e < rows) put(nt * 8 + 2 * t + e, m[nt][e], l[nt][e]);
-      }
+      if (tid < rows) put(tid, sh.cm[tid], sh.cl[tid]);
     };
 
     // ---- they are all there is, or a part
     const UnitAt at{s, tile, h, sp.t0};
     if (plan.chunks == 1) {
-      each_row([&](int r, float big, float sum) { sh.inv[team][r] = close_row(ap, at, tile * R + r, big, sum); });
-      team_sync();
-      each([&](int r, int dim, float4 v) { finish_row<T, HD>(ap, at, tile * R + r, dim, v, sh.inv[team][r]); });
-      team_sync();  // the sums are read before the next chunk's are written
+      each_row([&](int r, float big, float sum) { sh.inv[r] = close_row(ap, at, tile * R + r, big, sum); });
+      __syncthreads();
+      each([&](int r, int dim, float4 v) { finish_row<T, HD>(ap, at, tile * R + r, dim, v, sh.inv[r]); });
+      __syncthreads();  // the sums are read before the next chunk's are written
     } else {
       float* mine = unit_parts(ap, at) + chunk * ap.part_stride;
       const int l_at = (ap.part_rows + 3) & ~3;
@@ -724,10 +682,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
         __stcg(mine + l_at + r, sum);
       });
     }
-    if constexpr (TEAM > 1) {
-      fence_proxy_async_smem();  // O is overwritten by the next chunk's copies
-      __syncthreads();
-    }
+    fence_proxy_async_smem();  // O is overwritten by the next chunk's copies
+    __syncthreads();
     }
   }
 done:
@@ -745,14 +701,11 @@ struct PartSizes {
 PartSizes part_sizes(int nq, int nkv, int hd, int max_q, int max_kv) {
   PartSizes p;
   const long long rows = static_cast<long long>(max_q) * (nq / nkv);
-  const int R = tile_rows(rows), team = team_warps(R, max_kv);
+  const int R = tile_rows(rows);
   const int tokens = std::max(1, max_kv);
   p.tiles = static_cast<int>((rows + R - 1) / R);
-  p.parts = (tokens - 1) / chunk_tokens(tokens, team) + 1;
-  // just past a change of the step, a shorter cache has more chunks
-  if (team == 1 && tokens > 512) p.parts = std::max(p.parts, 8);
-  if (team == 1 && tokens > 2048) p.parts = std::max(p.parts, 16);
-  if (tokens > kMaxParts * 256) p.parts = kMaxParts;
+  p.parts = (tokens - 1) / chunk_tokens(tokens) + 1;
+  if (tokens > kMaxParts * kChunk) p.parts = kMaxParts;  // a shorter cache may have as many
   p.rows = static_cast<int>(std::min<long long>(R, rows));
   p.stride = 2 * ((p.rows + 3) & ~3) + p.rows * hd;
   p.unit_bytes = 4ll * p.parts * p.stride;
@@ -768,7 +721,7 @@ int resident_ctas(K kern, size_t smem, cudaError_t* err) {
   return std::min(per, kMaxCtasPerSm) * device_sm_count();
 }
 
-template <typename T, int HD, int NT, int TEAM>
+template <typename T, int HD, int NT>
 cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int max_kv, cudaStream_t s) {
   constexpr int R = 8 * NT;
   // the ring, which also takes the warps' O, 4 kWarps R HD bytes; and 1 KB to align it
@@ -783,7 +736,7 @@ cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int ma
   int rc = make_tmap_nd(&tk, ap.kpool, false, 2, dims, stride, box, step, HD);
   if (!rc) rc = make_tmap_nd(&tv, ap.vpool, false, 2, dims, stride, box, step, HD);
   if (rc) return static_cast<cudaError_t>(rc);
-  auto kern = cache_attn_rows<T, HD, NT, TEAM>;
+  auto kern = cache_attn_rows<T, HD, NT>;
   static std::atomic<int> resident[64];  // per instantiation and device
   int dev = 0;
   cudaGetDevice(&dev);
@@ -803,12 +756,12 @@ cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int ma
   ap.cap_units = ws ? ws_bytes / ps.unit_bytes : 0;
   // no more CTAs than chunks, as far as max_kv tells
   const long long chunks = static_cast<long long>(ap.seqs.n_seqs) * ps.tiles * ap.nkv * ps.parts;
-  grid = static_cast<int>(std::min<long long>(grid, (chunks * TEAM + kWarps - 1) / kWarps));
+  grid = static_cast<int>(std::min<long long>(grid, chunks));
   cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kWarps * 32), kSmem, s, tk, tv, ap);
   if (e == cudaSuccess && ps.parts > 1 && ap.cap_units > 0) {
     constexpr bool kMany = R > 8;  // rows enough for a warp each
-    e = kMany && ps.parts <= kJoinAlone ? launch_join<T, HD, RowsPlan<R, TEAM, kSlab, kMany>>(ap, s)
-                                        : launch_join<T, HD, RowsPlan<R, TEAM, kSlab, false>>(ap, s);
+    e = kMany && ps.parts <= kJoinAlone ? launch_join<T, HD, RowsPlan<R, kSlab, kMany>>(ap, s)
+                                        : launch_join<T, HD, RowsPlan<R, kSlab, false>>(ap, s);
   }
   return e;
 }
@@ -816,14 +769,15 @@ cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int ma
 template <typename T, int HD>
 cudaError_t launch_any(const CacheAttnParams& ap, void* ws, long long ws_bytes, int max_kv, cudaStream_t s) {
   const int R = tile_rows(static_cast<long long>(ap.seqs.max_q) * (ap.nq / ap.nkv));
-  if (R == 24) return launch_rows<T, HD, 3, kWarps>(ap, ws, ws_bytes, max_kv, s);
-  if (R == 8)
-    return team_warps(8, max_kv) == 1 ? launch_rows<T, HD, 1, 1>(ap, ws, ws_bytes, max_kv, s)
-                                      : launch_rows<T, HD, 1, kWarps>(ap, ws, ws_bytes, max_kv, s);
-  return launch_rows<T, HD, 2, kWarps>(ap, ws, ws_bytes, max_kv, s);
+  if (R == 8) return launch_rows<T, HD, 1>(ap, ws, ws_bytes, max_kv, s);
+  if (R == 16) return launch_rows<T, HD, 2>(ap, ws, ws_bytes, max_kv, s);
+  return launch_rows<T, HD, 3>(ap, ws, ws_bytes, max_kv, s);
 }
 
-// Rows of a K/V head and sequence up to which the few-row kernel is used.
+// Rows of a K/V head and sequence up to which the few-row kernel is used: as far as
+// its registers reach.  12 tokens, 24 rows, of 16 sessions over 5000 tokens: 109 us
+// here with chunks of 256 tokens, 125 on the tcgen05 kernel, which pads them to 128
+// rows (8 tokens, 16 rows: 84 and 123; one session of 24 rows: 33 and 39).
 constexpr int kFewRows = 24;
 
 }  // namespace
