@@ -187,8 +187,8 @@ int qa_k_cache_attention(const void* q, long long ldq, long long T, int nq, int 
 
 /*
  * out [M][N] = x [M][K] . W^T (+ bias [N] f32), the weights in 4 bits:
- * W[n][k] = scales[n][k / group] * (code[n][k] - zeros[n][k / group]), zeros 8
- * when NULL.  wq [N] rows of K / 2 bytes, ldw bytes apart, the even k of a pair
+ * W[n][k] = scales[n][k / group] * (code[n][k] - zeros[n][k / group]), zeros any
+ * byte, 8 when NULL.  wq [N] rows of K / 2 bytes, ldw bytes apart, the even k of a pair
  * in the low nibble; scales [N][K / group] in x's type; group 32, 64 or 128, K a
  * multiple of it.  f32 sums, one rounding.  Built for few rows, where the
  * weights are what has to be read; any M is taken.

@@ -667,7 +667,7 @@ def w4_linear(x, wq, scales, out, *, zeros=None, bias=None, stream=None):
     """out [M, N] = x [M, K] . W^T + bias, W in 4 bits (qa_k_w4_linear).
 
     wq uint8 [N, K / 2], low nibble first; scales [N, K / group] of x's type with
-    group 32, 64 or 128 (told by the shapes); zeros uint8 like scales (None: 8);
+    group 32, 64 or 128 (told by the shapes); zeros uint8 like scales, any value (None: 8);
     bias f32 [N].
     """
     if _F16 is None:

@@ -94,24 +94,40 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
 }
 
 // The pairs of nibbles (0,4) (1,5) (2,6) (3,7) of a word, less the zero, as
-// 16-bit values.  f16: 1024 + code with the code in the low four bits of the
-// mantissa, 64 + code with it four bits higher, so one shift serves two pairs.
-// bf16: 128 + code.  All exact, and so are the differences.
+// 16-bit values:  code - zero = (base + 15 - zero) - (base + (15 - code)).  The
+// nibble's complement 15 - code goes into the mantissa of a power of two by bit
+// work: f16 with 1024, its low four bits, and with 64, four bits higher, so one
+// shift serves two pairs; bf16 with 128.  base + 15 - zero lies in [-176, 1039] for
+// every byte (bf16: [-112, 143]) and is exact, which base + zero is not in bf16 (no
+// odd numbers above 256); so are the differences, at most 255 in size.
 template <typename T>
-struct Zero {  // base + zero, twice
+struct Zero {  // base + 15 - zero, twice
   uint32_t lo, hi;
-  __device__ __forceinline__ Zero() : Zero(8u) {}
-  __device__ __forceinline__ explicit Zero(uint32_t z) {
+  __device__ __forceinline__ Zero() {
     if constexpr (H16Traits<T>::kBf16) {
-      lo = hi = (0x4300u | z) * 0x10001u;
+      lo = hi = 0x43074307u;  // 135
     } else {
-      lo = (0x6400u | z) * 0x10001u;
-      hi = (0x5400u | z << 4) * 0x10001u;
+      lo = 0x64076407u;  // 1031
+      hi = 0x54705470u;  // 71
+    }
+  }
+  // the zero is byte `at` of w
+  __device__ __forceinline__ Zero(uint32_t w, int at) {
+    if constexpr (H16Traits<T>::kBf16) {
+      // 2^23 + zero, byte by byte; the difference is exact
+      const float f = 8388608.0f + 143.0f - __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7640u | at));
+      lo = hi = cvt2_rn<T>(make_float2(f, f));
+    } else {
+      const uint32_t z = __byte_perm(w, 0x00000064u, 0x4040u | at * 0x101u);  // 1024 + zero, twice
+      const __half2 h = __hsub2(__half2half2(__ushort_as_half(0x644F)), *reinterpret_cast<const __half2*>(&z));  // 1103 -
+      const __half2 l = __hadd2(h, __half2half2(__ushort_as_half(0x6380)));                                      // + 960
+      lo = *reinterpret_cast<const uint32_t*>(&l);
+      hi = *reinterpret_cast<const uint32_t*>(&h);
     }
   }
 };
 // The masks and bases in registers: an instruction takes one constant, and
-// (w & mask) | base is one instruction only when the other operand is a register.
+// (~w & mask) | base is one instruction only when the other operand is a register.
 template <typename T>
 struct Bits {
   uint32_t mask_lo, base_lo, mask_hi, base_hi;
@@ -122,9 +138,9 @@ struct Bits {
     asm volatile("mov.b32 %0, 0x54005400;" : "=r"(base_hi));
   }
 };
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t base) {
+__device__ __forceinline__ uint32_t andn_or(uint32_t a, uint32_t mask, uint32_t base) {
   uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(base));
+  asm("lop3.b32 %0, %1, %2, %3, 0xAE;" : "=r"(d) : "r"(a), "r"(mask), "r"(base));  // (~a & mask) | base
   return d;
 }
 template <typename T>
@@ -132,18 +148,18 @@ __device__ __forceinline__ void weights8(uint32_t w, const Zero<T>& z, const Bit
   if constexpr (H16Traits<T>::kBf16) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t v = and_or(w >> (4 * i), k.mask_lo, k.base_lo);
+      const uint32_t v = andn_or(w >> (4 * i), k.mask_lo, k.base_lo);
       const __nv_bfloat162 d =
-          __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&z.lo));
+          __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&z.lo), *reinterpret_cast<const __nv_bfloat162*>(&v));
       out[i] = *reinterpret_cast<const uint32_t*>(&d);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t u = i < 2 ? w : w >> 8;
-      const uint32_t v = i & 1 ? and_or(u, k.mask_hi, k.base_hi) : and_or(u, k.mask_lo, k.base_lo);
+      const uint32_t v = i & 1 ? andn_or(u, k.mask_hi, k.base_hi) : andn_or(u, k.mask_lo, k.base_lo);
       const __half2 d =
-          __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(i & 1 ? &z.hi : &z.lo));
+          __hsub2(*reinterpret_cast<const __half2*>(i & 1 ? &z.hi : &z.lo), *reinterpret_cast<const __half2*>(&v));
       out[i] = *reinterpret_cast<const uint32_t*>(&d);
     }
   }
@@ -325,7 +341,7 @@ __global__ void __launch_bounds__(kWarps * 32, Form<NT>::kCtas) w4_kernel(const 
 #pragma unroll
         for (int r = 0; r < 2 * kRb; ++r) {
           Zero<T> zero;
-          if constexpr (ZEROS) zero = Zero<T>(__shfl_sync(0xFFFFFFFFu, a.z, (lane & 28) + r) >> (8 * q) & 0xFFu);
+          if constexpr (ZEROS) zero = Zero<T>(__shfl_sync(0xFFFFFFFFu, a.z, (lane & 28) + r), q);
           const uint32_t word = w == 0 ? a.w[r].x : w == 1 ? a.w[r].y : w == 2 ? a.w[r].z : a.w[r].w;
           weights8<T>(word, zero, bits, k[r]);
         }
