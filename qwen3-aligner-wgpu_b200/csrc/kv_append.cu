@@ -226,7 +226,12 @@ __global__ void __launch_bounds__(kThreads, B8 ? (HD == 128 ? 2 : 3) : 4)
   uint32_t axes = 0;  // 2 bits for each of this lane's frequencies
   if (ap.rope.n_axes > 1)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) axes |= (ap.rope.axis_of[d0 + i] & 3) << (2 * i);
+    for (int i = 0; i < 8; ++i) {
+      const int a = ap.rope.axis_of[d0 + i];
+      const bool there = a >= 0 && a < ap.rope.n_axes;
+      bad |= !there;
+      axes |= static_cast<uint32_t>(there ? a : 0) << (2 * i);
+    }
 
   float kx[B8 ? kRounds : 1][16];
   float kmax = 0.0f, vmax = 0.0f;

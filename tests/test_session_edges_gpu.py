@@ -1,10 +1,10 @@
 """Edges of the operators of growing sessions, against the same plain
 implementations in 64 bits and with the same bounds as test_session_ops_gpu.py:
-zero points over the whole byte."""
+zero points over the whole byte, axes that are not there."""
 import pytest
 
 from conftest import cuda_ok, pkg
-from test_session_ops_gpu import _check_w4, _w4_case
+from test_session_ops_gpu import _append_case, _check_w4, _split, _w4_case
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +35,30 @@ def test_w4_zero_points_are_any_byte(dtype, group, m, pad):
     out = torch.full((m, n), float("nan"), dtype=c["x"].dtype, device="cuda")
     pkg()._lib.w4_linear(x, c["wq"].cuda(), c["scales"].cuda(), out, zeros=c["zeros"].cuda())
     _check_w4(c, out)
+
+# ---------------------------------------------------------------- kv_append
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_append_reports_an_axis_that_is_not_there(bits):
+    """Without `validate`, an axis outside [0, axes) sets the status and counts as
+    the first axis; the other frequencies are not affected."""
+    import torch
+    c = _append_case([(5, 70), (3, 3)], "f16", 64, 4, 2, bits, False, 3, seed=11)
+    d = {k: (v.cuda() if isinstance(v, torch.Tensor) else v) for k, v in c.items()}
+    q, k, v = _split(c, d["packed"])
+
+    def run(axis_of):
+        st, q_out = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.empty_like(q)
+        scales = {n: None if d[n] is None else d[n].clone() for n in ("kscale", "vscale")}
+        pkg()._lib.kv_append(q, k, v, q_out, d["q_start"], d["kv_len"], d["tab"], d["kpool"].clone(),
+                             d["vpool"].clone(), max_q=5, cos=d["cos"], sin=d["sin"], pos=d["pos"],
+                             axis_of=axis_of.cuda(), status=st, validate=False, **scales)
+        return int(st.item()), q_out
+
+    assert run(c["axis_of"])[0] == 0
+    for bad in (3, 4, 7, -1, 1 << 30, -(1 << 31)):
+        axis, as_first = c["axis_of"].clone(), c["axis_of"].clone()
+        axis[17], as_first[17] = bad, 0
+        status, q_out = run(axis)
+        assert status == 2, bad
+        assert torch.equal(q_out, run(as_first)[1]), bad
