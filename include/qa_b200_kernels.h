@@ -143,8 +143,8 @@ int qa_k_window_attention(const void* qkv, long long T, int dm, int nh, const in
  *
  * Rotation: cos_t / sin_t [table_rows][hd / 2] f32 (NULL: none), the halves of a
  * head paired (j, j + hd / 2).  Positions: pos [n_axes][pos_stride], NULL for the
- * cache index; with n_axes > 1 (at most 4), axis_of [hd / 2] names each
- * frequency's axis.  A position outside the tables or an axis outside
+ * cache index; with tables and n_axes > 1 (at most 4), axis_of [hd / 2] names
+ * each frequency's axis.  A position outside the tables or an axis outside
  * [0, n_axes) sets bit 2 of *status and counts as 0.  qn / kn [hd] (both or
  * neither): RMSNorm of each head before the rotation, with eps.  Arithmetic in
  * f32, rounded once.  kpool, vpool, cos_t and sin_t are 16-byte aligned.

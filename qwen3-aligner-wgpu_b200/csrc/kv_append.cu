@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, B8 ? (HD == 128 ? 2 : 3) : 4)
     bad = !page_ok;
   }
   uint32_t axes = 0;  // 2 bits for each of this lane's frequencies
-  if (ap.rope.n_axes > 1)
+  if (ap.rope.cos_t && ap.rope.n_axes > 1)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int a = ap.rope.axis_of[d0 + i];

@@ -1,10 +1,11 @@
 """Edges of the operators of growing sessions, against the same plain
 implementations in 64 bits and with the same bounds as test_session_ops_gpu.py:
-zero points over the whole byte, axes that are not there."""
+zero points over the whole byte, axes that are not there,
+calls without tables."""
 import pytest
 
 from conftest import cuda_ok, pkg
-from test_session_ops_gpu import _append_case, _check_w4, _split, _w4_case
+from test_session_ops_gpu import _append_case, _check_append, _check_w4, _split, _w4_case
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +63,29 @@ def test_append_reports_an_axis_that_is_not_there(bits):
         status, q_out = run(axis)
         assert status == 2, bad
         assert torch.equal(q_out, run(as_first)[1]), bad
+
+
+def _append_c(c, max_q, n_axes=1, axis_of=0):
+    """Through the C entry, without tables or positions: what a caller may leave out."""
+    import torch
+    L = pkg()._lib
+    d = {k: (v.cuda() if isinstance(v, torch.Tensor) else v) for k, v in c.items()}
+    q, k, v = _split(c, d["packed"])
+    q_out, st = torch.empty_like(q), torch.zeros(1, dtype=torch.int32, device="cuda")
+    rc = L.lib().qa_k_kv_append(
+        q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), q_out.data_ptr(),
+        q_out.stride(0), q.shape[0], c["nq"], c["nkv"], c["hd"], d["q_start"].data_ptr(), d["kv_len"].data_ptr(),
+        len(c["seqs"]), max_q, d["tab"].data_ptr(), d["tab"].shape[1], d["kpool"].data_ptr(), d["vpool"].data_ptr(),
+        c["pages"], d["kscale"].data_ptr(), d["vscale"].data_ptr(), 0, 0, 0, 0, 0, n_axes, axis_of, 0, 0, 1e-6,
+        1 if c["dtype"] == "bf16" else 0, st.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    c = dict(c, cos=torch.ones_like(c["cos"]), sin=torch.zeros_like(c["sin"]))  # what no rotation amounts to
+    return rc, int(st.item()), c, {n: x.cpu() for n, x in dict(q=q_out, kpool=d["kpool"], vpool=d["vpool"],
+                                                               kscale=d["kscale"], vscale=d["vscale"]).items()}
+
+
+def test_append_without_tables_reads_no_axes():
+    c = _append_case([(70, 75), (1, 9)], "bf16", 128, 4, 2, 8, False, 0, seed=13)
+    rc, status, c, got = _append_c(c, 70, n_axes=3)
+    assert rc == 0 and status == 0
+    _check_append(c, got)
