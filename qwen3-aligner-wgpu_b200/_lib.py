@@ -590,7 +590,14 @@ def kv_append(q, k, v, q_out, q_start, kv_len, block_tab, kpool, vpool, *, max_q
         check(rc)
 
 
-_workspaces: dict = {}  # (device, stream) -> the attention's workspace
+def _workspace(need, device, stream):
+    """`need` bytes that belong to the stream of the launch, so that whoever gets
+    them next is behind it; under graph capture they come from the graph's pool."""
+    import torch
+    if stream is None:
+        return torch.empty(need, dtype=_U8, device=device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+        return torch.empty(need, dtype=_U8, device=device)
 
 
 def cache_attention(q, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale, out, *, max_q,
@@ -601,9 +608,8 @@ def cache_attention(q, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale,
     q and out [T, nq * hd] 16-bit; the maps, pools and scales as for kv_append;
     lse f32 [T, nq] optional; scale defaults to 1 / sqrt(hd).  max_q and max_kv
     bound the sequences' new and cached tokens.  `validate` copies the maps to
-    the host to check them.  A workspace is kept for each stream and grows with
-    the sizes seen; under graph capture it comes from the graph's own pool, so that
-    a graph neither shares it with later calls nor outlives it.
+    the host to check them.  The workspace is torch's, taken and given back in the
+    order of the launch stream; a graph that captures the call has its own.
     """
     if _F16 is None:
         _types()
@@ -645,14 +651,7 @@ def cache_attention(q, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale,
     need = size(nq, nkv, hd, n, max_q, max_kv)
     ws = 0
     if need:
-        import torch
-        if torch.cuda.is_current_stream_capturing():
-            buf = torch.empty(need, dtype=_U8, device=q.device)  # the graph's own
-        else:
-            buf = _workspaces.get((dev, s))
-            if buf is None or buf.numel() < need:
-                torch.cuda.synchronize(dev)  # nobody uses the old one
-                buf = _workspaces[(dev, s)] = torch.empty(need, dtype=_U8, device=q.device)
+        buf = _workspace(need, q.device, stream)
         ws = buf.data_ptr()
     rc = call(_pack27(
         q.data_ptr(), ldq, T, nq, nkv, hd, q_start.data_ptr(), kv_len.data_ptr(), n, max_q,

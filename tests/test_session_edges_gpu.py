@@ -1,11 +1,11 @@
 """Edges of the operators of growing sessions, against the same plain
 implementations in 64 bits and with the same bounds as test_session_ops_gpu.py:
 zero points over the whole byte, axes that are not there,
-calls without tables."""
+calls without tables, captures of a stream that is not the current one."""
 import pytest
 
 from conftest import cuda_ok, pkg
-from test_session_ops_gpu import _append_case, _check_append, _check_w4, _split, _w4_case
+from test_session_ops_gpu import _append_case, _attn_case, _check_append, _check_attn, _check_w4, _split, _w4_case
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +89,33 @@ def test_append_without_tables_reads_no_axes():
     rc, status, c, got = _append_c(c, 70, n_axes=3)
     assert rc == 0 and status == 0
     _check_append(c, got)
+
+
+# ---------------------------------------------------------------- cache_attention
+
+def test_attention_captured_on_a_stream_that_is_not_the_current_one():
+    import torch
+    c = _attn_case([(1, 5000), (1, 3100)], "f16", 128, 16, 8, seed=43)
+    d = {k: (v.cuda() if isinstance(v, torch.Tensor) else v) for k, v in c.items()}
+    out, lse = torch.empty_like(d["buf"]), torch.empty(2, 16, device="cuda")
+
+    def run(stream):
+        pkg()._lib.cache_attention(d["buf"], d["q_start"], d["kv_len"], d["tab"], d["kpool"], d["vpool"], d["kscale"],
+                                   d["vscale"], out, lse=lse, max_q=1, max_kv=5000, stream=stream, validate=False)
+
+    s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    run(s.cuda_stream)
+    torch.cuda.synchronize()
+    want = out.clone()
+    with torch.cuda.stream(s):
+        graph.capture_begin()
+    run(s.cuda_stream)
+    with torch.cuda.stream(s):
+        graph.capture_end()
+    for _ in range(2):
+        out.zero_(), lse.zero_()
+        graph.replay()
+        run(s.cuda_stream)  # does not work in the graph's memory
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    _check_attn(c, (c["buf"], out.cpu(), lse.cpu()))

@@ -1,0 +1,126 @@
+"""Host side of the session operators, without a GPU: whose memory
+a call works in.
+
+The tensors here lie in host memory and say that they are on a device; the
+library's entry points are replaced by ones that record the call."""
+import contextlib
+
+import pytest
+import torch
+
+from conftest import pkg
+
+PAGE = 64
+
+
+class _OnDevice(torch.Tensor):
+    """A host tensor that calls itself one of device 1."""
+
+    def get_device(self):
+        return 1
+
+
+class _Gpu:
+    """What the wrappers ask of CUDA, with device `current` current; `calls` holds
+    (operator, current device, arguments) of each launch."""
+
+    def __init__(self, monkeypatch, current):
+        self.current, self.calls = current, []
+        lib = pkg()._lib
+
+        class Stream:
+            cuda_stream = 4321
+
+        @contextlib.contextmanager
+        def device(d):
+            was, self.current = self.current, d
+            try:
+                yield
+            finally:
+                self.current = was
+
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: self.current)
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: Stream)
+        monkeypatch.setattr(torch.cuda, "device", device)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+        monkeypatch.setattr(torch.cuda, "synchronize", lambda d=None: None)
+
+        def entry(name, n):
+            def call(packed, *rest):
+                import struct
+                self.calls.append((name, self.current, struct.unpack(f"{n}q", packed)))
+                return 0
+            return call
+
+        monkeypatch.setattr(lib, "_fn_kv_append", lambda: entry("append", 35))
+        monkeypatch.setattr(lib, "_fn_w4_linear", lambda: entry("w4", 15))
+        size = lib.lib().qa_k_cache_attention_workspace
+        monkeypatch.setattr(lib, "_fn_cache_attention", lambda: (entry("attend", 27), size))
+
+
+def _there(*shape, dtype=torch.float16):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(_OnDevice)
+
+
+def _codes(*shape):
+    return torch.zeros(*shape, dtype=torch.uint8).view(torch.float8_e4m3fn).as_subclass(_OnDevice)
+
+
+def _maps(n, pages, length):
+    qs = torch.arange(n + 1, dtype=torch.int32).as_subclass(_OnDevice)
+    kl = torch.full((n,), length, dtype=torch.int32).as_subclass(_OnDevice)
+    tab = torch.arange(n * pages, dtype=torch.int32).view(n, pages).as_subclass(_OnDevice)
+    return qs, kl, tab
+
+
+def _append(n=2, pages=2, nkv=2, nq=4, hd=64, **kw):
+    qs, kl, tab = _maps(n, pages, 70)
+    kw = {**dict(max_q=1), **kw}
+    pkg()._lib.kv_append(_there(n, nq * hd), _there(n, nkv * hd), _there(n, nkv * hd), _there(n, nq * hd), qs, kl, tab,
+                         _codes(n * pages, nkv, PAGE, hd), _codes(n * pages, nkv, PAGE, hd),
+                         kscale=_there(n * pages, nkv, dtype=torch.float32),
+                         vscale=_there(n * pages, nkv, dtype=torch.float32), **kw)
+
+
+def _attend(n=2, pages=2, nkv=2, nq=4, hd=64, **kw):
+    qs, kl, tab = _maps(n, pages, 70)
+    kw = {**dict(max_q=1, max_kv=70), **kw}
+    pkg()._lib.cache_attention(_there(n, nq * hd), qs, kl, tab, _codes(n * pages, nkv, PAGE, hd),
+                               _codes(n * pages, nkv, PAGE, hd), _there(n * pages, nkv, dtype=torch.float32),
+                               _there(n * pages, nkv, dtype=torch.float32), _there(n, nq * hd), **kw)
+
+
+def _w4(**kw):
+    pkg()._lib.w4_linear(_there(3, 256), _there(10, 128, dtype=torch.uint8), _there(10, 2), _there(3, 10), **kw)
+
+
+def test_the_attentions_workspace_belongs_to_the_launch_stream(monkeypatch):
+    """Taken with the launch's stream current (a capture of that stream is seen, and
+    memory given back is reused behind the call), and given back after the call."""
+    import weakref
+    gpu, on, taken = _Gpu(monkeypatch, 1), [4321], []
+
+    @contextlib.contextmanager
+    def stream(s):
+        on.append(s)
+        try:
+            yield
+        finally:
+            on.pop()
+
+    plain = torch.empty
+
+    def empty(*shape, **kw):
+        buf = plain(*shape, **kw)
+        if kw.get("dtype") is torch.uint8:
+            taken.append((on[-1], weakref.ref(buf)))
+        return buf
+
+    monkeypatch.setattr(torch.cuda, "stream", stream)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda handle, device=None: handle)
+    monkeypatch.setattr(torch, "empty", empty)
+    for handle in (None, 77, 77):
+        _attend(pages=40, max_kv=2500, stream=handle, validate=False)
+    assert [s for s, _ in taken] == [4321, 77, 77] == [c[2][-1] for c in gpu.calls]
+    assert all(buf() is None for _, buf in taken)
+    assert all(c[2][22] and c[2][23] > 0 for c in gpu.calls)  # and it was passed on
