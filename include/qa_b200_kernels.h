@@ -8,7 +8,8 @@
  * src/audio_encoder_gpu.rs), so each declaration names the reference stage it
  * computes instead.
  *
- * All functions return 0 on success or a QA_ERR_* code (see qa_b200.h).
+ * All functions return 0 on success or a QA_ERR_* code (see qa_b200.h).  They
+ * launch on the current device, which has to be the buffers' and the stream's.
  * 16-bit element buffers are f16 when `bf16 == 0`, bf16 otherwise.
  */
 #ifndef QA_B200_KERNELS_H

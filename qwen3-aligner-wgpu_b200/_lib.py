@@ -399,12 +399,13 @@ def gemm_qkv_rope(A, B, q_out, pos_of, clip_of, block_tab, kc, vc, cos_t, sin_t,
 # to the library as one array (qa_k_*_v).
 _pack35, _pack27, _pack15 = (struct.Struct(f"{n}q").pack for n in (35, 27, 15))
 
-_F16 = _BF16 = _F32 = _I32 = _U8 = _E4M3 = None
+_F16 = _BF16 = _F32 = _I32 = _U8 = _E4M3 = _cuda = None
 
 
 def _types():
-    global _F16, _BF16, _F32, _I32, _U8, _E4M3
+    global _F16, _BF16, _F32, _I32, _U8, _E4M3, _cuda
     import torch
+    _cuda = torch.cuda
     _F16, _BF16, _F32, _I32, _U8, _E4M3 = (torch.float16, torch.bfloat16, torch.float32, torch.int32,
                                            torch.uint8, torch.float8_e4m3fn)
     return _F16
@@ -476,8 +477,19 @@ def check_sequences(T, q_start, kv_len, block_tab, pages, max_q, appending) -> N
 
 
 def _stream(dev, stream):
-    import torch
-    return torch.cuda.current_stream(dev).cuda_stream if stream is None else stream
+    return _cuda.current_stream(dev).cuda_stream if stream is None else stream
+
+
+def _launch(dev, entry, *args) -> None:
+    """Calls a C entry with the tensors' device `dev` current: it launches there, and a
+    default stream's handle names no device."""
+    if _cuda.current_device() == dev:
+        rc = entry(*args)
+    else:
+        with _cuda.device(dev):
+            rc = entry(*args)
+    if rc:
+        check(rc)
 
 
 def _elsewhere():
@@ -581,13 +593,11 @@ def kv_append(q, k, v, q_out, q_start, kv_len, block_tab, kpool, vpool, *, max_q
             raise ValueError("kv_len outside the tables")
     if not here:
         _elsewhere()
-    rc = _fn_kv_append()(_pack35(
+    _launch(dev, _fn_kv_append(), _pack35(
         q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, q_out.data_ptr(), ldqo, T, nq, nkv,
         hd, q_start.data_ptr(), kv_len.data_ptr(), n, max_q, block_tab.data_ptr(), max_pages,
         kpool.data_ptr(), vpool.data_ptr(), pages, ks, vs, cs, sn, rows, ps, stride, axes, ax, gq, gk,
         1 if dt is _BF16 else 0, st, _stream(dev, stream)), eps)
-    if rc:
-        check(rc)
 
 
 def _workspace(need, device, stream):
@@ -653,13 +663,11 @@ def cache_attention(q, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale,
     if need:
         buf = _workspace(need, q.device, stream)
         ws = buf.data_ptr()
-    rc = call(_pack27(
+    _launch(dev, call, _pack27(
         q.data_ptr(), ldq, T, nq, nkv, hd, q_start.data_ptr(), kv_len.data_ptr(), n, max_q,
         max_kv, block_tab.data_ptr(), max_pages, kpool.data_ptr(), vpool.data_ptr(), pages,
         kscale.data_ptr(), vscale.data_ptr(), 1 if causal else 0, out.data_ptr(), ldo, ls, ws, need,
         1 if dt is _BF16 else 0, st, s), hd ** -0.5 if scale is None else scale)
-    if rc:
-        check(rc)
 
 
 def w4_linear(x, wq, scales, out, *, zeros=None, bias=None, stream=None):
@@ -700,11 +708,9 @@ def w4_linear(x, wq, scales, out, *, zeros=None, bias=None, stream=None):
         here = here and bias.get_device() == dev
     if not here:
         _elsewhere()
-    rc = _fn_w4_linear()(_pack15(
+    _launch(dev, _fn_w4_linear(), _pack15(
         x.data_ptr(), ldx, M, K, wq.data_ptr(), ldw, N, group, scales.data_ptr(), z, b,
         out.data_ptr(), ldo, 1 if dt is _BF16 else 0, _stream(dev, stream)))
-    if rc:
-        check(rc)
 
 
 # The C functions, looked up once: lib() takes a lock.

@@ -1,5 +1,5 @@
-"""Host side of the session operators, without a GPU: whose memory
-a call works in.
+"""Host side of the session operators, without a GPU: where a call
+launches, and whose memory it works in.
 
 The tensors here lie in host memory and say that they are on a device; the
 library's entry points are replaced by ones that record the call."""
@@ -124,3 +124,12 @@ def test_the_attentions_workspace_belongs_to_the_launch_stream(monkeypatch):
     assert [s for s, _ in taken] == [4321, 77, 77] == [c[2][-1] for c in gpu.calls]
     assert all(buf() is None for _, buf in taken)
     assert all(c[2][22] and c[2][23] > 0 for c in gpu.calls)  # and it was passed on
+
+
+@pytest.mark.parametrize("current", [0, 1])
+@pytest.mark.parametrize("op", [_append, _attend, _w4])
+def test_a_call_launches_on_its_tensors_device(monkeypatch, op, current):
+    gpu = _Gpu(monkeypatch, current)
+    op()
+    assert [c[1] for c in gpu.calls] == [1] and gpu.current == current
+    assert gpu.calls[0][2][-1] == 4321  # the stream that was asked for there
