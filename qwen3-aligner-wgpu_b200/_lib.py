@@ -578,6 +578,8 @@ def kv_append(q, k, v, q_out, q_start, kv_len, block_tab, kpool, vpool, *, max_q
         gq, gk = qn.data_ptr(), kn.data_ptr()
         here = here and qn.get_device() == dev and kn.get_device() == dev
     if status is not None:
+        if status.dtype is not _I32 or status.numel() == 0:
+            raise ValueError("status int32 [1]")
         st = status.data_ptr()
         here = here and status.get_device() == dev
     if validate:
@@ -648,6 +650,8 @@ def cache_attention(q, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale,
         ls = lse.data_ptr()
         here = here and lse.get_device() == dev
     if status is not None:
+        if status.dtype is not _I32 or status.numel() == 0:
+            raise ValueError("status int32 [1]")
         st = status.data_ptr()
         here = here and status.get_device() == dev
     if validate:

@@ -133,3 +133,14 @@ def test_a_call_launches_on_its_tensors_device(monkeypatch, op, current):
     op()
     assert [c[1] for c in gpu.calls] == [1] and gpu.current == current
     assert gpu.calls[0][2][-1] == 4321  # the stream that was asked for there
+
+
+@pytest.mark.parametrize("op", [_append, _attend])
+def test_a_status_that_cannot_take_the_bits_is_refused(monkeypatch, op):
+    gpu = _Gpu(monkeypatch, 1)
+    for dtype, size in ((torch.int32, 0), (torch.uint8, 1), (torch.int16, 2), (torch.float32, 1), (torch.int64, 1)):
+        with pytest.raises(ValueError, match="status"):
+            op(status=_there(size, dtype=dtype))
+    assert not gpu.calls
+    op(status=_there(1, dtype=torch.int32))
+    assert len(gpu.calls) == 1
