@@ -118,8 +118,8 @@ int qa_k_window_attention(const void* qkv, long long T, int dm, int nh, const in
  * counterpart in the reference, which prefills a whole clip at once.
  *
  * New tokens are packed: sequence s owns rows [q_start[s], q_start[s + 1]) of
- * every [T]-row buffer, at most max_q of them (0 is allowed), and its cache
- * holds kv_len[s] tokens, the new ones among them.  q_start [n_seqs + 1],
+ * every [T]-row buffer, at most max_q of them (0 is allowed; a max_q above T
+ * counts as T), and its cache holds kv_len[s] tokens, the new ones among them.  q_start [n_seqs + 1],
  * kv_len [n_seqs] and block_tab [n_seqs][max_pages] are device data; they are
  * checked on the device, and what contradicts the sizes given here (a sequence
  * outside [0, T) or longer than max_q or than its table, a page id outside
@@ -168,8 +168,9 @@ int qa_k_kv_append(const void* q, long long ldq, const void* k, long long ldk, c
  * sets bit 2 of *status and its tokens are left out.  lse [T][nq] f32 (natural
  * logarithm of the sum of exponentials) may be NULL.
  *
- * max_kv (the longest kv_len, as far as the caller knows) sizes the launch; a
- * smaller or larger value gives the same results up to the order of sums.
+ * max_kv (the longest kv_len, as far as the caller knows; above 64 * max_pages it
+ * counts as that) sizes the launch; a smaller or larger value gives the same
+ * results up to the order of sums.
  *
  * workspace: device memory, 16-byte aligned, of the size that
  * qa_k_cache_attention_workspace gives for these arguments (0: none is needed);

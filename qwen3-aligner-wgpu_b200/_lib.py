@@ -521,6 +521,7 @@ def kv_append(q, k, v, q_out, q_start, kv_len, block_tab, kpool, vpool, *, max_q
     nq = width // hd
     if nq == 0 or nq % nkv or nq * hd != width:
         raise ValueError("q has a multiple of the cache's heads")
+    max_q = min(max_q, T)  # no sequence has more
     kw = nkv * hd
     ldq, ldqo = _rows(q, T, width, dt, "q"), _rows(q_out, T, width, dt, "q_out")
     ldk, ldv = _rows(k, T, kw, dt, "k"), _rows(v, T, kw, dt, "v")
@@ -640,6 +641,7 @@ def cache_attention(q, q_start, kv_len, block_tab, kpool, vpool, kscale, vscale,
     ldq, ldo = _rows(q, T, width, dt, "q"), _rows(out, T, width, dt, "out")
     if max_kv < 0:
         raise ValueError("max_kv >= 0")
+    max_q, max_kv = min(max_q, T), min(max_kv, 64 * max_pages)  # no sequence has more
     ls = st = 0
     dev = q.get_device()
     here = dev >= 0 and (out.get_device() == q_start.get_device() == kv_len.get_device()

@@ -811,6 +811,8 @@ int cache_attention(const void* q, long long ldq, long long T, int nqh, int nkvh
                     void* out, long long ldo, float* lse, void* workspace,
                     long long workspace_bytes, bool bf16, unsigned* status, cudaStream_t s) {
   if (T <= 0 || seqs.n_seqs <= 0 || max_q <= 0) return 0;
+  max_q = static_cast<int>(std::min<long long>(max_q, T));  // no sequence has more
+  max_kv = static_cast<int>(std::min(static_cast<long long>(max_kv), 64ll * seqs.max_pages));
   CacheAttnParams ap{};
   ap.q = q;
   ap.ldq = ldq;

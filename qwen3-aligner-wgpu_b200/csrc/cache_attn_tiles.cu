@@ -893,7 +893,7 @@ PartSizes part_sizes(int nq, int nkv, int hd, int max_q, int max_kv) {
   PartSizes p;
   const long long rows = static_cast<long long>(max_q) * (nq / nkv);
   p.tiles = static_cast<int>((rows + kUnitRows - 1) / kUnitRows);
-  const int keys = std::max(1, (max_kv + kKeys - 1) / kKeys);
+  const int keys = (std::max(1, max_kv) - 1) / kKeys + 1;
   p.parts = 2 * std::min(kMaxChunks, (keys + kMinStep - 1) / kMinStep);
   p.rows = static_cast<int>(std::min<long long>(kUnitRows, rows));
   p.stride = 2 * ((p.rows + 3) & ~3) + p.rows * hd;

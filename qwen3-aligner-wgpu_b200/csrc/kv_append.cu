@@ -34,6 +34,8 @@
 // one token 9.4 us in the kernel, 18 with CTAs of 256 threads.
 #include <cuda_fp8.h>
 
+#include <algorithm>
+
 #include "kernels.cuh"
 #include "sm100.cuh"
 
@@ -394,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, B8 ? (HD == 128 ? 2 : 3) : 4)
 template <typename T, int HD, bool B8>
 cudaError_t launch(AppendParams& ap, cudaStream_t s) {
   constexpr int kTokens = tokens<HD, B8>();
-  ap.runs_per_seq = (ap.seqs.max_q + 2 * kTokens - 2) / kTokens;  // from a run's last slot on
+  ap.runs_per_seq = static_cast<int>((ap.seqs.max_q + 2ll * kTokens - 2) / kTokens);  // from a run's last slot on
   const int work = min(ap.seqs.max_q, kTokens) * (HD / 16);
   const int threads = min(kThreads, (work + 31) / 32 * 32);
   ap.rounds = (work + threads - 1) / threads;
@@ -441,7 +443,7 @@ int kv_append(const void* q, long long ldq, const void* k, long long ldk, const 
   ap.group = nqh / nkvh;
   ap.nkv = nkvh;
   ap.seqs = seqs;
-  ap.seqs.max_q = max_q;
+  ap.seqs.max_q = static_cast<int>(std::min<long long>(max_q, T));  // no sequence has more
   ap.kpool = kv.k;
   ap.vpool = kv.v;
   ap.kv_pages = kv_pages;

@@ -1,7 +1,8 @@
 """Edges of the operators of growing sessions, against the same plain
 implementations in 64 bits and with the same bounds as test_session_ops_gpu.py:
 zero points over the whole byte, axes that are not there,
-calls without tables, captures of a stream that is not the current one."""
+calls without tables, bounds that say nothing, captures of a stream that
+is not the current one."""
 import pytest
 
 from conftest import cuda_ok, pkg
@@ -91,6 +92,14 @@ def test_append_without_tables_reads_no_axes():
     _check_append(c, got)
 
 
+@pytest.mark.parametrize("max_q", [71, 1 << 20, (1 << 31) - 1])
+def test_append_with_a_bound_that_says_nothing(max_q):
+    c = _append_case([(70, 75), (1, 9)], "f16", 64, 4, 2, 8, False, 0, seed=13)
+    rc, status, c, got = _append_c(c, max_q)
+    assert rc == 0 and status == 0
+    _check_append(c, got)
+
+
 # ---------------------------------------------------------------- cache_attention
 
 def test_attention_captured_on_a_stream_that_is_not_the_current_one():
@@ -119,3 +128,31 @@ def test_attention_captured_on_a_stream_that_is_not_the_current_one():
         torch.cuda.synchronize()
         assert torch.equal(out, want)
     _check_attn(c, (c["buf"], out.cpu(), lse.cpu()))
+
+
+def _attend_c(c, max_q, max_kv, workspace=None, causal=1):
+    """Through the C entry, in a workspace of the caller's (none: a null pointer)."""
+    import torch
+    L = pkg()._lib
+    d = {k: (v.cuda() if isinstance(v, torch.Tensor) else v) for k, v in c.items()}
+    q, out = d["buf"], torch.full_like(d["buf"], float("nan"))
+    lse = torch.full((q.shape[0], c["nq"]), float("nan"), device="cuda")
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ws = 0 if workspace is None else workspace.data_ptr()
+    rc = L.lib().qa_k_cache_attention(
+        q.data_ptr(), q.stride(0), q.shape[0], c["nq"], c["nkv"], c["hd"], d["q_start"].data_ptr(),
+        d["kv_len"].data_ptr(), len(c["seqs"]), max_q, max_kv, d["tab"].data_ptr(), d["tab"].shape[1],
+        d["kpool"].data_ptr(), d["vpool"].data_ptr(), c["pages"], d["kscale"].data_ptr(), d["vscale"].data_ptr(),
+        c["hd"] ** -0.5, causal, out.data_ptr(), out.stride(0), lse.data_ptr(), ws,
+        0 if workspace is None else workspace.numel(), 1 if c["dtype"] == "bf16" else 0, st.data_ptr(),
+        torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert rc == 0 and int(st.item()) == 0
+    return c["buf"], out.cpu(), lse.cpu()
+
+
+@pytest.mark.parametrize("seqs", [[(1, 200), (1, 2100)], [(40, 300), (1, 1500)]])
+@pytest.mark.parametrize("bound", [1 << 20, (1 << 31) - 1])
+def test_attention_with_bounds_that_say_nothing(seqs, bound):
+    c = _attn_case(seqs, "bf16", 64, 14, 2, seed=47)
+    _check_attn(c, _attend_c(c, bound, bound))

@@ -144,3 +144,16 @@ def test_a_status_that_cannot_take_the_bits_is_refused(monkeypatch, op):
     assert not gpu.calls
     op(status=_there(1, dtype=torch.int32))
     assert len(gpu.calls) == 1
+
+
+def test_loose_bounds_are_cut_to_what_can_be(monkeypatch):
+    """No sequence has more new tokens than there are rows, nor more cached ones than
+    its pages hold: a caller that knows no better may give any bound."""
+    gpu = _Gpu(monkeypatch, 1)
+    for big in (3, 1 << 20, (1 << 31) - 1, 1 << 31, (1 << 32) + 1, 1 << 62):
+        gpu.calls.clear()
+        _append(n=2, max_q=big), _attend(n=2, pages=2, max_q=big, max_kv=64 * big)
+        assert [gpu.calls[0][2][15], gpu.calls[1][2][9], gpu.calls[1][2][10]] == [2, 2, 128]
+    gpu.calls.clear()
+    _append(n=2, max_q=1), _attend(n=2, pages=2, max_q=1, max_kv=70)
+    assert [gpu.calls[0][2][15], gpu.calls[1][2][9], gpu.calls[1][2][10]] == [1, 1, 70]
