@@ -79,6 +79,14 @@ class PageTable:
             self._pages[s] += [self._free.pop() for _ in range(want[s])]
             self._len[s] += n
 
+    def shrink(self, news: dict) -> None:
+        """Takes back the last `extend`, which was of these."""
+        for s, n in reversed(news.items()):
+            self._len[s] -= n
+            keep = -(-self._len[s] // PAGE)
+            self._free += reversed(self._pages[s][keep:])
+            del self._pages[s][keep:]
+
 
 class _Linear:
     def __init__(self, w, group, dtype, device):
@@ -152,16 +160,18 @@ class SessionDecoder:
     def close(self, sid: int) -> None:
         self.table.close(sid)
 
+    def _check(self, news: dict) -> None:
+        for s, ids in news.items():
+            if len(ids) and not 0 <= min(ids) <= max(ids) < self.cfg.vocab_size:
+                raise ValueError("a token id outside the vocabulary")
+            if self.table.length(s) + len(ids) > self.cfg.max_seq:
+                raise ValueError("a session longer than max_seq")
+
     def _maps(self, news: dict):
         """The step's token ids and sequence maps, in one copy to the device."""
         import torch
         sids = list(news)
         ids = [t for s in sids for t in news[s]]
-        if ids and not 0 <= min(ids) <= max(ids) < self.cfg.vocab_size:
-            raise ValueError("a token id outside the vocabulary")
-        if any(self.table.length(s) + len(news[s]) > self.cfg.max_seq for s in sids):
-            raise ValueError("a session longer than max_seq")
-        self.table.extend({s: len(news[s]) for s in sids})
         pages = [self.table.pages(s) for s in sids]
         wide = max([len(p) for p in pages] + [1])
         starts, lens = [0], [self.table.length(s) for s in sids]
@@ -179,10 +189,25 @@ class SessionDecoder:
 
     def step(self, news: dict):
         """Final hidden states (after the last norm) of the new tokens, in the
-        order of `news`, a map from session to its new token ids."""
+        order of `news`, a map from session to its new token ids.  A step that
+        raises leaves the sessions with the tokens that they had."""
         import torch
         if not news:
             return torch.empty(0, self.cfg.hidden_size, dtype=self.dtype, device=self.device)
+        self._check(news)
+        sizes = {s: len(ids) for s, ids in news.items()}
+        self.table.extend(sizes)
+        try:
+            return self._run(news)
+        except BaseException:
+            # What is queued still writes to the new slots, ahead of whatever is
+            # queued next; slots past a session's length are never read.  A page
+            # that was begun may keep the larger scale that a new value asked for.
+            self.table.shrink(sizes)
+            raise
+
+    def _run(self, news: dict):
+        import torch
         cfg = self.cfg
         ids, maps, max_q, max_kv = self._maps(news)
         nq, nkv, hd, eps = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, cfg.rms_norm_eps

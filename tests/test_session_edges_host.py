@@ -1,5 +1,5 @@
 """Host side of the session operators, without a GPU: where a call
-launches, and whose memory it works in.
+launches, whose memory it works in, and what a step that fails leaves behind.
 
 The tensors here lie in host memory and say that they are on a device; the
 library's entry points are replaced by ones that record the call."""
@@ -157,3 +157,63 @@ def test_loose_bounds_are_cut_to_what_can_be(monkeypatch):
     gpu.calls.clear()
     _append(n=2, max_q=1), _attend(n=2, pages=2, max_q=1, max_kv=70)
     assert [gpu.calls[0][2][15], gpu.calls[1][2][9], gpu.calls[1][2][10]] == [1, 1, 70]
+
+
+# ---------------------------------------------------------------- the session decoder
+
+def _decoder(pages=4, **kw):
+    import dataclasses
+    cfg = dataclasses.replace(pkg().synth.ModelConfig(), **{**dict(
+        num_layers=1, hidden_size=128, intermediate_size=128, num_heads=2, num_kv_heads=1, head_dim=64,
+        vocab_size=50, num_labels=10, max_seq=256), **kw})
+    g = torch.Generator().manual_seed(2)
+    w = {name: (torch.randn(*shape, generator=g) * 0.04).to(torch.bfloat16)
+         for name, shape, _ in pkg().synth.weight_specs(cfg)
+         if "language_model" in name or name.startswith("score")}
+    return pkg().incremental.SessionDecoder(cfg, w, pages=pages, device="cpu")
+
+
+def _table(dec):
+    t = dec.table
+    return {s: (t.length(s), list(t.pages(s))) for s in t._len}, sorted(t._free)
+
+
+@pytest.mark.parametrize("fails", ["w4_linear", "kv_append", "cache_attention", "device"])
+def test_a_step_that_fails_leaves_the_sessions_as_they_were(monkeypatch, fails):
+    """Whatever fails after the tokens were taken (memory, for one): the sessions do
+    not count tokens that their caches do not hold, and the step can be repeated."""
+    dec, lib = _decoder(pages=5), pkg()._lib
+
+    def quiet(*a, **k):
+        return None
+
+    def loud(*a, **k):
+        raise RuntimeError("no memory")
+
+    for name in ("w4_linear", "kv_append", "cache_attention"):
+        monkeypatch.setattr(lib, name, quiet)
+    a, b = dec.open(), dec.open()
+    dec.step({a: [1] * 60, b: [2]})
+    before = _table(dec)
+    with monkeypatch.context() as m:
+        if fails == "device":
+            m.setattr(torch.Tensor, "to", loud)
+        else:
+            m.setattr(lib, fails, loud)
+        with pytest.raises(RuntimeError, match="no memory"):
+            dec.step({a: [1] * 70, b: [], dec.open(): [3]})
+    dec.close(max(dec.table._len))
+    assert _table(dec) == before
+    assert dec.step({a: [1] * 70, b: [4]}).shape == (71, 128)
+    assert dec.table.length(a) == 130 and len(dec.table.pages(a)) == 3
+
+
+def test_a_step_with_what_is_no_token_leaves_the_sessions_as_they_were():
+    dec = _decoder()
+    a = dec.open()
+    for bad in (["x"], [None], [1, 2.5j]):
+        with pytest.raises((TypeError, ValueError)):
+            dec.step({a: bad})
+    with pytest.raises(KeyError):
+        dec.step({a: [1], a + 1: [1]})
+    assert dec.table.length(a) == 0 and len(dec.table._free) == 4
