@@ -30,7 +30,9 @@ def quantise4(w, group: int = 128, dtype=None):
     """4-bit codes of w [N, K] as `w4_linear` takes them: (wq uint8 [N, K / 2],
     scales [N, K / group] of `dtype`, zeros uint8).  Each group's range, widened
     to hold 0, is cut in 15 steps; a weight is off by half a step at most, plus
-    half a step where the zero point was rounded at the range's end."""
+    half a step at the range's end, where the zero point was rounded, plus what
+    rounding the step to `dtype` takes from the range.  float16's steps below 2^-14
+    are whole units of 2^-24, rounded up, so that groups of tiny weights keep them."""
     import torch
     dtype = dtype or torch.bfloat16
     N, K = w.shape
@@ -38,7 +40,10 @@ def quantise4(w, group: int = 128, dtype=None):
         raise ValueError("K a multiple of a group of 32, 64 or 128")
     g = w.float().reshape(N, K // group, group)
     lo, hi = g.amin(-1).clamp(max=0), g.amax(-1).clamp(min=0)
-    scales = ((hi - lo) / 15).clamp(min=torch.finfo(dtype).tiny).to(dtype)
+    step, tiny = (hi - lo) / 15, torch.finfo(dtype).tiny
+    if dtype is torch.float16:
+        step, tiny = torch.where(step < tiny, (step * 2 ** 24).ceil() * 2 ** -24, step), 2 ** -24
+    scales = step.clamp(min=tiny).to(dtype)
     s = scales.float()
     zeros = (-lo / s).round().clamp(0, 15)
     codes = ((g / s[..., None]).round() + zeros[..., None]).clamp(0, 15).to(torch.uint8).reshape(N, K)

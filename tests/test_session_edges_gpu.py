@@ -38,6 +38,21 @@ def test_w4_zero_points_are_any_byte(dtype, group, m, pad):
     pkg()._lib.w4_linear(x, c["wq"].cuda(), c["scales"].cuda(), out, zeros=c["zeros"].cuda())
     _check_w4(c, out)
 
+@pytest.mark.parametrize("pad", [0, 1])
+def test_w4_scales_below_the_normal_range(pad):
+    """What quantise4 gives for tiny weights in f16: steps of 2^-24 and up."""
+    import torch
+    m, n, k = 5, 200, 1024
+    c = _w4_case(m, n, k, 64, "f16", True, True, seed=61)
+    c["scales"] = (torch.randint(1, 1024, c["scales"].shape, generator=torch.Generator().manual_seed(62)) * 2.0 ** -24).half()
+    c["x"] = c["x"] * 512
+    x = torch.zeros(m, k + pad, dtype=torch.float16, device="cuda")[:, pad:]
+    x.copy_(c["x"])
+    out = torch.empty(m, n, dtype=torch.float16, device="cuda")
+    pkg()._lib.w4_linear(x, c["wq"].cuda(), c["scales"].cuda(), out, zeros=c["zeros"].cuda(), bias=c["bias"].cuda())
+    _check_w4(c, out)
+
+
 # ---------------------------------------------------------------- kv_append
 
 @pytest.mark.parametrize("bits", [8, 16])

@@ -1,5 +1,6 @@
 """Host side of the session operators, without a GPU: where a call
-launches, whose memory it works in, and what a step that fails leaves behind.
+launches, whose memory it works in, what a step that fails leaves
+behind, and 4-bit codes of tiny weights.
 
 The tensors here lie in host memory and say that they are on a device; the
 library's entry points are replaced by ones that record the call."""
@@ -217,3 +218,20 @@ def test_a_step_with_what_is_no_token_leaves_the_sessions_as_they_were():
     with pytest.raises(KeyError):
         dec.step({a: [1], a + 1: [1]})
     assert dec.table.length(a) == 0 and len(dec.table._free) == 4
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_tiny_weights_keep_their_steps(dtype):
+    """Half a step and half a step of the zero point; the step rounded to 16 bits moves
+    the range's end by 15 u, or is up to 2^-24 longer where float16 has no more bits."""
+    g = torch.Generator().manual_seed(6)
+    w = torch.randn(14, 128, generator=g) * 10.0 ** -torch.arange(1, 8).repeat(2)[:, None]
+    w[7:] = w[7:].abs()
+    wq, scales, zeros = pkg().incremental.quantise4(w, 64, dtype)
+    codes = torch.stack([wq & 15, wq >> 4], -1).reshape(14, 2, 64).double()
+    back = scales.double()[..., None] * (codes - zeros.double()[..., None])
+    w = w.double().reshape(14, 2, 64)
+    step = (w.amax(-1).clamp(min=0) - w.amin(-1).clamp(max=0)) / 15
+    u = 2.0 ** -11 if dtype is torch.float16 else 2.0 ** -8
+    bound = step * (1 + 15 * 2 * u) + (2.0 ** -24 if dtype is torch.float16 else 0)
+    assert ((back - w).abs() <= bound[..., None]).all()
