@@ -530,8 +530,16 @@ int w4_linear(const void* x, long long ldx, int M, int K, const uint8_t* wq, lon
   wp.vec_x = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0;
   wp.vec_w = reinterpret_cast<uintptr_t>(wq) % 16 == 0 && ldw % 16 == 0;
   wp.vec_o = reinterpret_cast<uintptr_t>(out) % 16 == 0 && ldo % 8 == 0;
-  const cudaError_t e = bf16 ? launch_any<__nv_bfloat16>(wp, s) : launch_any<__half>(wp, s);
-  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+  // a grid's y holds 65535 blocks of rows
+  constexpr int kMost = 65535 * 16;
+  for (long long m = 0; m < M; m += kMost) {
+    wp.x = static_cast<const uint8_t*>(x) + 2 * m * ldx;
+    wp.out = static_cast<uint8_t*>(out) + 2 * m * ldo;
+    wp.M = static_cast<int>(std::min<long long>(kMost, M - m));
+    const cudaError_t e = bf16 ? launch_any<__nv_bfloat16>(wp, s) : launch_any<__half>(wp, s);
+    if (e != cudaSuccess) return (int)e;
+  }
+  return (int)cudaGetLastError();
 }
 
 }  // namespace qa

@@ -53,6 +53,23 @@ def test_w4_scales_below_the_normal_range(pad):
     _check_w4(c, out)
 
 
+def test_w4_takes_any_number_of_rows():
+    """More rows than a grid has blocks for; compared where the pieces meet and at the
+    ends."""
+    import torch
+    at = 65535 * 16
+    m = at + 3
+    c = _w4_case(40, 6, 32, 32, "bf16", True, True, seed=67)
+    x = torch.zeros(m, 32, dtype=torch.bfloat16, device="cuda")
+    rows = list(range(16)) + list(range(at - 16, at + 3))
+    c["x"] = c["x"][: len(rows)]
+    x[torch.tensor(rows, device="cuda")] = c["x"].cuda()
+    out = torch.full((m, 6), float("nan"), dtype=torch.bfloat16, device="cuda")
+    pkg()._lib.w4_linear(x, c["wq"].cuda(), c["scales"].cuda(), out, zeros=c["zeros"].cuda(), bias=c["bias"].cuda())
+    _check_w4(c, out[torch.tensor(rows, device="cuda")])
+    assert bool((out[16: at - 16] == c["bias"].cuda().bfloat16()).all())
+
+
 # ---------------------------------------------------------------- kv_append
 
 @pytest.mark.parametrize("bits", [8, 16])
