@@ -171,11 +171,19 @@ struct Walk {
   }
 };
 
+__device__ __forceinline__ PartsAt unit_parts(const CacheAttnParams& ap, const UnitAt& at) {
+  const long long u = (static_cast<long long>(at.s) * ap.tiles_max + at.tile) * ap.nkv + at.h;
+  return PartsAt{ap.parts + u * ap.place_floats, ap.part_stride, padded_rows(ap.part_rows)};
+}
+
 // The parts that this kernel leaves, for the join.
 template <int R, int SLAB, bool ALONE>
 struct RowsPlan {
   static constexpr int kRows = R;
   static constexpr bool kAlone = ALONE;
+  __device__ static PartsAt place(const CacheAttnParams& ap, const SeqSpan&, const UnitAt& at) {
+    return unit_parts(ap, at);
+  }
   __device__ static int parts(const CacheAttnParams& ap, const SeqSpan& sp, int s, int) {
     const int n = seq_plan(ap, sp, s, ap.nq / ap.nkv, R, SLAB).chunks;
     return n > 1 ? n : 0;
@@ -672,8 +680,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
       each([&](int r, int dim, float4 v) { finish_row<T, HD>(ap, at, tile * R + r, dim, v, sh.inv[r]); });
       __syncthreads();  // the sums are read before the next chunk's are written
     } else {
-      float* mine = unit_parts(ap, at) + chunk * ap.part_stride;
-      const int l_at = (ap.part_rows + 3) & ~3;
+      const PartsAt parts = unit_parts(ap, at);
+      float* mine = parts.base + static_cast<long long>(chunk) * parts.stride;
+      const int l_at = parts.l_at;
       each([&](int r, int dim, float4 v) {
         __stcg(reinterpret_cast<float4*>(mine + 2 * l_at + r * HD + dim), v);
       });
@@ -696,7 +705,7 @@ int tile_rows(long long rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 24; }
 // The workspace of a unit, for caches of up to max_kv tokens.
 struct PartSizes {
   int tiles, parts, rows, stride;
-  long long unit_bytes;
+  long long place_floats;
 };
 PartSizes part_sizes(int nq, int nkv, int hd, int max_q, int max_kv) {
   PartSizes p;
@@ -707,8 +716,8 @@ PartSizes part_sizes(int nq, int nkv, int hd, int max_q, int max_kv) {
   p.parts = (tokens - 1) / chunk_tokens(tokens) + 1;
   if (tokens > kMaxParts * kChunk) p.parts = kMaxParts;  // a shorter cache may have as many
   p.rows = static_cast<int>(std::min<long long>(R, rows));
-  p.stride = 2 * ((p.rows + 3) & ~3) + p.rows * hd;
-  p.unit_bytes = 4ll * p.parts * p.stride;
+  p.stride = part_floats(p.rows, hd);
+  p.place_floats = static_cast<long long>(p.parts) * p.stride;
   return p;
 }
 
@@ -753,7 +762,8 @@ cudaError_t launch_rows(CacheAttnParams ap, void* ws, long long ws_bytes, int ma
   ap.part_rows = ps.rows;
   ap.part_stride = ps.stride;
   ap.parts = static_cast<float*>(ws);
-  ap.cap_units = ws ? ws_bytes / ps.unit_bytes : 0;
+  ap.place_floats = ps.place_floats;
+  ap.cap_units = ws ? ws_bytes / (4 * ps.place_floats) : 0;
   // no more CTAs than chunks, as far as max_kv tells
   const long long chunks = static_cast<long long>(ap.seqs.n_seqs) * ps.tiles * ap.nkv * ps.parts;
   grid = static_cast<int>(std::min<long long>(grid, chunks));
@@ -785,7 +795,7 @@ constexpr int kFewRows = 24;
 long long cache_rows_workspace(int nqh, int nkvh, int hd, int n_seqs, int max_q, int max_kv) {
   const PartSizes p = part_sizes(nqh, nkvh, hd, max_q, max_kv);
   if (p.parts == 1) return 0;
-  return static_cast<long long>(n_seqs) * p.tiles * nkvh * p.unit_bytes;
+  return places_bytes(static_cast<long long>(n_seqs) * p.tiles, nkvh, p.place_floats);
 }
 
 int cache_attention_rows(const CacheAttnParams& ap, int hd, bool bf16, int max_kv, void* ws,
@@ -798,11 +808,10 @@ int cache_attention_rows(const CacheAttnParams& ap, int hd, bool bf16, int max_k
 }
 
 long long cache_attention_workspace(int nqh, int nkvh, int hd, int n_seqs, int max_q, int max_kv) {
-  if (nkvh <= 0 || nqh < nkvh || n_seqs <= 0 || max_q <= 0) return 0;
+  if (nkvh <= 0 || nqh < nkvh || n_seqs <= 0 || max_q <= 0 || (hd != 64 && hd != 128)) return 0;
   const bool few = static_cast<long long>(max_q) * (nqh / nkvh) <= kFewRows;
-  const long long bytes = few ? cache_rows_workspace(nqh, nkvh, hd, n_seqs, max_q, max_kv)
-                              : cache_tiles_workspace(nqh, nkvh, hd, n_seqs, max_q, max_kv);
-  return std::min(bytes, 1ll << 30);
+  return few ? cache_rows_workspace(nqh, nkvh, hd, n_seqs, max_q, max_kv)
+             : cache_tiles_workspace(nqh, nkvh, hd, n_seqs, max_q, max_kv);
 }
 
 int cache_attention(const void* q, long long ldq, long long T, int nqh, int nkvh, int hd,

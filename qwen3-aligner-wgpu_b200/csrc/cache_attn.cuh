@@ -24,10 +24,12 @@ struct CacheAttnParams {
   float* lse;
   int vec;      // q and out rows can be read and written 16 bytes at a time
   int tiles_max;       // tiles of a sequence of max_q tokens
-  float* parts;        // workspace: the units' parts, part_stride floats each
-  long long cap_units; // units that have a place in the workspace
-  int cap_parts;       // parts a unit has place for
-  int part_rows, part_stride;
+  float* parts;        // workspace: place_floats for each unit (few-row kernel), or each sequence and K/V head
+  long long cap_units; // such places in the workspace
+  long long place_floats;
+  int cap_parts;       // parts a unit of the few-row kernel has place for
+  int part_rows, part_stride;  // most rows of a part, its floats
+  int half_stride;     // floats of a part of one tile of rows (tcgen05 kernel)
   unsigned* status;
 };
 
@@ -82,10 +84,13 @@ struct UnitAt {
   long long t0;  // the sequence's first row of q and out
 };
 
-__device__ __forceinline__ float* unit_parts(const CacheAttnParams& ap, const UnitAt& at) {
-  const long long u = (static_cast<long long>(at.s) * ap.tiles_max + at.tile) * ap.nkv + at.h;
-  return ap.parts + u * ap.cap_parts * ap.part_stride;
-}
+// A unit's parts: m and l of l_at rows (a multiple of four), O.
+struct PartsAt {
+  float* base;
+  int stride, l_at;
+};
+__host__ __device__ __forceinline__ int padded_rows(int rows) { return (rows + 3) & ~3; }
+__host__ __device__ __forceinline__ int part_floats(int rows, int hd) { return 2 * padded_rows(rows) + rows * hd; }
 
 // Row `row` of a sequence is done: its lse; returns what its O is multiplied by.
 __device__ __forceinline__ float close_row(const CacheAttnParams& ap, const UnitAt& at, int row,
@@ -135,16 +140,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32, Plan::kAlone ? 4 : 2) cache_a
   if (n == 0) return;
   constexpr bool alone = Plan::kAlone;
   const UnitAt at{s, tile, h, sp.t0};
-  const float* parts = unit_parts(ap, at);
-  const int l_at = (ap.part_rows + 3) & ~3;
+  const PartsAt parts = Plan::place(ap, sp, at);
   // the CTA's warps share row blockIdx.z, or take rows of their own
   for (int r = alone ? kJoinWarps * blockIdx.z + warp : blockIdx.z; r < rows; r += (alone ? kJoinWarps : 1) * gridDim.z) {
-  const int o_at = 2 * l_at + r * HD;
+  const int o_at = 2 * parts.l_at + r * HD;
   const int first = (alone ? 0 : warp * kPer) + lane / kLanes, step = alone ? kPer : kPer * kJoinWarps;
   const int d = lane % kLanes;
   float big = -INFINITY;
   for (int k = alone ? lane : threadIdx.x; k < n; k += alone ? 32 : 32 * kJoinWarps)
-    big = fmaxf(big, __ldcg(parts + static_cast<long long>(k) * ap.part_stride + r));
+    big = fmaxf(big, __ldcg(parts.base + static_cast<long long>(k) * parts.stride + r));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
   if constexpr (!alone) {
@@ -163,13 +167,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32, Plan::kAlone ? 4 : 2) cache_a
     float pm[kBatch], pl[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const float* part = parts + static_cast<long long>(k0 + i * step) * ap.part_stride;
+      const float* part = parts.base + static_cast<long long>(k0 + i * step) * parts.stride;
       y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       pm[i] = pl[i] = 0.0f;
       if (k0 + i * step < n) {
         y[i] = __ldcg(reinterpret_cast<const float4*>(part + o_at + 4 * d));
         pm[i] = __ldcg(part + r);
-        pl[i] = __ldcg(part + l_at + r);
+        pl[i] = __ldcg(part + parts.l_at + r);
       }
     }
 #pragma unroll
@@ -217,6 +221,13 @@ cudaError_t launch_join(const CacheAttnParams& ap, cudaStream_t s) {
 }
 
 }  // namespace
+
+// Bytes of units * nkvh places, at most 1 GiB: sequences past it are not split.
+inline long long places_bytes(long long units, int nkvh, long long place_floats) {
+  constexpr long long kMost = 1ll << 30;
+  const long long one = 4 * place_floats;
+  return units > kMost / one / nkvh ? kMost : units * nkvh * one;
+}
 
 // The two kernels' launches, and the workspace that each asks for.
 int cache_attention_rows(const CacheAttnParams& ap, int hd, bool bf16, int max_kv, void* ws,

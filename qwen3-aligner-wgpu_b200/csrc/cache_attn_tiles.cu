@@ -65,12 +65,15 @@ __host__ __device__ __forceinline__ int chunk_step(int keys, int tiles) {
 
 struct TilePlan {
   int tiles, step;
+  int chunks;  // of a unit, at most: each unit but the last has place for as many parts, if it is more than one
 };
 __device__ __forceinline__ TilePlan tile_plan(const CacheAttnParams& ap, const SeqSpan& sp) {
   const int group = ap.nq / ap.nkv;
   TilePlan p;
   p.tiles = sp.ok ? (sp.n * group + kUnitRows - 1) / kUnitRows : 0;
-  p.step = chunk_step(max(1, (sp.len + kKeys - 1) / kKeys), max(1, p.tiles));
+  const int keys = max(1, (sp.len + kKeys - 1) / kKeys);
+  p.step = chunk_step(keys, max(1, p.tiles));
+  p.chunks = (keys + p.step - 1) / p.step;
   return p;
 }
 
@@ -79,6 +82,7 @@ struct Unit {
   int rows, seen;    // rows; tokens that its last row sees
   int keys;          // key tiles, at least one: a row that sees nothing still gets zeros
   int step, chunks;  // key tiles of a chunk, chunks
+  int place;         // where its parts are in the sequence's and head's place
   bool pair;         // two tiles of rows, or no place for parts: streams are tiles
 };
 __device__ __forceinline__ Unit unit_of(const CacheAttnParams& ap, const SeqSpan& sp, const TilePlan& p,
@@ -92,8 +96,10 @@ __device__ __forceinline__ Unit unit_of(const CacheAttnParams& ap, const SeqSpan
   u.step = p.step;
   u.chunks = (u.keys + u.step - 1) / u.step;
   u.pair = u.rows > kRows;
-  if ((u.pair ? u.chunks : 2 * u.chunks) > ap.cap_parts ||
-      static_cast<long long>(s + 1) * ap.tiles_max * ap.nkv > ap.cap_units) {
+  // a part of both tiles for each chunk, or one of a tile for each chunk and stream
+  u.place = p.chunks > 1 ? tile * p.chunks * ap.part_stride : 0;
+  const int floats = !u.pair ? 2 * u.chunks * ap.half_stride : u.chunks > 1 ? u.chunks * ap.part_stride : 0;
+  if (u.place + floats > ap.place_floats || (s + 1ll) * ap.nkv > ap.cap_units) {
     u.pair = true;
     u.chunks = 1;
     u.step = u.keys;
@@ -101,10 +107,19 @@ __device__ __forceinline__ Unit unit_of(const CacheAttnParams& ap, const SeqSpan
   return u;
 }
 
+__device__ __forceinline__ PartsAt unit_parts(const CacheAttnParams& ap, const Unit& u, int s, int h) {
+  return PartsAt{ap.parts + (static_cast<long long>(s) * ap.nkv + h) * ap.place_floats + u.place,
+                 u.pair ? ap.part_stride : ap.half_stride,
+                 padded_rows(u.pair ? ap.part_rows : min(kRows, ap.part_rows))};
+}
+
 // The parts that this kernel leaves, for the join.
 struct TilesPlan {
   static constexpr int kRows = kUnitRows;
   static constexpr bool kAlone = true;
+  __device__ static PartsAt place(const CacheAttnParams& ap, const SeqSpan& sp, const UnitAt& at) {
+    return unit_parts(ap, unit_of(ap, sp, tile_plan(ap, sp), at.s, at.tile), at.s, at.h);
+  }
   __device__ static int parts(const CacheAttnParams& ap, const SeqSpan& sp, int s, int tile) {
     const Unit u = unit_of(ap, sp, tile_plan(ap, sp), s, tile);
     return u.pair ? (u.chunks > 1 ? u.chunks : 0) : 2 * u.chunks;
@@ -209,10 +224,8 @@ __device__ __forceinline__ Work work_of(const CacheAttnParams& ap, const TileWal
   w.k0 = it.k0;
   w.cnt = it.cnt;
   w.pair = u.pair;
-  w.parts = u.pair && u.chunks == 1
-                ? nullptr
-                : unit_parts(ap, UnitAt{it.s, it.tile, it.h, w.t0}) +
-                      (u.pair ? it.chunk : 2 * it.chunk) * static_cast<long long>(ap.part_stride);
+  const PartsAt parts = unit_parts(ap, u, it.s, it.h);
+  w.parts = u.pair && u.chunks == 1 ? nullptr : parts.base + (u.pair ? it.chunk : 2 * it.chunk) * parts.stride;
   return w;
 }
 
@@ -811,8 +824,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
       float inv = 1.0f;
       float* part = it.parts;
       if (part) {
-        const int l_at = (ap.part_rows + 3) & ~3;
-        if (!it.pair) part += h * static_cast<long long>(ap.part_stride);
+        const int l_at = padded_rows(it.pair ? ap.part_rows : min(kRows, ap.part_rows));
+        if (!it.pair) part += h * ap.half_stride;
         if (valid) {
           __stcg(part + ur, m);
           __stcg(part + l_at + ur, l);
@@ -886,18 +899,23 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_tiles(const __grid_con
 }
 
 struct PartSizes {
-  int tiles, parts, rows, stride;
-  long long unit_bytes;
+  int tiles, rows, stride, half;
+  long long place_floats;  // of a sequence and K/V head
 };
 PartSizes part_sizes(int nq, int nkv, int hd, int max_q, int max_kv) {
   PartSizes p;
   const long long rows = static_cast<long long>(max_q) * (nq / nkv);
   p.tiles = static_cast<int>((rows + kUnitRows - 1) / kUnitRows);
-  const int keys = (std::max(1, max_kv) - 1) / kKeys + 1;
-  p.parts = 2 * std::min(kMaxChunks, (keys + kMinStep - 1) / kMinStep);
   p.rows = static_cast<int>(std::min<long long>(kUnitRows, rows));
-  p.stride = 2 * ((p.rows + 3) & ~3) + p.rows * hd;
-  p.unit_bytes = 4ll * p.parts * p.stride;
+  p.stride = part_floats(p.rows, hd);
+  p.half = part_floats(std::min(kRows, p.rows), hd);
+  const int most = (std::max(1, max_kv) - 1) / kKeys / kMinStep + 1;  // chunks of a unit, whatever its tiles
+  // the most that a sequence of up to so many tiles asks for: 4096 rows or fewer
+  p.place_floats = 0;
+  for (int t = 1; t <= std::min(p.tiles, kMaxChunks); ++t) {
+    const long long chunks = std::min(kMaxChunks / t, most), whole = chunks > 1 ? chunks * p.stride : 0;
+    p.place_floats = std::max(p.place_floats, (t - 1) * whole + std::max(whole, 2 * chunks * p.half));
+  }
   return p;
 }
 
@@ -905,11 +923,12 @@ template <typename T, int HD>
 cudaError_t launch(CacheAttnParams ap, int max_kv, void* ws, long long ws_bytes, cudaStream_t s) {
   const PartSizes ps = part_sizes(ap.nq, ap.nkv, HD, ap.seqs.max_q, max_kv);
   ap.tiles_max = ps.tiles;
-  ap.cap_parts = ps.parts;
   ap.part_rows = ps.rows;
   ap.part_stride = ps.stride;
+  ap.half_stride = ps.half;
   ap.parts = static_cast<float*>(ws);
-  ap.cap_units = ws ? ws_bytes / ps.unit_bytes : 0;
+  ap.place_floats = ps.place_floats;
+  ap.cap_units = ws ? ws_bytes / (4 * ps.place_floats) : 0;
   CUtensorMap tk, tv;
   const long long rows = static_cast<long long>(ap.kv_pages) * ap.nkv * kPage;
   if (rows > 0x7FFFFFFFll) return cudaErrorInvalidValue;  // TMA row coordinates
@@ -932,7 +951,7 @@ cudaError_t launch(CacheAttnParams ap, int max_kv, void* ws, long long ws_bytes,
 
 long long cache_tiles_workspace(int nqh, int nkvh, int hd, int n_seqs, int max_q, int max_kv) {
   const PartSizes p = part_sizes(nqh, nkvh, hd, max_q, max_kv);
-  return static_cast<long long>(n_seqs) * p.tiles * nkvh * p.unit_bytes;
+  return places_bytes(n_seqs, nkvh, p.place_floats);
 }
 
 int cache_attention_tiles(const CacheAttnParams& ap, int hd, bool bf16, int max_kv, void* ws,

@@ -2,7 +2,7 @@
 implementations in 64 bits and with the same bounds as test_session_ops_gpu.py:
 zero points over the whole byte, axes that are not there,
 calls without tables, bounds that say nothing, captures of a stream that
-is not the current one."""
+is not the current one, workspaces of any size, a sequence's company."""
 import pytest
 
 from conftest import cuda_ok, pkg
@@ -188,3 +188,66 @@ def _attend_c(c, max_q, max_kv, workspace=None, causal=1):
 def test_attention_with_bounds_that_say_nothing(seqs, bound):
     c = _attn_case(seqs, "bf16", 64, 14, 2, seed=47)
     _check_attn(c, _attend_c(c, bound, bound))
+
+
+def _workspace(c, n_seqs, max_q, max_kv):
+    import torch
+    size = pkg()._lib.lib().qa_k_cache_attention_workspace(c["nq"], c["nkv"], c["hd"], n_seqs, max_q, max_kv)
+    return torch.empty(size, dtype=torch.uint8, device="cuda")
+
+
+def _only(c, s):
+    """Sequence s of a case by itself."""
+    a, b = int(c["q_start"][s]), int(c["q_start"][s + 1])
+    return dict(c, seqs=[c["seqs"][s]], buf=c["buf"][a:b].contiguous(), q_start=c["q_start"][s: s + 2] - a,
+                kv_len=c["kv_len"][s: s + 1], tab=c["tab"][s: s + 1].contiguous())
+
+
+COMPANY = [
+    [(1, 5000), (1, 20), (1, 3000), (0, 100)],
+    [(12, 5000), (3, 2100), (12, 1025)],
+    [(300, 2500), (129, 1500), (1, 3000), (40, 2000)],
+    # eight sessions, the last of them beside one that brings far more tokens
+    [(1024, 8192)] + [(16, 1200)] * 6 + [(16, 8192)],
+]
+
+
+@pytest.mark.parametrize("dtype,hd,nq,nkv", [("f16", 128, 16, 8), ("bf16", 64, 14, 2)])
+@pytest.mark.parametrize("seqs", COMPANY, ids=range(len(COMPANY)))
+def test_attention_of_a_sequence_does_not_depend_on_the_others(seqs, dtype, hd, nq, nkv):
+    """The same bits alone and at any place of a batch of one max_q."""
+    import torch
+    c = _attn_case(seqs, dtype, hd, nq, nkv, seed=53)
+    max_q, max_kv = max(n for n, _ in seqs), max(L for _, L in seqs)
+    _, out, lse = _attend_c(c, max_q, max_kv, _workspace(c, len(seqs), max_q, max_kv))
+    for s in range(len(seqs)):
+        a, b = int(c["q_start"][s]), int(c["q_start"][s + 1])
+        if a == b:
+            continue
+        # max_q counts as the rows that there are: rows of nobody keep it
+        one = _only(c, s)
+        one["buf"] = torch.cat([one["buf"], one["buf"].new_zeros(max_q - (b - a), nq * hd)])
+        _, o, e = _attend_c(one, max_q, max_kv, _workspace(c, 1, max_q, max_kv))
+        assert torch.equal(o[: b - a], out[a:b]) and torch.equal(e[: b - a], lse[a:b])
+
+
+@pytest.mark.parametrize("dtype,hd,nq,nkv", [("f16", 128, 16, 8), ("bf16", 64, 14, 2)])
+@pytest.mark.parametrize("seqs", COMPANY[:3], ids=range(3))
+def test_attention_in_a_workspace_of_any_size(seqs, dtype, hd, nq, nkv):
+    """None, and some of what is asked for: sequences without a place are not split."""
+    import torch
+    c = _attn_case(seqs, dtype, hd, nq, nkv, seed=59)
+    max_q, max_kv = max(n for n, _ in seqs), max(L for _, L in seqs)
+    whole = _workspace(c, len(seqs), max_q, max_kv)
+    want = _attend_c(c, max_q, max_kv, whole)
+    _check_attn(c, want)
+    _check_attn(c, _attend_c(c, max_q, max_kv))
+    one = whole.numel() // len(seqs)
+    for bytes_ in (16, one - 16, one, one + 16, whole.numel() - 16):
+        room = torch.full((whole.numel(),), 0x7F, dtype=torch.uint8, device="cuda")
+        got = _attend_c(c, max_q, max_kv, room[:bytes_])
+        assert bool((room[bytes_:] == 0x7F).all())
+        _check_attn(c, got)
+        if bytes_ >= one:
+            n = int(c["q_start"][1])
+            assert torch.equal(got[1][:n], want[1][:n]) and torch.equal(got[2][:n], want[2][:n])

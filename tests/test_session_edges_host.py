@@ -1,6 +1,6 @@
 """Host side of the session operators, without a GPU: where a call
-launches, whose memory it works in, what a step that fails leaves
-behind, and 4-bit codes of tiny weights.
+launches, whose memory it works in, how much of it, what a step
+that fails leaves behind, and 4-bit codes of tiny weights.
 
 The tensors here lie in host memory and say that they are on a device; the
 library's entry points are replaced by ones that record the call."""
@@ -235,3 +235,17 @@ def test_tiny_weights_keep_their_steps(dtype):
     u = 2.0 ** -11 if dtype is torch.float16 else 2.0 ** -8
     bound = step * (1 + 15 * 2 * u) + (2.0 ** -24 if dtype is torch.float16 else 0)
     assert ((back - w).abs() <= bound[..., None]).all()
+
+
+def test_the_attentions_workspace_is_what_its_parts_need():
+    """Many rows: 16 parts of 256 rows of a sequence and head at most, whatever their
+    number, and as much for each sequence; nothing for arguments that are none."""
+    size = pkg()._lib.lib().qa_k_cache_attention_workspace
+    most = 16 * 4 * (256 * 128 + 2 * 256)
+    for max_q in (128, 512, 1024, 8192, 100000):
+        assert size(16, 8, 128, 1, max_q, 8192) <= 8 * most
+        assert size(16, 8, 128, 8, max_q, 8192) == 8 * size(16, 8, 128, 1, max_q, 8192)
+    assert size(16, 8, 128, 1, 1024, 700) <= 8 * most // 8
+    for bad in ((0, 0, 128, 1, 64, 64), (16, 8, -2, 1, 64, 64), (16, 8, 128, 0, 64, 64), (16, 8, 128, 1, -5, 64)):
+        assert size(*bad) == 0
+    assert 0 < size(16, 8, 128, 1 << 30, (1 << 31) - 1, (1 << 31) - 1) <= 1 << 30
