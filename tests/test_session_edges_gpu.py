@@ -2,11 +2,13 @@
 implementations in 64 bits and with the same bounds as test_session_ops_gpu.py:
 zero points over the whole byte, axes that are not there,
 calls without tables, bounds that say nothing, captures of a stream that
-is not the current one, workspaces of any size, a sequence's company."""
+is not the current one, workspaces of any size, a sequence's company, many
+rows in many chunks, NaN codes that only some rows see."""
 import pytest
 
 from conftest import cuda_ok, pkg
-from test_session_ops_gpu import _append_case, _attn_case, _check_append, _check_attn, _check_w4, _split, _w4_case
+from test_session_ops_gpu import (PAGE, _append_case, _attn_case, _attn_run, _check_append, _check_attn, _check_w4,
+                                  _split, _w4_case)
 
 pytestmark = pytest.mark.gpu
 
@@ -251,3 +253,77 @@ def test_attention_in_a_workspace_of_any_size(seqs, dtype, hd, nq, nkv):
         if bytes_ >= one:
             n = int(c["q_start"][1])
             assert torch.equal(got[1][:n], want[1][:n]) and torch.equal(got[2][:n], want[2][:n])
+
+
+MANY = [
+    [(300, 2500), (129, 1500), (1, 3000)],  # units of two and of one tile of rows, one to three chunks
+    [(700, 1400), (64, 1100), (256, 256)],  # every token hidden from some rows, in two chunks
+    [(1100, 1100), (5, 9000)],              # many units of one chunk beside one of many
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("seqs", MANY, ids=range(len(MANY)))
+@pytest.mark.parametrize("dtype,hd,nq,nkv", [("f16", 128, 16, 8), ("bf16", 128, 14, 2), ("f16", 64, 14, 2),
+                                             ("bf16", 64, 16, 8), ("bf16", 128, 5, 5)])
+def test_attention_of_many_rows_in_many_chunks(dtype, hd, nq, nkv, seqs, causal):
+    c = _attn_case(seqs, dtype, hd, nq, nkv, seed=71)
+    _check_attn(c, _attn_run(c, causal), causal, device="cuda")
+
+
+def _spoil(c, pool, at):
+    """NaN codes at (sequence, token, head, dims); returns the case with zeros there."""
+    import torch
+    clean = dict(c, **{pool: c[pool].clone()})
+    for s, token, head, dims in at:
+        page = int(c["tab"][s, token // PAGE])
+        for x, code in ((c, 0x7F), (clean, 0)):
+            x[pool].view(torch.uint8)[page, head, token % PAGE, dims] = code
+    return clean
+
+
+SPOILED = [
+    ([(70, 200), (33, 300)], [131, 180, 199]),           # one unit a head, its streams' key tiles
+    ([(300, 2500), (40, 2500)], [2250, 2330, 2460, 2499]),  # units of two tiles of rows and of one, the last chunk
+    ([(700, 1400), (20, 1400)], [705, 900, 1050, 1399]),  # in the first chunk and in the second
+    ([(3, 100), (2, 3000)], [98, 99]),                     # few rows
+    ([(8, 3000), (12, 2000)], [2993, 2998, 2999]),         # few rows, the last chunk
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("seqs,tokens", SPOILED, ids=range(len(SPOILED)))
+@pytest.mark.parametrize("dtype,hd,nq,nkv", [("f16", 128, 4, 2), ("bf16", 64, 6, 3)])
+def test_attention_keeps_nan_values_to_the_rows_and_dims_that_see_them(dtype, hd, nq, nkv, seqs, tokens, causal):
+    """NaN codes of V of the first sequence: its last rows see them, the others not."""
+    import torch
+    c = _attn_case(seqs, dtype, hd, nq, nkv, seed=73)
+    n, L = seqs[0]
+    at = [(0, t, i % nkv, [3 * i, hd // 2 + i, hd - 1 - i]) for i, t in enumerate(tokens)]
+    clean = _attn_run(_spoil(c, "vpool", at), causal)
+    _, out, lse = _attn_run(c, causal)
+    want = torch.zeros(out.shape[0], nkv, nq // nkv, hd, dtype=torch.bool)
+    for _, t, head, dims in at:
+        want[max(0, t - (L - n)) if causal else 0: n, head][..., dims] = True
+    want = want.view(out.shape[0], -1)
+    assert torch.equal(out.isnan(), want)
+    assert torch.equal(out.masked_fill(want, 0), clean[1].masked_fill(want, 0)) and torch.equal(lse, clean[2])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("seqs,tokens", SPOILED, ids=range(len(SPOILED)))
+def test_attention_keeps_nan_keys_to_the_rows_that_see_them(seqs, tokens, causal):
+    import torch
+    nq, nkv, hd = 4, 2, 128
+    c = _attn_case(seqs, "f16", hd, nq, nkv, seed=79)
+    n, L = seqs[0]
+    t = tokens[-2]
+    clean = _attn_run(_spoil(c, "kpool", [(0, t, 1, [5])]), causal)
+    _, out, lse = _attn_run(c, causal)
+    want = torch.zeros(out.shape[0], nkv, nq // nkv, dtype=torch.bool)
+    want[max(0, t - (L - n)) if causal else 0: n, 1] = True
+    want = want.view(-1, nq)
+    assert torch.equal(lse.isnan(), want)
+    bad = want[..., None].expand(-1, -1, hd).reshape(out.shape)
+    assert torch.equal(out.isnan(), bad)
+    assert torch.equal(out[~bad], clean[1][~bad]) and torch.equal(lse[~want], clean[2][~want])
