@@ -408,7 +408,7 @@ cudaError_t launch(AppendParams& ap, cudaStream_t s) {
   const long long ctas = static_cast<long long>(ap.seqs.n_seqs) * ap.runs_per_seq * ap.ctas;
   if (ctas > 0x7FFFFFFFll) return cudaErrorInvalidValue;
   const uint32_t bytes = (ap.heads + 2) * slot;
-  if (bytes > 48 * 1024) {
+  if (bytes > 47 * 1024) {  // 48 KB without it, the kernel's own variables among them
     const cudaError_t e = cudaFuncSetAttribute(kv_append_kernel<T, HD, B8>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, kStage);
     if (e != cudaSuccess) return e;

@@ -1,14 +1,15 @@
 """Edges of the operators of growing sessions, against the same plain
 implementations in 64 bits and with the same bounds as test_session_ops_gpu.py:
-zero points over the whole byte, axes that are not there,
-calls without tables, bounds that say nothing, captures of a stream that
-is not the current one, workspaces of any size, a sequence's company, many
-rows in many chunks, NaN codes that only some rows see."""
+zero points over the whole byte, scales below the normal range, any number of
+rows; axes that are not there, any heads and tokens of a CTA, calls without
+tables; bounds that say nothing, captures of a stream that is not the current
+one, workspaces of any size, a sequence's company, many rows in many chunks,
+NaN codes that only some rows see."""
 import pytest
 
 from conftest import cuda_ok, pkg
-from test_session_ops_gpu import (PAGE, _append_case, _attn_case, _attn_run, _check_append, _check_attn, _check_w4,
-                                  _split, _w4_case)
+from test_session_ops_gpu import (PAGE, _append_case, _append_run, _attn_case, _attn_run, _check_append, _check_attn,
+                                  _check_w4, _split, _w4_case)
 
 pytestmark = pytest.mark.gpu
 
@@ -98,6 +99,16 @@ def test_append_reports_an_axis_that_is_not_there(bits):
         status, q_out = run(axis)
         assert status == 2, bad
         assert torch.equal(q_out, run(as_first)[1]), bad
+
+
+@pytest.mark.parametrize("hd,bits", [(128, 8), (128, 16), (64, 8), (64, 16)])
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 7, 10, 14, 22, 46])
+@pytest.mark.parametrize("n", [1, 2, 8, 16, 33, 64])
+def test_append_of_any_group_and_number_of_tokens(hd, bits, group, n):
+    """The heads of a CTA and its tokens make its shared memory: each size launches.
+    (48 KB with the kernel's own variables is where a launch has to ask for more.)"""
+    c = _append_case([(n, n + 70), (1, 1)], "f16", hd, group, 1, bits, False, 0, seed=group)
+    _check_append(c, _append_run(c))
 
 
 def _append_c(c, max_q, n_axes=1, axis_of=0):
