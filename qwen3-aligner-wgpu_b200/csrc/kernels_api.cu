@@ -120,6 +120,14 @@ bool cache_args_ok(int nq, int nkv, const int* q_start, const int* kv_len, int n
          max_pages > 0 && kv_pages > 0 && nq > 0 && nkv > 0 && nq % nkv == 0;
 }
 
+// The answer to a launch.  A failed one's error is taken off the runtime's record, or
+// the next call of anybody in the process would be told of it.
+int answer(int rc) {
+  if (rc == 0) return QA_OK;
+  cudaGetLastError();
+  return QA_ERR_CUDA;
+}
+
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace
@@ -151,7 +159,7 @@ extern "C" int qa_k_kv_append(const void* q, long long ldq, const void* k, long 
   const int rc = kv_append(q, ldq, k, ldk, v, ldv, q_out, ldqo, T, nq, nkv, hd, seqs, max_q,
                            PagedKV{kpool, vpool, 64}, kv_pages, kscale, vscale, rope, qn, kn, eps,
                            bf16 != 0, status, static_cast<cudaStream_t>(stream));
-  return rc == 0 ? QA_OK : QA_ERR_CUDA;
+  return answer(rc);
 }
 
 extern "C" int qa_k_cache_attention(const void* q, long long ldq, long long T, int nq, int nkv,
@@ -176,7 +184,7 @@ extern "C" int qa_k_cache_attention(const void* q, long long ldq, long long T, i
   const int rc = cache_attention(q, ldq, T, nq, nkv, hd, seqs, max_q, max_kv, kpool, vpool,
                                  kv_pages, kscale, vscale, scale, causal != 0, out, ldo, lse,
                                  workspace, workspace_bytes, bf16 != 0, status, static_cast<cudaStream_t>(stream));
-  return rc == 0 ? QA_OK : QA_ERR_CUDA;
+  return answer(rc);
 }
 
 extern "C" int64_t qa_k_cache_attention_workspace(int nq, int nkv, int hd, int n_seqs, int max_q,
@@ -195,7 +203,7 @@ extern "C" int qa_k_w4_linear(const void* x, long long ldx, int M, int K, const 
     return QA_ERR_SHAPE;
   const int rc = w4_linear(x, ldx, M, K, wq, ldw, N, group, scales, zeros, bias, out, ldo,
                            bf16 != 0, static_cast<cudaStream_t>(stream));
-  return rc == 0 ? QA_OK : QA_ERR_CUDA;
+  return answer(rc);
 }
 
 namespace {

@@ -1,7 +1,7 @@
 """Edges of the operators of growing sessions, against the same plain
 implementations in 64 bits and with the same bounds as test_session_ops_gpu.py:
 zero points over the whole byte, scales below the normal range, any number of
-rows; axes that are not there, any heads and tokens of a CTA, calls without
+rows, launches that fail; axes that are not there, any heads and tokens of a CTA, calls without
 tables; bounds that say nothing, captures of a stream that is not the current
 one, workspaces of any size, a sequence's company, many rows in many chunks,
 NaN codes that only some rows see."""
@@ -71,6 +71,34 @@ def test_w4_takes_any_number_of_rows():
     pkg()._lib.w4_linear(x, c["wq"].cuda(), c["scales"].cuda(), out, zeros=c["zeros"].cuda(), bias=c["bias"].cuda())
     _check_w4(c, out[torch.tensor(rows, device="cuda")])
     assert bool((out[16: at - 16] == c["bias"].cuda().bfloat16()).all())
+
+
+def test_a_launch_that_fails_is_not_told_to_the_next_caller():
+    """A stream whose capture has been invalidated takes no launch.  The call says so,
+    and the runtime's record of errors is as clean as before."""
+    import ctypes
+    import torch
+    rt = ctypes.CDLL("libcudart.so.12")
+    c = _w4_case(2, 64, 128, 128, "f16", False, False, seed=83)
+    x, wq, scales, out = c["x"].cuda(), c["wq"].cuda(), c["scales"].cuda(), torch.empty(2, 64, device="cuda").half()
+    s = torch.cuda.Stream()
+    pkg()._lib.w4_linear(x, wq, scales, out, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    stream, graph = ctypes.c_void_p(s.cuda_stream), ctypes.c_void_p()
+    assert rt.cudaStreamBeginCapture(stream, 2) == 0
+    try:
+        assert rt.cudaStreamSynchronize(stream) != 0  # not while it captures
+        rt.cudaGetLastError()
+        with pytest.raises(pkg().QaError):
+            pkg()._lib.w4_linear(x, wq, scales, out, stream=s.cuda_stream)
+        left = rt.cudaPeekAtLastError()
+    finally:
+        rt.cudaStreamEndCapture(stream, ctypes.byref(graph))
+        rt.cudaGetLastError()
+    assert left == 0
+    pkg()._lib.w4_linear(x, wq, scales, out, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    _check_w4(c, out)
 
 
 # ---------------------------------------------------------------- kv_append
