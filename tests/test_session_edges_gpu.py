@@ -1,10 +1,11 @@
 """Edges of the operators of growing sessions, against the same plain
 implementations in 64 bits and with the same bounds as test_session_ops_gpu.py:
 zero points over the whole byte, scales below the normal range, any number of
-rows, launches that fail; axes that are not there, any heads and tokens of a CTA, calls without
-tables; bounds that say nothing, captures of a stream that is not the current
-one, workspaces of any size, a sequence's company, many rows in many chunks,
-NaN codes that only some rows see."""
+rows, launches that fail; axes that are not there, any heads and tokens of a
+CTA, calls without tables; bounds that say nothing, captures of a stream that is
+not the current one, workspaces of any size, a sequence's company, many rows in
+many chunks, many sequences, wide groups of heads, NaN codes that only some rows
+see."""
 import pytest
 
 from conftest import cuda_ok, pkg
@@ -366,3 +367,34 @@ def test_attention_keeps_nan_keys_to_the_rows_that_see_them(seqs, tokens, causal
     bad = want[..., None].expand(-1, -1, hd).reshape(out.shape)
     assert torch.equal(out.isnan(), bad)
     assert torch.equal(out[~bad], clean[1][~bad]) and torch.equal(lse[~want], clean[2][~want])
+
+
+def _crowd(count, most, length, seed):
+    """Many sequences, some without new tokens, some without any."""
+    import random
+    r = random.Random(seed)
+    seqs = [(r.choice([0, 1, 1, most, r.randint(1, most)]), r.choice([0, 1, 64, r.randint(1, length)])) for _ in range(count)]
+    return [(min(n, max(L, 1)), max(L, min(n, 1))) for n, L in seqs]
+
+
+@pytest.mark.parametrize("most,length", [(1, 300), (1, 2600), (70, 500)])
+@pytest.mark.parametrize("count", [129, 449, 1500])
+def test_attention_of_many_sequences(count, most, length):
+    """More of them than a CTA has threads to look for its share with."""
+    seqs = _crowd(count, most, length, seed=count)
+    c = _attn_case(seqs, "f16", 64, 4, 2, seed=89)
+    _check_attn(c, _attn_run(c))
+
+
+def test_append_of_many_sequences():
+    seqs = _crowd(1500, 70, 500, seed=97)
+    c = _append_case([(min(n, L), L) for n, L in seqs], "bf16", 64, 4, 2, 8, True, 0, seed=97)
+    _check_append(c, _append_run(c))
+
+
+@pytest.mark.parametrize("seqs", [[(1, 300), (1, 1)], [(3, 2000), (2, 64)]])
+@pytest.mark.parametrize("nq", [24, 25, 300, 520])
+def test_attention_of_wide_groups(nq, seqs):
+    """A single token's heads of one K/V head fill a tile of rows, or several."""
+    c = _attn_case(seqs, "bf16", 64, nq, 1, seed=101)
+    _check_attn(c, _attn_run(c))
