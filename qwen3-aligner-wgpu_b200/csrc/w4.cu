@@ -94,20 +94,20 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
 }
 
 // The pairs of nibbles (0,4) (1,5) (2,6) (3,7) of a word, less the zero, as
-// 16-bit values:  code - zero = (base + 15 - zero) - (base + (15 - code)).  The
-// nibble's complement 15 - code goes into the mantissa of a power of two by bit
-// work: f16 with 1024, its low four bits, and with 64, four bits higher, so one
-// shift serves two pairs; bf16 with 128.  base + 15 - zero lies in [-176, 1039] for
-// every byte (bf16: [-112, 143]) and is exact, which base + zero is not in bf16 (no
-// odd numbers above 256); so are the differences, at most 255 in size.
+// 16-bit values, by bit work in the mantissa of a power of two.  f16 has 1024 + code
+// in its low four bits and 64 + 15 - code four bits higher, so one shift serves two
+// pairs; bf16 has 128 + 15 - code.  For every byte 1024 + zero, 64 + 15 - zero and
+// 128 + 15 - zero are exact (base + zero is not: no odd numbers above 256 in bf16,
+// and no room for it in the mantissa above 64), and so are the differences
+//   code - zero = (1024 + code) - (1024 + zero) = (base + 15 - zero) - (base + 15 - code).
 template <typename T>
-struct Zero {  // base + 15 - zero, twice
+struct Zero {  // f16: 1024 + zero and 79 - zero; bf16: 143 - zero; twice
   uint32_t lo, hi;
   __device__ __forceinline__ Zero() {
     if constexpr (H16Traits<T>::kBf16) {
       lo = hi = 0x43074307u;  // 135
     } else {
-      lo = 0x64076407u;  // 1031
+      lo = 0x64086408u;  // 1032
       hi = 0x54705470u;  // 71
     }
   }
@@ -118,16 +118,14 @@ struct Zero {  // base + 15 - zero, twice
       const float f = 8388608.0f + 143.0f - __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7640u | at));
       lo = hi = cvt2_rn<T>(make_float2(f, f));
     } else {
-      const uint32_t z = __byte_perm(w, 0x00000064u, 0x4040u | at * 0x101u);  // 1024 + zero, twice
-      const __half2 h = __hsub2(__half2half2(__ushort_as_half(0x644F)), *reinterpret_cast<const __half2*>(&z));  // 1103 -
-      const __half2 l = __hadd2(h, __half2half2(__ushort_as_half(0x6380)));                                      // + 960
-      lo = *reinterpret_cast<const uint32_t*>(&l);
+      lo = __byte_perm(w, 0x00000064u, 0x4040u | at * 0x101u);
+      const __half2 h = __hsub2(__half2half2(__ushort_as_half(0x644F)), *reinterpret_cast<const __half2*>(&lo));  // 1103 -
       hi = *reinterpret_cast<const uint32_t*>(&h);
     }
   }
 };
 // The masks and bases in registers: an instruction takes one constant, and
-// (~w & mask) | base is one instruction only when the other operand is a register.
+// (w & mask) | base is one instruction only when the other operand is a register.
 template <typename T>
 struct Bits {
   uint32_t mask_lo, base_lo, mask_hi, base_hi;
@@ -138,6 +136,11 @@ struct Bits {
     asm volatile("mov.b32 %0, 0x54005400;" : "=r"(base_hi));
   }
 };
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t base) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(base));
+  return d;
+}
 __device__ __forceinline__ uint32_t andn_or(uint32_t a, uint32_t mask, uint32_t base) {
   uint32_t d;
   asm("lop3.b32 %0, %1, %2, %3, 0xAE;" : "=r"(d) : "r"(a), "r"(mask), "r"(base));  // (~a & mask) | base
@@ -157,9 +160,10 @@ __device__ __forceinline__ void weights8(uint32_t w, const Zero<T>& z, const Bit
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t u = i < 2 ? w : w >> 8;
-      const uint32_t v = i & 1 ? andn_or(u, k.mask_hi, k.base_hi) : andn_or(u, k.mask_lo, k.base_lo);
-      const __half2 d =
-          __hsub2(*reinterpret_cast<const __half2*>(i & 1 ? &z.hi : &z.lo), *reinterpret_cast<const __half2*>(&v));
+      const uint32_t v = i & 1 ? andn_or(u, k.mask_hi, k.base_hi) : and_or(u, k.mask_lo, k.base_lo);
+      const __half2 c = *reinterpret_cast<const __half2*>(&v);
+      const __half2 d = i & 1 ? __hsub2(*reinterpret_cast<const __half2*>(&z.hi), c)
+                              : __hsub2(c, *reinterpret_cast<const __half2*>(&z.lo));
       out[i] = *reinterpret_cast<const uint32_t*>(&d);
     }
   }
