@@ -175,9 +175,13 @@ int qa_k_kv_append(const void* q, long long ldq, const void* k, long long ldk, c
  * workspace: device memory, 16-byte aligned, of the size that
  * qa_k_cache_attention_workspace gives for these arguments (0: none is needed);
  * what it holds does not matter, and two calls that may run at the same time
- * need one each.  With less of it, or NULL, some or all sequences are not split
- * over CTAs, which is slow for few long caches.  A sequence's result does not
- * depend on the others of the batch, as long as the workspace has the size given.
+ * need one each.  With less of it, or NULL, the last or all sequences are not
+ * split over CTAs, which is slow for few long caches.  More than 1 GiB is never
+ * asked for: of the sequences past it the same holds.
+ *
+ * The others of the batch bear on a sequence's result only through max_q, which
+ * chooses the kernel and its tiles of rows (other sums, within rounding), and
+ * where they leave it no place in the workspace.
  */
 int64_t qa_k_cache_attention_workspace(int nq, int nkv, int hd, int n_seqs, int max_q, int max_kv);
 int qa_k_cache_attention(const void* q, long long ldq, long long T, int nq, int nkv, int hd,
@@ -192,8 +196,8 @@ int qa_k_cache_attention(const void* q, long long ldq, long long T, int nq, int 
  * W[n][k] = scales[n][k / group] * (code[n][k] - zeros[n][k / group]), zeros any
  * byte, 8 when NULL.  wq [N] rows of K / 2 bytes, ldw bytes apart, the even k of a pair
  * in the low nibble; scales [N][K / group] in x's type; group 32, 64 or 128, K a
- * multiple of it.  f32 sums, one rounding.  Built for few rows, where the
- * weights are what has to be read; any M is taken.
+ * multiple of it.  f32 sums, one rounding; M and N bear on their order.  Built
+ * for few rows, where the weights are what has to be read; any M is taken.
  */
 int qa_k_w4_linear(const void* x, long long ldx, int M, int K, const uint8_t* wq, long long ldw,
                    int N, int group, const void* scales, const uint8_t* zeros, const float* bias,

@@ -24,7 +24,7 @@ namespace {
 // Bound: the cache's bytes, read once (2 hd a token and head), so what matters
 // is that every SM reads all the time, bytes in flight and instructions a byte.
 //  - A unit's cached tokens are cut into chunks by the unit's own length alone
-//    (so a sequence's result does not depend on the batch it is in).  The slabs
+//    (the batch it is in does not move a sequence's cuts).  The slabs
 //    of 32 tokens of all units, laid end to end, are shared out evenly over the
 //    CTAs that the GPU holds; a CTA takes the chunks that begin in its share,
 //    which it finds from kv_len and q_start itself.  Its four warps take every
@@ -49,8 +49,9 @@ namespace {
 // PRMT per two pairs); P^T comes from S^T's layout by movmatrix.
 //
 // e4m3 codes are exact in f16.  So are bf16 queries once a row is scaled by a
-// power of two that brings its largest component to [2^14, 2^15): what falls
-// into f16's subnormals lies 2^-39 below that.  P is rounded to f16.
+// power of two that brings its largest component to [2^14, 2^15): components up to
+// 2^28 smaller keep all their bits, and what is lost of others lies 2^-39 below the
+// largest.  P is rounded to f16 (cache_attn.cuh says what that costs).
 //
 // As M moves rarely, a slab usually needs one vote instead of a maximum across
 // lanes.
@@ -785,9 +786,9 @@ cudaError_t launch_any(const CacheAttnParams& ap, void* ws, long long ws_bytes, 
 }
 
 // Rows of a K/V head and sequence up to which the few-row kernel is used: as far as
-// its registers reach.  12 tokens, 24 rows, of 16 sessions over 5000 tokens: 109 us
-// here with chunks of 256 tokens, 125 on the tcgen05 kernel, which pads them to 128
-// rows (8 tokens, 16 rows: 84 and 123; one session of 24 rows: 33 and 39).
+// its registers reach.  24 rows over 5000 tokens each (16/8 heads of 128), 16 sessions:
+// 80 us here, 124 on the tcgen05 kernel, which pads them to 128 rows; 16 rows: 65 and
+// 122.  One session of 24 rows over 8192 tokens: 38 and 42, over 131,000: 104 and 156.
 constexpr int kFewRows = 24;
 
 }  // namespace

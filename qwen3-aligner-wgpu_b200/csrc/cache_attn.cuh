@@ -45,8 +45,15 @@ constexpr float kLog2e = 1.4426950408889634f;
 // 2^kSlack (any reference gives the same quotient); kLift keeps the small p of a
 // long cache out of f16's subnormals, and 2^(kLift + kSlack) is below its largest
 // value.
+//
+// P is f16 because the matrix instructions take 16 bits and V's codes are exact in
+// f16; m, l and O stay in f32.  A p is off by 2^-11 of itself, or by 2^-25 where it
+// is below 2^-14, which is 2^-22 or less of the row's largest: a token that counts
+// that little beside another (its probability times its page's V scale) keeps fewer
+// bits, and is lost below 2^-33.  Against 64 bits, outputs of 421 tokens are off by
+// 2.3e-4 of their norm in f16 (2.1e-4 with P in 32 bits: the outputs' own rounding)
+// and by 1.7e-3 in bf16 either way.
 constexpr float kLift = 8.0f, kSlack = 6.0f;
-
 
 // Four e4m3 codes (low byte first) as two f16x2; NaN codes stay NaN.
 __device__ __forceinline__ void e4m3x4_f16x2(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -117,8 +124,10 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& ap, const Unit
 // then summed in turn.  Many rows of few parts (kAlone): a warp a row.  Bound by
 // latency: a part's row is one line of 4 hd bytes.
 constexpr int kJoinWarps = 8;
-// Parts up to which a warp joins a row alone (16 sessions of 24 rows over 8192 tokens,
-// 32 parts: 162 us in all against 176; one session 29 against 25).
+// Parts up to which a warp joins a row alone.  24 rows a head (16/8 heads of 128), in
+// all, against a CTA a row: 16 sessions over 8192 tokens, 11 parts, 103 and 124 us;
+// over 24,576, 32 parts, 259 and 276, but one session 36 and 32.  More parts: one
+// session over 50,000, 66 parts, 73 and 60; four over 100,000 292 and 276.
 constexpr int kJoinAlone = 32;
 
 // grid: (sequences x tiles, K/V heads, rows, or rows / 8)

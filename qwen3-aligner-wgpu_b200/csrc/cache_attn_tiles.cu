@@ -25,9 +25,11 @@
 //
 // TMEM: S_h (P_h over it) at 128 h, O_h at 256 + 128 h.
 //
-// Bound by the softmax's chain (about 4,000 of a key tile's 6,600 cycles) and an
-// item's fixed cost (25,000 cycles).  Measured on a B200: four sessions of up to 1024
-// new tokens over 8192 (16/8 heads of 128) 323 us, 328 TFLOP/s.
+// Bound by the softmax's chain and by what an item costs besides its key tiles.
+// Measured on a B200: one unit of 256 rows a CTA, nothing masked, takes 21 us and 2.4 us
+// (4,800 cycles, where the products need 2,900) a key tile; four sessions of up to 1024
+// new tokens over 8192 (16/8 heads of 128) 323 us, 328 TFLOP/s, the join among them (40
+// us by itself), with the tensor pipes active for a quarter of the time.
 #include <algorithm>
 
 #include "cache_attn.cuh"
@@ -53,9 +55,9 @@ constexpr int kMaxChunks = 16;
 
 // Key tiles of a chunk of a sequence with `keys` key tiles and `tiles` units a
 // head: enough chunks to fill the GPU from one sequence, as few as that takes.  1024
-// new tokens over 8192, 16/8 heads: one session 123 us with 16 in kMaxChunks and 182
-// with 8, which leaves SMs idle; eight sessions 760 and 707 (no parts).  256 new
-// tokens: 72 and 82.  The number of sequences must not decide: a sequence's result
+// new tokens over 8192, 16/8 heads: one session 125 us with 16 in kMaxChunks and 185
+// with 8, which leaves SMs idle; eight sessions 767 and 704 (no parts).  256 new
+// tokens: 71 and 83.  The number of sequences must not decide: a sequence's result
 // would depend on the others.
 __host__ __device__ __forceinline__ int chunk_step(int keys, int tiles) {
   const int want = kMaxChunks / tiles > 1 ? kMaxChunks / tiles : 1;

@@ -28,8 +28,8 @@
 //
 // Bound by bytes for long prompts, by the latency of a chain of dependent loads
 // (maps, positions, rows) and the launch for few tokens.  Measured on a B200: four
-// prompts of up to 8192 tokens into the 16-bit cache (16/8 heads of 128) 65 us,
-// 5.0 TB/s; 24 ragged sequences (14/2 heads of 64, three axes, 8 bits) 16.5 us, 3.5
+// prompts of up to 8192 tokens into the 16-bit cache (16/8 heads of 128) 68 us,
+// 4.9 TB/s; 24 ragged sequences (14/2 heads of 64, three axes, 8 bits) 16.5 us, 3.5
 // TB/s, 26 with the inputs in registers and a loop over the heads; 64 sequences of
 // one token 9.4 us in the kernel, 18 with CTAs of 256 threads.
 #include <cuda_fp8.h>

@@ -27,10 +27,10 @@
 // shared memory in the CTAs' order.  No atomics, the same bits each time.
 //
 // Bound by the latency of a warp's step (copies, bit work, products and scales in
-// one chain, 16 warps an SM; an issue slot is used every second cycle, DRAM at up to
-// 45 %).  Measured on a B200: 4096 x 1024, one row, 8.1 us a call (10.2 without the
-// split of K); 8191 x 8192, 5 rows, groups of 64 with zeros, 20.1 us (63 without the
-// split); 151936 x 1024, 16 rows, 30 us, 2.8 TB/s.  W through a ring in shared memory
+// one chain, 16 warps an SM; 32 to 42 % of the issue slots are used, and 19 to 29 % of
+// DRAM's time).  Measured on a B200: 4096 x 1024, one row, 8.5 us a call (10.2 without
+// the split of K); 8191 x 8192, 5 rows, groups of 64 with zeros, 20.2 us (63 without
+// the split); 151936 x 1024, 16 rows, 30 us, 2.8 TB/s.  W through a ring in shared memory
 // came out the same or slower (22 and 30 us), 24 warps with fewer registers too (29
 // and 35).
 #include <algorithm>

@@ -16,7 +16,9 @@ set of sessions:
 
 A layer is `w4_linear` (q, k and v as one), `kv_append` (q/k RMSNorm, rotation,
 cache), `cache_attention`, `w4_linear` (output), and `w4_linear` twice for the
-gated MLP; the norms and the gate between them are plain tensor operations.
+gated MLP; the norms and the gate between them are plain tensor operations.  How
+many tokens a step takes, and the most of one session, bear on the order of sums:
+a session beside others agrees with itself alone within rounding.
 """
 from __future__ import annotations
 
